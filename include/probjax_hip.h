@@ -499,6 +499,137 @@ int pjx_mla_project_bwd(int dtype, const void* cache, const void* wk, const void
                         size_t workspace_bytes, int64_t batch, int64_t kv_len, int64_t heads, int64_t rank,
                         int64_t qk_dim, int64_t v_dim, int64_t width, void* stream);
 
+/*
+ * Elements between consecutive sequences, tokens and heads of a K and a V cache
+ * (features are contiguous); every one whole 16-byte chunks.  Pass NULL for
+ * contiguous [B, Lk, Hkv, row_dim] caches.
+ */
+typedef struct pjx_cache_strides {
+  int64_t k_batch, k_token, k_head;
+  int64_t v_batch, v_token, v_head;
+} pjx_cache_strides;
+
+/*
+ * Attention of q_len drafted tokens, which form a tree, over a KV cache: the
+ * verification step of speculative decoding.  No counterpart in the reference,
+ * whose split-KV decode (kernels/attention_splitkv.py:137-250) takes no mask.
+ *
+ * Sequence b's prefix is its keys [0, P), P = kv_lengths[b] clamped to [0, kv_len]
+ * (NULL: kv_len - q_len); the drafted tokens' own keys are slots P .. P + q_len - 1
+ * of the same cache, as far as it reaches.  Token t sees the prefix and, of the
+ * drafted keys, those of
+ *   parents   -- int32 [trees, q_len]: t itself, parents[t], its parent, and so on
+ *                until a negative one.  A parent that is no earlier token counts as
+ *                -1.  Below -1 the slot holds no token: its row has no valid key.
+ *   tree_mask -- bytes [trees, q_len, q_len]: j where tree_mask[t][j] != 0.
+ * One of the two is given; trees is 1 (one tree for the batch) or batch.
+ * What a row does not see does not reach it, infinities and NaN included.  Rows
+ * without a valid key give output 0 and LSE +inf.
+ *
+ * q, o [B, q_len, Hq, row_dim]; k, v [B, kv_len, Hkv, row_dim] (or strides); all
+ * start on 16 bytes.  head_dim, the kernel's width: 64, 128 or 256; row_dim:
+ * head_dim, or in 16 bits a multiple of 8 up to a head_dim of 64 or 128.
+ * q_len <= 256.  dtype, lse, chunk and workspace as pjx_splitkv_decode with
+ * v_dim = head_dim.
+ */
+int pjx_tree_decode(int dtype, const void* q, const void* k, const void* v, const int32_t* kv_lengths,
+                    const int32_t* parents, const uint8_t* tree_mask, int64_t trees, void* o, float* lse,
+                    void* workspace, size_t workspace_bytes, int64_t batch, int64_t q_len, int64_t kv_len,
+                    int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t row_dim,
+                    const pjx_cache_strides* strides, float sm_scale, int64_t chunk, void* stream);
+
+/*
+ * The softmax weight that every key was given, added to weights [B, Hkv, kv_len]
+ * (NULL: zeros) into weights_out (the same memory or none of it):
+ *   weights_out[b, g, j] = weights[b, g, j] + sum over rows t and heads h of g's
+ *                          group of exp(sm_scale q_ht.k_gj - lse_ht)
+ * in float32; keys that no row sees keep theirs.  What eviction goes by
+ * (pjx_evict_keys); no counterpart in the reference, whose kernels return no
+ * weights.
+ *
+ * pjx_weighted_decode: a decode step (pjx_splitkv_decode with head_dim = v_dim; up
+ * to 64 rows (Hq/Hkv)*q_len per KV head) that gives the weights beside its output.
+ * Shapes, row_dim, strides and alignment as pjx_tree_decode.  workspace: on 16
+ * bytes, at least pjx_weighted_decode_workspace_size() bytes (the decode's partials
+ * and the scores) with the same chunk.
+ *
+ * pjx_key_weights: for any number of rows, from the LSE [B, Hq, q_len] of
+ * pjx_flash_fwd (+inf rows give nothing) with its masks: kv_lengths, and with causal
+ * != 0 k <= q + causal_shift.  q [B, q_len, Hq, row_dim], k [B, kv_len, Hkv,
+ * row_dim], contiguous, on 16 bytes; head_dim 64, 128 or 256; row_dim: head_dim, or
+ * in 16 bits a multiple of 8 up to it.  workspace: pjx_key_weights_workspace_size()
+ * bytes of partial sums, added in a fixed order.
+ */
+size_t pjx_weighted_decode_workspace_size(int64_t batch, int64_t kv_heads, int64_t rows, int64_t kv_len,
+                                          int64_t head_dim, int64_t chunk);
+int pjx_weighted_decode(int dtype, const void* q, const void* k, const void* v, const int32_t* kv_lengths,
+                        const float* weights, float* weights_out, void* o, float* lse, void* workspace,
+                        size_t workspace_bytes, int64_t batch, int64_t q_len, int64_t kv_len, int64_t q_heads,
+                        int64_t kv_heads, int64_t head_dim, int64_t row_dim, const pjx_cache_strides* strides,
+                        float sm_scale, int64_t chunk, void* stream);
+size_t pjx_key_weights_workspace_size(int64_t batch, int64_t q_len, int64_t kv_len, int64_t q_heads);
+int pjx_key_weights(int dtype, const void* q, const void* k, const float* lse, const int32_t* kv_lengths,
+                    const float* weights, float* weights_out, void* workspace, size_t workspace_bytes,
+                    int64_t batch, int64_t q_len, int64_t kv_len, int64_t q_heads, int64_t kv_heads,
+                    int64_t head_dim, int64_t row_dim, int causal, int64_t causal_shift, float sm_scale,
+                    void* stream);
+
+/*
+ * Rotary positions of 1 to 4 axes (time, height and width of images and video)
+ * applied to q and k in one launch, or undone (inverse != 0: the gradient).
+ * The reference's RotaryPosEncode (layers/encoding.py:107-211) is one axis,
+ * interleaved.
+ *
+ * Of every row of head_dim features the first R = sum(sections) are rotated, in
+ * R/2 pairs; the rest pass.  Section a (sections[a] features, even, 0 or more) is
+ * turned by the positions of axis a:
+ *   shared_spectrum 0 -- every section is an embedding of its own: its pair i has
+ *     frequency base^(-2i / sections[a]);
+ *   shared_spectrum 1 -- the R features are one embedding whose pair p has
+ *     frequency base^(-2p / R); the sections deal the pairs to the axes.
+ * interleaved 1: a pair is two neighbouring features; 0: feature i of an
+ * embedding's first half and feature i of its second half.
+ *   (a, b) -> (a cos - b sin, b cos + a sin), angle = position * frequency
+ * Angles are formed in float64 (reduced to one turn), the rest in float32,
+ * rounded once.
+ *
+ * q [B, T, q_heads, D] and k [B, T, k_heads, D] (k_heads 0: none) with `strides`
+ * in elements (k_* of the struct for q, v_* for k; NULL: contiguous); q_out and
+ * k_out are contiguous.  positions: PJX_POSITION_* values, element (b, t, a) at
+ * b * position_batch_stride + t * position_token_stride + a (a batch stride of 0:
+ * the same for every sequence).  sections: host array.  head_dim <= 256.
+ */
+#define PJX_POSITION_I32 0
+#define PJX_POSITION_I64 1
+#define PJX_POSITION_F32 2
+#define PJX_POSITION_F64 3
+int pjx_rotary(int dtype, const void* q, const void* k, void* q_out, void* k_out, const void* positions,
+               int position_type, int64_t position_batch_stride, int64_t position_token_stride, int64_t batch,
+               int64_t len, int64_t q_heads, int64_t k_heads, int64_t head_dim, const pjx_cache_strides* strides,
+               const int32_t* sections, int64_t axes, double base, int interleaved, int shared_spectrum,
+               int inverse, void* stream);
+
+/*
+ * Eviction from a KV cache: every (sequence, KV head) is cut to its `keep` keys of
+ * most weight.  No counterpart in the reference.  Of n = kv_lengths[b] keys (clamped
+ * to [0, kv_len]; NULL: kv_len) n <= keep are all kept; else the first `sinks`, the
+ * last `recent` and, between them, those of the largest weights [B, Hkv, kv_len]
+ * (NaN before all others, -0 as 0, ties to the lower slot).  Kept keys stay in their
+ * order:
+ *   index       [B, Hkv, keep] int32: the slot each came from, -1 behind the last
+ *   lengths_out [B] int32: min(n, keep)
+ *   k_out, v_out rows, weights_out [B, Hkv, out_len] (out_len >= keep): what they held
+ * Rows at and behind lengths_out[b] up to keep are zeroed with fill != 0, and all
+ * of them left as they are without.  Out buffers must not overlap the inputs.
+ * elem_size: bytes of an element of k and v (2 or 4); strides in elements, features
+ * contiguous (NULL: contiguous, [B, kv_len, Hkv, D] and [B, out_len, Hkv, D]).
+ */
+int pjx_evict_keys(int64_t elem_size, const void* k, const void* v, const float* weights, const int32_t* kv_lengths,
+                   void* k_out, void* v_out, float* weights_out, int32_t* lengths_out, int32_t* index, int64_t batch,
+                   int64_t kv_len, int64_t kv_heads, int64_t head_dim, int64_t out_len, int64_t keep, int64_t sinks,
+                   int64_t recent, const pjx_cache_strides* strides, const pjx_cache_strides* out_strides, int fill,
+                   void* stream);
+
 #ifdef __cplusplus
 }
 #endif

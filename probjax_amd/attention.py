@@ -39,6 +39,7 @@ from __future__ import annotations
 import functools
 import math
 import os
+from typing import NamedTuple
 
 import torch
 
@@ -590,6 +591,222 @@ def splitkv_forward(q, k, v, *, sm_scale: float, num_splits: int | None = None,
     if v_width == dv or rows is not None:
         return res
     return (res[0][..., :dv], res[1]) if return_lse else res[..., :dv]
+
+
+def tree_attention(q, k, v, *, parents=None, tree_mask=None, kv_lengths=None, sm_scale: float | None = None,
+                   return_lse: bool = False):
+    """Attention of drafted tokens that form a tree over a KV cache, the
+    verification step of speculative decoding (no counterpart in the reference).
+
+    ``q [B, T, Hq, D]`` are the T drafted tokens (up to 256), ``k`` / ``v``
+    ``[B, S, Hkv, D]`` the caches: sequence b's prefix is its first
+    ``kv_lengths[b]`` keys (None: all but the last T slots), and the drafted
+    tokens' own keys follow it in the same cache, as far as it reaches.  Every
+    token sees the prefix and the drafted keys that the tree gives it:
+
+    * ``parents`` (int ``[T]``, or ``[B, T]`` for a tree per sequence): token t
+      sees itself, ``parents[t]``, its parent, and so on; a negative parent is
+      the prefix.  Parents come before their children (one that does not counts
+      as -1).  A parent below -1 marks a slot without a token (batches of trees
+      of different sizes): its output is 0 and its LSE +inf, and no token whose
+      ancestors do not name it sees it.
+    * ``tree_mask`` (bool ``[T, T]`` or ``[B, T, T]``): token t sees drafted key
+      j where ``tree_mask[t, j]``.
+
+    What a token does not see does not reach its output, infinities and NaN
+    included; a token that sees nothing gets 0 and LSE +inf.  bf16, fp16 or
+    fp32, head dims up to 256, caches in any order of their first three axes.
+    ``sm_scale`` defaults to ``1/sqrt(D)``.  With ``return_lse`` also the
+    natural-log LSE ``[B, Hq, T]``.  No gradient: inputs that require one raise.
+    """
+    if sm_scale is None:
+        sm_scale = 1.0 / math.sqrt(q.shape[-1])
+    d = q.shape[-1]
+    res = hip.tree_decode(q, k, v, sm_scale=sm_scale, parents=parents, tree_mask=tree_mask, kv_lengths=kv_lengths,
+                          return_lse=return_lse)
+    out = res[0] if return_lse else res
+    if out.shape[-1] != d:
+        out = out[..., :d]
+    return (out, res[1]) if return_lse else out
+
+
+def attention_with_key_weights(q, k, v, key_weights=None, *, mask=None, sm_scale: float | None = None,
+                               return_lse: bool = False):
+    """Softmax attention that also adds up the weight every key was given
+    (no counterpart in the reference; ``evict_keys`` goes by the sums).
+
+    ``q [B, T, Hq, D]``, ``k`` / ``v`` ``[B, S, Hkv, D]``; ``key_weights`` float32
+    ``[B, Hkv, S]``, the sums so far (None: zeros).  Returns ``(out,
+    key_weights)``, a new tensor each: ``key_weights[b, g, j]`` plus the softmax
+    weights of key j over the T rows of the Hq/Hkv query heads that share it.
+    Masks: None, ``KVLenMask``, ``CausalMask``, ``CausalFromBottomRightMask`` and
+    their intersections.  bf16, fp16 or fp32, head dims up to 256; ``sm_scale``
+    defaults to ``1/sqrt(D)``.  With ``return_lse`` also the LSE ``[B, Hq, T]``.
+
+    Steps of up to 64 rows ``(Hq/Hkv)*T`` without a causal mask run the
+    split-KV decode, which keeps its scores; longer ones the flash forward and a
+    second pass over the scores.  No gradient: inputs that require one raise.
+    """
+    who = "attention with key weights"
+    if q.ndim != 4 or k.ndim != 4 or v.ndim != 4:
+        raise ValueError(f"{who}: q must be [B, T, Hq, D], k and v [B, S, Hkv, D]")
+    _gqa_group(q.shape[-2], k.shape[-2])
+    B, T, Hq, D = q.shape
+    if _needs_grad(q, k, v) or (key_weights is not None and _needs_grad(key_weights)):
+        raise ValueError(f"{who} has no gradient: call it under torch.no_grad() or on detached tensors")
+    lm = lower_mask(mask)
+    if lm is not None and lm.row_kv_lengths is not None and T == 1:  # one row: per-batch lengths
+        lm.kv_lengths, lm.row_kv_lengths = _row_kv_lengths(lm.row_kv_lengths, B, 1, q.device)[:, 0], None
+    if lm is None or lm.q_valid is not None or lm.kv_valid is not None or lm.extended and not _only_shifted(lm):
+        raise ValueError(f"{who} takes no mask, KVLenMask and causal masks, got {type(mask).__name__}")
+    if sm_scale is None:
+        sm_scale = 1.0 / math.sqrt(D)
+    lse = None
+    if not lm.causal and (Hq // k.shape[2]) * T <= hip.WEIGHTED_DECODE_MAX_ROWS and T > 0:
+        out, weights, *lse = hip.weighted_decode(q, k, v, key_weights, sm_scale=sm_scale, kv_lengths=lm.kv_lengths,
+                                                 return_lse=return_lse)
+        lse = lse[0] if lse else None
+    else:
+        width = _kernel_width(D, q.dtype)
+        if width is None:
+            raise ValueError(f"{who}: head dims up to {FLASH_HEAD_DIMS[-1]}, got {D}")
+        rows = None
+        if width != D:
+            rows = hip.rows_width(D, max(Hq, k.shape[2])) if q.dtype in HALF_DTYPES else None
+            if rows is None:
+                q, k, v = _pad_features(q, width), _pad_features(k, width), _pad_features(v, width)
+        mods = hip.ScoreModsArgs(causal_shift=lm.causal_shift) if lm.causal_shift else None
+        out, lse = hip.flash_attention_fwd(q, k, v, sm_scale=float(sm_scale), causal=lm.causal,
+                                           kv_lengths=lm.kv_lengths, return_lse=True, mods=mods, width=rows)
+        weights = hip.key_weights(q, k, lse, key_weights, sm_scale=float(sm_scale), causal=lm.causal,
+                                  causal_shift=lm.causal_shift or 0, kv_lengths=lm.kv_lengths, width=rows)
+    if out.shape[-1] != D:
+        out = out[..., :D]
+    return (out, weights, lse) if return_lse else (out, weights)
+
+
+def _only_shifted(lm: LoweredMask) -> bool:
+    """A causal mask moved to another corner is all that is extended."""
+    return (lm.causal and lm.causal_shift is not None and lm.window_left is None and lm.window_right is None
+            and lm.prefix_lengths is None and lm.seq_lengths is None and lm.row_kv_lengths is None
+            and lm.segment_q is None and lm.segment_k is None)
+
+
+class EvictedKeys(NamedTuple):
+    """What ``evict_keys`` kept."""
+
+    k: torch.Tensor  # [B, keep, Hkv, D]
+    v: torch.Tensor
+    key_weights: torch.Tensor  # [B, Hkv, keep]
+    kv_lengths: torch.Tensor  # [B] int32
+    index: torch.Tensor  # [B, Hkv, keep] int32: the slot each key came from, -1 behind the last
+
+
+def evict_keys(k, v, key_weights, keep: int, *, kv_lengths=None, sinks: int = 0, recent: int = 0,
+               out=None) -> EvictedKeys:
+    """Cuts KV caches to the keys of the largest accumulated weight (no
+    counterpart in the reference).
+
+    ``k`` / ``v`` ``[B, S, Hkv, D]``, ``key_weights`` float32 ``[B, Hkv, S]`` (the
+    sums of ``attention_with_key_weights``), ``kv_lengths`` int ``[B]`` (None: S).
+    Every head of every sequence chooses for itself: up to ``keep`` keys are all
+    kept; of more, the first ``sinks``, the last ``recent`` and between them those
+    of the largest weights (equal ones: the earlier slot; NaN before all).  Kept
+    keys stay in their order, so one length per sequence, ``min(kv_lengths[b],
+    keep)``, holds for all heads.
+
+    Returns new caches of ``keep`` slots, zeros behind the kept keys.  With
+    ``out=(k, v, key_weights)``, buffers of at least ``keep`` slots that share no
+    memory with the inputs, those are written and returned, and what they hold
+    behind the kept keys stays (a layer's spare caches, say, with room for the
+    tokens to come).  No gradient: inputs that require one raise.
+    """
+    return EvictedKeys(*hip.evict_keys(k, v, key_weights, keep, kv_lengths=kv_lengths, sinks=sinks, recent=recent,
+                                       out=out))
+
+
+class _RotaryFunction(torch.autograd.Function):
+    """Differentiable rotation of q and k: the gradient turns back by the same
+    angles (and is differentiable itself)."""
+
+    @staticmethod
+    def forward(ctx, q, k, positions, options):
+        ctx.save_for_backward(positions)
+        ctx.options = options
+        ctx.set_materialize_grads(False)
+        q, k = hip.rotary(q, k, positions, **options)
+        return q if k is None else (q, k)
+
+    @staticmethod
+    def backward(ctx, dq, dk=None):
+        (positions,) = ctx.saved_tensors
+        options = dict(ctx.options, inverse=not ctx.options["inverse"])
+        grads = [g for g in (dq, dk) if g is not None]
+        if not grads:
+            return None, None, None, None
+        res = _RotaryFunction.apply(grads[0], grads[1] if len(grads) == 2 else None, positions, options)
+        if dq is None:
+            return None, res, None, None
+        return (*res, None, None) if len(grads) == 2 else (res, None, None, None)
+
+
+def rotary(q, k, positions, *, sections=None, base: float = 10000.0, interleaved: bool = True,
+           shared_spectrum: bool = False):
+    """Rotary positions of one or several axes, on q and k in one launch.
+
+    ``q [B, T, Hq, D]`` and ``k [B, T, Hk, D]`` (None: q alone, returned alone);
+    ``positions [T, A]`` or ``[B, T, A]`` for A axes (up to 4: time, height and
+    width of a video's patches), or ``[T]`` for one; integers, or floats for
+    positions between patches.  ``sections``: how many features of a row each axis
+    turns, even, in order from the first feature (features behind the last section
+    pass); None: D / A each.
+
+    The defaults are the reference's ``RotaryPosEncode`` (layers/encoding.py:
+    107-211): pairs of neighbouring features, pair i of a section of d features at
+    frequency ``base^(-2i/d)``.  ``interleaved=False`` pairs a section's first half
+    with its second.  ``shared_spectrum=True``: one embedding over all sections
+    (frequencies ``base^(-2p/sum(sections))`` and, not interleaved, halves of the
+    whole), of whose pairs each axis turns those in its section.  Angles are formed
+    in float64, so far positions keep their fraction of a turn.
+
+    bf16, fp16 or fp32, D up to 256, any strides (a slice of the features is read
+    in place).  Differentiable in q and k.
+    """
+    if q.ndim != 4 or (k is not None and k.ndim != 4):
+        raise ValueError("rotary: q and k must be [B, T, H, D]")
+    B, T, _, D = q.shape
+    if k is not None and ((k.shape[0], k.shape[1], k.shape[3]) != (B, T, D) or k.dtype != q.dtype):
+        raise ValueError(f"rotary: incompatible q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype}")
+    if D > 256:
+        raise ValueError(f"rotary: head dims up to 256, got {D}")
+    positions = torch.as_tensor(positions, device=q.device)
+    if positions.ndim == 1:
+        positions = positions[:, None]
+    A = positions.shape[-1] if positions.ndim else 0
+    if tuple(positions.shape) not in ((T, A), (B, T, A)) or not 1 <= A <= 4:
+        raise ValueError(f"rotary: positions must be [{T}], [{T}, A] or [{B}, {T}, A] with 1 to 4 axes, got "
+                         f"{tuple(positions.shape)}")
+    if positions.requires_grad:
+        raise ValueError("rotary has no gradient in the positions")
+    if positions.dtype not in hip._POSITION_TYPES:
+        if positions.dtype == torch.bool or positions.dtype.is_complex:
+            raise ValueError(f"rotary: positions must be integers or floats, got {positions.dtype}")
+        positions = positions.to(torch.float32 if positions.dtype.is_floating_point else torch.int64)
+    if sections is None:
+        if D % (2 * A):
+            raise ValueError(f"rotary: {D} features do not divide into pairs of {A} axes; give sections")
+        sections = (D // A,) * A
+    sections = tuple(int(x) for x in sections)
+    if len(sections) != A or any(x < 0 or x % 2 for x in sections) or sum(sections) > D:
+        raise ValueError(f"rotary: sections must be {A} even numbers that add up to at most {D}, got {sections}")
+    if not 0.0 < base < 1e300:
+        raise ValueError(f"rotary: base must be positive, got {base}")
+    options = dict(sections=sections, base=float(base), interleaved=bool(interleaved),
+                   shared_spectrum=bool(shared_spectrum), inverse=False)
+    if _needs_grad(q) or (k is not None and _needs_grad(k)):
+        return _RotaryFunction.apply(q, k, positions, options)
+    y, z = hip.rotary(q, k, positions, **options)
+    return y if z is None else (y, z)
 
 
 class _MaterializedMLAFunction(torch.autograd.Function):

@@ -1,0 +1,414 @@
+// The softmax weight that every key of a cache was given, for gfx950:
+//   w'[b, g, j] = w[b, g, j] + sum over the rows t and heads h of group g of
+//                 exp(s_htj - lse_ht),
+// what eviction from a KV cache goes by (evict.hip).
+//
+// Decode steps (few rows): the split-KV decode (decode_common.h) also keeps its
+// scores, 4 bytes a row and key beside the 2 (D + D) bytes of a 16-bit key, and
+// a second kernel sums their exponentials once the rows' statistics are known.
+// Forming the scores again instead would read K, half of the cache, again.
+//
+// Prompts (many rows): the scores are too many to keep.  They are formed again
+// on the matrix units, keys as MFMA rows, so a lane's accumulators are sums of
+// its own 16 keys and nothing is exchanged until the end.
+#include <stdio.h>
+
+#include "decode_common.h"
+
+namespace pjx {
+
+template <typename E, int D, int NRB, bool ROWS>
+__global__ __launch_bounds__(256, (decode_occupancy<D, D, NRB>())) void scored_decode_kernel(DecodeArgs a) {
+  gqa_decode<E, D, D, NRB, false, ROWS, kScores>(a);
+}
+
+template <int D, int NRB>
+__global__ __launch_bounds__(256, 1) void scored_decode_f32_kernel(DecodeArgs a) {
+  gqa_decode_f32<D, D, NRB, kScores>(a);
+}
+
+constexpr int kWeightThreads = 256;
+constexpr int kMaxScoredRows = 64;
+
+// Keys of the weights' kernel: 4 consecutive ones per thread.
+__global__ __launch_bounds__(kWeightThreads) void score_weights_kernel(DecodeArgs a, const float* w_in, float* w_out) {
+  __shared__ float stat[kMaxScoredRows][2];  // running max (log2 units), 1 / sum
+  const int bg = blockIdx.y + blockIdx.z * 65535;
+  if (bg >= a.B * a.G) return;
+  const int b = bg / a.G, tid = threadIdx.x;
+  const int L = seq_len(a, b), n = (L + a.chunk - 1) / a.chunk;
+  const int j0 = (blockIdx.x * kWeightThreads + tid) * 4;
+  if (tid < a.rows) {
+    const float* ml = a.ws_ml + ((size_t)bg * a.nch * a.rows + tid) * 2;
+    float M = kMaxInit, sum = 0.f;
+    for (int c = 0; c < n; ++c) {
+      const float m = ml[(size_t)c * a.rows * 2], l = ml[(size_t)c * a.rows * 2 + 1];
+      const float m_new = fmaxf(M, m);
+      sum = fmaf(sum, fast_exp2(M - m_new), l * fast_exp2(m - m_new));
+      M = m_new;
+    }
+    stat[tid][0] = M;
+    stat[tid][1] = 1.f / sum;
+  }
+  __syncthreads();
+  if (j0 >= a.Lk) return;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  if (j0 < L) {
+    const float* s = a.scores + (size_t)bg * a.rows * a.score_ld + j0;
+#pragma unroll 4
+    for (int r = 0; r < a.rows; ++r) {
+      const f32x4 x = *(const f32x4*)(s + (size_t)r * a.score_ld);
+      const float M = stat[r][0], inv = stat[r][1];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] = fmaf(fast_exp2(x[e] - M), inv, acc[e]);
+    }
+  }
+  const size_t at = (size_t)bg * a.Lk + j0;
+  for (int e = 0; e < 4 && j0 + e < a.Lk; ++e)
+    w_out[at + e] = (w_in ? w_in[at + e] : 0.f) + (j0 + e < L ? acc[e] : 0.f);
+}
+
+template <auto K>
+static int run_scored(DecodeArgs& a, const float* w_in, float* w_out, void* ws, size_t ws_bytes, hipStream_t s) {
+  const char* who = "pjx_weighted_decode";
+  int rc = run_chunks<K>(a, ws, ws_bytes, s, who);
+  if (rc == PJX_OK) rc = launch_decode_merge(a, s, who);
+  if (rc != PJX_OK) return rc;
+  const int64_t bg = (int64_t)a.B * a.G;
+  const dim3 grid((unsigned)((a.Lk + 4 * kWeightThreads - 1) / (4 * kWeightThreads)), (unsigned)std::min<int64_t>(bg, 65535),
+                  (unsigned)((bg + 65534) / 65535));
+  launch_kernel<score_weights_kernel>(grid, dim3(kWeightThreads), 0, s, a, w_in, w_out);
+  return check_launch(who);
+}
+
+template <typename E, int D, bool ROWS>
+static int run_scored_rows(DecodeArgs& a, int nrb, const float* wi, float* wo, void* ws, size_t n, hipStream_t s) {
+  if (nrb == 1) return run_scored<scored_decode_kernel<E, D, 1, ROWS>>(a, wi, wo, ws, n, s);
+  if (nrb == 2) return run_scored<scored_decode_kernel<E, D, 2, ROWS>>(a, wi, wo, ws, n, s);
+  if constexpr (D <= 128) return run_scored<scored_decode_kernel<E, D, 4, ROWS>>(a, wi, wo, ws, n, s);
+  return fail(PJX_ERR_INVALID, "pjx_weighted_decode: row blocks");
+}
+
+template <typename E>
+static int run_scored_16(DecodeArgs& a, int d, int nrb, const float* wi, float* wo, void* ws, size_t n, hipStream_t s) {
+  const bool rows = a.orow != d;
+  if (d == 64)
+    return rows ? run_scored_rows<E, 64, true>(a, nrb, wi, wo, ws, n, s)
+                : run_scored_rows<E, 64, false>(a, nrb, wi, wo, ws, n, s);
+  if (d == 128)
+    return rows ? run_scored_rows<E, 128, true>(a, nrb, wi, wo, ws, n, s)
+                : run_scored_rows<E, 128, false>(a, nrb, wi, wo, ws, n, s);
+  return run_scored_rows<E, 256, false>(a, nrb, wi, wo, ws, n, s);
+}
+
+template <int D>
+static int run_scored_f32(DecodeArgs& a, int nrb, const float* wi, float* wo, void* ws, size_t n, hipStream_t s) {
+  return nrb == 1 ? run_scored<scored_decode_f32_kernel<D, 1>>(a, wi, wo, ws, n, s)
+                  : run_scored<scored_decode_f32_kernel<D, 2>>(a, wi, wo, ws, n, s);
+}
+
+// Workspace of a weighted decode: the decode's partials, then the scores.
+static size_t partial_bytes(int64_t batch, int64_t groups, int64_t rows, int64_t kv_len, int64_t v_dim, int64_t chunk) {
+  return (ws_size(batch, groups, rows, kv_len, v_dim, chunk) + 255) & ~(size_t)255;
+}
+static int64_t score_stride(int64_t kv_len) { return (kv_len + 3) & ~(int64_t)3; }
+
+// ---------------------------------------------------------------------------
+// Prompts
+// ---------------------------------------------------------------------------
+struct KeyWeightArgs {
+  const void* q;
+  const void* k;
+  const float* lse;
+  const int32_t* lengths;
+  float* part;  // [splits][B * G][Lk]
+  int B, Lq, Lk, Hq, G, rdim;
+  int causal, shift;
+  int q_step;   // query rows of a split
+  int splits;   // splits of the query rows (each per head)
+  float cx;
+};
+
+// Rows of a tile of queries in LDS: 16-byte chunks XOR-swizzled by the row, so
+// that 32 lanes reading one chunk of 32 rows touch distinct banks.
+template <int D>
+struct QueryTile {
+  static constexpr int BQ = 32, NC = D / 8, ROWB = 2 * D;
+  __device__ static int swz(int r) { return NC >= 16 ? (r & 15) : (r & 7); }
+};
+
+// One workgroup: 128 keys (32 per wave, their fragments in registers) of one
+// (batch, KV head), against the query rows of one split of one head of its group.
+template <typename E, int D>
+__global__ __launch_bounds__(256) void key_weights_kernel(KeyWeightArgs a) {
+  using T = QueryTile<D>;
+  __shared__ __attribute__((aligned(1024))) unsigned char qs[2][T::BQ * T::ROWB];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, col = lane & 31, half = lane >> 5;
+  const int per = a.Hq / a.G;
+  const int hs = blockIdx.y % (per * a.splits), bg = blockIdx.y / (per * a.splits);
+  const int b = bg / a.G, g = bg % a.G, h = g * per + hs / a.splits, split = hs % a.splits;
+  const int k0 = blockIdx.x * 128 + 32 * w;
+  const int L = a.lengths ? min(a.Lk, max(a.lengths[b], 0)) : a.Lk;
+  // rows of this split that see the workgroup's first key
+  int q_lo = split * a.q_step, q_hi = min(q_lo + a.q_step, a.Lq);
+  if (a.causal) q_lo = max(q_lo, (max((int)blockIdx.x * 128 - a.shift, 0)) / T::BQ * T::BQ);
+  const bool any = (int)blockIdx.x * 128 < L && q_lo < q_hi;
+  f32x16 acc = {};
+  if (any) {
+    typename E::v8 kf[D / 16];
+    const int key = k0 + col;
+    const uint16_t* krow = (const uint16_t*)a.k + ((size_t)(b * (int64_t)a.Lk + min(key, a.Lk - 1)) * a.G + g) * a.rdim;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) {
+      u32x4 r = {0u, 0u, 0u, 0u};
+      if (key < L && 16 * s + 8 * half < a.rdim) r = *(const u32x4*)(krow + 16 * s + 8 * half);
+      kf[s] = E::as8(r);
+    }
+    const float* lse = a.lse + ((size_t)b * a.Hq + h) * a.Lq;
+    const uint16_t* Q = (const uint16_t*)a.q + ((size_t)b * a.Lq * a.Hq + h) * a.rdim;
+    constexpr int NLD = T::BQ * T::NC / 256;
+    u32x4 qr[NLD];
+    float lr;
+    auto load = [&](int t0) {
+#pragma unroll
+      for (int i = 0; i < NLD; ++i) {
+        const int u = tid + 256 * i, r = u / T::NC, c = u % T::NC;
+        qr[i] = u32x4{0u, 0u, 0u, 0u};
+        if (t0 + r < q_hi && 8 * c < a.rdim) qr[i] = *(const u32x4*)(Q + (size_t)(t0 + r) * a.Hq * a.rdim + 8 * c);
+      }
+      lr = t0 + col < q_hi ? lse[t0 + col] : INFINITY;
+    };
+    load(q_lo);
+    int st = 0;
+    for (int t0 = q_lo; t0 < q_hi; t0 += T::BQ, st ^= 1) {
+#pragma unroll
+      for (int i = 0; i < NLD; ++i) {
+        const int u = tid + 256 * i, r = u / T::NC, c = u % T::NC;
+        *(u32x4*)(qs[st] + r * T::ROWB + 16 * (c ^ T::swz(r))) = qr[i];
+      }
+      const float l2 = lr * kLog2e;  // +inf: no row, or one without a valid key
+      __syncthreads();
+      if (t0 + T::BQ < q_hi) load(t0 + T::BQ);
+      f32x16 s = {};
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        const u32x4 q8 = *(const u32x4*)(qs[st] + col * T::ROWB + 16 * ((2 * i + half) ^ T::swz(col)));
+        s = E::mma32(kf[i], E::as8(q8), s);
+      }
+      // register r: key k0 + 8 (r / 4) + 4 half + r % 4, query t0 + col
+      if (a.causal && k0 + 31 > t0 + a.shift) {
+        const int lim = t0 + col + a.shift - (k0 + 4 * half);
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (8 * (r >> 2) + (r & 3) > lim) s[r] = -INFINITY;
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[r] += fast_exp2(fmaf(s[r], a.cx, -l2));
+    }
+  }
+  // sums over the 32 queries of a half wave
+  float* part = a.part + ((size_t)hs * a.B * a.G + bg) * a.Lk;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    float x = acc[r];
+#pragma unroll
+    for (int m = 1; m < 32; m *= 2) x += __shfl_xor(x, m);
+    const int key = k0 + 8 * (r >> 2) + 4 * half + (r & 3);
+    if (col == r && key < a.Lk) part[key] = key < L ? x : 0.f;
+  }
+}
+
+__device__ __forceinline__ f32x16 mma_f32(float a, float b, f32x16 c) { return mfma32x32x2f32(a, b, c); }
+
+// float32: the same on v_mfma_f32_32x32x2f32, two features a step.  K's lane
+// holds feature half + 2 i of key col in register i.
+template <int D>
+__global__ __launch_bounds__(256) void key_weights_f32_kernel(KeyWeightArgs a) {
+  constexpr int BQ = 32, LD = D + 4;  // padded rows: 32 lanes reading a feature pair touch distinct banks
+  __shared__ __attribute__((aligned(16))) float qs[BQ * LD];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, col = lane & 31, half = lane >> 5;
+  const int per = a.Hq / a.G;
+  const int hs = blockIdx.y % (per * a.splits), bg = blockIdx.y / (per * a.splits);
+  const int b = bg / a.G, g = bg % a.G, h = g * per + hs / a.splits, split = hs % a.splits;
+  const int k0 = blockIdx.x * 128 + 32 * w;
+  const int L = a.lengths ? min(a.Lk, max(a.lengths[b], 0)) : a.Lk;
+  int q_lo = split * a.q_step, q_hi = min(q_lo + a.q_step, a.Lq);
+  if (a.causal) q_lo = max(q_lo, (max((int)blockIdx.x * 128 - a.shift, 0)) / BQ * BQ);
+  const bool any = (int)blockIdx.x * 128 < L && q_lo < q_hi;
+  f32x16 acc = {};
+  if (any) {
+    // features 4 i + 2 half .. + 1 of key col: step 2 i contracts 4 i and 4 i + 2
+    float2 kf[D / 4];
+    const int key = k0 + col;
+    const float* krow = (const float*)a.k + ((size_t)(b * (int64_t)a.Lk + min(key, a.Lk - 1)) * a.G + g) * D;
+#pragma unroll
+    for (int i = 0; i < D / 4; ++i) kf[i] = key < L ? *(const float2*)(krow + 4 * i + 2 * half) : make_float2(0.f, 0.f);
+    const float* lse = a.lse + ((size_t)b * a.Hq + h) * a.Lq;
+    const float* Q = (const float*)a.q + ((size_t)b * a.Lq * a.Hq + h) * D;
+    for (int t0 = q_lo; t0 < q_hi; t0 += BQ) {
+      __syncthreads();
+      for (int u = tid; u < BQ * D / 4; u += 256) {
+        const int r = u / (D / 4), c = u % (D / 4);
+        f32x4 x = {};
+        if (t0 + r < q_hi) x = *(const f32x4*)(Q + (size_t)(t0 + r) * a.Hq * D + 4 * c);
+        *(f32x4*)(qs + r * LD + 4 * c) = x;
+      }
+      const float l2 = (t0 + col < q_hi ? lse[t0 + col] : INFINITY) * kLog2e;
+      __syncthreads();
+      f32x16 s = {};
+#pragma unroll
+      for (int i = 0; i < D / 4; ++i) {
+        const float2 q2 = *(const float2*)(qs + col * LD + 4 * i + 2 * half);
+        s = mma_f32(kf[i].x, q2.x, s);
+        s = mma_f32(kf[i].y, q2.y, s);
+      }
+      if (a.causal && k0 + 31 > t0 + a.shift) {
+        const int lim = t0 + col + a.shift - (k0 + 4 * half);
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (8 * (r >> 2) + (r & 3) > lim) s[r] = -INFINITY;
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[r] += fast_exp2(fmaf(s[r], a.cx, -l2));
+    }
+  }
+  float* part = a.part + ((size_t)hs * a.B * a.G + bg) * a.Lk;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    float x = acc[r];
+#pragma unroll
+    for (int m = 1; m < 32; m *= 2) x += __shfl_xor(x, m);
+    const int key = k0 + 8 * (r >> 2) + 4 * half + (r & 3);
+    if (col == r && key < a.Lk) part[key] = key < L ? x : 0.f;
+  }
+}
+
+// Adds the parts, in their order, to the weights so far.
+__global__ __launch_bounds__(256) void add_weights_kernel(const float* part, const float* w_in, float* w_out, int parts,
+                                                         int64_t n) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    float x = 0.f;
+    for (int p = 0; p < parts; ++p) x += part[p * n + i];
+    w_out[i] = (w_in ? w_in[i] : 0.f) + x;
+  }
+}
+
+// Splits of the query rows: enough workgroups for two rounds of the device.
+static int64_t row_splits(int64_t batch, int64_t q_len, int64_t kv_len, int64_t q_heads) {
+  const int64_t blocks = (kv_len + 127) / 128 * batch * q_heads;
+  return std::clamp<int64_t>(2048 / std::max<int64_t>(blocks, 1), 1, std::max<int64_t>((q_len + 255) / 256, 1));
+}
+
+}  // namespace pjx
+
+using namespace pjx;
+
+extern "C" size_t pjx_weighted_decode_workspace_size(int64_t batch, int64_t kv_heads, int64_t rows, int64_t kv_len,
+                                                     int64_t head_dim, int64_t chunk) {
+  return partial_bytes(batch, kv_heads, rows, kv_len, head_dim, chunk) +
+         (size_t)(batch * kv_heads * rows * score_stride(kv_len)) * 4;
+}
+
+extern "C" int pjx_weighted_decode(int dtype, const void* q, const void* k, const void* v, const int32_t* kv_lengths,
+                                   const float* weights, float* weights_out, void* o, float* lse, void* workspace,
+                                   size_t workspace_bytes, int64_t batch, int64_t q_len, int64_t kv_len,
+                                   int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t row_dim,
+                                   const pjx_cache_strides* strides, float sm_scale, int64_t chunk, void* stream) {
+  clear_error();
+  const char* who = "pjx_weighted_decode";
+  DecodeArgs a = {};
+  const int rc = fill_cache_decode(a, who, dtype, q, k, v, kv_lengths, o, lse, batch, q_len, kv_len, q_heads, kv_heads,
+                                   head_dim, row_dim, strides, sm_scale, chunk);
+  if (rc != PJX_OK) return rc;
+  const int64_t rows = q_heads / kv_heads * q_len;
+  if (rows > kMaxScoredRows) return fail(PJX_ERR_INVALID, "pjx_weighted_decode: at most 64 rows per KV head");
+  if (batch == 0) return PJX_OK;
+  hipStream_t s = (hipStream_t)stream;
+  const bool f32 = dtype == PJX_DTYPE_F32;
+  if (kv_len == 0)
+    return write_keyless(o, lse, (size_t)(batch * q_len * q_heads * row_dim), f32, (size_t)(batch * q_heads * q_len), s,
+                         who);
+  if (!weights_out) return fail(PJX_ERR_INVALID, "pjx_weighted_decode: null pointer");
+  if (batch * kv_heads > (int64_t)65535 * 65535) return fail(PJX_ERR_INVALID, "pjx_weighted_decode: sizes out of range");
+  if (!workspace || workspace_bytes < pjx_weighted_decode_workspace_size(batch, kv_heads, rows, kv_len, head_dim, a.chunk))
+    return fail(PJX_ERR_WORKSPACE, "pjx_weighted_decode: workspace missing or too small");
+  if ((uintptr_t)workspace % 16) return fail(PJX_ERR_INVALID, "pjx_weighted_decode: the workspace must start on 16 bytes");
+  const size_t parts = partial_bytes(batch, kv_heads, rows, kv_len, head_dim, a.chunk);
+  a.scores = (float*)((char*)workspace + parts);
+  a.score_ld = score_stride(kv_len);
+  const int d = (int)head_dim;
+  const int nrb = gqa_row_blocks(a.rows, d, d, f32);
+  a.rpg = kRows * nrb;
+  if (f32)
+    return d == 64    ? run_scored_f32<64>(a, nrb, weights, weights_out, workspace, parts, s)
+           : d == 128 ? run_scored_f32<128>(a, nrb, weights, weights_out, workspace, parts, s)
+                      : run_scored_f32<256>(a, nrb, weights, weights_out, workspace, parts, s);
+  return a.f16 ? run_scored_16<F16Fmt>(a, d, nrb, weights, weights_out, workspace, parts, s)
+               : run_scored_16<Bf16Fmt>(a, d, nrb, weights, weights_out, workspace, parts, s);
+}
+
+extern "C" size_t pjx_key_weights_workspace_size(int64_t batch, int64_t q_len, int64_t kv_len, int64_t q_heads) {
+  return (size_t)(batch * q_heads * kv_len * row_splits(batch, q_len, kv_len, q_heads)) * 4;
+}
+
+extern "C" int pjx_key_weights(int dtype, const void* q, const void* k, const float* lse, const int32_t* kv_lengths,
+                               const float* weights, float* weights_out, void* workspace, size_t workspace_bytes,
+                               int64_t batch, int64_t q_len, int64_t kv_len, int64_t q_heads, int64_t kv_heads,
+                               int64_t head_dim, int64_t row_dim, int causal, int64_t causal_shift, float sm_scale,
+                               void* stream) {
+  clear_error();
+  char buf[256];
+  auto bad = [&](const char* what) {
+    snprintf(buf, sizeof(buf), "pjx_key_weights: %s", what);
+    return fail(PJX_ERR_INVALID, buf);
+  };
+  if (dtype != PJX_DTYPE_BF16 && dtype != PJX_DTYPE_F16 && dtype != PJX_DTYPE_F32)
+    return bad("dtype must be PJX_DTYPE_BF16, PJX_DTYPE_F16 or PJX_DTYPE_F32");
+  const bool f32 = dtype == PJX_DTYPE_F32;
+  if (batch < 0 || q_len < 0 || kv_len < 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads) return bad("bad sizes");
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256) return bad("head_dim must be 64, 128 or 256");
+  if (row_dim != head_dim && (f32 || row_dim <= 0 || row_dim > head_dim || row_dim % 8))
+    return bad("row_dim must be head_dim, or in 16 bits a multiple of 8 up to it");
+  if (!(sm_scale > 0.f)) return bad("sm_scale must be > 0");
+  const int64_t most = (int64_t)1 << 40;
+  if (q_len > (1 << 28) || kv_len > (1 << 28) || causal_shift > (1 << 28) || causal_shift < -(1 << 28) ||
+      batch * q_heads > (1 << 22) || batch * q_heads * std::max(q_len, kv_len) > most / head_dim)
+    return bad("sizes out of range");
+  if (batch * kv_len == 0) return PJX_OK;
+  if (!weights_out || !k || (q_len > 0 && (!q || !lse))) return bad("null pointer");
+  if (((uintptr_t)q | (uintptr_t)k) % 16) return bad("q and k must start on 16 bytes");
+  if (!workspace || workspace_bytes < pjx_key_weights_workspace_size(batch, q_len, kv_len, q_heads))
+    return fail(PJX_ERR_WORKSPACE, "pjx_key_weights: workspace missing or too small");
+  KeyWeightArgs a = {};
+  a.q = q; a.k = k; a.lse = lse; a.lengths = kv_lengths; a.part = (float*)workspace;
+  a.B = (int)batch; a.Lq = (int)q_len; a.Lk = (int)kv_len; a.Hq = (int)q_heads; a.G = (int)kv_heads;
+  a.rdim = (int)row_dim;
+  a.causal = causal != 0;
+  a.shift = (int)causal_shift;
+  a.splits = (int)row_splits(batch, q_len, kv_len, q_heads);
+  a.q_step = (int)(((q_len + a.splits - 1) / a.splits + 31) / 32 * 32);
+  a.cx = sm_scale * kLog2e;
+  const int64_t rows = batch * q_heads * a.splits, groups = (kv_len + 127) / 128;
+  if (rows > 65535 || groups > 0xffffffffLL / 256) return bad("sizes out of range");
+  hipStream_t s = (hipStream_t)stream;
+  const dim3 grid((unsigned)groups, (unsigned)rows), block(256);
+  if (f32) {
+    if (head_dim == 64) launch_kernel<key_weights_f32_kernel<64>>(grid, block, 0, s, a);
+    else if (head_dim == 128) launch_kernel<key_weights_f32_kernel<128>>(grid, block, 0, s, a);
+    else launch_kernel<key_weights_f32_kernel<256>>(grid, block, 0, s, a);
+  } else if (dtype == PJX_DTYPE_F16) {
+    if (head_dim == 64) launch_kernel<key_weights_kernel<F16Fmt, 64>>(grid, block, 0, s, a);
+    else if (head_dim == 128) launch_kernel<key_weights_kernel<F16Fmt, 128>>(grid, block, 0, s, a);
+    else launch_kernel<key_weights_kernel<F16Fmt, 256>>(grid, block, 0, s, a);
+  } else {
+    if (head_dim == 64) launch_kernel<key_weights_kernel<Bf16Fmt, 64>>(grid, block, 0, s, a);
+    else if (head_dim == 128) launch_kernel<key_weights_kernel<Bf16Fmt, 128>>(grid, block, 0, s, a);
+    else launch_kernel<key_weights_kernel<Bf16Fmt, 256>>(grid, block, 0, s, a);
+  }
+  const int rc = check_launch("pjx_key_weights");
+  if (rc != PJX_OK) return rc;
+  const int64_t n = batch * kv_heads * kv_len;
+  launch_kernel<add_weights_kernel>(dim3((unsigned)std::min<int64_t>((n + 255) / 256, 65536)), block, 0, s,
+                                    (const float*)a.part, weights, weights_out, (int)(q_heads / kv_heads * a.splits), n);
+  return check_launch("pjx_key_weights");
+}

@@ -42,10 +42,18 @@ class ScoreMods(ctypes.Structure):
     ]
 
 
+class CacheStrides(ctypes.Structure):
+    """``pjx_cache_strides``: elements between sequences, tokens and heads of a
+    K and a V cache."""
+
+    _fields_ = [(n, ctypes.c_int64) for n in ("k_batch", "k_token", "k_head", "v_batch", "v_token", "v_head")]
+
+
 # (name, restype, argtypes) of every exported entry point.
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _MODS = ctypes.POINTER(ScoreMods)
+_STRIDES = ctypes.POINTER(CacheStrides)
 _SIGNATURES = {
     "pjx_version": (ctypes.c_int, []),
     "pjx_last_error": (ctypes.c_char_p, []),
@@ -128,6 +136,33 @@ _SIGNATURES = {
         ctypes.c_int,
         [ctypes.c_int, _P, _P, _P, _P, _P, _P, _P, _P, _P, ctypes.c_size_t, _I64, _I64, _I64, _I64, _I64, _I64,
          _I64, _P],
+    ),
+    "pjx_tree_decode": (
+        ctypes.c_int,
+        [ctypes.c_int, _P, _P, _P, _P, _P, _P, _I64, _P, _P, _P, ctypes.c_size_t, _I64, _I64, _I64, _I64, _I64, _I64,
+         _I64, _STRIDES, ctypes.c_float, _I64, _P],
+    ),
+    "pjx_weighted_decode_workspace_size": (ctypes.c_size_t, [_I64, _I64, _I64, _I64, _I64, _I64]),
+    "pjx_weighted_decode": (
+        ctypes.c_int,
+        [ctypes.c_int, _P, _P, _P, _P, _P, _P, _P, _P, _P, ctypes.c_size_t, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
+         _STRIDES, ctypes.c_float, _I64, _P],
+    ),
+    "pjx_key_weights_workspace_size": (ctypes.c_size_t, [_I64, _I64, _I64, _I64]),
+    "pjx_key_weights": (
+        ctypes.c_int,
+        [ctypes.c_int, _P, _P, _P, _P, _P, _P, _P, ctypes.c_size_t, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
+         ctypes.c_int, _I64, ctypes.c_float, _P],
+    ),
+    "pjx_rotary": (
+        ctypes.c_int,
+        [ctypes.c_int, _P, _P, _P, _P, _P, ctypes.c_int, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _STRIDES,
+         ctypes.POINTER(ctypes.c_int32), _I64, ctypes.c_double, ctypes.c_int, ctypes.c_int, ctypes.c_int, _P],
+    ),
+    "pjx_evict_keys": (
+        ctypes.c_int,
+        [_I64, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _STRIDES, _STRIDES,
+         ctypes.c_int, _P],
     ),
 }
 EXPORTED = tuple(_SIGNATURES)
