@@ -49,7 +49,7 @@ HIPCC_FLAGS = [
 # 4%).  decode.hip: the same copies around the accumulators of the 64-row GQA
 # decode and of the fp32 decodes (GQA-8 with 8 query rows 5.7% faster, fp32
 # decode 3%; the bf16 C3 / latent decode unchanged); tree_decode.hip and
-# key_weights.hip hold the same kernel.  flash_fwd.hip and
+# key_weights.hip hold the same kernel, tree_wide.hip is like flash_fwd.hip's.  flash_fwd.hip and
 # flash_f32.hip: the fp32 forward kernels likewise (7-8.5% faster); the 16-bit
 # ones use no AGPRs and compile to the same code either way.  flash_bwd.hip:
 # the 16-bit backward kernels (1%); its D = 256 dK/dV kernel, which the
@@ -62,6 +62,7 @@ FILE_FLAGS = {
     "flash_wide.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "decode.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "tree_decode.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "tree_wide.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "key_weights.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "flash_fwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "flash_f32.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],

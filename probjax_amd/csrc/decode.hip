@@ -121,7 +121,7 @@ __global__ __launch_bounds__(kDecThreads, 1) void mla_decode_kernel(DecodeArgs a
   const int c16 = lane & 15, q4 = lane >> 4;
   __shared__ int sched[4 + 2 * kSchedMaxBatch];
   int b, g, chunk_id, L;
-  if (!decode_item(a, sched, b, g, chunk_id, L)) return;  // nothing past the length is read
+  if (!decode_item(a, sched, b, g, chunk_id, L, blockIdx.x)) return;  // nothing past the length is read
   const int c0 = chunk_id * a.chunk;
   const int c1 = min(c0 + a.chunk, L);
   const int n_tiles = (c1 - c0 + BK - 1) / BK;

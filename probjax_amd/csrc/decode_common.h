@@ -208,7 +208,7 @@ __device__ __forceinline__ void emit_row_elem(const DecodeArgs& a, int b, int g,
   }
 }
 
-// Work item of a decode workgroup: (batch b, kv group g, chunk chunk_id).
+// Work item `item` of a decode: (batch b, kv group g, chunk chunk_id).
 // The hardware starts workgroups in index order as slots free up, so the
 // index order is the schedule.  With per-sequence lengths (B <=
 // kSchedMaxBatch) the items run longest first: every full chunk (sequence by
@@ -220,18 +220,18 @@ __device__ __forceinline__ void emit_row_elem(const DecodeArgs& a, int b, int g,
 // the sequence's clamped length; false: the item has no keys.
 constexpr int kSchedMaxBatch = 256;
 static_assert(kSchedMaxBatch <= kDecThreads, "one length per thread");
-__device__ bool decode_item(const DecodeArgs& a, int* sched, int& b, int& g, int& chunk_id, int& L) {
+__device__ bool decode_item(const DecodeArgs& a, int* sched, int& b, int& g, int& chunk_id, int& L, unsigned item) {
   if (!a.lengths || a.B > kSchedMaxBatch) {
     const int BG = a.B * a.G;
-    chunk_id = blockIdx.x / BG;
-    const int bg = blockIdx.x % BG;
+    chunk_id = item / BG;
+    const int bg = item % BG;
     b = bg / a.G;
     g = bg % a.G;
     L = seq_len(a, b);
     return chunk_id * a.chunk < L;
   }
-  const int q = blockIdx.x / a.G, t = threadIdx.x;
-  g = blockIdx.x % a.G;
+  const int q = item / a.G, t = threadIdx.x;
+  g = item % a.G;
   int* nfs = sched + 4;                 // full chunks per sequence
   int* rms = nfs + kSchedMaxBatch;      // keys of the partial last chunk
   int Lt = 0, nf = 0, rt = 0;
@@ -455,7 +455,7 @@ __device__ __forceinline__ void gqa_decode(const DecodeArgs& a) {
   const int c16 = lane & 15, q4 = lane >> 4;
   __shared__ int sched[4 + 2 * kSchedMaxBatch];
   int b, g, chunk_id, L;
-  if (!decode_item(a, sched, b, g, chunk_id, L)) return;  // nothing past the length is read
+  if (!decode_item(a, sched, b, g, chunk_id, L, blockIdx.x)) return;  // nothing past the length is read
   const int bg = b * a.G + g;
   const int c0 = chunk_id * a.chunk;
   // the item's keys split evenly over the 4 waves (32-key steps), so a
@@ -787,7 +787,7 @@ __device__ __forceinline__ void gqa_decode_f32(const DecodeArgs& a) {
   const int c16 = lane & 15, q4 = lane >> 4;
   __shared__ int sched[4 + 2 * kSchedMaxBatch];
   int b, g, chunk_id, L;
-  if (!decode_item(a, sched, b, g, chunk_id, L)) return;
+  if (!decode_item(a, sched, b, g, chunk_id, L, blockIdx.x)) return;
   const int bg = b * a.G + g;
   const int c0 = chunk_id * a.chunk;
   const int per_wave = ((min(L - c0, a.chunk) + 127) >> 7) << 5;
@@ -971,6 +971,11 @@ int fill_cache_decode(DecodeArgs& a, const char* who, int dtype, const void* q, 
                       const int32_t* kv_lengths, void* o, float* lse, int64_t batch, int64_t q_len, int64_t kv_len,
                       int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t row_dim,
                       const pjx_cache_strides* strides, float sm_scale, int64_t chunk);
+// Drafts of many rows (tree_wide.hip): whether its kernel takes them, and the
+// launch (auto_chunk_size: the chunk is the kernel's to choose, from a.chunk up).
+bool tree_wide_takes(const DecodeArgs& a, int head_dim, bool f32);
+int run_tree_wide(DecodeArgs& a, int head_dim, bool auto_chunk_size, void* ws, size_t ws_bytes, hipStream_t s,
+                  const char* who);
 // Merges the chunk partials of a decode whose chunk kernel was launched with `a`.
 int launch_decode_merge(const DecodeArgs& a, hipStream_t stream, const char* name);
 

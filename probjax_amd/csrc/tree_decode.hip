@@ -28,7 +28,6 @@ template <typename E, int D, bool ROWS>
 static int run_tree_rows(DecodeArgs& a, int nrb, void* ws, size_t ws_bytes, hipStream_t s, const char* who) {
   if (nrb == 1) return run_decode<tree_decode_kernel<E, D, 1, ROWS>>(a, ws, ws_bytes, s, who);
   if (nrb == 2) return run_decode<tree_decode_kernel<E, D, 2, ROWS>>(a, ws, ws_bytes, s, who);
-  if constexpr (D <= 128) return run_decode<tree_decode_kernel<E, D, 4, ROWS>>(a, ws, ws_bytes, s, who);
   return fail(PJX_ERR_INVALID, "tree decode: row blocks");
 }
 
@@ -139,6 +138,7 @@ extern "C" int pjx_tree_decode(int dtype, const void* q, const void* k, const vo
   a.tree_mask = tree_mask;
   a.tree_step = trees == 1 ? 0 : parents ? q_len : q_len * q_len;
   const int d = (int)head_dim;
+  if (tree_wide_takes(a, d, f32)) return run_tree_wide(a, d, chunk == 0, workspace, workspace_bytes, s, who);
   const int nrb = gqa_row_blocks(a.rows, d, d, f32);
   a.rpg = kRows * nrb;
   if (f32)

@@ -72,6 +72,8 @@ CASES = [
     ("bf16", 2, 16, 700, 8, 2, 128, [684, 120], 128),  # the draft straddles two chunks
     ("bf16", 2, 33, 400, 4, 1, 64, [300, 127], 128),   # 132 rows, sets of two words
     ("bf16", 1, 64, 1200, 8, 2, 128, [1136], 256),     # 256 rows
+    ("f16", 3, 16, 900, 8, 2, 64, [0, 884, 401], 256),  # 64 rows
+    ("bf16", 5, 61, 400, 8, 2, 120, [300, 10, 339, 0, 77], 0),
     ("bf16", 1, 100, 300, 4, 2, 256, [200], 0),
     ("bf16", 1, 256, 600, 2, 1, 64, [300], 128),       # the widest draft
     ("f16", 2, 7, 333, 6, 3, 80, [320, 55], 128),      # rows of 80 features
@@ -117,8 +119,9 @@ def test_matches_definition(device, case, form):
     check(got[..., :D], lse, want, dtype, D, S)
 
 
+@pytest.mark.parametrize("hq", [2, 8])  # 20 or 80 rows per KV head
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
-def test_unseen_infinities_do_not_reach_a_row(device, dtype):
+def test_unseen_infinities_do_not_reach_a_row(device, dtype, hq):
     """K and V of the drafted keys hold infinities and NaN; rows that do not see
     such a key are what they are with ordinary numbers there, rows that see it
     follow the sum."""
@@ -126,7 +129,7 @@ def test_unseen_infinities_do_not_reach_a_row(device, dtype):
     from probjax_amd.attention import tree_attention
 
     dt = _types()[dtype]
-    B, T, S, Hq, Hkv, D = 2, 20, 400, 8, 2, 128
+    B, T, S, Hq, Hkv, D = 2, 20, 400, hq, 2, 128
     (q, k, v), _ = _inputs(6, dt, B, T, S, Hq, Hkv, D, device)
     parents = torch.from_numpy(random_parents(np.random.default_rng(2), 1, T)[0]).to(device)
     L = torch.tensor([370, 100], dtype=torch.int32, device=device)
