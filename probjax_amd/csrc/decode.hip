@@ -304,93 +304,8 @@ __global__ __launch_bounds__(kDecThreads, 1) void mla_decode_kernel(DecodeArgs a
   }
 }
 
-// Exact merge of the chunk partials of one (batch, group, query row):
-// M = max_c m_c, O = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c
-// (attention_splitkv.py:236-245, with unnormalised partials).  One thread per
-// 4 output dims.  The partials are taken in batches of kMergeBatch chunks whose
-// loads (m, l and 4 dims of O per chunk) are all issued before any is used, so
-// a batch costs one memory round trip (the first one overlapping the length
-// load); batches are combined online (running max, rescaled sums).  Sequences that fit one chunk were finished by the
-// chunk kernel; empty sequences (length 0, no chunk ran) get a zero output and
-// LSE = +inf (attention_xla.py:417-420).
-constexpr int kMergeThreads = 128;
-constexpr int kMergeBatch = 16;
 __global__ __launch_bounds__(kMergeThreads) void decode_merge_kernel(DecodeArgs a) {
-  const int nq = a.orow / 4;
-  const long gid = (long)blockIdx.x * kMergeThreads + threadIdx.x;
-  const long item = gid / nq;
-  const int u = (int)(gid % nq);
-  if (item >= (long)a.B * a.G * a.rows) return;
-  const int bg = (int)(item / a.rows), r = (int)(item % a.rows);
-  const int b = bg / a.G, g = bg % a.G;
-  const size_t base = (size_t)bg * a.nch;
-  const float* ml = a.ws_ml + (base * a.rows + r) * 2;  // chunk c at ml[c * ml_stride]
-  const size_t ml_stride = (size_t)a.rows * 2;
-  const float* po = a.ws_o + (base * a.rows + r) * a.dv + 4 * u;  // chunk c at po[c * o_stride]
-  const size_t o_stride = (size_t)a.rows * a.dv;
-  // The sequence length is needed only after the first batch's loads are
-  // issued: partial addresses are clamped to the workspace's a.nch chunks,
-  // and slots at or past this sequence's chunk count n (never written by this
-  // call) are dropped by selects, so whatever they hold cannot leak in.
-  // (A buffer load of the length: unconditional, so nothing waits for it
-  // before the partial loads; without lengths the buffer is empty.)
-  const int len_raw = (int)__builtin_amdgcn_raw_buffer_load_b32(
-      make_rsrc(a.lengths, a.lengths ? (uint32_t)a.B * 4u : 0u), b * 4, 0, 0);
-  float M = kMaxInit, den = 0.f;
-  f32x4 num = {0.f, 0.f, 0.f, 0.f};
-  float mv[kMergeBatch], lv[kMergeBatch];
-  f32x4 ov[kMergeBatch];
-  auto load_batch = [&](int c0) {
-#pragma unroll
-    for (int i = 0; i < kMergeBatch; ++i) {
-      const size_t c = (size_t)min(c0 + i, a.nch - 1);
-      mv[i] = ml[c * ml_stride];
-      lv[i] = ml[c * ml_stride + 1];
-      ov[i] = *(const f32x4*)(po + c * o_stride);
-    }
-    __builtin_amdgcn_sched_barrier(0);  // keep every load of the batch ahead of the arithmetic
-  };
-  auto add_batch = [&](int c0, int n) {
-    float bm = M;
-#pragma unroll
-    for (int i = 0; i < kMergeBatch; ++i)
-      if (c0 + i < n) bm = fmaxf(bm, mv[i]);
-    const float sc = fast_exp2(M - bm);
-    M = bm;
-    den *= sc;
-    num *= sc;
-#pragma unroll
-    for (int i = 0; i < kMergeBatch; ++i) {
-      if (c0 + i < n) {
-        const float wt = fast_exp2(mv[i] - M);
-        den = fmaf(wt, lv[i], den);
-        num += wt * ov[i];
-      }
-    }
-  };
-  load_batch(0);
-  const int L = a.lengths ? min(a.Lk, min(a.Lk, max(len_raw, 0)) + a.extra) : a.Lk;  // as seq_len
-  const int n = (L + a.chunk - 1) / a.chunk;
-  if (n == 1) return;  // the chunk kernel wrote this row's output
-  add_batch(0, n);
-  for (int c0 = kMergeBatch; c0 < n; c0 += kMergeBatch) {
-    load_batch(c0);
-    add_batch(c0, n);
-  }
-  int t, h;
-  row_to_head(a, g, r, t, h);
-  const bool some = a.extra ? some_key(den) : den > 0.f;
-  const float inv = some ? 1.f / den : 0.f;
-  const size_t oi = ((size_t)(b * a.Lq + t) * a.Hq + h) * a.orow + 4 * u;
-  if (a.o32) {
-    *(f32x4*)(a.o32 + oi) = num * inv;
-  } else {
-    const u32x2 pk = a.f16 ? u32x2{F16Fmt::pack2(num[0] * inv, num[1] * inv), F16Fmt::pack2(num[2] * inv, num[3] * inv)}
-                           : u32x2{Bf16Fmt::pack2(num[0] * inv, num[1] * inv), Bf16Fmt::pack2(num[2] * inv, num[3] * inv)};
-    *(u32x2*)(a.o + oi) = pk;
-  }
-  if (a.lse && u == 0)
-    a.lse[((size_t)b * a.Hq + h) * a.Lq + t] = some ? (M + __log2f(den)) * kLn2 : INFINITY;
+  merge_chunks(a, (long)blockIdx.x * kMergeThreads + threadIdx.x);
 }
 
 // Keys per work item when the caller passes chunk = 0: the smallest power of

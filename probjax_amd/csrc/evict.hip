@@ -38,12 +38,36 @@ __device__ __forceinline__ uint32_t weight_key(uint32_t u) {
   return u >> 31 ? ~u : u | 0x80000000u;
 }
 
+// Sum over the 16 lanes of a row, in every lane of it.
+__device__ __forceinline__ int row_sum(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x128, 0xf, 0xf, false);  // row_ror:8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x124, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x122, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x121, 0xf, 0xf, false);
+  return x;
+}
+
+// Inclusive prefix sum over a wave.
+__device__ __forceinline__ int wave_scan(int x) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int y = __shfl_up(x, d);
+    x += lane >= d ? y : 0;
+  }
+  return x;
+}
+
 // R: keys of a thread's registers (the cache has at most R * kSelThreads); 0:
 // read again in every round.
+constexpr int kPlaceTiles = 8;  // tiles of kSelThreads keys ranked together
 template <int R>
 __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) {
-  __shared__ __attribute__((aligned(16))) int count[2][3][kSelWaves];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ int count[2][3 * kSelWaves];
+  __shared__ int rank_above[kPlaceTiles * kSelWaves], rank_at[kPlaceTiles * kSelWaves];
+  __shared__ int total[2];
+  static_assert(kSelWaves == 16 && kPlaceTiles * kSelWaves == 128, "two ranks per lane of a wave");
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int bh = blockIdx.x, b = bh / a.H;
   const int n = a.lengths ? min(max(a.lengths[b], 0), a.S) : a.S;
   const int kept = min(n, a.keep);
@@ -91,68 +115,83 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
       } else {
         for (int j = tid; j < (n + kSelThreads - 1) / kSelThreads * kSelThreads; j += kSelThreads) look(key_at(j));
       }
-      if (lane < 3) count[round][lane][wave] = lane == 0 ? c[0] : lane == 1 ? c[1] : c[2];
+      // (the counts are the same in every lane: the ballots' sums are scalars)
+      if (lane < 3) count[round][16 * lane + wave] = lane == 0 ? c[0] : lane == 1 ? c[1] : c[2];
       __syncthreads();
+      const int sums = row_sum(lane < 48 ? count[round][lane] : 0);
       int at = 0, reached = 0;
 #pragma unroll
-      for (int j = 0; j < 3; ++j) {
-        int sum = 0;
-#pragma unroll
-        for (int i = 0; i < kSelWaves; ++i) sum += count[round][j][i];
-        if (sum >= need) {
-          at = j + 1;
-          reached = sum;
-        } else {
-          above = sum;
-          break;
+      for (int j = 2; j >= 0; --j) {  // the largest digit that enough keys reach
+        const int sum = __builtin_amdgcn_readlane(sums, 16 * j);
+        if (at == 0) {
+          if (sum >= need) {
+            at = j + 1;
+            reached = sum;
+          } else {
+            above = sum;
+          }
         }
       }
       T |= (uint32_t)at << bit;
       exact = at > 0 && reached == need;
     }
-    __syncthreads();
   }
   // Keys above T are kept, and of those at T the first `ties`.
-  const int ties = need == 0 ? 0 : exact ? need : need - above;
+  const int ties = need == 0 || exact ? 0 : need - above;
   if (exact) T -= 1;
-  const int ties_at_T = exact ? 0 : ties;
-  int done_above = 0, done_at = 0, buf = 0;
-  auto place = [&](int j, uint32_t u) {
-    const bool g = j < n && (j < lo || j >= hi || u > T);
-    const bool e = j >= lo && j < hi && u == T;
-    const uint64_t gm = __builtin_amdgcn_ballot_w64(g), em = __builtin_amdgcn_ballot_w64(e);
-    if (lane == 0) {
-      count[buf][0][wave] = __popcll(gm);
-      count[buf][1][wave] = __popcll(em);
+  // Ranks, kPlaceTiles tiles at a time: every wave counts its kept and tied keys
+  // of each tile, one wave sums them in the keys' order.
+  int done_above = 0, done_at = 0;
+  auto place = [&](int j0, const uint32_t* u) {
+    uint64_t gm[kPlaceTiles], em[kPlaceTiles];
+#pragma unroll
+    for (int i = 0; i < kPlaceTiles; ++i) {
+      const int j = j0 + i * kSelThreads + tid;
+      gm[i] = __builtin_amdgcn_ballot_w64(j < n && (j < lo || j >= hi || u[i] > T));
+      em[i] = __builtin_amdgcn_ballot_w64(j >= lo && j < hi && u[i] == T);
+      if (lane == 0) {
+        rank_above[kSelWaves * i + wave] = __popcll(gm[i]);
+        rank_at[kSelWaves * i + wave] = __popcll(em[i]);
+      }
     }
     __syncthreads();
-    int g0 = done_above, e0 = done_at, ga = 0, ea = 0;
-#pragma unroll
-    for (int i = 0; i < kSelWaves; ++i) {
-      const int cg = count[buf][0][i], ce = count[buf][1][i];
-      g0 += i < wave ? cg : 0;
-      e0 += i < wave ? ce : 0;
-      ga += cg;
-      ea += ce;
+    if (wave < 2) {
+      int* r = wave == 0 ? rank_above : rank_at;
+      const int x = r[2 * lane], y = r[2 * lane + 1], end = wave_scan(x + y);
+      r[2 * lane] = end - y - x;
+      r[2 * lane + 1] = end - y;
+      if (lane == 63) total[wave] = end;
     }
-    done_above += ga;
-    done_at += ea;
-    buf ^= 1;
+    __syncthreads();
     const uint64_t below = ((uint64_t)1 << lane) - 1;
-    g0 += __popcll(gm & below);
-    e0 += __popcll(em & below);
-    if (g || (e && e0 < ties_at_T)) {
-      const int at = g0 + min(e0, ties_at_T);
-      index[at] = j;
-      wout[at] = w[j];
+#pragma unroll
+    for (int i = 0; i < kPlaceTiles; ++i) {
+      const int g0 = done_above + rank_above[kSelWaves * i + wave] + __popcll(gm[i] & below);
+      const int e0 = done_at + rank_at[kSelWaves * i + wave] + __popcll(em[i] & below);
+      if ((gm[i] >> lane & 1) || ((em[i] >> lane & 1) && e0 < ties)) {
+        const int at = g0 + min(e0, ties), j = j0 + i * kSelThreads + tid;
+        index[at] = j;
+        wout[at] = w[j];
+      }
     }
+    done_above += total[0];
+    done_at += total[1];
   };
   if constexpr (R > 0) {
 #pragma unroll
-    for (int i = 0; i < R; ++i)
-      if (i * kSelThreads < n) place(tid + i * kSelThreads, key[i]);
+    for (int i = 0; i < R; i += kPlaceTiles)
+      if (i * kSelThreads < n) {
+        if (i > 0) __syncthreads();  // the last tiles' ranks have been read
+        place(i * kSelThreads, key + i);
+      }
   } else {
-    for (int j0 = 0; j0 < n; j0 += kSelThreads) place(j0 + tid, key_at(j0 + tid));
+    for (int j0 = 0; j0 < n; j0 += kPlaceTiles * kSelThreads) {
+      uint32_t u[kPlaceTiles];
+#pragma unroll
+      for (int i = 0; i < kPlaceTiles; ++i) u[i] = key_at(j0 + i * kSelThreads + tid);
+      __syncthreads();
+      place(j0, u);
+    }
   }
 }
 

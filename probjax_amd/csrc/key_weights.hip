@@ -17,9 +17,9 @@
 
 namespace pjx {
 
-template <typename E, int D, int NRB, bool ROWS>
+template <typename E, int D, int NRB, bool STREAM, bool ROWS>
 __global__ __launch_bounds__(256, (decode_occupancy<D, D, NRB>())) void scored_decode_kernel(DecodeArgs a) {
-  gqa_decode<E, D, D, NRB, false, ROWS, kScores>(a);
+  gqa_decode<E, D, D, NRB, STREAM, ROWS, kScores>(a);
 }
 
 template <int D, int NRB>
@@ -27,29 +27,45 @@ __global__ __launch_bounds__(256, 1) void scored_decode_f32_kernel(DecodeArgs a)
   gqa_decode_f32<D, D, NRB, kScores>(a);
 }
 
-constexpr int kWeightThreads = 256;
+constexpr int kWeightThreads = 128;  // the merge's, which shares the launch
+constexpr int kWeightKeys = 4 * kWeightThreads;
 constexpr int kMaxScoredRows = 64;
+static_assert(kWeightThreads == kMergeThreads && kMaxScoredRows <= kWeightThreads, "one launch");
 
-// Keys of the weights' kernel: 4 consecutive ones per thread.
-__global__ __launch_bounds__(kWeightThreads) void score_weights_kernel(DecodeArgs a, const float* w_in, float* w_out) {
-  __shared__ float stat[kMaxScoredRows][2];  // running max (log2 units), 1 / sum
-  const int bg = blockIdx.y + blockIdx.z * 65535;
-  if (bg >= a.B * a.G) return;
+// After the chunk kernel: the first merge_blocks workgroups merge the outputs,
+// every further one forms the weights of 512 keys, 4 consecutive ones a thread.
+// Each of these finds the statistics of its rows itself, from the chunks'.
+__global__ __launch_bounds__(kWeightThreads) void scored_merge_kernel(DecodeArgs a, const float* w_in, float* w_out,
+                                                                     int merge_blocks, int key_blocks) {
+  if ((int)blockIdx.x < merge_blocks) {
+    merge_chunks(a, (long)blockIdx.x * kWeightThreads + threadIdx.x);
+    return;
+  }
+  __shared__ float2 stat[kMaxScoredRows];  // running max (log2 units), 1 / sum
+  const int block = blockIdx.x - merge_blocks, bg = block / key_blocks;
   const int b = bg / a.G, tid = threadIdx.x;
   const int L = seq_len(a, b), n = (L + a.chunk - 1) / a.chunk;
-  const int j0 = (blockIdx.x * kWeightThreads + tid) * 4;
-  if (tid < a.rows) {
-    const float* ml = a.ws_ml + ((size_t)bg * a.nch * a.rows + tid) * 2;
-    float M = kMaxInit, sum = 0.f;
-    for (int c = 0; c < n; ++c) {
-      const float m = ml[(size_t)c * a.rows * 2], l = ml[(size_t)c * a.rows * 2 + 1];
-      const float m_new = fmaxf(M, m);
-      sum = fmaf(sum, fast_exp2(M - m_new), l * fast_exp2(m - m_new));
+  const int j0 = block % key_blocks * kWeightKeys + 4 * tid;
+  // each row's chunks over the lanes it gets: a power of two of them, in one wave
+  int per = 64;
+  while (per * a.rows > kWeightThreads) per /= 2;
+  const int row = tid / per, l0 = tid % per;
+  float M = kMaxInit, sum = 0.f;
+  if (row < a.rows) {
+    const float2* ml = (const float2*)a.ws_ml + (size_t)bg * a.nch * a.rows + row;
+    for (int c = l0; c < n; c += per) {
+      const float2 x = ml[(size_t)c * a.rows];
+      const float m_new = fmaxf(M, x.x);
+      sum = fmaf(sum, fast_exp2(M - m_new), x.y * fast_exp2(x.x - m_new));
       M = m_new;
     }
-    stat[tid][0] = M;
-    stat[tid][1] = 1.f / sum;
   }
+  for (int d = per / 2; d > 0; d /= 2) {
+    const float m2 = __shfl_xor(M, d), s2 = __shfl_xor(sum, d), m_new = fmaxf(M, m2);
+    sum = sum * fast_exp2(M - m_new) + s2 * fast_exp2(m2 - m_new);
+    M = m_new;
+  }
+  if (row < a.rows && l0 == 0) stat[row] = make_float2(M, 1.f / sum);
   __syncthreads();
   if (j0 >= a.Lk) return;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
@@ -58,9 +74,9 @@ __global__ __launch_bounds__(kWeightThreads) void score_weights_kernel(DecodeArg
 #pragma unroll 4
     for (int r = 0; r < a.rows; ++r) {
       const f32x4 x = *(const f32x4*)(s + (size_t)r * a.score_ld);
-      const float M = stat[r][0], inv = stat[r][1];
+      const float2 st = stat[r];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] = fmaf(fast_exp2(x[e] - M), inv, acc[e]);
+      for (int e = 0; e < 4; ++e) acc[e] = fmaf(fast_exp2(x[e] - st.x), st.y, acc[e]);
     }
   }
   const size_t at = (size_t)bg * a.Lk + j0;
@@ -71,21 +87,28 @@ __global__ __launch_bounds__(kWeightThreads) void score_weights_kernel(DecodeArg
 template <auto K>
 static int run_scored(DecodeArgs& a, const float* w_in, float* w_out, void* ws, size_t ws_bytes, hipStream_t s) {
   const char* who = "pjx_weighted_decode";
-  int rc = run_chunks<K>(a, ws, ws_bytes, s, who);
-  if (rc == PJX_OK) rc = launch_decode_merge(a, s, who);
+  const int rc = run_chunks<K>(a, ws, ws_bytes, s, who);
   if (rc != PJX_OK) return rc;
-  const int64_t bg = (int64_t)a.B * a.G;
-  const dim3 grid((unsigned)((a.Lk + 4 * kWeightThreads - 1) / (4 * kWeightThreads)), (unsigned)std::min<int64_t>(bg, 65535),
-                  (unsigned)((bg + 65534) / 65535));
-  launch_kernel<score_weights_kernel>(grid, dim3(kWeightThreads), 0, s, a, w_in, w_out);
+  const int64_t merge = ((int64_t)a.B * a.G * a.rows * (a.orow / 4) + kWeightThreads - 1) / kWeightThreads;
+  const int64_t keys = (a.Lk + kWeightKeys - 1) / kWeightKeys, blocks = merge + keys * a.B * a.G;
+  if (blocks > 0xffffffffLL / kWeightThreads) return fail(PJX_ERR_INVALID, "pjx_weighted_decode: sizes out of range");
+  launch_kernel<scored_merge_kernel>(dim3((unsigned)blocks), dim3(kWeightThreads), 0, s, a, w_in, w_out, (int)merge,
+                                     (int)keys);
   return check_launch(who);
 }
 
+// Caches past decode_streams_kv's threshold are read with non-temporal loads, as
+// the plain decode reads them (up to 32 rows at head dims up to 128).
 template <typename E, int D, bool ROWS>
 static int run_scored_rows(DecodeArgs& a, int nrb, const float* wi, float* wo, void* ws, size_t n, hipStream_t s) {
-  if (nrb == 1) return run_scored<scored_decode_kernel<E, D, 1, ROWS>>(a, wi, wo, ws, n, s);
-  if (nrb == 2) return run_scored<scored_decode_kernel<E, D, 2, ROWS>>(a, wi, wo, ws, n, s);
-  if constexpr (D <= 128) return run_scored<scored_decode_kernel<E, D, 4, ROWS>>(a, wi, wo, ws, n, s);
+  if constexpr (!ROWS && D <= 128) {
+    if (nrb <= 2 && decode_streams_kv((int64_t)a.B * a.Lk * a.G * 2 * D * 2, kStreamBytes))
+      return nrb == 1 ? run_scored<scored_decode_kernel<E, D, 1, true, false>>(a, wi, wo, ws, n, s)
+                      : run_scored<scored_decode_kernel<E, D, 2, true, false>>(a, wi, wo, ws, n, s);
+  }
+  if (nrb == 1) return run_scored<scored_decode_kernel<E, D, 1, false, ROWS>>(a, wi, wo, ws, n, s);
+  if (nrb == 2) return run_scored<scored_decode_kernel<E, D, 2, false, ROWS>>(a, wi, wo, ws, n, s);
+  if constexpr (D <= 128) return run_scored<scored_decode_kernel<E, D, 4, false, ROWS>>(a, wi, wo, ws, n, s);
   return fail(PJX_ERR_INVALID, "pjx_weighted_decode: row blocks");
 }
 
@@ -329,7 +352,6 @@ extern "C" int pjx_weighted_decode(int dtype, const void* q, const void* k, cons
     return write_keyless(o, lse, (size_t)(batch * q_len * q_heads * row_dim), f32, (size_t)(batch * q_heads * q_len), s,
                          who);
   if (!weights_out) return fail(PJX_ERR_INVALID, "pjx_weighted_decode: null pointer");
-  if (batch * kv_heads > (int64_t)65535 * 65535) return fail(PJX_ERR_INVALID, "pjx_weighted_decode: sizes out of range");
   if (!workspace || workspace_bytes < pjx_weighted_decode_workspace_size(batch, kv_heads, rows, kv_len, head_dim, a.chunk))
     return fail(PJX_ERR_WORKSPACE, "pjx_weighted_decode: workspace missing or too small");
   if ((uintptr_t)workspace % 16) return fail(PJX_ERR_INVALID, "pjx_weighted_decode: the workspace must start on 16 bytes");
