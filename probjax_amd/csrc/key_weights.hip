@@ -14,6 +14,7 @@
 #include <stdio.h>
 
 #include "decode_common.h"
+#include "flash_common.h"
 
 namespace pjx {
 
@@ -152,93 +153,219 @@ struct KeyWeightArgs {
   float cx;
 };
 
-// Rows of a tile of queries in LDS: 16-byte chunks XOR-swizzled by the row, so
-// that 32 lanes reading one chunk of 32 rows touch distinct banks.
-template <int D>
-struct QueryTile {
-  static constexpr int BQ = 32, NC = D / 8, ROWB = 2 * D;
-  __device__ static int swz(int r) { return NC >= 16 ? (r & 15) : (r & 7); }
-};
+// Keys of a wave, in blocks of 32 (their fragments stay in registers): a query
+// fragment read from LDS serves all of them.  With one block, the four waves'
+// reads of a query tile take as long as their products.
+constexpr int key_blocks(int head_dim) { return head_dim <= 128 ? 2 : 1; }
 
-// One workgroup: 128 keys (32 per wave, their fragments in registers) of one
-// (batch, KV head), against the query rows of one split of one head of its group.
+// What a workgroup works on: keys k_first .. of one (batch, KV head), against the
+// query rows [q_lo, q_hi) of one split of one head of its group.
+struct KeyWork {
+  int b, g, h, hs, L, q_lo, q_hi;
+};
+// Workgroup x works on key block x / (rows of the grid); of the rest, heads vary
+// slower than splits, and the split is turned by the key block and the head: under
+// a causal mask early splits and late key blocks have little to do, and workgroup
+// x runs on XCD x % 8, so any fixed order gives some XCDs the heavy ones (key
+// block fastest: 100 us for 70 on the prompt below).
+__device__ __forceinline__ KeyWork key_work(const KeyWeightArgs& a, int keys, int& k_first) {
+  KeyWork u;
+  const int per = a.Hq / a.G, units = a.B * a.Hq * a.splits;
+  const int block = blockIdx.x / units, y = blockIdx.x % units, hb = y / a.splits;
+  const int split = (y + hb + block) % a.splits;
+  k_first = block * keys;
+  u.b = hb / a.Hq;
+  u.h = hb % a.Hq;
+  u.g = u.h / per;
+  u.hs = u.h % per * a.splits + split;
+  // (a scalar: loaded as a vector, everything up to the loop's count became one)
+  u.L = a.lengths ? min(a.Lk, max(__builtin_amdgcn_readfirstlane(a.lengths[u.b]), 0)) : a.Lk;
+  u.q_lo = split * a.q_step;
+  u.q_hi = min(u.q_lo + a.q_step, a.Lq);
+  // (rows before it see none of the keys)
+  if (a.causal) u.q_lo = max(u.q_lo, max(k_first - a.shift, 0) / 32 * 32);
+  if (k_first >= u.L) u.q_hi = u.q_lo;
+  return u;
+}
+
+template <int N>
+__device__ __forceinline__ void halve(float* x, int d) {
+  const bool up = (threadIdx.x & d) != 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    float keep = x[i], give = x[i + N];
+    asm volatile("" : "+v"(keep), "+v"(give));  // (two selects; merged over the registers they became hundreds)
+    const float k = up ? give : keep, g = up ? keep : give;
+    x[i] = k + __shfl_xor(g, d);
+  }
+}
+
+// Writes the sums over the 32 queries of a half wave of one block of 32 keys.
+// Each exchange halves the registers: a lane keeps the half that its bit names and
+// adds its partner's, so 16 exchanges do for 16 registers; lane c ends with
+// register bit-reverse(c % 16).
+__device__ __forceinline__ void put_weights(const KeyWeightArgs& a, const KeyWork& u, const f32x16& sums, int k0) {
+  const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
+  float* part = a.part + ((size_t)u.hs * a.B * a.G + u.b * a.G + u.g) * a.Lk;
+  float x[16];
+#pragma unroll
+  for (int r = 0; r < 16; ++r) x[r] = sums[r];
+  if (u.q_lo < u.q_hi) {
+    halve<8>(x, 1);
+    halve<4>(x, 2);
+    halve<2>(x, 4);
+    halve<1>(x, 8);
+    x[0] += __shfl_xor(x[0], 16);
+  }
+  const int r = (col & 1) << 3 | (col & 2) << 1 | (col & 4) >> 1 | (col & 8) >> 3;
+  const int key = k0 + 8 * (r >> 2) + 4 * half + (r & 3);
+  if (col < 16 && key < a.Lk) part[key] = key < u.L ? x[0] : 0.f;
+}
+
+// 16 bits: tiles of 32 query rows (and their LSE) go HBM -> LDS by loads that
+// write LDS, three tiles ahead in a ring of four, and tile t + 1's products run
+// beside tile t's exponentials.  The ring's slots are LDS objects of their own and
+// the loop is unrolled over them, so that the compiler sees that no load in flight
+// writes the slot being read; with an index it waits for every load first.
 template <typename E, int D>
-__global__ __launch_bounds__(256) void key_weights_kernel(KeyWeightArgs a) {
-  using T = QueryTile<D>;
-  __shared__ __attribute__((aligned(1024))) unsigned char qs[2][T::BQ * T::ROWB];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, col = lane & 31, half = lane >> 5;
-  const int per = a.Hq / a.G;
-  const int hs = blockIdx.y % (per * a.splits), bg = blockIdx.y / (per * a.splits);
-  const int b = bg / a.G, g = bg % a.G, h = g * per + hs / a.splits, split = hs % a.splits;
-  const int k0 = blockIdx.x * 128 + 32 * w;
-  const int L = a.lengths ? min(a.Lk, max(a.lengths[b], 0)) : a.Lk;
-  // rows of this split that see the workgroup's first key
-  int q_lo = split * a.q_step, q_hi = min(q_lo + a.q_step, a.Lq);
-  if (a.causal) q_lo = max(q_lo, (max((int)blockIdx.x * 128 - a.shift, 0)) / T::BQ * T::BQ);
-  const bool any = (int)blockIdx.x * 128 < L && q_lo < q_hi;
-  f32x16 acc = {};
-  if (any) {
-    typename E::v8 kf[D / 16];
-    const int key = k0 + col;
-    const uint16_t* krow = (const uint16_t*)a.k + ((size_t)(b * (int64_t)a.Lk + min(key, a.Lk - 1)) * a.G + g) * a.rdim;
+__global__ __launch_bounds__(256, 2) void key_weights_kernel(KeyWeightArgs a) {
+  using T = Bf16Tile<D, 32>;
+  constexpr int KB = key_blocks(D), ROWB = T::ROWB;
+  constexpr int NLD = 32 / 4 / T::RPI > 0 ? 32 / 4 / T::RPI : 1;  // loads per wave per tile
+  static_assert(T::RPI * NLD * 4 == 32, "tile rows");
+  __shared__ __attribute__((aligned(1024))) unsigned char qs0[T::TILE_B + 1024], qs1[T::TILE_B + 1024],
+      qs2[T::TILE_B + 1024], qs3[T::TILE_B + 1024];  // a tile, then each wave's copy of its LSE
+  auto slot = [&](auto i) -> unsigned char* {
+    constexpr int I = decltype(i)::value & 3;
+    if constexpr (I == 0) return qs0;
+    else if constexpr (I == 1) return qs1;
+    else if constexpr (I == 2) return qs2;
+    else return qs3;
+  };
+  const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int k_first;
+  const KeyWork u = key_work(a, 128 * KB, k_first);
+  const int k0 = k_first + 32 * KB * w;
+  f32x16 acc[KB];
 #pragma unroll
-    for (int s = 0; s < D / 16; ++s) {
-      u32x4 r = {0u, 0u, 0u, 0u};
-      if (key < L && 16 * s + 8 * half < a.rdim) r = *(const u32x4*)(krow + 16 * s + 8 * half);
-      kf[s] = E::as8(r);
+  for (int kb = 0; kb < KB; ++kb) acc[kb] = f32x16{};
+  const int n = (u.q_hi - u.q_lo + 31) / 32;
+  if (n > 0) {
+    const uint32_t rowstride = (uint32_t)a.Hq * a.rdim * 2;
+    const unsigned char* Q = (const unsigned char*)a.q + ((size_t)u.b * a.Lq * a.Hq + u.h) * a.rdim * 2;
+    uint32_t voff[NLD];
+#pragma unroll
+    for (int j = 0; j < NLD; ++j) {
+      const int r = 8 * w + T::RPI * j + lane / T::NC, slot = lane % T::NC;
+      voff[j] = row_chunk(r, rowstride, slot ^ T::swz_k(r), a.rdim);
     }
-    const float* lse = a.lse + ((size_t)b * a.Hq + h) * a.Lq;
-    const uint16_t* Q = (const uint16_t*)a.q + ((size_t)b * a.Lq * a.Hq + h) * a.rdim;
-    constexpr int NLD = T::BQ * T::NC / 256;
-    u32x4 qr[NLD];
-    float lr;
-    auto load = [&](int t0) {
+    const float* lse = a.lse + ((size_t)u.b * a.Hq + u.h) * a.Lq;
+    auto issue = [&](int t, unsigned char* q) {
+      const int t0 = u.q_lo + 32 * t;
+      // (a tile past the end: empty buffers, so that every path issues the same loads)
+      const int rows = max(min(32, u.q_hi - t0), 0);
+      const uint32_t bytes = rows > 0 ? (uint32_t)(rows - 1) * rowstride + a.rdim * 2 : 0u;
+      const rsrc_t rq = make_rsrc(Q + (size_t)min(t0, a.Lq - 1) * rowstride, bytes);
+      const rsrc_t rl = make_rsrc(lse + min(t0, a.Lq - 1), 4 * rows);
 #pragma unroll
-      for (int i = 0; i < NLD; ++i) {
-        const int u = tid + 256 * i, r = u / T::NC, c = u % T::NC;
-        qr[i] = u32x4{0u, 0u, 0u, 0u};
-        if (t0 + r < q_hi && 8 * c < a.rdim) qr[i] = *(const u32x4*)(Q + (size_t)(t0 + r) * a.Hq * a.rdim + 8 * c);
-      }
-      lr = t0 + col < q_hi ? lse[t0 + col] : INFINITY;
+      for (int j = 0; j < NLD; ++j) buffer_load_lds16(rq, q + (8 * w + T::RPI * j) * ROWB, voff[j]);
+      buffer_load_lds4(rl, q + T::TILE_B + 256 * w, 4 * lane);
     };
-    load(q_lo);
-    int st = 0;
-    for (int t0 = q_lo; t0 < q_hi; t0 += T::BQ, st ^= 1) {
+    typename E::v8 kf[KB][D / 16];
 #pragma unroll
-      for (int i = 0; i < NLD; ++i) {
-        const int u = tid + 256 * i, r = u / T::NC, c = u % T::NC;
-        *(u32x4*)(qs[st] + r * T::ROWB + 16 * (c ^ T::swz(r))) = qr[i];
+    for (int kb = 0; kb < KB; ++kb) {
+      const int key = k0 + 32 * kb + col;
+      const uint16_t* krow = (const uint16_t*)a.k + (((size_t)u.b * a.Lk + min(key, a.Lk - 1)) * a.G + u.g) * a.rdim;
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s) {
+        u32x4 r = {0u, 0u, 0u, 0u};
+        if (key < u.L && 16 * s + 8 * half < a.rdim) r = *(const u32x4*)(krow + 16 * s + 8 * half);
+        kf[kb][s] = E::as8(r);
       }
-      const float l2 = lr * kLog2e;  // +inf: no row, or one without a valid key
-      __syncthreads();
-      if (t0 + T::BQ < q_hi) load(t0 + T::BQ);
-      f32x16 s = {};
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        const u32x4 q8 = *(const u32x4*)(qs[st] + col * T::ROWB + 16 * ((2 * i + half) ^ T::swz(col)));
-        s = E::mma32(kf[i], E::as8(q8), s);
-      }
-      // register r: key k0 + 8 (r / 4) + 4 half + r % 4, query t0 + col
-      if (a.causal && k0 + 31 > t0 + a.shift) {
-        const int lim = t0 + col + a.shift - (k0 + 4 * half);
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (8 * (r >> 2) + (r & 3) > lim) s[r] = -INFINITY;
-      }
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[r] += fast_exp2(fmaf(s[r], a.cx, -l2));
     }
-  }
-  // sums over the 32 queries of a half wave
-  float* part = a.part + ((size_t)hs * a.B * a.G + bg) * a.Lk;
+    uint32_t offQ[D / 16];
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    float x = acc[r];
+    for (int st = 0; st < D / 16; ++st) offQ[st] = col * ROWB + 16 * ((2 * st + half) ^ T::swz_k(col));
+    auto scores = [&](const unsigned char* q, f32x16* s) {
 #pragma unroll
-    for (int m = 1; m < 32; m *= 2) x += __shfl_xor(x, m);
-    const int key = k0 + 8 * (r >> 2) + 4 * half + (r & 3);
-    if (col == r && key < a.Lk) part[key] = key < L ? x : 0.f;
+      for (int kb = 0; kb < KB; ++kb) s[kb] = f32x16{};
+#pragma unroll
+      for (int st = 0; st < D / 16; ++st) {
+        const typename E::v8 qf = E::as8(*(const u32x4*)(q + offQ[st]));
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) s[kb] = E::mma32(kf[kb][st], qf, s[kb]);
+      }
+    };
+    // register r of block kb: key k0 + 32 kb + 8 (r / 4) + 4 half + r % 4, query t0 + col
+    auto mask = [&](int t, f32x16* s) {
+      const int t0 = u.q_lo + 32 * t;
+      if (a.causal && k0 + 32 * KB - 1 > t0 + a.shift) {
+        asm volatile("");  // (a branch: as selects the comparisons ran on every tile)
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+          const int lim = t0 + col + a.shift - (k0 + 32 * kb + 4 * half);
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (8 * (r >> 2) + (r & 3) > lim) s[kb][r] = -INFINITY;
+        }
+      }
+    };
+    auto add = [&](f32x16* s, float l2) {
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[kb][r] += fast_exp2(fmaf(s[kb][r], a.cx, -l2));
+    };
+    f32x16 sa[KB], sb[KB];
+    auto lse_of = [&](int t, const unsigned char* q) {  // in log2 units; +inf: no row, or one without a valid key
+      const float l = ((const float*)(q + T::TILE_B + 256 * w))[col];
+      return u.q_lo + 32 * t + col < u.q_hi ? l * kLog2e : INFINITY;
+    };
+    issue(0, qs0);
+    issue(1, qs1);
+    issue(2, qs2);
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    scores(qs0, sa);
+    float l = lse_of(0, qs0);
+    // Iteration t forms the scores of tile t + 1, which has landed, and loads tile
+    // t + 3 into the slot of tile t - 1, last read in iteration t - 2.  Its end waits
+    // for tile t + 2, loaded two iterations before it is read.
+    auto step = [&](auto i, int t, f32x16* s, f32x16* next) {
+      constexpr int I = decltype(i)::value;
+      unsigned char* q = slot(std::integral_constant<int, I + 1>{});
+      issue(t + 3, slot(std::integral_constant<int, I + 3>{}));
+      const float l_next = lse_of(t + 1, q);
+      mask(t, s);
+      // one basic block from here: the products beside the exponentials
+      scores(q, next);
+      add(s, l);
+      // issue order: the first fragments, then each MFMA with the sums of two scores
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // DS reads
+#pragma unroll
+      for (int j = 0; j < KB * D / 16; ++j) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
+        __builtin_amdgcn_sched_group_barrier(0x402, 768 / D, 0);  // VALU incl. transcendental
+        if (j % KB == KB - 1) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      l = l_next;
+      wait_vmcnt<NLD + 1>();  // all but tile t + 3's
+      stage_barrier();
+    };
+    for (int t = 0; t < n; t += 4) {
+      step(std::integral_constant<int, 0>{}, t, sa, sb);
+      if (t + 1 >= n) break;
+      step(std::integral_constant<int, 1>{}, t + 1, sb, sa);
+      if (t + 2 >= n) break;
+      step(std::integral_constant<int, 2>{}, t + 2, sa, sb);
+      if (t + 3 >= n) break;
+      step(std::integral_constant<int, 3>{}, t + 3, sb, sa);
+    }
+    wait_vmcnt<0>();  // the last (empty) tiles' loads still write LDS
   }
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb) put_weights(a, u, acc[kb], k0 + 32 * kb);
 }
 
 __device__ __forceinline__ f32x16 mma_f32(float a, float b, f32x16 c) { return mfma32x32x2f32(a, b, c); }
@@ -250,33 +377,28 @@ __global__ __launch_bounds__(256) void key_weights_f32_kernel(KeyWeightArgs a) {
   constexpr int BQ = 32, LD = D + 4;  // padded rows: 32 lanes reading a feature pair touch distinct banks
   __shared__ __attribute__((aligned(16))) float qs[BQ * LD];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, col = lane & 31, half = lane >> 5;
-  const int per = a.Hq / a.G;
-  const int hs = blockIdx.y % (per * a.splits), bg = blockIdx.y / (per * a.splits);
-  const int b = bg / a.G, g = bg % a.G, h = g * per + hs / a.splits, split = hs % a.splits;
-  const int k0 = blockIdx.x * 128 + 32 * w;
-  const int L = a.lengths ? min(a.Lk, max(a.lengths[b], 0)) : a.Lk;
-  int q_lo = split * a.q_step, q_hi = min(q_lo + a.q_step, a.Lq);
-  if (a.causal) q_lo = max(q_lo, (max((int)blockIdx.x * 128 - a.shift, 0)) / BQ * BQ);
-  const bool any = (int)blockIdx.x * 128 < L && q_lo < q_hi;
+  int k_first;
+  const KeyWork u = key_work(a, 128, k_first);
+  const int k0 = k_first + 32 * w;
   f32x16 acc = {};
-  if (any) {
+  if (u.q_lo < u.q_hi) {
     // features 4 i + 2 half .. + 1 of key col: step 2 i contracts 4 i and 4 i + 2
     float2 kf[D / 4];
     const int key = k0 + col;
-    const float* krow = (const float*)a.k + ((size_t)(b * (int64_t)a.Lk + min(key, a.Lk - 1)) * a.G + g) * D;
+    const float* krow = (const float*)a.k + (((size_t)u.b * a.Lk + min(key, a.Lk - 1)) * a.G + u.g) * D;
 #pragma unroll
-    for (int i = 0; i < D / 4; ++i) kf[i] = key < L ? *(const float2*)(krow + 4 * i + 2 * half) : make_float2(0.f, 0.f);
-    const float* lse = a.lse + ((size_t)b * a.Hq + h) * a.Lq;
-    const float* Q = (const float*)a.q + ((size_t)b * a.Lq * a.Hq + h) * D;
-    for (int t0 = q_lo; t0 < q_hi; t0 += BQ) {
+    for (int i = 0; i < D / 4; ++i) kf[i] = key < u.L ? *(const float2*)(krow + 4 * i + 2 * half) : make_float2(0.f, 0.f);
+    const float* lse = a.lse + ((size_t)u.b * a.Hq + u.h) * a.Lq;
+    const float* Q = (const float*)a.q + ((size_t)u.b * a.Lq * a.Hq + u.h) * D;
+    for (int t0 = u.q_lo; t0 < u.q_hi; t0 += BQ) {
       __syncthreads();
-      for (int u = tid; u < BQ * D / 4; u += 256) {
-        const int r = u / (D / 4), c = u % (D / 4);
+      for (int i = tid; i < BQ * D / 4; i += 256) {
+        const int r = i / (D / 4), c = i % (D / 4);
         f32x4 x = {};
-        if (t0 + r < q_hi) x = *(const f32x4*)(Q + (size_t)(t0 + r) * a.Hq * D + 4 * c);
+        if (t0 + r < u.q_hi) x = *(const f32x4*)(Q + (size_t)(t0 + r) * a.Hq * D + 4 * c);
         *(f32x4*)(qs + r * LD + 4 * c) = x;
       }
-      const float l2 = (t0 + col < q_hi ? lse[t0 + col] : INFINITY) * kLog2e;
+      const float l2 = (t0 + col < u.q_hi ? lse[t0 + col] : INFINITY) * kLog2e;
       __syncthreads();
       f32x16 s = {};
 #pragma unroll
@@ -295,15 +417,7 @@ __global__ __launch_bounds__(256) void key_weights_f32_kernel(KeyWeightArgs a) {
       for (int r = 0; r < 16; ++r) acc[r] += fast_exp2(fmaf(s[r], a.cx, -l2));
     }
   }
-  float* part = a.part + ((size_t)hs * a.B * a.G + bg) * a.Lk;
-#pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    float x = acc[r];
-#pragma unroll
-    for (int m = 1; m < 32; m *= 2) x += __shfl_xor(x, m);
-    const int key = k0 + 8 * (r >> 2) + 4 * half + (r & 3);
-    if (col == r && key < a.Lk) part[key] = key < L ? x : 0.f;
-  }
+  put_weights(a, u, acc, k0);
 }
 
 // Adds the parts, in their order, to the weights so far.
@@ -311,14 +425,16 @@ __global__ __launch_bounds__(256) void add_weights_kernel(const float* part, con
                                                          int64_t n) {
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
     float x = 0.f;
+#pragma unroll 8
     for (int p = 0; p < parts; ++p) x += part[p * n + i];
     w_out[i] = (w_in ? w_in[i] : 0.f) + x;
   }
 }
 
-// Splits of the query rows: enough workgroups for two rounds of the device.
+// Splits of the query rows: enough workgroups that the causal half of them still
+// fills the device.
 static int64_t row_splits(int64_t batch, int64_t q_len, int64_t kv_len, int64_t q_heads) {
-  const int64_t blocks = (kv_len + 127) / 128 * batch * q_heads;
+  const int64_t blocks = (kv_len + 255) / 256 * batch * q_heads;
   return std::clamp<int64_t>(2048 / std::max<int64_t>(blocks, 1), 1, std::max<int64_t>((q_len + 255) / 256, 1));
 }
 
@@ -394,7 +510,7 @@ extern "C" int pjx_key_weights(int dtype, const void* q, const void* k, const fl
   if (!(sm_scale > 0.f)) return bad("sm_scale must be > 0");
   const int64_t most = (int64_t)1 << 40;
   if (q_len > (1 << 28) || kv_len > (1 << 28) || causal_shift > (1 << 28) || causal_shift < -(1 << 28) ||
-      batch * q_heads > (1 << 22) || batch * q_heads * std::max(q_len, kv_len) > most / head_dim)
+      batch * q_heads > (1 << 22) || q_heads * row_dim > (1 << 24) || batch * q_heads * std::max(q_len, kv_len) > most / head_dim)
     return bad("sizes out of range");
   if (batch * kv_len == 0) return PJX_OK;
   if (!weights_out || !k || (q_len > 0 && (!q || !lse))) return bad("null pointer");
@@ -410,10 +526,11 @@ extern "C" int pjx_key_weights(int dtype, const void* q, const void* k, const fl
   a.splits = (int)row_splits(batch, q_len, kv_len, q_heads);
   a.q_step = (int)(((q_len + a.splits - 1) / a.splits + 31) / 32 * 32);
   a.cx = sm_scale * kLog2e;
-  const int64_t rows = batch * q_heads * a.splits, groups = (kv_len + 127) / 128;
-  if (rows > 65535 || groups > 0xffffffffLL / 256) return bad("sizes out of range");
+  const int64_t units = batch * q_heads * a.splits, per = f32 ? 128 : 128 * key_blocks((int)head_dim),
+                groups = (kv_len + per - 1) / per;
+  if (units * groups > 0xffffffffLL / 256) return bad("sizes out of range");
   hipStream_t s = (hipStream_t)stream;
-  const dim3 grid((unsigned)groups, (unsigned)rows), block(256);
+  const dim3 grid((unsigned)(units * groups)), block(256);
   if (f32) {
     if (head_dim == 64) launch_kernel<key_weights_f32_kernel<64>>(grid, block, 0, s, a);
     else if (head_dim == 128) launch_kernel<key_weights_f32_kernel<128>>(grid, block, 0, s, a);
