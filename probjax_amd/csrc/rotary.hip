@@ -7,8 +7,10 @@
 // Bound by HBM: every feature is read and written once.  Angles cost float64
 // arithmetic (a position times a frequency loses the turn's fraction in float32
 // from a few thousand on), so a workgroup forms the cosines and sines of its
-// tokens once, in LDS, and all heads of q and k use them; a thread keeps its
-// place within the rows, so it reads the table once per token.
+// tokens once, in LDS, and all heads of q and k use them.  A thread keeps its place
+// within the rows and takes four of them at a time, their loads issued before the
+// first store.  bf16, 12288 tokens of 16 + 16 heads of 128 (201 MB): see the table
+// at the launch.
 #include <stdio.h>
 
 #include "pjx_common.h"
@@ -17,7 +19,7 @@
 namespace pjx {
 
 constexpr int kRotThreads = 256;
-constexpr int kRotTokens = 4;    // tokens of a workgroup at most
+constexpr int kRotTokens = 16;   // tokens of a workgroup at most
 constexpr int kRotPairs = 128;   // rotated pairs of a row at most
 constexpr int kRotAxes = 4;
 
@@ -30,13 +32,12 @@ struct RotaryArgs {
   int64_t pos_b, pos_t;  // elements between sequences and tokens of the positions
   int pos_type;
   int axes, T, D;
-  int64_t tokens;        // B * T
+  int tokens;            // B * T
   int first_pair[kRotAxes + 1];  // pairs of axis a: first_pair[a] .. first_pair[a + 1]
   int interleaved, shared;
-  double log2_base;
+  double rate[kRotAxes];  // log2 of the frequency's step from pair to pair
   float sign;
   int per_wg, heads_per_wg;
-  int64_t block0;  // first block of a launch
 };
 
 __device__ __forceinline__ double rotary_position(const RotaryArgs& a, int64_t i) {
@@ -53,56 +54,58 @@ constexpr int kInChunk = 0;   // interleaved: both in the chunk
 constexpr int kChunk = 1;     // halves of whole chunks: in another chunk, at the same places
 constexpr int kAnywhere = 2;  // one by one
 
-// N elements of type T (uint16_t bits or float) as floats, and back.
+// A chunk of N elements of format E in memory and as floats.
+struct F32Fmt {};
 template <typename E, int N>
 struct RotChunk;
 template <typename E>
 struct RotChunk<E, 8> {
   typedef u32x4 raw;
-  __device__ static void get(const char* p, float* v) {
-    const u32x4 r = *(const u32x4*)p;
+  __device__ static void get(const raw& r, float* v) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       v[2 * i] = E::lo(r[i]);
       v[2 * i + 1] = E::hi(r[i]);
     }
   }
-  __device__ static void put(char* p, const float* v) {
-    u32x4 r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = E::pack2(v[2 * i], v[2 * i + 1]);
-    *(u32x4*)p = r;
+  __device__ static raw put(const float* v) {
+    return raw{E::pack2(v[0], v[1]), E::pack2(v[2], v[3]), E::pack2(v[4], v[5]), E::pack2(v[6], v[7])};
   }
 };
 template <typename E>
 struct RotChunk<E, 1> {
-  __device__ static void get(const char* p, float* v) { v[0] = E::lo(*(const uint16_t*)p); }
-  __device__ static void put(char* p, const float* v) { *(uint16_t*)p = E::bits(v[0]); }
+  typedef uint16_t raw;
+  __device__ static void get(raw r, float* v) { v[0] = E::lo(r); }
+  __device__ static raw put(const float* v) { return E::bits(v[0]); }
 };
-struct F32Fmt {};
 template <>
 struct RotChunk<F32Fmt, 4> {
-  __device__ static void get(const char* p, float* v) {
-    const f32x4 r = *(const f32x4*)p;
+  typedef f32x4 raw;
+  __device__ static void get(const raw& r, float* v) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = r[i];
   }
-  __device__ static void put(char* p, const float* v) { *(f32x4*)p = f32x4{v[0], v[1], v[2], v[3]}; }
+  __device__ static raw put(const float* v) { return raw{v[0], v[1], v[2], v[3]}; }
 };
 template <>
 struct RotChunk<F32Fmt, 1> {
-  __device__ static void get(const char* p, float* v) { v[0] = *(const float*)p; }
-  __device__ static void put(char* p, const float* v) { *(float*)p = v[0]; }
+  typedef float raw;
+  __device__ static void get(raw r, float* v) { v[0] = r; }
+  __device__ static raw put(const float* v) { return v[0]; }
 };
 
 template <typename E, int N, int MODE>
 __global__ __launch_bounds__(kRotThreads) void rotary_kernel(RotaryArgs a) {
+  typedef RotChunk<E, N> C;
+  typedef typename C::raw Raw;
+  typedef RotChunk<E, 1> One;
   constexpr int SZ = std::is_same<E, F32Fmt>::value ? 4 : 2;
-  __shared__ float2 turn[kRotTokens][kRotPairs];  // cos, sin
+  constexpr int CH = MODE == kChunk ? 2 : 1;          // chunks of a thread's unit
+  constexpr int ROWS = MODE == kChunk ? 2 : 4;        // rows of a thread at a time
+  __shared__ float2 turn[kRotTokens * kRotPairs];     // cos, sin of pair p of token t at t * pairs + p
   const int tid = threadIdx.x;
   const int np = a.first_pair[a.axes];
-  const int64_t n0 = (a.block0 + blockIdx.x) * a.per_wg;
-  const int nt = (int)min((int64_t)a.per_wg, a.tokens - n0);
+  const int n0 = blockIdx.x * a.per_wg, nt = min(a.per_wg, a.tokens - n0);
 
   for (int i = tid; i < nt * np; i += kRotThreads) {
     const int tok = i / np, p = i - tok * np;
@@ -110,102 +113,151 @@ __global__ __launch_bounds__(kRotThreads) void rotary_kernel(RotaryArgs a) {
 #pragma unroll
     for (int j = 1; j < kRotAxes; ++j)
       if (j < a.axes && p >= a.first_pair[j]) axis = j;
-    const int lo = a.shared ? 0 : a.first_pair[axis], hi = a.shared ? np : a.first_pair[axis + 1];
-    const int64_t n = n0 + tok, b = n / a.T, t = n - b * a.T;
+    const int n = n0 + tok, b = n / a.T, t = n - b * a.T;
     const double x = rotary_position(a, b * a.pos_b + t * a.pos_t + axis);
+    double rate = a.rate[0];
+#pragma unroll
+    for (int j = 1; j < kRotAxes; ++j) rate = axis == j ? a.rate[j] : rate;
+    int lo = a.first_pair[0];
+#pragma unroll
+    for (int j = 1; j < kRotAxes; ++j) lo = axis == j && !a.shared ? a.first_pair[j] : lo;
     // turns, less the whole ones
-    const double f = exp2(-a.log2_base * (double)(p - lo) / (double)(hi - lo)) * 0.15915494309189535;
-    const double r = x * f;
+    const double r = x * (exp2(rate * (double)(p - lo)) * 0.15915494309189535);
     float s, c;
     sincospif((float)(2.0 * (r - rint(r))), &s, &c);
-    turn[tok][p] = make_float2(c, a.sign * s);
+    turn[i] = make_float2(c, a.sign * s);
   }
-  __syncthreads();
 
-  // this thread's chunk within the rows, and the pair, side and partner of its features
-  const int cpr = a.D / N, rows = kRotThreads / cpr;
-  const int c = tid % cpr, r0 = tid / cpr;
-  if (r0 >= rows) return;
-  int pair[N], other[N];  // other: elements to the partner (kAnywhere: of each feature)
-#pragma unroll
-  for (int e = 0; e < N; ++e) {
-    const int d = N * c + e;
-    pair[e] = -1;
-    other[e] = 0;
-    if (d >= 2 * np) continue;
+  // This thread's unit of a row: its first feature (kChunk: of the first half, the
+  // second `apart` features on), its first pair, how many of its features turn.
+  const int units = MODE == kChunk ? np / N + (a.D - 2 * np) / N : a.D / N;
+  const int per_pass = kRotThreads / units;
+  const int u = tid % units, r0 = tid / units;
+  int d0 = N * u, apart = 0, pair0 = N * u / 2, turns = min(max(2 * np - N * u, 0), N);
+  if constexpr (MODE == kChunk) {
     int lo = 0, hi = np;
     if (!a.shared) {
 #pragma unroll
       for (int j = 0; j < kRotAxes; ++j)
-        if (j < a.axes && d >= 2 * a.first_pair[j] && d < 2 * a.first_pair[j + 1]) {
+        if (j < a.axes && N * u >= a.first_pair[j] && N * u < a.first_pair[j + 1]) {
           lo = a.first_pair[j];
           hi = a.first_pair[j + 1];
         }
     }
-    const int in = d - 2 * lo, half = hi - lo;
-    if (a.interleaved) {
-      pair[e] = lo + in / 2;
-      other[e] = in & 1 ? -1 : 1;
-    } else {
-      pair[e] = lo + (in < half ? in : in - half);
-      other[e] = in < half ? half : -half;
-    }
+    pair0 = N * u;
+    turns = N * u < np ? N : 0;
+    d0 = turns ? lo + N * u : N * u + np;
+    apart = hi - lo;
   }
-  const int h_end = min((int)(blockIdx.y + 1) * a.heads_per_wg, a.heads[1]);
-  for (int tok = 0; tok < nt; ++tok) {
-    const int64_t n = n0 + tok, b = n / a.T, t = n - b * a.T;
-    float co[N], si[N];  // out = x co + partner si
+  int pair[MODE == kAnywhere ? N : 1], other[MODE == kAnywhere ? N : 1];  // of each feature, elements to its partner
+  if constexpr (MODE == kAnywhere) {
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-      const float2 cs = pair[e] < 0 ? make_float2(1.f, 0.f) : turn[tok][pair[e]];
-      co[e] = cs.x;
-      si[e] = other[e] > 0 ? -cs.y : cs.y;
+      const int d = d0 + e;
+      int lo = 0, hi = np;
+      if (!a.shared) {
+#pragma unroll
+        for (int j = 0; j < kRotAxes; ++j)
+          if (j < a.axes && d >= 2 * a.first_pair[j] && d < 2 * a.first_pair[j + 1]) {
+            lo = a.first_pair[j];
+            hi = a.first_pair[j + 1];
+          }
+      }
+      const int in = d - 2 * lo, half = hi - lo;
+      const bool first = a.interleaved ? !(in & 1) : in < half;
+      pair[e] = d < 2 * np ? lo + (a.interleaved ? in / 2 : first ? in : in - half) : 0;
+      other[e] = d < 2 * np ? (a.interleaved ? 1 : half) * (first ? 1 : -1) : 0;
     }
-#pragma unroll 2
-    for (int h = blockIdx.y * a.heads_per_wg + r0; h < h_end; h += rows) {
+  }
+  __syncthreads();
+  if (r0 >= per_pass) return;
+
+  const int h0 = blockIdx.y * a.heads_per_wg, nh = min(a.heads_per_wg, a.heads[1] - h0);
+  const int last = nt * nh;
+  for (int i0 = r0; i0 < last; i0 += ROWS * per_pass) {
+    Raw v[ROWS][CH];
+    char* to[ROWS];
+    int tok[ROWS];
+    float o[ROWS][MODE == kAnywhere ? N : 1];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const int row = i0 + i * per_pass;
+      if (row >= last) break;
+      tok[i] = row / nh;
+      const int h = h0 + row - tok[i] * nh, n = n0 + tok[i], b = n / a.T, t = n - b * a.T;
       const int w = h >= a.heads[0], hh = w ? h - a.heads[0] : h, H = w ? a.heads[1] - a.heads[0] : a.heads[0];
-      const char* row = a.x[w] + b * a.sb[w] + t * a.st[w] + hh * a.sh[w];
-      const char* px = row + (int64_t)c * N * SZ;
-      float v[N], o[N];
-      RotChunk<E, N>::get(px, v);
+      const char* px = a.x[w] + b * a.sb[w] + t * a.st[w] + hh * a.sh[w] + d0 * SZ;
+      to[i] = a.y[w] + (((int64_t)n * H + hh) * a.D + d0) * SZ;
+      v[i][0] = *(const Raw*)px;
+      if constexpr (MODE == kChunk)
+        if (turns) v[i][1] = *(const Raw*)(px + apart * SZ);
+      if constexpr (MODE == kAnywhere)
+#pragma unroll
+        for (int e = 0; e < N; ++e) One::get(*(const typename One::raw*)(px + (e + other[e]) * SZ), o[i] + e);
+    }
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      if (i0 + i * per_pass >= last) break;
+      const float2* cs = turn + tok[i] * np;
+      if (turns == 0) {  // features that are not rotated pass whatever they hold
+        *(Raw*)to[i] = v[i][0];
+        continue;
+      }
+      float x[N], y[N];
+      C::get(v[i][0], x);
       if constexpr (MODE == kInChunk) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) o[e] = v[e ^ 1];
+        for (int e = 0; e < N; e += 2) {
+          const float2 k = cs[pair0 + min(e, turns - 2) / 2];
+          y[e] = e < turns ? fmaf(x[e], k.x, -x[e + 1] * k.y) : x[e];
+          y[e + 1] = e < turns ? fmaf(x[e + 1], k.x, x[e] * k.y) : x[e + 1];
+        }
       } else if constexpr (MODE == kChunk) {
-        RotChunk<E, N>::get(px + (int64_t)other[0] * SZ, o);
+        float z[N], q[N];
+        C::get(v[i][1], z);
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const float2 k = cs[pair0 + e];
+          y[e] = fmaf(x[e], k.x, -z[e] * k.y);
+          q[e] = fmaf(z[e], k.x, x[e] * k.y);
+        }
+        *(Raw*)(to[i] + apart * SZ) = C::put(q);
       } else {
 #pragma unroll
-        for (int e = 0; e < N; ++e) RotChunk<E, 1>::get(px + (int64_t)(e + other[e]) * SZ, o + e);
+        for (int e = 0; e < N; ++e) {
+          const float2 k = cs[pair[e]];
+          const float s = other[e] > 0 ? -k.y : k.y;
+          y[e] = e < turns ? fmaf(x[e], k.x, o[i][e] * s) : x[e];
+        }
       }
-#pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const float y = fmaf(v[e], co[e], o[e] * si[e]);
-        v[e] = pair[e] < 0 ? v[e] : y;  // a feature that is not rotated passes whatever it holds
-      }
-      RotChunk<E, N>::put(a.y[w] + ((n * H + hh) * a.D + (int64_t)c * N) * SZ, v);
+      *(Raw*)to[i] = C::put(y);
     }
   }
 }
 
 template <typename E, int N, int MODE>
-static int launch_rotary(const RotaryArgs& a, int64_t blocks, hipStream_t s) {
-  const int64_t most = 0xffffffffLL / kRotThreads;  // work-items of a launch: 32 bits
-  const unsigned gy = (unsigned)((a.heads[1] + a.heads_per_wg - 1) / a.heads_per_wg);
-  for (int64_t b = 0; b < blocks; b += most) {
-    RotaryArgs args = a;
-    args.block0 = b;
-    launch_kernel<rotary_kernel<E, N, MODE>>(dim3((unsigned)std::min(most, blocks - b), gy), dim3(kRotThreads), 0, s,
-                                             args);
-  }
+static int launch_rotary(RotaryArgs& a, hipStream_t s) {
+  // Tokens of a workgroup: enough for a round or more of its threads' rows; where
+  // that leaves few workgroups, fewer, and the heads of one spread over several.
+  const int64_t np = a.first_pair[a.axes], rows = a.heads[1];
+  const int64_t units = MODE == kChunk ? np / N + (a.D - 2 * np) / N : a.D / N, per_pass = kRotThreads / units;
+  const int64_t want = 1024, full = (8 / (MODE == kChunk ? 2 : 1) * per_pass + rows - 1) / rows;
+  a.per_wg = (int)std::clamp<int64_t>(std::min<int64_t>(full, a.tokens / want), 1, kRotTokens);
+  const int64_t blocks = (a.tokens + a.per_wg - 1) / a.per_wg;
+  const int64_t gy = std::clamp<int64_t>(want / blocks, 1, (rows + per_pass - 1) / per_pass);
+  a.heads_per_wg = (int)((rows + gy - 1) / gy);
+  if (blocks > 0xffffffffLL / kRotThreads) return fail(PJX_ERR_INVALID, "pjx_rotary: too many tokens");
+  const dim3 grid((unsigned)blocks, (unsigned)((rows + a.heads_per_wg - 1) / a.heads_per_wg));
+  launch_kernel<rotary_kernel<E, N, MODE>>(grid, dim3(kRotThreads), 0, s, a);
   return check_launch("pjx_rotary");
 }
 
 template <typename E, int N>
-static int run_rotary(const RotaryArgs& a, int mode, bool chunks, int64_t blocks, hipStream_t s) {
-  if (!chunks) return launch_rotary<E, 1, kAnywhere>(a, blocks, s);
-  if (mode == kInChunk) return launch_rotary<E, N, kInChunk>(a, blocks, s);
-  if (mode == kChunk) return launch_rotary<E, N, kChunk>(a, blocks, s);
-  return launch_rotary<E, N, kAnywhere>(a, blocks, s);
+static int run_rotary(RotaryArgs& a, int mode, bool chunks, hipStream_t s) {
+  if (!chunks) return launch_rotary<E, 1, kAnywhere>(a, s);
+  if (mode == kInChunk) return launch_rotary<E, N, kInChunk>(a, s);
+  if (mode == kChunk) return launch_rotary<E, N, kChunk>(a, s);
+  return launch_rotary<E, N, kAnywhere>(a, s);
 }
 
 }  // namespace pjx
@@ -227,7 +279,7 @@ extern "C" int pjx_rotary(int dtype, const void* q, const void* k, void* q_out, 
     return bad("dtype must be PJX_DTYPE_BF16, PJX_DTYPE_F16 or PJX_DTYPE_F32");
   if (position_type < PJX_POSITION_I32 || position_type > PJX_POSITION_F64) return bad("position type");
   if (batch < 0 || len < 0 || q_heads < 0 || k_heads < 0 || head_dim < 1 || head_dim > 256 ||
-      q_heads + k_heads > (1 << 20) || batch > (1 << 30) || len > (1 << 30) || batch * len > ((int64_t)1 << 40))
+      q_heads + k_heads > (1 << 20) || batch > (1 << 30) || len > (1 << 30) || batch > 0x7fffffffLL / std::max<int64_t>(len, 1))
     return bad("sizes out of range (head_dim at most 256)");
   if (axes < 1 || axes > kRotAxes || !sections) return bad("1 to 4 axes");
   if (!(base > 0.0) || base > 1e300) return bad("base must be a positive number");
@@ -278,10 +330,13 @@ extern "C" int pjx_rotary(int dtype, const void* q, const void* k, void* q_out, 
   a.axes = (int)axes;
   a.T = (int)len;
   a.D = (int)d;
-  a.tokens = batch * len;
+  a.tokens = (int)(batch * len);
   a.interleaved = interleaved != 0;
   a.shared = shared_spectrum != 0;
-  a.log2_base = log2(base);
+  for (int i = 0; i < axes; ++i) {
+    const int pairs = a.shared ? width / 2 : sections[i] / 2;
+    a.rate[i] = pairs > 0 ? -log2(base) / pairs : 0.0;
+  }
   a.sign = inverse ? -1.f : 1.f;
   int mode = kInChunk;
   if (!a.interleaved) {
@@ -292,16 +347,8 @@ extern "C" int pjx_rotary(int dtype, const void* q, const void* k, void* q_out, 
       for (int i = 0; i < axes; ++i) whole = whole && sections[i] / 2 % n == 0;
     mode = whole ? kChunk : kAnywhere;
   }
-  // Few tokens: a workgroup takes one, and their heads spread over several.
-  const int64_t want = 1024;
-  a.per_wg = (int)std::clamp<int64_t>(a.tokens / want, 1, kRotTokens);
-  const int64_t blocks = (a.tokens + a.per_wg - 1) / a.per_wg;
-  const int rows_per_pass = std::max<int>(1, kRotThreads / (int)(chunks ? d / n : d));
-  const int64_t most_y = (rows + rows_per_pass - 1) / rows_per_pass;
-  const int64_t gy = std::clamp<int64_t>(want / blocks, 1, most_y);
-  a.heads_per_wg = (int)((rows + gy - 1) / gy);
   hipStream_t s = (hipStream_t)stream;
-  if (f32) return run_rotary<F32Fmt, 4>(a, mode, chunks, blocks, s);
-  return dtype == PJX_DTYPE_F16 ? run_rotary<F16Fmt, 8>(a, mode, chunks, blocks, s)
-                                : run_rotary<Bf16Fmt, 8>(a, mode, chunks, blocks, s);
+  if (f32) return run_rotary<F32Fmt, 4>(a, mode, chunks, s);
+  return dtype == PJX_DTYPE_F16 ? run_rotary<F16Fmt, 8>(a, mode, chunks, s)
+                                : run_rotary<Bf16Fmt, 8>(a, mode, chunks, s);
 }
