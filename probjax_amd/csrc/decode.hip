@@ -336,6 +336,19 @@ size_t ws_size(int64_t batch, int64_t groups, int64_t rows, int64_t kv_len,
   return (size_t)(parts * v_dim + parts * 2) * sizeof(float);
 }
 
+// At most kFewChunks partials a row (wide drafts, tree_wide.hip): the merge above
+// issues the loads of 16 whatever there is (8192 rows of 128, 4 chunks: 8 us for 5).
+__global__ __launch_bounds__(kMergeThreads) void decode_merge_few_kernel(DecodeArgs a) {
+  merge_chunks<kFewChunks>(a, (long)blockIdx.x * kMergeThreads + threadIdx.x);
+}
+
+int launch_merge_few(const DecodeArgs& a, hipStream_t stream, const char* name) {
+  const long merge_threads = (long)a.B * a.G * a.rows * (a.orow / 4);
+  launch_kernel<decode_merge_few_kernel>(dim3((unsigned)((merge_threads + kMergeThreads - 1) / kMergeThreads)),
+                     dim3(kMergeThreads), 0, stream, a);
+  return check_launch(name);
+}
+
 int launch_decode_merge(const DecodeArgs& a, hipStream_t stream, const char* name) {
   const long merge_threads = (long)a.B * a.G * a.rows * (a.orow / 4);
   launch_kernel<decode_merge_kernel>(dim3((unsigned)((merge_threads + kMergeThreads - 1) / kMergeThreads)),

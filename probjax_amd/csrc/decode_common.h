@@ -123,17 +123,26 @@ __device__ __forceinline__ void build_tree(const DecodeArgs& a, int b, TreeTable
       __syncthreads();
     }
   } else {
+    // 64 bytes of a row a time, the loads of 8 of them issued before the first is used
     const uint8_t* m = a.tree_mask + (size_t)b * a.tree_step;
-    const int lane = tid & 63;
-    for (int t = tid >> 6; t < T; t += kDecThreads / 64)
-      for (int i = 0; i < (T + 63) / 64; ++i) {
-        const int j = 64 * i + lane;
-        const uint64_t seen = __builtin_amdgcn_ballot_w64(j < T && m[(size_t)t * T + j] != 0);
-        if (lane == 0) {
-          tt.bits[t][2 * i] = (uint32_t)seen;
-          tt.bits[t][2 * i + 1] = (uint32_t)(seen >> 32);
+    const int lane = tid & 63, per_row = (T + 63) / 64, n = T * per_row;
+    for (int i0 = tid >> 6; i0 < n; i0 += 8 * (kDecThreads / 64)) {
+      uint8_t x[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int i = i0 + u * (kDecThreads / 64), t = i / per_row, j = 64 * (i - t * per_row) + lane;
+        x[u] = i < n && j < T ? m[t * T + j] : 0;
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int i = i0 + u * (kDecThreads / 64), t = i / per_row, w = 2 * (i - t * per_row);
+        const uint64_t seen = __builtin_amdgcn_ballot_w64(x[u] != 0);
+        if (lane == 0 && i < n) {
+          tt.bits[t][w] = (uint32_t)seen;
+          tt.bits[t][w + 1] = (uint32_t)(seen >> 32);
         }
       }
+    }
     __syncthreads();
   }
 }
@@ -995,6 +1004,7 @@ __device__ __forceinline__ void gqa_decode_f32(const DecodeArgs& a) {
 // LSE = +inf (attention_xla.py:417-420).
 constexpr int kMergeThreads = 128;
 constexpr int kMergeBatch = 16;
+template <int BATCH = kMergeBatch>
 __device__ __forceinline__ void merge_chunks(const DecodeArgs& a, long gid) {
   const int nq = a.orow / 4;
   const long item = gid / nq;
@@ -1017,11 +1027,11 @@ __device__ __forceinline__ void merge_chunks(const DecodeArgs& a, long gid) {
       make_rsrc(a.lengths, a.lengths ? (uint32_t)a.B * 4u : 0u), b * 4, 0, 0);
   float M = kMaxInit, den = 0.f;
   f32x4 num = {0.f, 0.f, 0.f, 0.f};
-  float mv[kMergeBatch], lv[kMergeBatch];
-  f32x4 ov[kMergeBatch];
+  float mv[BATCH], lv[BATCH];
+  f32x4 ov[BATCH];
   auto load_batch = [&](int c0) {
 #pragma unroll
-    for (int i = 0; i < kMergeBatch; ++i) {
+    for (int i = 0; i < BATCH; ++i) {
       const size_t c = (size_t)min(c0 + i, a.nch - 1);
       mv[i] = ml[c * ml_stride];
       lv[i] = ml[c * ml_stride + 1];
@@ -1032,14 +1042,14 @@ __device__ __forceinline__ void merge_chunks(const DecodeArgs& a, long gid) {
   auto add_batch = [&](int c0, int n) {
     float bm = M;
 #pragma unroll
-    for (int i = 0; i < kMergeBatch; ++i)
+    for (int i = 0; i < BATCH; ++i)
       if (c0 + i < n) bm = fmaxf(bm, mv[i]);
     const float sc = fast_exp2(M - bm);
     M = bm;
     den *= sc;
     num *= sc;
 #pragma unroll
-    for (int i = 0; i < kMergeBatch; ++i) {
+    for (int i = 0; i < BATCH; ++i) {
       if (c0 + i < n) {
         const float wt = fast_exp2(mv[i] - M);
         den = fmaf(wt, lv[i], den);
@@ -1052,7 +1062,7 @@ __device__ __forceinline__ void merge_chunks(const DecodeArgs& a, long gid) {
   const int n = (L + a.chunk - 1) / a.chunk;
   if (n == 1) return;  // the chunk kernel wrote this row's output
   add_batch(0, n);
-  for (int c0 = kMergeBatch; c0 < n; c0 += kMergeBatch) {
+  for (int c0 = BATCH; c0 < n; c0 += BATCH) {
     load_batch(c0);
     add_batch(c0, n);
   }
@@ -1095,6 +1105,9 @@ int run_tree_wide(DecodeArgs& a, int head_dim, bool auto_chunk_size, void* ws, s
                   const char* who);
 // Merges the chunk partials of a decode whose chunk kernel was launched with `a`.
 int launch_decode_merge(const DecodeArgs& a, hipStream_t stream, const char* name);
+// The same where a row has at most kFewChunks partials.
+constexpr int kFewChunks = 4;
+int launch_merge_few(const DecodeArgs& a, hipStream_t stream, const char* name);
 
 // Launches chunk kernel K over the work items of `a`, whose partials it places
 // in the workspace.

@@ -1,15 +1,20 @@
 // Tree attention for drafts of many rows (tree_decode.hip takes few): 16 bits,
 // head dims 64 and 128.  With R = (Hq/Hkv)*T rows a key costs 4 D R operations
 // and 4 D bytes, so from some 64 rows on the key loop is a flash forward's: one
-// workgroup owns 32 * RW rows and a chunk of keys, whose K and V tiles all of its
-// waves share in LDS.  Each wave owns 32 rows (RW of the 4 waves different ones;
-// the 4 / RW waves of the same rows take different 32-key blocks of a tile and
-// are joined at the end).  The narrow kernel gives each wave keys of its own and
-// all rows, 16 at a time: it reads K and V without LDS, but its accumulators of
-// 64 rows leave one wave per SIMD, and every further 64 rows read the cache again.
+// workgroup owns 32 RW rows and a chunk of keys, whose K and V tiles all of its
+// RW KG waves share in LDS.  Each wave owns 32 rows (KG waves the same ones: they
+// take different 32-key blocks of a tile and are joined at the end); the scores of
+// the next tile are formed beside this one's exponentials.  The narrow kernel gives
+// each wave keys of its own and all rows, 16 at a time: it reads K and V without
+// LDS, but its accumulators of 64 rows leave one wave per SIMD, and every further
+// 64 rows read the cache again (1 / 16 / 8 sequences of the table at the launch:
+// 55 / 128 / 296 us for 19 / 76 / 58).
 //
 // Row groups of one work item are placed 8 workgroups apart, on one XCD, whose
-// L2 gives all but the first their K and V.
+// L2 gives all but the first their K and V (HBM traffic of 244 rows, two groups:
+// that of one).  Bound by latency on one sequence (launch, lengths, first tile,
+// table and four tiles in turn: 16 us), by HBM on 16 (285 MB in 68 us), by the waves'
+// chains of a tile (1.5 us for two) and the partial results on the widest.
 #include "decode_common.h"
 #include "flash_common.h"
 
@@ -26,15 +31,17 @@ __device__ __forceinline__ uint32_t tree_bits(const TreeTable& tt, int t, int j)
   return s ? word(j >> 5) >> s | word((j >> 5) + 1) << (32 - s) : word(j >> 5);
 }
 
-template <typename E, int D, int RW>
-__global__ __launch_bounds__(256, 2) void tree_wide_kernel(DecodeArgs a, int groups) {
+template <typename E, int D, int RW, int KG>
+__global__ __launch_bounds__(64 * RW * KG, 2) void tree_wide_kernel(DecodeArgs a, int groups) {
   using T = Bf16Tile<D>;
-  constexpr int BK = T::BK, ROWB = T::ROWB, TILE_B = T::TILE_B, STAGE_B = T::STAGE_B;
-  constexpr int KG = 4 / RW;       // waves of the same rows
-  constexpr int NB = BK / 32 / KG;  // 32-key blocks of a wave's tile
-  static_assert(BK == kWideKeys && NB >= 1, "tile");
-  __shared__ __attribute__((aligned(1024))) unsigned char smem0[STAGE_B];
-  __shared__ __attribute__((aligned(1024))) unsigned char smem1[STAGE_B];
+  constexpr int BK = T::BK, ROWB = T::ROWB, TILE_B = T::TILE_B;
+  constexpr int NB = BK / 32 / KG;        // 32-key blocks of a wave's tile
+  constexpr int NW = RW * KG, RPW = BK / NW;  // waves, rows of a tile that each loads
+  constexpr int NLD = RPW / T::RPI;
+  static_assert(BK == kWideKeys && NB >= 1 && NLD * T::RPI == RPW, "tile");
+  // (objects of their own: the compiler waits for every load in flight before it
+  // reads an object that one of them writes)
+  __shared__ __attribute__((aligned(1024))) unsigned char k_lds0[TILE_B], k_lds1[TILE_B], v_lds0[TILE_B], v_lds1[TILE_B];
   __shared__ TreeTable tree;
   __shared__ int sched[4 + 2 * kSchedMaxBatch];
 
@@ -47,33 +54,16 @@ __global__ __launch_bounds__(256, 2) void tree_wide_kernel(DecodeArgs a, int gro
   if (!decode_item(a, sched, b, g, chunk_id, L, item)) return;
   const int c0 = chunk_id * a.chunk, c1 = min(c0 + a.chunk, L);
   const int P = prefix_len(a, b);
-  if (c1 > P) build_tree(a, b, tree);
-
   const int rdim = a.orow;
-  const int row = rg * 32 * RW + 32 * rw + col;
-  const bool row_in = row < a.rows;
-  int tok = 0, h = 0;
-  if (row_in) row_to_head(a, g, row, tok, h);
-  typename E::v8 qf[D / 16];
-  {
-    const uint16_t* qrow = a.q + ((size_t)(b * a.Lq + tok) * a.Hq + h) * rdim;
-#pragma unroll
-    for (int s = 0; s < D / 16; ++s) {
-      u32x4 raw = {0u, 0u, 0u, 0u};
-      if (row_in && 16 * s + 8 * half < rdim) raw = *(const u32x4*)(qrow + 16 * s + 8 * half);
-      qf[s] = E::as8(raw);
-    }
-  }
-
   // Loads: the tile's first token is the buffer's base, so offsets within a tile
   // stay below 64 token strides (the launcher checks 32 bits).
   const uint32_t krow = (uint32_t)a.k_t * 2, vrow = (uint32_t)a.v_t * 2;
   const unsigned char* Kb = (const unsigned char*)(a.k + b * a.k_b + g * a.k_h);
   const unsigned char* Vb = (const unsigned char*)(a.v + b * a.v_b + g * a.v_h);
-  uint32_t voffK[T::NLD], voffV[T::NLD];
+  uint32_t voffK[NLD], voffV[NLD];
 #pragma unroll
-  for (int j = 0; j < T::NLD; ++j) {
-    const int r = 16 * w + T::RPI * j + lane / T::NC, slot = lane % T::NC;
+  for (int j = 0; j < NLD; ++j) {
+    const int r = RPW * w + T::RPI * j + lane / T::NC, slot = lane % T::NC;
     voffK[j] = row_chunk(r, krow, slot ^ T::swz_k(r), rdim);
     voffV[j] = row_chunk(r, vrow, slot ^ T::swz_v(r), rdim);
   }
@@ -97,28 +87,61 @@ __global__ __launch_bounds__(256, 2) void tree_wide_kernel(DecodeArgs a, int gro
   float m_run = kMaxInit, l_run = 0.f;
 
   const int n_tiles = (c1 - c0 + BK - 1) / BK;
-  auto issue = [&](int t, unsigned char* ks) {
+  auto issue = [&](const unsigned char* base, int64_t stride, uint32_t row_b, const uint32_t* voff, int t,
+                   unsigned char* dst) {
+    if (t >= n_tiles) return;
     const int k0 = c0 + t * BK, nvalid = min(BK, c1 - k0);
-    const rsrc_t rk = make_rsrc(Kb + (size_t)k0 * a.k_t * 2, (uint32_t)(nvalid - 1) * krow + rdim * 2);
-    const rsrc_t rv = make_rsrc(Vb + (size_t)k0 * a.v_t * 2, (uint32_t)(nvalid - 1) * vrow + rdim * 2);
+    const rsrc_t rs = make_rsrc(base + (size_t)k0 * stride * 2, (uint32_t)(nvalid - 1) * row_b + rdim * 2);
 #pragma unroll
-    for (int j = 0; j < T::NLD; ++j) {
-      const int r0 = 16 * w + T::RPI * j;
-      buffer_load_lds16(rk, ks + r0 * ROWB, voffK[j]);
-      buffer_load_lds16(rv, ks + TILE_B + r0 * ROWB, voffV[j]);
+    for (int j = 0; j < NLD; ++j) buffer_load_lds16(rs, dst + (RPW * w + T::RPI * j) * ROWB, voff[j]);
+  };
+  auto issue_k = [&](int t, unsigned char* dst) { issue(Kb, a.k_t, krow, voffK, t, dst); };
+  auto issue_v = [&](int t, unsigned char* dst) { issue(Vb, a.v_t, vrow, voffV, t, dst); };
+
+  // Tile t lives in stage t % 2; K is loaded one tile ahead of V.  The first tile
+  // comes while the queries do and the table is built.
+  issue_k(0, k_lds0);
+  issue_v(0, v_lds0);
+  issue_k(1, k_lds1);
+  const int row = rg * 32 * RW + 32 * rw + col;
+  const bool row_in = row < a.rows;
+  int tok = 0, h = 0;
+  if (row_in) row_to_head(a, g, row, tok, h);
+  typename E::v8 qf[D / 16];
+  {
+    const uint16_t* qrow = a.q + ((size_t)(b * a.Lq + tok) * a.Hq + h) * rdim;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) {
+      u32x4 raw = {0u, 0u, 0u, 0u};
+      if (row_in && 16 * s + 8 * half < rdim) raw = *(const u32x4*)(qrow + 16 * s + 8 * half);
+      qf[s] = E::as8(raw);
+    }
+  }
+
+  if (c1 > P) build_tree(a, b, tree);
+
+  auto scores = [&](const unsigned char* ks, f32x16* s) {
+#pragma unroll
+    for (int kb = 0; kb < NB; ++kb) {
+      s[kb] = f32x16{};
+#pragma unroll
+      for (int st = 0; st < D / 16; ++st) {
+        const typename E::v8 kf = E::as8(*(const u32x4*)(ks + (kg * NB + kb) * 32 * ROWB + offK[st]));
+        s[kb] = E::mma32(kf, qf[st], s[kb]);
+      }
     }
   };
-
-  auto compute = [&](int t, unsigned char* ks) {
+  // Tile t's softmax and products with V, and beside them the scores of tile t + 1
+  // (of whatever its slot holds past the last tile).
+  auto compute = [&](int t, f32x16* s, unsigned char* vs, const unsigned char* next, f32x16* sn) {
     const int k0 = c0 + t * BK;
-    unsigned char* vs = ks + TILE_B;
     const bool tail = k0 + BK > P;
     bool unbounded = false;  // as in gqa_decode
     if (tail) {
       bool any = false;
 #pragma unroll
-      for (int i = 0; i < TILE_B / (16 * 256); ++i) {
-        u32x4* p = (u32x4*)(vs + 16 * (tid + 256 * i));
+      for (int i = 0; i < TILE_B / (16 * 64 * NW); ++i) {
+        u32x4* p = (u32x4*)(vs + 16 * (tid + 64 * NW * i));
         u32x4 x = *p;
         bool odd = false;
 #pragma unroll
@@ -131,16 +154,6 @@ __global__ __launch_bounds__(256, 2) void tree_wide_kernel(DecodeArgs a, int gro
         any |= odd;
       }
       unbounded = __syncthreads_or(any);
-    }
-    f32x16 s[NB];
-#pragma unroll
-    for (int kb = 0; kb < NB; ++kb) {
-      s[kb] = f32x16{};
-#pragma unroll
-      for (int st = 0; st < D / 16; ++st) {
-        const typename E::v8 kf = E::as8(*(const u32x4*)(ks + (kg * NB + kb) * 32 * ROWB + offK[st]));
-        s[kb] = E::mma32(kf, qf[st], s[kb]);
-      }
     }
     // Register r of block kb holds key k0 + 32 (kg NB + kb) + 8 (r / 4) + 4 half + r % 4.
     if (tail || k0 + BK > c1) {
@@ -171,16 +184,20 @@ __global__ __launch_bounds__(256, 2) void tree_wide_kernel(DecodeArgs a, int gro
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[i][r] *= corr;
     }
-    float rs = 0.f;
+    scores(next, sn);
+    float rs0 = 0.f, rs1 = 0.f;
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float p = fast_exp2(fmaf(s[kb][r], a.cx, -m_run));
-        rs += p;
-        s[kb][r] = p;
+      for (int r = 0; r < 16; r += 2) {
+        const float p0 = fast_exp2(fmaf(s[kb][r], a.cx, -m_run));
+        const float p1 = fast_exp2(fmaf(s[kb][r + 1], a.cx, -m_run));
+        rs0 += p0;
+        rs1 += p1;
+        s[kb][r] = p0;
+        s[kb][r + 1] = p1;
       }
-    l_run += rs;
+    l_run += rs0 + rs1;
     typename E::v8 pf[2 * NB];
 #pragma unroll
     for (int c = 0; c < 2 * NB; ++c) {
@@ -232,33 +249,42 @@ __global__ __launch_bounds__(256, 2) void tree_wide_kernel(DecodeArgs a, int gro
     }
   };
 
-  // Tile t lives in stage t % 2, loaded while tile t - 1 is computed.
-  issue(0, smem0);
+  f32x16 sa[NB], sb[NB];
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  scores(k_lds0, sa);
+  // Iteration t: K of tile t + 1 and V of tile t have landed; K of tile t + 2 takes
+  // the place of tile t's, V of tile t + 1 that of tile t - 1's.
   for (int t = 0; t < n_tiles; t += 2) {
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    if (t + 1 < n_tiles) issue(t + 1, smem1);
-    compute(t, smem0);
+    issue_k(t + 2, k_lds0);
+    issue_v(t + 1, v_lds1);
+    compute(t, sa, v_lds0, k_lds1, sb);
     if (t + 1 >= n_tiles) break;
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    if (t + 2 < n_tiles) issue(t + 2, smem0);
-    compute(t + 1, smem1);
+    issue_k(t + 3, k_lds1);
+    issue_v(t + 2, v_lds0);
+    compute(t + 1, sb, v_lds1, k_lds0, sa);
   }
 
   if constexpr (KG > 1) {
     // Waves of the same rows: the second hands (max, sum, O) to the first
     // through LDS, in the same register layout.
-    static_assert(KG == 2 && (D / 32) * 4 * RW * 64 * 16 <= STAGE_B && RW * 64 * 8 <= STAGE_B, "hand-over");
+    static_assert(KG == 2 && RW <= 4 && (D / 32) * 4 * 64 * 16 == TILE_B && RW * 64 * 8 <= sizeof(TreeTable),
+                  "hand-over");
     __syncthreads();
-    f32x4* xo = (f32x4*)smem0 + rw * 64 + lane;
-    float* xml = (float*)smem1 + 2 * (rw * 64 + lane);
+    // (each wave's O in a tile's place of its own, (max, sum) in the table's)
+    unsigned char* own = rw == 0 ? v_lds0 : rw == 1 ? v_lds1 : rw == 2 ? k_lds0 : k_lds1;
+    f32x4* xo = (f32x4*)own + lane;
+    float* xml = (float*)&tree + 2 * (rw * 64 + lane);
     if (kg == 1) {
 #pragma unroll
       for (int i = 0; i < D / 32; ++i)
 #pragma unroll
         for (int r = 0; r < 16; r += 4)
-          xo[(4 * i + r / 4) * RW * 64] = f32x4{acc[i][r], acc[i][r + 1], acc[i][r + 2], acc[i][r + 3]};
+          xo[(4 * i + r / 4) * 64] = f32x4{acc[i][r], acc[i][r + 1], acc[i][r + 2], acc[i][r + 3]};
       xml[0] = m_run;
       xml[1] = l_run;
     }
@@ -270,7 +296,7 @@ __global__ __launch_bounds__(256, 2) void tree_wide_kernel(DecodeArgs a, int gro
     for (int i = 0; i < D / 32; ++i)
 #pragma unroll
       for (int r = 0; r < 16; r += 4) {
-        const f32x4 o1 = xo[(4 * i + r / 4) * RW * 64];
+        const f32x4 o1 = xo[(4 * i + r / 4) * 64];
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][r + j] = fmaf(acc[i][r + j], f0, o1[j] * f1);
       }
@@ -315,7 +341,8 @@ __global__ __launch_bounds__(256, 2) void tree_wide_kernel(DecodeArgs a, int gro
   }
 }
 
-template <typename E, int D, int RW>
+// (one item per sequence and head: the chunk kernel wrote every row)
+template <typename E, int D, int RW, int KG>
 static int launch_wide(DecodeArgs& a, void* ws, size_t ws_bytes, hipStream_t s, const char* who) {
   if (!ws || ws_bytes < ws_size(a.B, a.G, a.rows, a.Lk, a.dv, a.chunk))
     return fail(PJX_ERR_WORKSPACE, "tree decode: workspace missing or too small");
@@ -323,18 +350,19 @@ static int launch_wide(DecodeArgs& a, void* ws, size_t ws_bytes, hipStream_t s, 
   a.ws_ml = a.ws_o + (size_t)a.B * a.G * a.nch * a.rows * a.dv;
   const int64_t items = (int64_t)a.B * a.G * a.nch, groups = (a.rows + 32 * RW - 1) / (32 * RW);
   const int64_t blocks = (items + 7) / 8 * 8 * groups;
-  if (blocks > 0xffffffffLL / 256 || (int64_t)a.B * a.G * a.rows > 0x7fffffffLL)
+  if (blocks > 0xffffffffLL / (64 * RW * KG) || (int64_t)a.B * a.G * a.rows > 0x7fffffffLL)
     return fail(PJX_ERR_INVALID, "tree decode: grid too large");
-  launch_kernel<tree_wide_kernel<E, D, RW>>(dim3((unsigned)blocks), dim3(256), 0, s, a, (int)groups);
+  launch_kernel<tree_wide_kernel<E, D, RW, KG>>(dim3((unsigned)blocks), dim3(64 * RW * KG), 0, s, a, (int)groups);
   const int rc = check_launch(who);
-  return rc ? rc : launch_decode_merge(a, s, who);
+  if (rc || a.nch == 1) return rc;
+  return a.nch <= kFewChunks ? launch_merge_few(a, s, who) : launch_decode_merge(a, s, who);
 }
 
 template <typename E>
 static int run_wide(DecodeArgs& a, int d, int rw, void* ws, size_t n, hipStream_t s, const char* who) {
   if (d == 64)
-    return rw == 2 ? launch_wide<E, 64, 2>(a, ws, n, s, who) : launch_wide<E, 64, 4>(a, ws, n, s, who);
-  return rw == 2 ? launch_wide<E, 128, 2>(a, ws, n, s, who) : launch_wide<E, 128, 4>(a, ws, n, s, who);
+    return rw == 2 ? launch_wide<E, 64, 2, 2>(a, ws, n, s, who) : launch_wide<E, 64, 4, 2>(a, ws, n, s, who);
+  return rw == 2 ? launch_wide<E, 128, 2, 2>(a, ws, n, s, who) : launch_wide<E, 128, 4, 2>(a, ws, n, s, who);
 }
 
 bool tree_wide_takes(const DecodeArgs& a, int head_dim, bool f32) {
@@ -343,11 +371,20 @@ bool tree_wide_takes(const DecodeArgs& a, int head_dim, bool f32) {
 
 int run_tree_wide(DecodeArgs& a, int head_dim, bool auto_chunk_size, void* ws, size_t ws_bytes, hipStream_t s,
                   const char* who) {
-  const int rw = a.rows <= 64 ? 2 : 4;
+  // 128 rows a workgroup (of eight waves), unless they are fewer or would leave the
+  // device idle; else 64 (of four).  Chunks from 256 keys on, doubled while some
+  // workgroups per CU remain, one of eight waves or two of four: every chunk's
+  // partial results cost as much traffic as a key a row, written and read again.
+  // MI355X, us, chunk 256 / 512 / 1024 / 2048 / 4096, 8 KV heads of 128:
+  //   1 x 4096, 104 rows   64 rows 20 / 21 / 27 / 40 / 66      128 rows 21 / 25 / 36 / 59 (four waves)
+  //   16 x 8192, 64 rows   64 rows 107 / 91 / 82 / 77 / 99
+  //   8 x 4096, 244 rows   128 rows 115 / 80 / 71 / 58 / 83    (four waves: 91 / 72 / 61 / 68 / 106)
+  const int64_t pairs = (int64_t)a.B * a.G;
+  const int rw = a.rows <= 64 || pairs * ((a.Lk + 511) / 512) * ((a.rows + 127) / 128) < 512 ? 2 : 4;
   if (auto_chunk_size) {
-    const int64_t work = (int64_t)a.B * a.G * a.Lk * ((a.rows + 32 * rw - 1) / (32 * rw));
-    int64_t c = a.chunk;
-    while (c < 2048 && work / c > 768) c *= 2;
+    const int64_t work = pairs * a.Lk * ((a.rows + 32 * rw - 1) / (32 * rw)), most = rw == 2 ? 640 : 320;
+    int64_t c = std::max(a.chunk, 256);
+    while (c < 2048 && work / c > most) c *= 2;
     a.chunk = (int)c;
     a.nch = (int)std::max<int64_t>((a.Lk + c - 1) / c, 1);
   }
