@@ -734,20 +734,23 @@ class _RotaryFunction(torch.autograd.Function):
         ctx.save_for_backward(positions)
         ctx.options = options
         ctx.set_materialize_grads(False)
-        q, k = hip.rotary(q, k, positions, **options)
+        q, k = hip.rotary(q, k, positions, *options)
         return q if k is None else (q, k)
 
     @staticmethod
     def backward(ctx, dq, dk=None):
         (positions,) = ctx.saved_tensors
-        options = dict(ctx.options, inverse=not ctx.options["inverse"])
-        grads = [g for g in (dq, dk) if g is not None]
-        if not grads:
+        if dq is None and dk is None:
             return None, None, None, None
-        res = _RotaryFunction.apply(grads[0], grads[1] if len(grads) == 2 else None, positions, options)
-        if dq is None:
-            return None, res, None, None
-        return (*res, None, None) if len(grads) == 2 else (res, None, None, None)
+        *options, inverse = ctx.options
+        options = (*options, not inverse)
+        one, two = (dk, None) if dq is None else (dq, dk)
+        if _needs_grad(one) or (two is not None and _needs_grad(two)):
+            res = _RotaryFunction.apply(one, two, positions, options)
+            one, two = res if two is not None else (res, None)
+        else:
+            one, two = hip.rotary(one, two, positions, *options)
+        return (None, one, None, None) if dq is None else (one, two, None, None)
 
 
 def rotary(q, k, positions, *, sections=None, base: float = 10000.0, interleaved: bool = True,
@@ -775,15 +778,18 @@ def rotary(q, k, positions, *, sections=None, base: float = 10000.0, interleaved
     if q.ndim != 4 or (k is not None and k.ndim != 4):
         raise ValueError("rotary: q and k must be [B, T, H, D]")
     B, T, _, D = q.shape
-    if k is not None and ((k.shape[0], k.shape[1], k.shape[3]) != (B, T, D) or k.dtype != q.dtype):
-        raise ValueError(f"rotary: incompatible q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype}")
+    if k is not None:
+        Bk, Tk, _, Dk = k.shape
+        if Bk != B or Tk != T or Dk != D or k.dtype is not q.dtype:
+            raise ValueError(f"rotary: incompatible q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype}")
     if D > 256:
         raise ValueError(f"rotary: head dims up to 256, got {D}")
-    positions = torch.as_tensor(positions, device=q.device)
+    if not isinstance(positions, torch.Tensor) or positions.device != q.device:
+        positions = torch.as_tensor(positions, device=q.device)
     if positions.ndim == 1:
         positions = positions[:, None]
     A = positions.shape[-1] if positions.ndim else 0
-    if tuple(positions.shape) not in ((T, A), (B, T, A)) or not 1 <= A <= 4:
+    if positions.shape not in ((T, A), (B, T, A)) or not 1 <= A <= 4:
         raise ValueError(f"rotary: positions must be [{T}], [{T}, A] or [{B}, {T}, A] with 1 to 4 axes, got "
                          f"{tuple(positions.shape)}")
     if positions.requires_grad:
@@ -796,16 +802,17 @@ def rotary(q, k, positions, *, sections=None, base: float = 10000.0, interleaved
         if D % (2 * A):
             raise ValueError(f"rotary: {D} features do not divide into pairs of {A} axes; give sections")
         sections = (D // A,) * A
-    sections = tuple(int(x) for x in sections)
-    if len(sections) != A or any(x < 0 or x % 2 for x in sections) or sum(sections) > D:
-        raise ValueError(f"rotary: sections must be {A} even numbers that add up to at most {D}, got {sections}")
+    else:
+        sections = tuple(map(int, sections))
+        if len(sections) != A or min(sections) < 0 or sum(sections) > D or any(x & 1 for x in sections):
+            raise ValueError(f"rotary: sections must be {A} even numbers that add up to at most {D}, got {sections}")
     if not 0.0 < base < 1e300:
         raise ValueError(f"rotary: base must be positive, got {base}")
-    options = dict(sections=sections, base=float(base), interleaved=bool(interleaved),
-                   shared_spectrum=bool(shared_spectrum), inverse=False)
+    # sections, base, interleaved, shared_spectrum, inverse, as hip.rotary takes them
+    options = (sections, float(base), bool(interleaved), bool(shared_spectrum), False)
     if _needs_grad(q) or (k is not None and _needs_grad(k)):
         return _RotaryFunction.apply(q, k, positions, options)
-    y, z = hip.rotary(q, k, positions, **options)
+    y, z = hip.rotary(q, k, positions, *options)
     return y if z is None else (y, z)
 
 

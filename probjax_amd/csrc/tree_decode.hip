@@ -139,7 +139,8 @@ extern "C" int pjx_tree_decode(int dtype, const void* q, const void* k, const vo
   a.tree_step = trees == 1 ? 0 : parents ? q_len : q_len * q_len;
   const int d = (int)head_dim;
   if (tree_wide_takes(a, d, f32)) return run_tree_wide(a, d, chunk == 0, workspace, workspace_bytes, s, who);
-  const int nrb = gqa_row_blocks(a.rows, d, d, f32);
+  // (at most 32 rows, or rows too far apart in memory for the wide kernel)
+  const int nrb = std::min(gqa_row_blocks(a.rows, d, d, f32), 2);
   a.rpg = kRows * nrb;
   if (f32)
     return d == 64    ? run_tree_f32<64>(a, nrb, workspace, workspace_bytes, s, who)

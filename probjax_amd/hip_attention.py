@@ -9,6 +9,7 @@ device; nothing is copied between host and device.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from dataclasses import dataclass
 
@@ -609,59 +610,94 @@ def mla_project_bwd_supported(cache, wk, wv, width: int) -> bool:
             and cache.numel() > 0 and max(R, wk.shape[0] * width) <= 1 << 20)
 
 
-def _on_its_device(dev, entry, *args) -> None:
-    """``entry(*args)``, raising on an error, with ``dev`` as the current device
-    (a launch takes the current device's kernels)."""
-    if dev.index in (None, torch._C._cuda_getDevice()):
-        native.check(entry(*args))
+# The operators below take a few microseconds of kernels on small sizes, so their
+# host path is kept short: devices are compared by index, what is already as the
+# kernels need it is passed on after one look, and outputs shaped like an input
+# come from empty_like.
+
+def _gpu(*ts) -> int:
+    """Index of the ROCm device that all tensors (None: absent) are on."""
+    index = None
+    for t in ts:
+        if t is None:
+            continue
+        i = t.get_device() if isinstance(t, torch.Tensor) else -1
+        if i < 0 or (index is not None and i != index):
+            _on_device(*ts)  # says which
+        index = i
+    return index
+
+
+def _call(index: int, entry, *args) -> None:
+    """``entry(*args, stream)``, raising on an error, on the current stream of
+    device ``index`` and with it as the current device (a launch takes the current
+    device's kernels)."""
+    if index == torch._C._cuda_getDevice():
+        rc = entry(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(dev):
-            native.check(entry(*args))
+        with torch.cuda.device(index):
+            rc = entry(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        native.check(rc)
 
 
-def _int32(t, what: str, dev, shapes):
-    """``t`` as a contiguous int32 tensor on ``dev`` of one of ``shapes``."""
-    if not isinstance(t, torch.Tensor) or t.device != dev:
-        t = torch.as_tensor(t, device=dev)
-    if t.dtype.is_floating_point or t.dtype.is_complex or t.dtype == torch.bool:
-        raise ValueError(f"{what} must hold integers, got {t.dtype}")
-    if tuple(t.shape) not in shapes:
+def _int32(t, what: str, like, *shapes):
+    """``t`` as a contiguous int32 tensor on the device of ``like``, of one of
+    ``shapes``."""
+    if not (isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.get_device() == like.get_device()
+            and t.is_contiguous()):
+        t = torch.as_tensor(t, device=like.device)
+        if t.dtype.is_floating_point or t.dtype.is_complex or t.dtype == torch.bool:
+            raise ValueError(f"{what} must hold integers, got {t.dtype}")
+        t = t.to(torch.int32).contiguous()
+    if t.shape not in shapes:
         raise ValueError(f"{what} must have shape {' or '.join(map(str, shapes))}, got {tuple(t.shape)}")
-    return t.to(torch.int32).contiguous()
+    return t
+
+
+def _scratch(nbytes: int, like, workspace=None):
+    """``nbytes`` of workspace on the device of ``like``: ``workspace`` if it holds
+    them, else new."""
+    if workspace is None:
+        return like.new_empty((nbytes,), dtype=torch.uint8)
+    return _workspace(nbytes, like.device, workspace)
 
 
 def _cache_call(who: str, q, k, v):
-    """What the operators over a KV cache check and prepare alike: ``(dev, code,
-    width, row, q, k, v, strides)`` for 16-bit or float32 ``q [B, T, Hq, D]`` and
-    caches ``[B, S, Hkv, D]``.  ``width`` is the kernel's head dim and ``row``
-    the features of a row in memory; rows that no kernel takes as they lie are
-    zero-padded to the width, caches whose rows are no whole 16-byte chunks
-    copied, any other order of the caches' axes is read in place (``strides``)."""
-    dev = _on_device(q, k, v)
+    """What the operators over a KV cache check and prepare alike: ``(index, width,
+    row, q, k, v, strides)`` for 16-bit or float32 ``q [B, T, Hq, D]`` and caches
+    ``[B, S, Hkv, D]``.  ``width`` is the kernel's head dim and ``row`` the features
+    of a row in memory; rows that no kernel takes as they lie are zero-padded to the
+    width, caches whose rows are no whole 16-byte chunks copied, any other order of
+    the caches' axes is read in place (``strides``)."""
+    index = _gpu(q, k, v)
     if q.ndim != 4 or k.ndim != 4 or v.ndim != 4:
         raise ValueError(f"{who}: q must be [B, T, Hq, D], k and v [B, S, Hkv, D]")
     B, _, Hq, D = q.shape
-    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D or k.shape[2] < 1 or Hq < 1 or Hq % k.shape[2]:
+    Bk, _, Hkv, Dk = k.shape
+    if k.shape != v.shape or Bk != B or Dk != D or Hkv < 1 or Hq < 1 or Hq % Hkv:
         raise ValueError(f"{who}: incompatible shapes q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
-    if q.dtype not in _DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+    dtype = q.dtype
+    if dtype not in _DTYPES or k.dtype is not dtype or v.dtype is not dtype:
         raise ValueError(f"{who} takes bfloat16, float16 or float32 q, k and v of one dtype")
     if not 1 <= D <= 256:
         raise ValueError(f"{who}: head dims up to 256, got {D}")
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
         raise ValueError(f"{who} has no gradient: call it under torch.no_grad() or on detached tensors")
     width = 64 if D <= 64 else 128 if D <= 128 else 256
-    half = q.dtype != torch.float32
     row = D
-    if D != width and not (half and width < 256 and D % 8 == 0):
+    if D != width and (dtype is torch.float32 or width == 256 or D % 8):
         row = width
         q, k, v = (torch.nn.functional.pad(x, (0, width - D)) for x in (q, k, v))
-    q = _aligned(q.contiguous())
     strides = None
     if not (k.is_contiguous() and v.is_contiguous()):
         k, v = _whole_chunks(k), _whole_chunks(v)
         # (an axis of one element has a stride of no meaning)
         strides = native.CacheStrides(*(x.stride(i) if x.shape[i] > 1 else 0 for x in (k, v) for i in range(3)))
-    return dev, _DTYPES[q.dtype], width, row, q, _aligned(k), _aligned(v), strides
+    q = q.contiguous()
+    if (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16:
+        q, k, v = _aligned(q), _aligned(k), _aligned(v)
+    return index, width, row, q, k, v, strides
 
 
 def _whole_chunks(x):
@@ -681,37 +717,36 @@ def tree_decode(
     sequence's ``kv_lengths[b]`` keys (None: the last T slots).  The tree is
     ``parents`` (int ``[T]`` or ``[B, T]``) or ``tree_mask`` (bool ``[T, T]`` or
     ``[B, T, T]``)."""
-    dev, code, width, row, q, k, v, strides = _cache_call("tree attention", q, k, v)
-    B, T, Hq, D = q.shape
-    S, Hkv = k.shape[1], k.shape[2]
+    index, width, row, q, k, v, strides = _cache_call("tree attention", q, k, v)
+    B, T, Hq, _ = q.shape
+    _, S, Hkv, _ = k.shape
     if not 1 <= T <= 256:
         raise ValueError(f"tree attention takes 1 to 256 drafted tokens, got {T}")
     if (parents is None) == (tree_mask is None):
         raise ValueError("tree attention takes parents or tree_mask, and not both")
+    p = m = None
     if parents is not None:
-        parents = _int32(parents, "parents", dev, ((T,), (B, T)))
-        trees = 1 if parents.ndim == 1 else B
+        tree = _int32(parents, "parents", q, (T,), (B, T))
+        trees, p = (1 if tree.ndim == 1 else B), tree.data_ptr()
     else:
-        if not isinstance(tree_mask, torch.Tensor) or tree_mask.device != dev:
-            tree_mask = torch.as_tensor(tree_mask, device=dev)
-        if tree_mask.dtype not in (torch.bool, torch.uint8):
-            raise ValueError(f"tree_mask must be boolean, got {tree_mask.dtype}")
-        if tuple(tree_mask.shape) not in ((T, T), (B, T, T)):
-            raise ValueError(f"tree_mask must have shape {(T, T)} or {(B, T, T)}, got {tuple(tree_mask.shape)}")
-        tree_mask = tree_mask.contiguous()
-        trees = 1 if tree_mask.ndim == 2 else B
+        tree = torch.as_tensor(tree_mask, device=q.device)
+        if tree.dtype not in (torch.bool, torch.uint8):
+            raise ValueError(f"tree_mask must be boolean, got {tree.dtype}")
+        if tree.shape not in ((T, T), (B, T, T)):
+            raise ValueError(f"tree_mask must have shape {(T, T)} or {(B, T, T)}, got {tuple(tree.shape)}")
+        tree = tree.contiguous()
+        trees, m = (1 if tree.ndim == 2 else B), tree.data_ptr()
     if kv_lengths is None and S < T:
         raise ValueError(f"a cache of {S} slots does not hold {T} drafted tokens")
-    L = None if kv_lengths is None else _int32(kv_lengths, "kv_lengths", dev, ((B,),))
+    L = None if kv_lengths is None else _int32(kv_lengths, "kv_lengths", q, (B,))
     lib = native.load()
     nbytes = lib.pjx_decode_workspace_size(B, Hkv, (Hq // Hkv) * T, S, width, chunk)
-    ws = _workspace(nbytes, dev, workspace)
-    o = torch.empty((B, T, Hq, row), dtype=q.dtype, device=dev)
-    lse = torch.empty((B, Hq, T), dtype=torch.float32, device=dev) if return_lse else None
-    _on_its_device(
-        dev, lib.pjx_tree_decode, code, _ptr(q), _ptr(k), _ptr(v), _ptr(L), _ptr(parents), _ptr(tree_mask), trees,
-        _ptr(o), _ptr(lse), _ptr(ws), nbytes, B, T, S, Hq, Hkv, width, row, strides, float(sm_scale), int(chunk),
-        _stream(dev),
+    ws = _scratch(nbytes, q, workspace)
+    o = torch.empty_like(q)
+    lse = torch.empty((B, Hq, T), dtype=torch.float32, device=q.device) if return_lse else None
+    _call(
+        index, lib.pjx_tree_decode, _DTYPES[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(L), p, m, trees,
+        o.data_ptr(), _ptr(lse), ws.data_ptr(), nbytes, B, T, S, Hq, Hkv, width, row, strides, sm_scale, chunk,
     )
     return (o, lse) if return_lse else o
 
@@ -720,14 +755,15 @@ def tree_decode(
 WEIGHTED_DECODE_MAX_ROWS = 64
 
 
-def _key_weights(weights, shape, dev):
+def _key_weights(weights, like, B, H, S):
     if weights is None:
         return None
-    if not isinstance(weights, torch.Tensor) or weights.device != dev or weights.dtype != torch.float32:
-        raise ValueError(f"key weights must be a float32 tensor on {dev}")
-    if tuple(weights.shape) != shape:
-        raise ValueError(f"key weights must have shape {shape}, got {tuple(weights.shape)}")
-    return weights.detach().contiguous()
+    if not isinstance(weights, torch.Tensor) or weights.get_device() != like.get_device() \
+            or weights.dtype is not torch.float32:
+        raise ValueError(f"key weights must be a float32 tensor on {like.device}")
+    if weights.shape != (B, H, S):
+        raise ValueError(f"key weights must have shape {(B, H, S)}, got {tuple(weights.shape)}")
+    return weights.contiguous()
 
 
 def weighted_decode(
@@ -738,23 +774,24 @@ def weighted_decode(
     ``[B, S, Hkv, D]`` that also adds every key's softmax weight to ``weights
     [B, Hkv, S]`` (float32; None: zeros) -> ``(o, weights)``; at most 64 rows
     ``(Hq/Hkv)*T``.  Zero-padded head dims come back padded."""
-    dev, code, width, row, q, k, v, strides = _cache_call("attention with key weights", q, k, v)
-    B, T, Hq, D = q.shape
-    S, Hkv = k.shape[1], k.shape[2]
+    index, width, row, q, k, v, strides = _cache_call("attention with key weights", q, k, v)
+    B, T, Hq, _ = q.shape
+    _, S, Hkv, _ = k.shape
     rows = (Hq // Hkv) * T
     if not 1 <= rows <= WEIGHTED_DECODE_MAX_ROWS:
         raise ValueError(f"a weighted decode step takes 1 to {WEIGHTED_DECODE_MAX_ROWS} rows per KV head, got {rows}")
-    weights = _key_weights(weights, (B, Hkv, S), dev)
-    L = None if kv_lengths is None else _int32(kv_lengths, "kv_lengths", dev, ((B,),))
+    weights = _key_weights(weights, q, B, Hkv, S)
+    L = None if kv_lengths is None else _int32(kv_lengths, "kv_lengths", q, (B,))
     lib = native.load()
     nbytes = lib.pjx_weighted_decode_workspace_size(B, Hkv, rows, S, width, chunk)
-    ws = _workspace(nbytes, dev, workspace)
-    o = torch.empty((B, T, Hq, row), dtype=q.dtype, device=dev)
-    out = torch.empty((B, Hkv, S), dtype=torch.float32, device=dev)
-    lse = torch.empty((B, Hq, T), dtype=torch.float32, device=dev) if return_lse else None
-    _on_its_device(
-        dev, lib.pjx_weighted_decode, code, _ptr(q), _ptr(k), _ptr(v), _ptr(L), _ptr(weights), _ptr(out), _ptr(o),
-        _ptr(lse), _ptr(ws), nbytes, B, T, S, Hq, Hkv, width, row, strides, float(sm_scale), int(chunk), _stream(dev),
+    ws = _scratch(nbytes, q, workspace)
+    o = torch.empty_like(q)
+    out = torch.empty((B, Hkv, S), dtype=torch.float32, device=q.device) if weights is None else torch.empty_like(weights)
+    lse = torch.empty((B, Hq, T), dtype=torch.float32, device=q.device) if return_lse else None
+    _call(
+        index, lib.pjx_weighted_decode, _DTYPES[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(L),
+        _ptr(weights), out.data_ptr(), o.data_ptr(), _ptr(lse), ws.data_ptr(), nbytes, B, T, S, Hq, Hkv, width, row,
+        strides, sm_scale, chunk,
     )
     return (o, out, lse) if return_lse else (o, out)
 
@@ -766,27 +803,27 @@ def key_weights(
     """``pjx_key_weights``: adds to ``weights [B, Hkv, S]`` (None: zeros) the softmax
     weight that the rows of ``q [B, T, Hq, D]`` give each key of ``k [B, S, Hkv,
     D]``, from the LSE ``[B, Hq, T]`` of the flash forward with the same masks."""
-    dev = _on_device(q, k, lse)
+    index = _gpu(q, k, lse)
     if q.ndim != 4 or k.ndim != 4:
         raise ValueError("q must be [B, T, Hq, D] and k [B, S, Hkv, D]")
     B, T, Hq, D = q.shape
-    S, Hkv = k.shape[1], k.shape[2]
-    if k.shape[0] != B or k.shape[3] != D or Hkv < 1 or Hq % Hkv or tuple(lse.shape) != (B, Hq, T):
+    _, S, Hkv, _ = k.shape
+    if k.shape[0] != B or k.shape[3] != D or Hkv < 1 or Hq % Hkv or lse.shape != (B, Hq, T):
         raise ValueError(f"incompatible shapes q {tuple(q.shape)}, k {tuple(k.shape)}, lse {tuple(lse.shape)}")
     if q.dtype != k.dtype or lse.dtype != torch.float32:
         raise ValueError("q and k must share a dtype and lse be float32")
     code = _dtype_code(q)
-    weights = _key_weights(weights, (B, Hkv, S), dev)
-    L = None if kv_lengths is None else _int32(kv_lengths, "kv_lengths", dev, ((B,),))
+    weights = _key_weights(weights, q, B, Hkv, S)
+    L = None if kv_lengths is None else _int32(kv_lengths, "kv_lengths", q, (B,))
     q, k, lse = _aligned(q.contiguous()), _aligned(k.contiguous()), lse.contiguous()
     lib = native.load()
     nbytes = lib.pjx_key_weights_workspace_size(B, T, S, Hq)
-    ws = _workspace(nbytes, dev, workspace)
-    out = torch.empty((B, Hkv, S), dtype=torch.float32, device=dev)
-    _on_its_device(
-        dev, lib.pjx_key_weights, code, _ptr(q), _ptr(k), _ptr(lse), _ptr(L), _ptr(weights), _ptr(out), _ptr(ws),
-        nbytes, B, T, S, Hq, Hkv, D if width is None else int(width), D, int(bool(causal)), int(causal_shift),
-        float(sm_scale), _stream(dev),
+    ws = _scratch(nbytes, q, workspace)
+    out = torch.empty((B, Hkv, S), dtype=torch.float32, device=q.device)
+    _call(
+        index, lib.pjx_key_weights, code, q.data_ptr(), k.data_ptr(), lse.data_ptr(), _ptr(L), _ptr(weights),
+        out.data_ptr(), ws.data_ptr(), nbytes, B, T, S, Hq, Hkv, D if width is None else width, D, int(bool(causal)),
+        causal_shift, sm_scale,
     )
     return out
 
@@ -809,74 +846,98 @@ def evict_keys(k, v, weights, keep: int, *, kv_lengths=None, sinks: int = 0, rec
     ``[B, S, Hkv, D]`` cut to ``keep`` keys per sequence and head; ``out``: buffers
     ``(k, v, weights)`` of at least ``keep`` slots to write into, whose rows behind
     the kept ones stay as they are."""
-    dev = _on_device(k, v, weights)
-    if k.ndim != 4 or k.shape != v.shape or k.dtype != v.dtype:
+    index = _gpu(k, v, weights)
+    if k.ndim != 4 or k.shape != v.shape or k.dtype is not v.dtype:
         raise ValueError(f"k and v must be [B, S, Hkv, D] of one shape and dtype, got {tuple(k.shape)} {k.dtype} and "
                          f"{tuple(v.shape)} {v.dtype}")
     if k.dtype not in _DTYPES:
         raise ValueError(f"unsupported dtype {k.dtype}; expected bfloat16, float16 or float32")
-    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or weights.requires_grad):
+    if (k.requires_grad or v.requires_grad or weights.requires_grad) and torch.is_grad_enabled():
         raise ValueError("eviction has no gradient: call it under torch.no_grad() or on detached tensors")
     B, S, H, D = k.shape
     keep, sinks, recent = int(keep), int(sinks), int(recent)
     if keep < 1 or sinks < 0 or recent < 0 or sinks + recent > keep:
         raise ValueError(f"keep must be at least 1 and at least sinks + recent, got keep={keep}, sinks={sinks}, "
                          f"recent={recent}")
-    weights = _key_weights(weights, (B, H, S), dev)
-    L = None if kv_lengths is None else _int32(kv_lengths, "kv_lengths", dev, ((B,),))
-    fill = out is None
-    if fill:
-        k_out, v_out = (torch.empty((B, keep, H, D), dtype=k.dtype, device=dev) for _ in range(2))
-        w_out = torch.empty((B, H, keep), dtype=torch.float32, device=dev)
+    weights = _key_weights(weights, k, B, H, S)
+    L = None if kv_lengths is None else _int32(kv_lengths, "kv_lengths", k, (B,))
+    out_strides = None
+    if out is None:
+        k_out = k.new_empty((B, keep, H, D))
+        v_out = torch.empty_like(k_out)
+        w_out = weights.new_empty((B, H, keep))
     else:
         k_out, v_out, w_out = out
-        C = k_out.shape[1] if k_out.ndim == 4 else 0
-        for t, shape, dtype in ((k_out, (B, C, H, D), k.dtype), (v_out, (B, C, H, D), k.dtype),
-                                (w_out, (B, H, C), torch.float32)):
-            if t.device != dev or t.dtype != dtype or tuple(t.shape) != shape or C < keep:
-                raise ValueError(f"out must be k and v {(B, f'>= {keep}', H, D)} of {k.dtype} and weights "
-                                 f"{(B, H, f'>= {keep}')} of float32 on {dev}")
-        if k_out.stride(3) != 1 or v_out.stride(3) != 1 or not w_out.is_contiguous():
-            raise ValueError("out needs contiguous features and contiguous weights")
-        places = [t.untyped_storage().data_ptr() for t in (k, v, weights, k_out, v_out, w_out) if t.numel()]
-        ins = 3 if k.numel() else 0
-        if set(places[:ins]) & set(places[ins:]) or len(set(places[ins:])) != len(places[ins:]):
-            raise ValueError("out must not share memory with the inputs, nor its buffers with each other")
-    lengths = torch.empty((B,), dtype=torch.int32, device=dev)
-    index = torch.empty((B, H, keep), dtype=torch.int32, device=dev)
+        _check_evict_out(out, (k, v, weights), keep)
+        out_strides = _pair_strides(k_out, v_out)
+    lengths_index = torch.empty((B * (1 + H * keep),), dtype=torch.int32, device=k.device)
+    lengths, index_out = lengths_index[:B], lengths_index[B:].view(B, H, keep)
     k, v = _features_contiguous(k), _features_contiguous(v)
-    _on_its_device(
-        dev, native.load().pjx_evict_keys, k.element_size(), _ptr(k), _ptr(v), _ptr(weights), _ptr(L), _ptr(k_out),
-        _ptr(v_out), _ptr(w_out), _ptr(lengths), _ptr(index), B, S, H, D, k_out.shape[1], keep, sinks, recent,
-        _pair_strides(k, v), _pair_strides(k_out, v_out), int(fill), _stream(dev),
+    _call(
+        index, native.load().pjx_evict_keys, k.element_size(), k.data_ptr(), v.data_ptr(), weights.data_ptr(), _ptr(L),
+        k_out.data_ptr(), v_out.data_ptr(), w_out.data_ptr(), lengths.data_ptr(), index_out.data_ptr(), B, S, H, D,
+        k_out.shape[1], keep, sinks, recent, _pair_strides(k, v), out_strides, int(out is None),
     )
-    return k_out, v_out, w_out, lengths, index
+    return k_out, v_out, w_out, lengths, index_out
+
+
+def _check_evict_out(out, ins, keep: int) -> None:
+    """Refuses buffers that ``evict_keys`` cannot write ``keep`` keys of ``ins`` into."""
+    k, v, weights = ins
+    k_out, v_out, w_out = out
+    B, _, H, D = k.shape
+    C = k_out.shape[1] if k_out.ndim == 4 else 0
+    for t, shape, dtype in ((k_out, (B, C, H, D), k.dtype), (v_out, (B, C, H, D), k.dtype),
+                            (w_out, (B, H, C), torch.float32)):
+        if t.device != k.device or t.dtype != dtype or tuple(t.shape) != shape or C < keep:
+            raise ValueError(f"out must be k and v {(B, f'>= {keep}', H, D)} of {k.dtype} and weights "
+                             f"{(B, H, f'>= {keep}')} of float32 on {k.device}")
+    if (D > 1 and (k_out.stride(3) != 1 or v_out.stride(3) != 1)) or not w_out.is_contiguous():
+        raise ValueError("out needs contiguous features and contiguous weights")
+    if any(n > 1 and s == 0 for t in (k_out, v_out) for n, s in zip(t.shape, t.stride())):
+        raise ValueError("out must not be expanded")
+    read = {t.untyped_storage().data_ptr() for t in ins if t.numel()}
+    write = [t.untyped_storage().data_ptr() for t in out if t.numel()]
+    if read & set(write) or len(set(write)) != len(write):
+        raise ValueError("out must not share memory with the inputs, nor its buffers with each other")
 
 
 _POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2, torch.float64: 3}  # PJX_POSITION_*
 
 
-def rotary(q, k, positions, *, sections, base: float, interleaved: bool, shared_spectrum: bool, inverse: bool = False):
+def rotary(q, k, positions, sections, base: float, interleaved: bool, shared_spectrum: bool, inverse: bool = False):
     """``pjx_rotary``: ``q [B, T, Hq, D]`` and ``k [B, T, Hk, D]`` (or None) turned
     by ``positions [T, A]`` or ``[B, T, A]`` (``inverse``: back) -> contiguous
     ``(q, k)``."""
-    dev = _on_device(q, k, positions)
+    index = _gpu(q, k, positions)
     B, T, Hq, D = q.shape
     code = _dtype_code(q)
-    q = _features_contiguous(q)
-    Hk = 0
+    if q.is_contiguous():
+        y = torch.empty_like(q)
+    else:
+        q = _features_contiguous(q)
+        y = torch.empty((B, T, Hq, D), dtype=q.dtype, device=q.device)
+    Hk, z = 0, None
     if k is not None:
-        k = _features_contiguous(k)
         Hk = k.shape[2]
-    if positions.shape[-1] > 1 and positions.stride(-1) != 1:
+        if k.is_contiguous():
+            z = torch.empty_like(k)
+        else:
+            k = _features_contiguous(k)
+            z = torch.empty((B, T, Hk, D), dtype=q.dtype, device=q.device)
+    *lead, token, last = positions.stride()
+    if last != 1 and positions.shape[-1] > 1:
         positions = positions.contiguous()
-    pb = positions.stride(0) if positions.ndim == 3 else 0
-    y = torch.empty((B, T, Hq, D), dtype=q.dtype, device=dev)
-    z = None if k is None else torch.empty((B, T, Hk, D), dtype=q.dtype, device=dev)
-    _on_its_device(
-        dev, native.load().pjx_rotary, code, _ptr(q), _ptr(k), _ptr(y), _ptr(z), _ptr(positions),
-        _POSITION_TYPES[positions.dtype], pb, positions.stride(-2), B, T, Hq, Hk, D, _pair_strides(q, k),
-        (ctypes.c_int32 * len(sections))(*sections), len(sections), float(base), int(interleaved),
-        int(shared_spectrum), int(inverse), _stream(dev),
+        *lead, token, last = positions.stride()
+    _call(
+        index, native.load().pjx_rotary, code, q.data_ptr(), _ptr(k), y.data_ptr(), _ptr(z), positions.data_ptr(),
+        _POSITION_TYPES[positions.dtype], lead[0] if lead else 0, token, B, T, Hq, Hk, D, _pair_strides(q, k),
+        _int_array(sections), len(sections), base, interleaved, shared_spectrum, inverse,
     )
     return y, z
+
+
+@functools.lru_cache(maxsize=64)
+def _int_array(values):
+    """``values`` (a tuple) as a C array of int32."""
+    return (ctypes.c_int32 * len(values))(*values)

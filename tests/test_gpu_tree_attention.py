@@ -184,6 +184,25 @@ def test_caches_in_any_order_of_axes(device):
     assert torch.equal(tree_attention(qt, k, v, parents=parents, kv_lengths=L), want)
 
 
+def test_slots_far_apart_in_memory(device):
+    """A cache whose slots lie 2^24 + 8 elements apart (a slice of a much longer
+    row), with more rows per KV head than one 16-row block twice: offsets of a tile
+    of keys pass 32 bits."""
+    import torch
+
+    B, T, S, Hq, Hkv, D, step = 1, 12, 150, 4, 1, 64, 2 ** 24 + 8
+    (q, k, v), (qn, kn, vn) = _inputs(31, torch.bfloat16, B, T, S, Hq, Hkv, D, device)
+    far = torch.empty((S * step,), dtype=torch.bfloat16, device=device).as_strided((B, S, Hkv, D), (0, step, D, 1))
+    far.copy_(k)
+    parents = random_parents(np.random.default_rng(31), B, T)
+    from probjax_amd.hip_attention import tree_decode
+
+    sees, token = ref.tree_sees(parents[0])
+    want = ref.tree_attention(qn, kn, vn, [S - T], [sees], [token], D ** -0.5)
+    out, lse = tree_decode(q, far, v, parents=torch.from_numpy(parents).to(device), sm_scale=D ** -0.5, return_lse=True)
+    check(out, lse, want, torch.bfloat16, D, S)
+
+
 def test_without_lengths_the_draft_is_the_cache_end(device):
     import torch
     from probjax_amd.attention import tree_attention
