@@ -2,12 +2,14 @@
 // `sinks` and last `recent` keys and, of those between, the ones of the largest
 // accumulated weight, in their order.
 //
-// Two kernels.  The selection runs one workgroup per (sequence, head), bound by
-// the latency of its rounds: the weights stay in registers as order-preserving
-// integers, the threshold is found two bits a round by counting (ballots, so the
-// time does not depend on how the weights are spread, as that of a histogram in
-// LDS does), and one more pass ranks the kept keys.  The gather reads and writes
-// every kept K and V row once, 16 bytes a lane, bound by HBM.
+// Two kernels.  The selection runs one workgroup per (sequence, head), its weights
+// in registers as order-preserving integers, and finds the threshold by counting
+// digits of 11 bits in LDS, two or three passes; one more pass ranks the kept keys.
+// It is bound by the latency of those steps (8 x 4096 weights 9 us, 128 x 8192 of
+// them 11; bits counted two a round by ballots kept the scalar unit, which 16 waves
+// share, busy for 9 us more).  The gather reads and writes every kept K and V row
+// once, 16 bytes a lane, bound by HBM (16 x 8192 keys of 8 heads of 128 cut to half
+// their capacity, 490 MB: 97 us, 5.0 TB/s).
 #include <stdio.h>
 
 #include "pjx_common.h"
@@ -38,38 +40,36 @@ __device__ __forceinline__ uint32_t weight_key(uint32_t u) {
   return u >> 31 ? ~u : u | 0x80000000u;
 }
 
-// Sum over the 16 lanes of a row, in every lane of it.
-__device__ __forceinline__ int row_sum(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x128, 0xf, 0xf, false);  // row_ror:8
-  x += __builtin_amdgcn_update_dpp(0, x, 0x124, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x122, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x121, 0xf, 0xf, false);
+// Inclusive prefix sums over the 16 lanes of a row, and over a wave.
+__device__ __forceinline__ int row_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);  // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
   return x;
 }
-
-// Inclusive prefix sum over a wave.
 __device__ __forceinline__ int wave_scan(int x) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const int y = __shfl_up(x, d);
-    x += lane >= d ? y : 0;
-  }
+  x = row_scan(x);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2 and 3
   return x;
 }
 
-// R: keys of a thread's registers (the cache has at most R * kSelThreads); 0:
-// read again in every round.
-constexpr int kPlaceTiles = 8;  // tiles of kSelThreads keys ranked together
+// R: weights of a thread's registers (the cache has at most R * kSelThreads); 0:
+// read again in every pass.
+constexpr int kTiles = 8;  // tiles of kSelThreads keys ranked, or loaded, together
+constexpr int kDigit = 11, kBins = 1 << kDigit;
 template <int R>
 __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) {
-  __shared__ int count[2][3 * kSelWaves];
-  __shared__ int rank_above[kPlaceTiles * kSelWaves], rank_at[kPlaceTiles * kSelWaves];
+  __shared__ __attribute__((aligned(8))) int bins[kBins];
+  __shared__ int wave_sum[kSelWaves], found[3];
+  __shared__ int rank_above[kTiles * kSelWaves], rank_at[kTiles * kSelWaves];
   __shared__ int total[2];
-  static_assert(kSelWaves == 16 && kPlaceTiles * kSelWaves == 128, "two ranks per lane of a wave");
+  static_assert(kSelWaves == 16 && kTiles * kSelWaves == 128, "two ranks per lane of a wave");
+  static_assert(kBins == 2 * kSelThreads, "two bins per thread");
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int bh = blockIdx.x, b = bh / a.H;
-  const int n = a.lengths ? min(max(a.lengths[b], 0), a.S) : a.S;
+  const int n = __builtin_amdgcn_readfirstlane(a.lengths ? min(max(a.lengths[b], 0), a.S) : a.S);
   const int kept = min(n, a.keep);
   const uint32_t* w = a.weights + (size_t)bh * a.S;
   int32_t* index = a.index + (size_t)bh * a.keep;
@@ -86,70 +86,98 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
     }
     return;
   }
+  // (loads without a condition: a branch around each would wait for it)
+  auto weight_at = [&](int j) { return w[min(j, n - 1)]; };
   const int lo = a.sinks, hi = n - a.recent, need = a.keep - a.sinks - a.recent;
-  auto key_at = [&](int j) { return j >= lo && j < hi ? weight_key(w[j]) : 0u; };  // 0: protected, or no key
-  uint32_t key[R > 0 ? R : 1];
+  auto key_of = [&](int j, uint32_t u) { return ((j >= lo) & (j < hi)) ? weight_key(u) : 0u; };  // 0: protected, or no key
+  uint32_t raw[R > 0 ? R : kTiles];
   if constexpr (R > 0) {
 #pragma unroll
-    for (int i = 0; i < R; ++i) key[i] = key_at(tid + i * kSelThreads);
+    for (int i = 0; i < R; ++i) raw[i] = weight_at(tid + i * kSelThreads);
   }
 
-  // T: the largest threshold that at least `need` keys reach, two bits a round;
-  // above: how many reach the smallest one known to be too high.
-  uint32_t T = 0;
-  int above = 0;
-  bool exact = false;  // exactly `need` keys reach T
-  if (need == 0) {
-    T = 0xffffffffu;
-  } else {
-    int round = 0;
-    for (int bit = 30; bit >= 0 && !exact; bit -= 2, round ^= 1) {
-      int c[3] = {0, 0, 0};
+  // T: the key of rank hi - lo - need from below among those between, kDigit bits a
+  // pass: the keys that agree with T so far are counted by their next digit, and the
+  // digit is the one in whose count the rank falls.
+  uint32_t T = 0xffffffffu;
+  int ties = 0;  // of the keys equal to T, so many are kept
+  if (need > 0) {
+    int2* own = (int2*)bins + tid;
+    *own = {0, 0};
+    __syncthreads();
+    T = 0u;
+    int skip = hi - lo - need;
+#pragma unroll 1
+    for (int shift = 32 - kDigit, before = 32;;) {
       auto look = [&](uint32_t u) {
-#pragma unroll
-        for (int j = 0; j < 3; ++j) c[j] += __popcll(__builtin_amdgcn_ballot_w64(u >= (T | (uint32_t)(j + 1) << bit)));
+        const bool in = (u != 0u) & (before == 32 || (u ^ T) >> (before & 31) == 0u);
+        const int d = (int)(u >> shift) & (kBins - 1);
+        const uint64_t m = __builtin_amdgcn_ballot_w64(in);
+        if (!m) return;
+        // One atomic for all lanes of the first one's digit: weights often share one,
+        // and atomics on one word take their turns.
+        const int d0 = __builtin_amdgcn_readlane(d, __builtin_ctzll(m));
+        const uint64_t same = __builtin_amdgcn_ballot_w64(in & (d == d0));
+        if (lane == __builtin_ctzll(m)) atomicAdd(&bins[d0], __popcll(same));
+        else if (in & (d != d0)) atomicAdd(&bins[d], 1);
       };
       if constexpr (R > 0) {
 #pragma unroll
-        for (int i = 0; i < R; ++i) look(key[i]);
+        for (int i = 0; i < R; ++i) look(key_of(tid + i * kSelThreads, raw[i]));
       } else {
-        for (int j = tid; j < (n + kSelThreads - 1) / kSelThreads * kSelThreads; j += kSelThreads) look(key_at(j));
-      }
-      // (the counts are the same in every lane: the ballots' sums are scalars)
-      if (lane < 3) count[round][16 * lane + wave] = lane == 0 ? c[0] : lane == 1 ? c[1] : c[2];
-      __syncthreads();
-      const int sums = row_sum(lane < 48 ? count[round][lane] : 0);
-      int at = 0, reached = 0;
+        for (int j0 = tid; j0 - tid < n; j0 += kTiles * kSelThreads) {
 #pragma unroll
-      for (int j = 2; j >= 0; --j) {  // the largest digit that enough keys reach
-        const int sum = __builtin_amdgcn_readlane(sums, 16 * j);
-        if (at == 0) {
-          if (sum >= need) {
-            at = j + 1;
-            reached = sum;
-          } else {
-            above = sum;
-          }
+          for (int i = 0; i < kTiles; ++i) raw[i] = weight_at(j0 + i * kSelThreads);
+#pragma unroll
+          for (int i = 0; i < kTiles; ++i) look(key_of(j0 + i * kSelThreads, raw[i]));
         }
       }
-      T |= (uint32_t)at << bit;
-      exact = at > 0 && reached == need;
+      __syncthreads();
+      const int2 c = *own;
+      *own = {0, 0};
+      const int sum = c.x + c.y, incl = wave_scan(sum);
+      if (lane == 63) wave_sum[wave] = incl;
+      __syncthreads();
+      const int sums = row_scan(wave_sum[lane & 15]);
+      const int first = (wave ? __builtin_amdgcn_readlane(sums, wave - 1) : 0) + incl - sum;
+      if ((first <= skip) & (skip < first + sum)) {
+        const bool y = skip >= first + c.x;
+        found[0] = 2 * tid + y;
+        found[1] = y ? first + c.x : first;  // keys of smaller digits
+        found[2] = y ? c.y : c.x;
+      }
+      __syncthreads();
+      const int digit = __builtin_amdgcn_readfirstlane(found[0]), count = __builtin_amdgcn_readfirstlane(found[2]);
+      skip -= __builtin_amdgcn_readfirstlane(found[1]);
+      T |= (uint32_t)digit << shift;
+      if (skip == 0) {  // every key from T on is kept, whatever its further bits
+        T -= 1;
+        break;
+      }
+      if (shift == 0) {
+        ties = count - skip;
+        break;
+      }
+      before = shift;
+      shift = max(shift - kDigit, 0);
     }
   }
   // Keys above T are kept, and of those at T the first `ties`.
-  const int ties = need == 0 || exact ? 0 : need - above;
-  if (exact) T -= 1;
-  // Ranks, kPlaceTiles tiles at a time: every wave counts its kept and tied keys
-  // of each tile, one wave sums them in the keys' order.
+  // Ranks, kTiles tiles at a time: every wave counts its kept and tied keys of each
+  // tile, one wave sums them in the keys' order.
   int done_above = 0, done_at = 0;
   auto place = [&](int j0, const uint32_t* u) {
-    uint64_t gm[kPlaceTiles], em[kPlaceTiles];
+    uint64_t gm[kTiles], em[kTiles];
 #pragma unroll
-    for (int i = 0; i < kPlaceTiles; ++i) {
+    for (int i = 0; i < kTiles; ++i) {
       const int j = j0 + i * kSelThreads + tid;
-      gm[i] = __builtin_amdgcn_ballot_w64(j < n && (j < lo || j >= hi || u[i] > T));
-      em[i] = __builtin_amdgcn_ballot_w64(j >= lo && j < hi && u[i] == T);
-      if (lane == 0) {
+      const uint32_t x = key_of(j, u[i]);
+      gm[i] = __builtin_amdgcn_ballot_w64((j < n) & ((x > T) | (x == 0u)));
+      em[i] = __builtin_amdgcn_ballot_w64(x == T);
+    }
+    if (lane == 0) {
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i) {
         rank_above[kSelWaves * i + wave] = __popcll(gm[i]);
         rank_at[kSelWaves * i + wave] = __popcll(em[i]);
       }
@@ -164,14 +192,18 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
     }
     __syncthreads();
     const uint64_t below = ((uint64_t)1 << lane) - 1;
+    int g0[kTiles], e0[kTiles];
 #pragma unroll
-    for (int i = 0; i < kPlaceTiles; ++i) {
-      const int g0 = done_above + rank_above[kSelWaves * i + wave] + __popcll(gm[i] & below);
-      const int e0 = done_at + rank_at[kSelWaves * i + wave] + __popcll(em[i] & below);
-      if ((gm[i] >> lane & 1) || ((em[i] >> lane & 1) && e0 < ties)) {
-        const int at = g0 + min(e0, ties), j = j0 + i * kSelThreads + tid;
-        index[at] = j;
-        wout[at] = w[j];
+    for (int i = 0; i < kTiles; ++i) {
+      g0[i] = done_above + rank_above[kSelWaves * i + wave] + __popcll(gm[i] & below);
+      e0[i] = done_at + rank_at[kSelWaves * i + wave] + __popcll(em[i] & below);
+    }
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) {
+      if ((gm[i] >> lane & 1) | ((em[i] >> lane & 1) & (e0[i] < ties))) {
+        const int at = g0[i] + min(e0[i], ties);
+        index[at] = j0 + i * kSelThreads + tid;
+        wout[at] = u[i];
       }
     }
     done_above += total[0];
@@ -179,18 +211,17 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
   };
   if constexpr (R > 0) {
 #pragma unroll
-    for (int i = 0; i < R; i += kPlaceTiles)
+    for (int i = 0; i < R; i += kTiles)
       if (i * kSelThreads < n) {
         if (i > 0) __syncthreads();  // the last tiles' ranks have been read
-        place(i * kSelThreads, key + i);
+        place(i * kSelThreads, raw + i);
       }
   } else {
-    for (int j0 = 0; j0 < n; j0 += kPlaceTiles * kSelThreads) {
-      uint32_t u[kPlaceTiles];
+    for (int j0 = 0; j0 < n; j0 += kTiles * kSelThreads) {
 #pragma unroll
-      for (int i = 0; i < kPlaceTiles; ++i) u[i] = key_at(j0 + i * kSelThreads + tid);
+      for (int i = 0; i < kTiles; ++i) raw[i] = weight_at(j0 + i * kSelThreads + tid);
       __syncthreads();
-      place(j0, u);
+      place(j0, raw);
     }
   }
 }
