@@ -89,13 +89,35 @@ struct TreeTable {
 };
 static_assert(kTreeMax <= kDecThreads, "one thread per token");
 
-// Fills the table; every thread of a workgroup of kDecThreads calls it.  From
+// Fills the table; every thread of a workgroup of WAVES waves calls it.  From
 // parents: each token's set starts as itself and every round adds the set of
 // the token it jumps to while the jumps double in length, so a chain of T
-// tokens takes log2(T) rounds.  A parent that is no earlier token ends a chain.
+// tokens takes log2(T) rounds; up to 64 tokens by one wave between its lanes
+// (26 tokens: 2.1 us with a barrier after every round).  A parent that is no
+// earlier token ends a chain.
+template <int WAVES>
 __device__ __forceinline__ void build_tree(const DecodeArgs& a, int b, TreeTable& tt) {
-  const int tid = threadIdx.x, T = a.Lq;
-  if (a.parents) {
+  const int tid = threadIdx.x, lane = tid & 63, T = a.Lq;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  if (a.parents && T <= 64) {
+    if (wave == 0) {
+      const int p = a.parents[(size_t)b * a.tree_step + min(lane, T - 1)];
+      int jump = p < lane ? p : -1;
+      uint32_t lo = lane < 32 ? 1u << lane : 0u, hi = lane < 32 ? 0u : 1u << (lane - 32);
+      for (int span = 1; span < T; span *= 2) {
+        const int src = max(jump, 0), next = __shfl(jump, src);
+        const uint32_t more_lo = __shfl(lo, src), more_hi = __shfl(hi, src);
+        if (jump >= 0) {
+          lo |= more_lo;
+          hi |= more_hi;
+          jump = next;
+        }
+      }
+#pragma unroll
+      for (int w = 0; w < kTreeWords; ++w)
+        if (lane < T) tt.bits[lane][w] = w == 0 ? lo : w == 1 ? hi : 0u;
+    }
+  } else if (a.parents) {
     if (tid < T) {
       const int p = a.parents[(size_t)b * a.tree_step + tid];
       tt.jump[tid] = p < tid ? p : -1;
@@ -123,28 +145,28 @@ __device__ __forceinline__ void build_tree(const DecodeArgs& a, int b, TreeTable
       __syncthreads();
     }
   } else {
-    // 64 bytes of a row a time, the loads of 8 of them issued before the first is used
+    // 64 bytes of a row a time, the loads of 8 rows issued before the first is used
     const uint8_t* m = a.tree_mask + (size_t)b * a.tree_step;
-    const int lane = tid & 63, per_row = (T + 63) / 64, n = T * per_row;
-    for (int i0 = tid >> 6; i0 < n; i0 += 8 * (kDecThreads / 64)) {
-      uint8_t x[8];
+    for (int j0 = 0; j0 < T; j0 += 64) {
+      const int j = min(j0 + lane, T - 1);
+      const bool in = j0 + lane < T;
+      for (int t0 = wave; t0 < T; t0 += 8 * WAVES) {
+        uint8_t x[8];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const int i = i0 + u * (kDecThreads / 64), t = i / per_row, j = 64 * (i - t * per_row) + lane;
-        x[u] = i < n && j < T ? m[t * T + j] : 0;
-      }
+        for (int u = 0; u < 8; ++u) x[u] = m[min(t0 + u * WAVES, T - 1) * T + j];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const int i = i0 + u * (kDecThreads / 64), t = i / per_row, w = 2 * (i - t * per_row);
-        const uint64_t seen = __builtin_amdgcn_ballot_w64(x[u] != 0);
-        if (lane == 0 && i < n) {
-          tt.bits[t][w] = (uint32_t)seen;
-          tt.bits[t][w + 1] = (uint32_t)(seen >> 32);
+        for (int u = 0; u < 8; ++u) {
+          const int t = t0 + u * WAVES;
+          const uint64_t seen = __builtin_amdgcn_ballot_w64(in & (x[u] != 0));
+          if (lane == 0 && t < T) {
+            tt.bits[t][j0 >> 5] = (uint32_t)seen;
+            tt.bits[t][(j0 >> 5) + 1] = (uint32_t)(seen >> 32);
+          }
         }
       }
     }
-    __syncthreads();
   }
+  __syncthreads();
 }
 
 // Whether token t sees the key `j` slots behind the prefix's end (j < 0: a key
@@ -481,7 +503,7 @@ __device__ __forceinline__ void gqa_decode(const DecodeArgs& a) {
   __shared__ typename std::conditional<X == kTree, TreeTable, int>::type tree;
   __shared__ float tree_p[X == kTree ? 4 * 512 : 1];
   if constexpr (X == kTree) {
-    if (c0 + a.chunk > P) build_tree(a, b, tree);
+    if (c0 + a.chunk > P) build_tree<kDecThreads / 64>(a, b, tree);
   }
   int tok[NRB];
   const int rd = ROWS ? a.orow : D, rdv = ROWS ? a.orow : DV;
@@ -837,7 +859,7 @@ __device__ __forceinline__ void gqa_decode_f32(const DecodeArgs& a) {
   __shared__ typename std::conditional<X == kTree, TreeTable, int>::type tree;
   __shared__ float tree_p[X == kTree ? 4 * 512 : 1];
   if constexpr (X == kTree) {
-    if (c0 + a.chunk > P) build_tree(a, b, tree);
+    if (c0 + a.chunk > P) build_tree<kDecThreads / 64>(a, b, tree);
   }
   int tok[NRB];
 

@@ -67,20 +67,6 @@ __global__ __launch_bounds__(64 * RW * KG, 2) void tree_wide_kernel(DecodeArgs a
     voffK[j] = row_chunk(r, krow, slot ^ T::swz_k(r), rdim);
     voffV[j] = row_chunk(r, vrow, slot ^ T::swz_v(r), rdim);
   }
-  uint32_t offK[D / 16];
-#pragma unroll
-  for (int st = 0; st < D / 16; ++st) offK[st] = col * ROWB + 16 * ((2 * st + half) ^ T::swz_k(col));
-  uint32_t offV[D / 32];
-  {
-    const int s16 = lane & 15, grp = lane >> 4;
-    const int r = 4 * half + s16 / 4;
-#pragma unroll
-    for (int db = 0; db < D / 32; ++db) {
-      const int chunk = 4 * db + 2 * (grp & 1) + ((s16 & 3) >> 1);
-      offV[db] = r * ROWB + 16 * (chunk ^ T::swz_v(r)) + 8 * (s16 & 1);
-    }
-  }
-
   f32x16 acc[D / 32];
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) acc[i] = f32x16{};
@@ -118,7 +104,21 @@ __global__ __launch_bounds__(64 * RW * KG, 2) void tree_wide_kernel(DecodeArgs a
     }
   }
 
-  if (c1 > P) build_tree(a, b, tree);
+  if (c1 > P) build_tree<NW>(a, b, tree);
+
+  uint32_t offK[D / 16];
+#pragma unroll
+  for (int st = 0; st < D / 16; ++st) offK[st] = col * ROWB + 16 * ((2 * st + half) ^ T::swz_k(col));
+  uint32_t offV[D / 32];
+  {
+    const int s16 = lane & 15, grp = lane >> 4;
+    const int r = 4 * half + s16 / 4;
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db) {
+      const int chunk = 4 * db + 2 * (grp & 1) + ((s16 & 3) >> 1);
+      offV[db] = r * ROWB + 16 * (chunk ^ T::swz_v(r)) + 8 * (s16 & 1);
+    }
+  }
 
   auto scores = [&](const unsigned char* ks, f32x16* s) {
 #pragma unroll
