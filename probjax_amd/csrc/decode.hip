@@ -50,8 +50,10 @@ __global__ __launch_bounds__(256, (decode_occupancy<D, D, NRB>())) void gqa_deco
   gqa_decode<E, D, D, NRB, false, true>(a);
 }
 
+// Two waves per SIMD where 256 registers do: one 16-row block of widths 128 and 256
+// needs 262 otherwise (8 sequences of 2048 keys, 4 KV heads: 29.7 us).
 template <int D, int DV, int NRB>
-__global__ __launch_bounds__(256, 1) void gqa_decode_f32_kernel(DecodeArgs a) {
+__global__ __launch_bounds__(256, NRB == 1 && D + DV < 512 ? 2 : 1) void gqa_decode_f32_kernel(DecodeArgs a) {
   gqa_decode_f32<D, DV, NRB, kPlain>(a);
 }
 

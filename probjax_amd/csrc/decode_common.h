@@ -502,9 +502,6 @@ __device__ __forceinline__ void gqa_decode(const DecodeArgs& a) {
   const int P = X == kTree ? prefix_len(a, b) : 0;
   __shared__ typename std::conditional<X == kTree, TreeTable, int>::type tree;
   __shared__ float tree_p[X == kTree ? 4 * 512 : 1];
-  if constexpr (X == kTree) {
-    if (c0 + a.chunk > P) build_tree<kDecThreads / 64>(a, b, tree);
-  }
   int tok[NRB];
   const int rd = ROWS ? a.orow : D, rdv = ROWS ? a.orow : DV;
   typename E::v8 qf[NRB][KSTEPS];
@@ -647,6 +644,9 @@ __device__ __forceinline__ void gqa_decode(const DecodeArgs& a) {
   if (w0 < w1) {
     load_k(w0);
     load_v(w0);
+  }
+  if constexpr (X == kTree) {
+    if (c0 + a.chunk > P) build_tree<kDecThreads / 64>(a, b, tree);
   }
   for (int k0 = w0; k0 < w1; k0 += 32) {
     const int kn = k0 + 32;
@@ -888,24 +888,13 @@ __device__ __forceinline__ void gqa_decode_f32(const DecodeArgs& a) {
   }
 
   for (int k0 = w0; k0 < w1; k0 += 32) {
-    // S^T for keys k0 + 16*kb + 4*q4 + r, query row 16rb + c16.
-    f32x4 s[NRB][2];
+    // (loads without a condition, all issued before the first is used)
+    f32x4 kf[2][NJ];
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
-      const int key = k0 + 16 * kb + c16;
-      const bool ok = key < w1;
-      const float* kp = Kb + (size_t)(ok ? key : 0) * k_tok + 4 * q4;
-      f32x4 kf[NJ];
+      const float* kp = Kb + (size_t)min(k0 + 16 * kb + c16, w1 - 1) * k_tok + 4 * q4;
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) kf[j] = ok ? *(const f32x4*)(kp + 16 * j) : f32x4{};
-#pragma unroll
-      for (int rb = 0; rb < NRB; ++rb) {
-        s[rb][kb] = f32x4{};
-#pragma unroll
-        for (int j = 0; j < NJ; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[rb][kb] = mfma16x16x4f32(kf[j][e], qf[rb][j][e], s[rb][kb]);
-      }
+      for (int j = 0; j < NJ; ++j) kf[kb][j] = *(const f32x4*)(kp + 16 * j);
     }
     // V[key 16kb + 4*q4 + e][dim 16i + c16] for the A operands of P.V
     float vv[2][4][NDB];
@@ -914,12 +903,30 @@ __device__ __forceinline__ void gqa_decode_f32(const DecodeArgs& a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int key = k0 + 16 * kb + 4 * q4 + e;
-        const bool ok = key < w1;
-        const float* vp = Vb + (size_t)(ok ? key : 0) * v_tok + c16;
+        const float* vp = Vb + (size_t)min(key, w1 - 1) * v_tok + c16;
 #pragma unroll
-        for (int i = 0; i < NDB; ++i) vv[kb][e][i] = ok ? vp[16 * i] : 0.f;
+        for (int i = 0; i < NDB; ++i) vv[kb][e][i] = vp[16 * i];
       }
+    // S^T for keys k0 + 16*kb + 4*q4 + r, query row 16rb + c16.
+    f32x4 s[NRB][2];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+      for (int rb = 0; rb < NRB; ++rb) {
+        s[rb][kb] = f32x4{};
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[rb][kb] = mfma16x16x4f32(kf[kb][j][e], qf[rb][j][e], s[rb][kb]);
+      }
+    }
     if (k0 + 32 > w1) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int i = 0; i < NDB; ++i) vv[kb][e][i] = k0 + 16 * kb + 4 * q4 + e < w1 ? vv[kb][e][i] : 0.f;
 #pragma unroll
       for (int rb = 0; rb < NRB; ++rb)
 #pragma unroll
@@ -1152,7 +1159,8 @@ int run_chunks(DecodeArgs& a, void* workspace, size_t ws_bytes, hipStream_t stre
 template <auto K>
 int run_decode(DecodeArgs& a, void* workspace, size_t ws_bytes, hipStream_t stream, const char* name) {
   const int rc = run_chunks<K>(a, workspace, ws_bytes, stream, name);
-  return rc ? rc : launch_decode_merge(a, stream, name);
+  if (rc) return rc;
+  return a.extra && a.nch <= kFewChunks ? launch_merge_few(a, stream, name) : launch_decode_merge(a, stream, name);
 }
 
 }  // namespace pjx
