@@ -188,8 +188,8 @@ __device__ __forceinline__ uint32_t plain_bits(float x) {
   asm volatile("" : "+v"(u));
   return u;
 }
-// Whether a float is an infinity or NaN.
-__device__ __forceinline__ bool not_finite(float x) { return (plain_bits(x) & 0x7f800000u) == 0x7f800000u; }
+// Whether a float's bits are those of an infinity or NaN.
+__device__ __forceinline__ bool not_finite(uint32_t u) { return (u & 0x7f800000u) == 0x7f800000u; }
 
 // 16-bit elements of a dword whose exponent is all ones (infinities, NaN) -> 0.
 template <typename E>
@@ -211,27 +211,39 @@ __device__ __forceinline__ void wave_lds_sync() {
 // Whether a row with this sum of weights has a valid key (a NaN sum: yes).
 __device__ __forceinline__ bool some_key(float sum) { return plain_bits(sum) != 0u; }
 
-// Writes the combined result of one work item: the final 16-bit output and LSE
-// when the item covers the whole sequence, else the unnormalised partial
-// (O relative to max M, plus M and the sum) for the merge kernel.
+// Writes 4 consecutive dims d..d+3 (d a multiple of 4) of one work item's combined
+// result: the final output and LSE when the item covers the whole sequence, else
+// the unnormalised partial (O relative to max M, plus M and the sum) for the merge
+// kernel.  (kPlain promises no alignment of a final output.)
 template <int X>
-__device__ __forceinline__ void emit_row_elem(const DecodeArgs& a, int b, int g, int r, int d,
-                                              size_t part, bool final_out, float M, float Ls,
-                                              float O) {
+__device__ __forceinline__ void emit_row(const DecodeArgs& a, int b, int g, int r, int d, size_t part, bool final_out,
+                                         float M, float Ls, f32x4 O) {
   if (final_out) {
     int t, h;
     row_to_head(a, g, r, t, h);
     const bool some = X == kPlain ? Ls > 0.f : some_key(Ls);
-    const float out = some ? O / Ls : 0.f;
+    f32x4 out;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[e] = some ? O[e] / Ls : 0.f;
     const size_t oi = ((size_t)(b * a.Lq + t) * a.Hq + h) * a.orow + d;
-    if (a.o32)
-      a.o32[oi] = out;
-    else
-      a.o[oi] = a.f16 ? F16Fmt::bits(out) : Bf16Fmt::bits(out);
+    if constexpr (X == kPlain) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (a.o32)
+          a.o32[oi + e] = out[e];
+        else
+          a.o[oi + e] = a.f16 ? F16Fmt::bits(out[e]) : Bf16Fmt::bits(out[e]);
+      }
+    } else if (a.o32) {
+      *(f32x4*)(a.o32 + oi) = out;
+    } else {
+      *(u32x2*)(a.o + oi) = a.f16 ? u32x2{F16Fmt::pack2(out[0], out[1]), F16Fmt::pack2(out[2], out[3])}
+                                  : u32x2{Bf16Fmt::pack2(out[0], out[1]), Bf16Fmt::pack2(out[2], out[3])};
+    }
     if (a.lse && d == 0)
       a.lse[((size_t)b * a.Hq + h) * a.Lq + t] = some ? (M + __log2f(Ls)) * kLn2 : INFINITY;
   } else {
-    a.ws_o[(part * a.rows + r) * a.dv + d] = O;
+    *(f32x4*)(a.ws_o + (part * a.rows + r) * a.dv + d) = O;
     if (d == 0) {
       a.ws_ml[(part * a.rows + r) * 2] = M;
       a.ws_ml[(part * a.rows + r) * 2 + 1] = Ls;
@@ -315,7 +327,7 @@ __device__ bool decode_item(const DecodeArgs& a, int* sched, int& b, int& g, int
   return true;
 }
 
-// emit_row_elem for 4 consecutive dims d..d+3 (d a multiple of 4).
+// emit_row of the latent decode, whose outputs are products with 1 / sum.
 __device__ __forceinline__ void emit_row_quad(const DecodeArgs& a, int b, int g, int r, int d,
                                               size_t part, bool final_out, float M, float Ls,
                                               f32x4 O) {
@@ -364,12 +376,16 @@ __device__ __forceinline__ void emit_row_quad(const DecodeArgs& a, int b, int g,
 
 // Combines the 4 waves' (max, sum, O^T) of row block rb through LDS scratch
 // red (>= 4 x 16 x D floats + 4 x 16 x 2) and emits rows row0 + 16rb .. of the
-// item (D = the output dims).  acc[i] holds O^T[dim 16i + 4*q4 + r][row
-// row0 + 16rb + c16].
-template <int D, int X = kPlain>
-__device__ __forceinline__ void combine_rows(const DecodeArgs& a, float* red, const f32x4* acc,
+// item (D = the output dims).  acc[i] holds quad quad_of(i) of row
+// row0 + 16rb + c16 of O, a quad being 4 consecutive dims.  Rows lie in quads of dims, quad c of row r at c ^ r, so that
+// neither the writes (16 rows at once) nor the reads (a row at once) meet in a bank,
+// and each thread combines a quad (32 rows of 128 element by element: 7 us of the 17
+// of a float32 work item).
+template <int D, int X, typename Q>
+__device__ __forceinline__ void combine_rows(const DecodeArgs& a, float* red, const f32x4* acc, Q quad_of,
                                              float m_run, float l_run, int row0, int rb, int b, int g,
                                              size_t part, bool final_out) {
+  static_assert(D % 64 == 0, "16 quads or more");
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int c16 = lane & 15, q4 = lane >> 4;
   float* red_o = red;                  // [4][16 rows][D]
@@ -377,33 +393,33 @@ __device__ __forceinline__ void combine_rows(const DecodeArgs& a, float* red, co
   __syncthreads();  // the scratch is free (every wave is done with it)
 #pragma unroll
   for (int db = 0; db < D / 16; ++db)
-    *(f32x4*)(red_o + (w * 16 + c16) * D + 16 * db + 4 * q4) = acc[db];
-  if (q4 == 0) {
-    red_ml[(w * 16 + c16) * 2] = m_run;
-    red_ml[(w * 16 + c16) * 2 + 1] = l_run;
-  }
+    *(f32x4*)(red_o + (w * 16 + c16) * D + 4 * (quad_of(db) ^ c16)) = acc[db];
+  if (q4 == 0) *(float2*)(red_ml + (w * 16 + c16) * 2) = make_float2(m_run, l_run);
   __syncthreads();
   const int nr = min(16, a.rows - row0 - 16 * rb);
-  for (int e = tid; e < nr * D; e += 256) {
-    const int r = e / D, d = e % D;
+  for (int e = tid; e < nr * (D / 4); e += 256) {
+    const int r = e / (D / 4), c = e % (D / 4), d = 4 * c;
     if (d >= a.orow) continue;
+    float2 ml[4];
     float M = kMaxInit;
 #pragma unroll
-    for (int ww = 0; ww < 4; ++ww) M = fmaxf(M, red_ml[(ww * 16 + r) * 2]);
-    float Ls = 0.f, O = 0.f;
+    for (int ww = 0; ww < 4; ++ww) {
+      ml[ww] = *(const float2*)(red_ml + (ww * 16 + r) * 2);
+      M = fmaxf(M, ml[ww].x);
+    }
+    float Ls = 0.f;
+    f32x4 O = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int ww = 0; ww < 4; ++ww) {
-      const float wt = fast_exp2(red_ml[(ww * 16 + r) * 2] - M);
-      Ls = fmaf(wt, red_ml[(ww * 16 + r) * 2 + 1], Ls);
-      O = fmaf(wt, red_o[(ww * 16 + r) * D + d], O);
+      const float wt = fast_exp2(ml[ww].x - M);
+      Ls = fmaf(wt, ml[ww].y, Ls);
+      const f32x4 o = *(const f32x4*)(red_o + (ww * 16 + r) * D + 4 * (c ^ r));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) O[i] = fmaf(wt, o[i], O[i]);
     }
-    if constexpr (X == kTree) {
-      if (!tree_token(a, b, (row0 + 16 * rb + r) % a.Lq)) {  // a row without a valid key
-        M = kMaxInit;
-        Ls = O = 0.f;
-      }
-    }
-    emit_row_elem<X>(a, b, g, row0 + 16 * rb + r, d, part, final_out, M, Ls, O);
+    if constexpr (X == kTree)
+      if (!some_key(Ls)) O = f32x4{0.f, 0.f, 0.f, 0.f};  // a row without a valid key
+    emit_row<X>(a, b, g, row0 + 16 * rb + r, d, part, final_out, M, Ls, O);
     if constexpr (X == kScores) {  // the weights' kernel reads every item's statistics
       if (final_out && d == 0) {
         a.ws_ml[(part * a.rows + row0 + 16 * rb + r) * 2] = M;
@@ -414,8 +430,8 @@ __device__ __forceinline__ void combine_rows(const DecodeArgs& a, float* red, co
 }
 
 // kTree: adds p * v for the infinite and NaN elements v of a 32-key step's V
-// rows to the rows that see the key; v_at(key, dim, odd) gives 4 elements from
-// dim and the mask of such ones.
+// rows to the rows that see the key; v_at(key, db, odd) gives the lane's 4 elements
+// of output block db and the mask of such ones.
 // s holds the step's p (lane layout of S^T), px 512 floats of this wave.
 template <int NRB, int NDB, typename V>
 __device__ __forceinline__ void add_unbounded(const DecodeArgs& a, const TreeTable& tree, float* px,
@@ -437,7 +453,7 @@ __device__ __forceinline__ void add_unbounded(const DecodeArgs& a, const TreeTab
 #pragma unroll
       for (int db = 0; db < NDB; ++db) {
         int odd = 0;
-        const f32x4 v = v_at(k0 + i, 16 * db + 4 * q4, odd);
+        const f32x4 v = v_at(k0 + i, db, odd);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           if (sees && (odd >> e & 1)) acc[rb][db][e] = fmaf(p, v[e], acc[rb][db][e]);
@@ -503,6 +519,7 @@ __device__ __forceinline__ void gqa_decode(const DecodeArgs& a) {
   __shared__ typename std::conditional<X == kTree, TreeTable, int>::type tree;
   __shared__ float tree_p[X == kTree ? 4 * 512 : 1];
   int tok[NRB];
+  bool has[NRB];  // kTree: the row's slot holds a token
   const int rd = ROWS ? a.orow : D, rdv = ROWS ? a.orow : DV;
   typename E::v8 qf[NRB][KSTEPS];
 #pragma unroll
@@ -512,6 +529,7 @@ __device__ __forceinline__ void gqa_decode(const DecodeArgs& a) {
     int t = 0, h = 0;
     if (rv) row_to_head(a, g, row, t, h);
     tok[rb] = t;
+    has[rb] = X != kTree || tree_token(a, b, t);
     const uint16_t* qrow = a.q + ((size_t)(b * a.Lq + t) * a.Hq + h) * rd;
 #pragma unroll
     for (int s = 0; s < KSTEPS; ++s) {
@@ -656,7 +674,7 @@ __device__ __forceinline__ void gqa_decode(const DecodeArgs& a) {
     bool unbounded = false;
     if constexpr (X == kTree) {
       if (kn > P) {
-        bool any = false;
+        uint32_t odd = 0;
 #pragma unroll
         for (int i = 0; i < VU; ++i)
 #pragma unroll
@@ -664,10 +682,10 @@ __device__ __forceinline__ void gqa_decode(const DecodeArgs& a) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const uint32_t x = finite_halves<E>(vr[i][j][e]);
-              any |= x != vr[i][j][e];
+              odd |= x ^ vr[i][j][e];
               vr[i][j][e] = x;
             }
-        unbounded = wave_any(any);
+        unbounded = wave_any(odd != 0u);
       }
     }
     store_vt();
@@ -790,7 +808,8 @@ __device__ __forceinline__ void gqa_decode(const DecodeArgs& a) {
     wave_lds_sync();
     if constexpr (X == kTree) {
       if (unbounded)
-        add_unbounded<NRB, NDB>(a, tree, tree_p + 512 * w, s, acc, tok, k0, w1, P, [&](int key, int d, int& odd) {
+        add_unbounded<NRB, NDB>(a, tree, tree_p + 512 * w, s, acc, tok, k0, w1, P, [&](int key, int db, int& odd) {
+          const int d = 16 * db + 4 * q4;
           if (ROWS && d >= rdv) return f32x4{};
           const u32x2 u = *(const u32x2*)(Vb + (size_t)key * v_tok + d);
 #pragma unroll
@@ -811,8 +830,8 @@ __device__ __forceinline__ void gqa_decode(const DecodeArgs& a) {
   const size_t part = (size_t)bg * a.nch + chunk_id;
 #pragma unroll
   for (int rb = 0; rb < NRB; ++rb)
-    combine_rows<DV, X>(a, (float*)vt_lds, acc[rb], m_run[rb], xor32_sum(xor16_sum(l_run[rb])), row0, rb, b, g,
-                     part, final_out);
+    combine_rows<DV, X>(a, (float*)vt_lds, acc[rb], [&](int i) { return 4 * i + q4; }, has[rb] ? m_run[rb] : kMaxInit,
+                        has[rb] ? xor32_sum(xor16_sum(l_run[rb])) : 0.f, row0, rb, b, g, part, final_out);
 }
 
 // ---------------------------------------------------------------------------
@@ -823,8 +842,8 @@ __device__ __forceinline__ void gqa_decode(const DecodeArgs& a) {
 // index q4, so each lane's K and Q^T operands are float4 loads of dims
 // 16j + 4*q4 .. +3.  P.V's B operand for step e is the score register e
 // itself (keys 4*q4 + e of a 16-key block), and its A operand V[key][dim] is
-// loaded per lane (16 lanes read 16 consecutive dims of one key row).  Up to
-// 32 rows (2 row blocks).
+// loaded per lane, 4 consecutive dims, one for each of 4 blocks (block i's rows are
+// the dims 64(i/4) + 4*row + i%4).  Up to 32 rows (2 row blocks).
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ f32x4 mfma16x16x4f32(float a, float b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
@@ -862,6 +881,7 @@ __device__ __forceinline__ void gqa_decode_f32(const DecodeArgs& a) {
     if (c0 + a.chunk > P) build_tree<kDecThreads / 64>(a, b, tree);
   }
   int tok[NRB];
+  bool has[NRB];
 
   f32x4 qf[NRB][NJ];
 #pragma unroll
@@ -871,6 +891,7 @@ __device__ __forceinline__ void gqa_decode_f32(const DecodeArgs& a) {
     int t = 0, h = 0;
     if (rv) row_to_head(a, g, row, t, h);
     tok[rb] = t;
+    has[rb] = X != kTree || tree_token(a, b, t);
     const float* qrow = Q + ((size_t)(b * a.Lq + t) * a.Hq + h) * D;
 #pragma unroll
     for (int j = 0; j < NJ; ++j) qf[rb][j] = rv ? *(const f32x4*)(qrow + 16 * j + 4 * q4) : f32x4{};
@@ -896,16 +917,22 @@ __device__ __forceinline__ void gqa_decode_f32(const DecodeArgs& a) {
 #pragma unroll
       for (int j = 0; j < NJ; ++j) kf[kb][j] = *(const f32x4*)(kp + 16 * j);
     }
-    // V[key 16kb + 4*q4 + e][dim 16i + c16] for the A operands of P.V
-    float vv[2][4][NDB];
+    // V[key 16kb + 4*q4 + e][dim 64(i/4) + 4*c16 + i%4] for the A operands of P.V, as
+    // bits: 16 bytes a load, which give the rows of four blocks (a dword a load, of
+    // dims 16i + c16: 5 us of 17 to issue, at 128 dims)
+    uint32_t vv[2][4][NDB];
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int key = k0 + 16 * kb + 4 * q4 + e;
-        const float* vp = Vb + (size_t)min(key, w1 - 1) * v_tok + c16;
+        const float* vp = Vb + (size_t)min(key, w1 - 1) * v_tok + 4 * c16;
 #pragma unroll
-        for (int i = 0; i < NDB; ++i) vv[kb][e][i] = vp[16 * i];
+        for (int i = 0; i < NDB; i += 4) {
+          const u32x4 u = *(const u32x4*)(vp + 16 * i);
+#pragma unroll
+          for (int t = 0; t < 4; ++t) vv[kb][e][i + t] = u[t];
+        }
       }
     // S^T for keys k0 + 16*kb + 4*q4 + r, query row 16rb + c16.
     f32x4 s[NRB][2];
@@ -926,7 +953,7 @@ __device__ __forceinline__ void gqa_decode_f32(const DecodeArgs& a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
 #pragma unroll
-          for (int i = 0; i < NDB; ++i) vv[kb][e][i] = k0 + 16 * kb + 4 * q4 + e < w1 ? vv[kb][e][i] : 0.f;
+          for (int i = 0; i < NDB; ++i) vv[kb][e][i] = k0 + 16 * kb + 4 * q4 + e < w1 ? vv[kb][e][i] : 0u;
 #pragma unroll
       for (int rb = 0; rb < NRB; ++rb)
 #pragma unroll
@@ -944,11 +971,11 @@ __device__ __forceinline__ void gqa_decode_f32(const DecodeArgs& a) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
 #pragma unroll
-            for (int i = 0; i < NDB; ++i)
-              if (not_finite(vv[kb][e][i])) {
-                vv[kb][e][i] = 0.f;
-                any = true;
-              }
+            for (int i = 0; i < NDB; ++i) {
+              const bool out = not_finite(vv[kb][e][i]);
+              any |= out;
+              vv[kb][e][i] = out ? 0u : vv[kb][e][i];
+            }
 #pragma unroll
             for (int rb = 0; rb < NRB; ++rb)
               if (!tree_sees(tree, a.Lq, tok[rb], k0 + 16 * kb + 4 * q4 + e - P)) s[rb][kb][e] = -INFINITY;
@@ -1000,16 +1027,21 @@ __device__ __forceinline__ void gqa_decode_f32(const DecodeArgs& a) {
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[rb][i] = mfma16x16x4f32(vv[kb][e][i], s[rb][kb][e], acc[rb][i]);
+          for (int e = 0; e < 4; ++e) acc[rb][i] = mfma16x16x4f32(__uint_as_float(vv[kb][e][i]), s[rb][kb][e], acc[rb][i]);
       }
     }
     if constexpr (X == kTree) {
       if (unbounded)
-        add_unbounded<NRB, NDB>(a, tree, tree_p + 512 * w, s, acc, tok, k0, w1, P, [&](int key, int d, int& odd) {
-          const u32x4 u = *(const u32x4*)(Vb + (size_t)key * v_tok + d);
+        add_unbounded<NRB, NDB>(a, tree, tree_p + 512 * w, s, acc, tok, k0, w1, P, [&](int key, int db, int& odd) {
+          const uint32_t* vr = (const uint32_t*)(Vb + (size_t)key * v_tok) + 64 * (db / 4) + 16 * q4 + db % 4;
+          f32x4 v;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) odd |= not_finite(__uint_as_float(u[e])) ? 1 << e : 0;
-          return __builtin_bit_cast(f32x4, u);
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t u = vr[4 * e];
+            odd |= not_finite(u) ? 1 << e : 0;
+            v[e] = __uint_as_float(u);
+          }
+          return v;
         });
     }
   }
@@ -1017,9 +1049,15 @@ __device__ __forceinline__ void gqa_decode_f32(const DecodeArgs& a) {
   const bool final_out = c0 == 0 && L <= a.chunk;
   const size_t part = (size_t)bg * a.nch + chunk_id;
 #pragma unroll
-  for (int rb = 0; rb < NRB; ++rb)
-    combine_rows<DV, X>(a, red, acc[rb], m_run[rb], xor32_sum(xor16_sum(l_run[rb])), row0, rb, b, g, part,
-                     final_out);
+  for (int rb = 0; rb < NRB; ++rb) {
+    f32x4 o[NDB];  // quad 16j + 4*q4 + r: element r of the four blocks 4j ..
+#pragma unroll
+    for (int i = 0; i < NDB; ++i)
+#pragma unroll
+      for (int t = 0; t < 4; ++t) o[i][t] = acc[rb][i / 4 * 4 + t][i % 4];
+    combine_rows<DV, X>(a, red, o, [&](int i) { return i / 4 * 16 + 4 * q4 + i % 4; }, has[rb] ? m_run[rb] : kMaxInit,
+                        has[rb] ? xor32_sum(xor16_sum(l_run[rb])) : 0.f, row0, rb, b, g, part, final_out);
+  }
 }
 
 // Exact merge of the chunk partials of one (batch, group, query row):

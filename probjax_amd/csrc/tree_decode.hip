@@ -45,8 +45,9 @@ static int run_tree(DecodeArgs& a, int d, int nrb, void* ws, size_t ws_bytes, hi
 
 template <int D>
 static int run_tree_f32(DecodeArgs& a, int nrb, void* ws, size_t ws_bytes, hipStream_t s, const char* who) {
-  return nrb == 1 ? run_decode<tree_decode_f32_kernel<D, 1>>(a, ws, ws_bytes, s, who)
-                  : run_decode<tree_decode_f32_kernel<D, 2>>(a, ws, ws_bytes, s, who);
+  if constexpr (D <= 128)
+    if (nrb > 1) return run_decode<tree_decode_f32_kernel<D, 2>>(a, ws, ws_bytes, s, who);
+  return run_decode<tree_decode_f32_kernel<D, 1>>(a, ws, ws_bytes, s, who);
 }
 
 // Argument checks shared by the decode forms of this library's cache operators:
@@ -140,7 +141,7 @@ extern "C" int pjx_tree_decode(int dtype, const void* q, const void* k, const vo
   const int d = (int)head_dim;
   if (tree_wide_takes(a, d, f32)) return run_tree_wide(a, d, chunk == 0, workspace, workspace_bytes, s, who);
   // (at most 32 rows, or rows too far apart in memory for the wide kernel)
-  const int nrb = std::min(gqa_row_blocks(a.rows, d, d, f32), 2);
+  const int nrb = std::min(gqa_row_blocks(a.rows, d, d, f32), f32 && d == 256 ? 1 : 2);
   a.rpg = kRows * nrb;
   if (f32)
     return d == 64    ? run_tree_f32<64>(a, nrb, workspace, workspace_bytes, s, who)

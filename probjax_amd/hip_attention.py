@@ -655,6 +655,13 @@ def _int32(t, what: str, like, *shapes):
     return t
 
 
+@functools.lru_cache(maxsize=256)
+def _workspace_size(entry: str, *sizes) -> int:
+    """What the entry point's size query answers (a function of the sizes alone; a
+    call of the library takes 1 us)."""
+    return getattr(native.load(), entry)(*sizes)
+
+
 def _scratch(nbytes: int, like, workspace=None):
     """``nbytes`` of workspace on the device of ``like``: ``workspace`` if it holds
     them, else new."""
@@ -740,7 +747,7 @@ def tree_decode(
         raise ValueError(f"a cache of {S} slots does not hold {T} drafted tokens")
     L = None if kv_lengths is None else _int32(kv_lengths, "kv_lengths", q, (B,))
     lib = native.load()
-    nbytes = lib.pjx_decode_workspace_size(B, Hkv, (Hq // Hkv) * T, S, width, chunk)
+    nbytes = _workspace_size("pjx_decode_workspace_size", B, Hkv, (Hq // Hkv) * T, S, width, chunk)
     ws = _scratch(nbytes, q, workspace)
     o = torch.empty_like(q)
     lse = torch.empty((B, Hq, T), dtype=torch.float32, device=q.device) if return_lse else None
@@ -783,7 +790,7 @@ def weighted_decode(
     weights = _key_weights(weights, q, B, Hkv, S)
     L = None if kv_lengths is None else _int32(kv_lengths, "kv_lengths", q, (B,))
     lib = native.load()
-    nbytes = lib.pjx_weighted_decode_workspace_size(B, Hkv, rows, S, width, chunk)
+    nbytes = _workspace_size("pjx_weighted_decode_workspace_size", B, Hkv, rows, S, width, chunk)
     ws = _scratch(nbytes, q, workspace)
     o = torch.empty_like(q)
     out = torch.empty((B, Hkv, S), dtype=torch.float32, device=q.device) if weights is None else torch.empty_like(weights)
@@ -817,7 +824,7 @@ def key_weights(
     L = None if kv_lengths is None else _int32(kv_lengths, "kv_lengths", q, (B,))
     q, k, lse = _aligned(q.contiguous()), _aligned(k.contiguous()), lse.contiguous()
     lib = native.load()
-    nbytes = lib.pjx_key_weights_workspace_size(B, T, S, Hq)
+    nbytes = _workspace_size("pjx_key_weights_workspace_size", B, T, S, Hq)
     ws = _scratch(nbytes, q, workspace)
     out = torch.empty((B, Hkv, S), dtype=torch.float32, device=q.device)
     _call(
