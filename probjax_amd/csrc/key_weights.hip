@@ -6,11 +6,18 @@
 // Decode steps (few rows): the split-KV decode (decode_common.h) also keeps its
 // scores, 4 bytes a row and key beside the 2 (D + D) bytes of a 16-bit key, and
 // a second kernel sums their exponentials once the rows' statistics are known.
-// Forming the scores again instead would read K, half of the cache, again.
+// Forming the scores again instead would read K, half of the cache, again.  bf16, 8 KV
+// heads of 128, 4 rows each: 32 sequences of 512 .. 8192 keys (588 MB) 125 us, bound by
+// HBM (the decode without scores 107), and 12 us for the second kernel; one of 4096
+// keys 8 and 4.7 us, bound by latency.
 //
 // Prompts (many rows): the scores are too many to keep.  They are formed again
 // on the matrix units, keys as MFMA rows, so a lane's accumulators are sums of
-// its own 16 keys and nothing is exchanged until the end.
+// its own 16 keys and nothing is exchanged until the end.  bf16, 4096 causal rows of
+// 16 heads over 4 KV heads of 128: 58 us, 590 TFLOP/s, bound by the exponentials (one
+// for every 256 operations) beside the products; the sum over the splits 4.8 us.
+//
+// Scores, their exponentials and every sum are float32, in a fixed order.
 #include <stdio.h>
 
 #include "decode_common.h"

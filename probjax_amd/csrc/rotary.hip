@@ -9,8 +9,10 @@
 // from a few thousand on), so a workgroup forms the cosines and sines of its
 // tokens once, in LDS, and all heads of q and k use them.  A thread keeps its place
 // within the rows and takes four of them at a time, their loads issued before the
-// first store.  bf16, 12288 tokens of 16 + 16 heads of 128 (201 MB): see the table
-// at the launch.
+// first store.  The products and the sum are float32, rounded to the type once.  bf16,
+// 12288 tokens of 16 + 16 heads of 128 (201 MB): 45 us interleaved, 4.5 TB/s; halves,
+// 2 x 4096 tokens of 16 + 4 heads (84 MB): 21.6 us, 3.9 TB/s; one row a thread at a
+// time took 51 and 30.
 #include <stdio.h>
 
 #include "pjx_common.h"

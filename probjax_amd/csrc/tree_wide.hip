@@ -8,13 +8,16 @@
 // each wave keys of its own and all rows, 16 at a time: it reads K and V without
 // LDS, but its accumulators of 64 rows leave one wave per SIMD, and every further
 // 64 rows read the cache again (1 / 16 / 8 sequences of the table at the launch:
-// 55 / 128 / 296 us for 19 / 76 / 58).
+// 55 / 128 / 296 us for 18 / 68 / 50).
 //
 // Row groups of one work item are placed 8 workgroups apart, on one XCD, whose
 // L2 gives all but the first their K and V (HBM traffic of 244 rows, two groups:
-// that of one).  Bound by latency on one sequence (launch, lengths, first tile,
-// table and four tiles in turn: 16 us), by HBM on 16 (285 MB in 68 us), by the waves'
-// chains of a tile (1.5 us for two) and the partial results on the widest.
+// that of one).  Bound by latency on one sequence (launch, lengths, first tile and
+// four tiles in turn, 1 us each: 15 us), by HBM on 16 (285 MB in 68 us, 4.2 TB/s), on
+// the widest by a tile's work on each SIMD and in LDS, about 1000 cycles each of
+// matrix instructions, exponentials and reads for the 2500 that a tile takes.
+// The weights p enter their product with V rounded to the 16-bit type, as the flash
+// forward's do; scores, sums and outputs are float32 until the last store.
 #include "decode_common.h"
 #include "flash_common.h"
 
@@ -376,9 +379,10 @@ int run_tree_wide(DecodeArgs& a, int head_dim, bool auto_chunk_size, void* ws, s
   // workgroups per CU remain, one of eight waves or two of four: every chunk's
   // partial results cost as much traffic as a key a row, written and read again.
   // MI355X, us, chunk 256 / 512 / 1024 / 2048 / 4096, 8 KV heads of 128:
-  //   1 x 4096, 104 rows   64 rows 20 / 21 / 27 / 40 / 66      128 rows 21 / 25 / 36 / 59 (four waves)
-  //   16 x 8192, 64 rows   64 rows 107 / 91 / 82 / 77 / 99
-  //   8 x 4096, 244 rows   128 rows 115 / 80 / 71 / 58 / 83    (four waves: 91 / 72 / 61 / 68 / 106)
+  //   1 x 4096, 104 rows               64 rows 18 / 20 / 26 / 39 / 65   128 rows 20 / 22 / 28 / 44 / 73
+  //   16 x 512 .. 8192 keys, 64 rows   64 rows 103 / 88 / 75 / 68 / 90
+  //   8 x 1500 .. 4096 keys, 244 rows  64 rows 92 / 70 / 58 / 50 / 67   128 rows 105 / 74 / 63 / 50 / 75
+  //   8 x 4096, 244 rows, the chunk as chosen: 64 rows 56, 128 rows 52; 8 x 2048, 1024 rows: 119, 105
   const int64_t pairs = (int64_t)a.B * a.G;
   const int rw = a.rows <= 64 || pairs * ((a.Lk + 511) / 512) * ((a.rows + 127) / 128) < 512 ? 2 : 4;
   if (auto_chunk_size) {
