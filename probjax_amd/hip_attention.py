@@ -903,6 +903,8 @@ def _check_evict_out(out, ins, keep: int) -> None:
         raise ValueError("out needs contiguous features and contiguous weights")
     if any(n > 1 and s == 0 for t in (k_out, v_out) for n, s in zip(t.shape, t.stride())):
         raise ValueError("out must not be expanded")
+    if any(t.requires_grad for t in out):
+        raise ValueError("out must not require a gradient")
     read = {t.untyped_storage().data_ptr() for t in ins if t.numel()}
     write = [t.untyped_storage().data_ptr() for t in out if t.numel()]
     if read & set(write) or len(set(write)) != len(write):

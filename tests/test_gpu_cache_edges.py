@@ -1,0 +1,172 @@
+"""Calls of the cache and position operators that their documentation allows at the
+edges: nothing to do, one tensor given twice, shared and overlapping views, the
+largest drafts, calls on two streams at once."""
+
+import math
+
+import numpy as np
+import pytest
+
+from oracle import cache_ops as ref
+from tests._helpers import to_np
+from tests.test_gpu_key_weights import check_weights
+from tests.test_gpu_tree_attention import _inputs, _types, check, random_parents
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("name", ["bf16", "f32"])
+@pytest.mark.parametrize("B,T,S", [(0, 3, 70), (2, 0, 70), (2, 1, 0), (2, 70, 0), (0, 0, 0)])
+def test_nothing_to_do(device, name, B, T, S):
+    import torch
+    from probjax_amd import masks
+    from probjax_amd.attention import attention_with_key_weights, evict_keys, rotary, tree_attention
+
+    (q, k, v), _ = _inputs(1, _types()[name], B, T, S, 4, 2, 64, device)
+    w = torch.rand((B, 2, S), device=device)
+    for mask in (None, masks.CausalMask()):
+        out, sums, lse = attention_with_key_weights(q, k, v, w, mask=mask, return_lse=True)
+        torch.cuda.synchronize()
+        assert out.shape == q.shape and not out.any()
+        assert torch.equal(sums, w) and torch.isposinf(lse).all()
+    y, z = rotary(q, q, torch.arange(T, device=device))
+    assert y.shape == z.shape == q.shape
+    kept = evict_keys(k, v, w, 5)
+    torch.cuda.synchronize()
+    assert kept.k.shape == (B, 5, 2, 64)
+    if S:
+        assert torch.equal(kept.kv_lengths, torch.full((B,), 5, dtype=torch.int32, device=device))
+    else:
+        assert not kept.kv_lengths.any() and not kept.k.any() and (kept.index == -1).all()
+    if T:
+        got, lse = tree_attention(q, k, v, parents=list(range(-1, T - 1)),
+                                  kv_lengths=torch.zeros(B, dtype=torch.int32, device=device), return_lse=True)
+        torch.cuda.synchronize()
+        assert got.shape == q.shape
+        if S == 0:
+            assert not got.any() and torch.isposinf(lse).all()
+
+
+@pytest.mark.parametrize("name,Hq,Hkv,T,D", [("bf16", 8, 2, 5, 64), ("f16", 16, 2, 9, 128), ("f32", 4, 1, 5, 64)])
+def test_one_cache_for_every_sequence_and_for_k_and_v(device, name, Hq, Hkv, T, D):
+    """k and v the same tensor, shared by the batch (stride 0), windows of one
+    longer buffer that overlap."""
+    import torch
+    from probjax_amd import masks
+    from probjax_amd.attention import attention_with_key_weights, tree_attention
+
+    B, S = 3, 200
+    dtype, scale = _types()[name], 1.0 / math.sqrt(D)
+    (q, k, _), (qn, kn, _) = _inputs(2, dtype, B, T, S, Hq, Hkv, D, device)
+    shared, shared_n = k[:1].expand(B, S, Hkv, D), np.broadcast_to(kn[:1], kn.shape)
+    slide = torch.as_strided(k.contiguous(), (B, S, Hkv, D), (64 * Hkv * D, Hkv * D, D, 1))
+    for kk, host in ((shared, shared_n), (slide, to_np(slide).astype(np.float64))):
+        L = [150, 3, 0]
+        parents = random_parents(np.random.default_rng(5), B, T)
+        sees, token = zip(*(ref.tree_sees(p) for p in parents))
+        lengths = torch.tensor(L, dtype=torch.int32, device=device)
+        out, lse = tree_attention(q, kk, kk, parents=parents, kv_lengths=lengths, return_lse=True)
+        check(out, lse, ref.tree_attention(qn, host, host, L, sees, token, scale), dtype, D, S)
+        one = q[:, 1:2]
+        out, w, lse = attention_with_key_weights(one, kk, kk, mask=masks.KVLenMask(lengths), return_lse=True)
+        keep = np.arange(S)[None, None, :] < np.array(L)[:, None, None]
+        zero = np.zeros((B, Hkv, S))
+        want = ref.key_weight_attention(qn[:, 1:2], host, host, zero, keep, scale)
+        check(out, lse, want, dtype, D, S)
+        check_weights(w, want, zero, D, S, Hq // Hkv)
+
+
+@pytest.mark.parametrize("name,Hq,Hkv,T,D,S", [
+    ("bf16", 4, 1, 256, 64, 700), ("f16", 2, 2, 256, 128, 300), ("f32", 2, 1, 256, 64, 300), ("bf16", 2, 1, 200, 256, 260),
+    ("f32", 3, 1, 40, 256, 150), ("f16", 1, 1, 65, 72, 129), ("bf16", 64, 1, 1, 64, 257), ("f32", 64, 1, 1, 128, 257),
+])
+def test_the_largest_drafts_and_groups(device, name, Hq, Hkv, T, D, S):
+    import torch
+    from probjax_amd.attention import attention_with_key_weights, tree_attention
+
+    B, dtype, scale = 2, _types()[name], 1.0 / math.sqrt(D)
+    (q, k, v), host = _inputs(6, dtype, B, T, S, Hq, Hkv, D, device)
+    rng = np.random.default_rng(T)
+    parents = random_parents(rng, B, T, absent=True)
+    sees, token = zip(*(ref.tree_sees(p) for p in parents))
+    L = [max(S - T, 0), 17]
+    out, lse = tree_attention(q, k, v, parents=parents, kv_lengths=torch.tensor(L, device=device), return_lse=True)
+    check(out, lse, ref.tree_attention(*host, L, sees, token, scale), dtype, D, S)
+    mask = rng.random((T, T)) < 0.1
+    out, lse = tree_attention(q, k, v, tree_mask=torch.from_numpy(mask).to(device), return_lse=True,
+                              kv_lengths=torch.tensor([0, S], device=device))
+    check(out, lse, ref.tree_attention(*host, [0, S], [mask] * B, np.ones((B, T), bool), scale), dtype, D, S)
+    if T == 1:
+        zero, keep = np.zeros((B, Hkv, S)), np.ones((B, 1, S), bool)
+        out, w, lse = attention_with_key_weights(q, k, v, return_lse=True)
+        want = ref.key_weight_attention(*host, zero, keep, scale)
+        check(out, lse, want, dtype, D, S)
+        check_weights(w, want, zero, D, S, Hq)
+
+
+def test_two_streams_at_once(device):
+    """The same inputs used by calls on two streams, each result its own."""
+    import torch
+    from probjax_amd import masks
+    from probjax_amd.attention import attention_with_key_weights, evict_keys, rotary, tree_attention
+
+    B, S, T = 4, 2000, 9
+    (q, k, v), _ = _inputs(7, torch.bfloat16, B, T, S, 8, 2, 128, device)
+    L = torch.tensor([2000, 700, 1, 1300], dtype=torch.int32, device=device)
+    w = torch.rand((B, 2, S), device=device)
+    pos = torch.arange(T, device=device)
+
+    def step():
+        y = rotary(q, None, pos)
+        out, sums = attention_with_key_weights(y[:, :1], k, v, w, mask=masks.KVLenMask(L))
+        prompt = attention_with_key_weights(k, k, v, w, mask=masks.CausalMask())
+        return (out, sums, *prompt, *evict_keys(k, v, sums, 500, kv_lengths=L, recent=8),
+                tree_attention(y, k, v, parents=[-1, 0, 0, 1, 1, 2, 2, 3, 3], kv_lengths=L - T))
+
+    want = step()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(device) for _ in range(2)]
+    for _ in range(3):
+        got = []
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(step())
+        torch.cuda.synchronize()
+        for g in got:
+            for x, y in zip(g, want):
+                assert torch.equal(x, y)
+
+
+def test_evicting_into_buffers_that_require_a_gradient_is_refused(device):
+    import torch
+    from probjax_amd.attention import evict_keys
+
+    (_, k, v), _ = _inputs(8, torch.bfloat16, 1, 1, 40, 2, 2, 64, device)
+    w = torch.rand((1, 2, 40), device=device)
+    out = [torch.zeros((1, 10, 2, 64), dtype=torch.bfloat16, device=device) for _ in range(2)]
+    out.append(torch.zeros((1, 2, 10), device=device))
+    out[0].requires_grad_()
+    with pytest.raises(ValueError, match="gradient"):
+        evict_keys(k, v, w, 10, out=tuple(out))
+
+
+@pytest.mark.parametrize("Hq", [2, 16])  # 6 and 48 rows per KV head
+def test_more_sequences_than_the_schedule_sorts(device, Hq):
+    import torch
+    from probjax_amd import masks
+    from probjax_amd.attention import attention_with_key_weights, tree_attention
+
+    B, T, S, D = 300, 6, 300, 64
+    (q, k, v), host = _inputs(9, torch.bfloat16, B, T, S, Hq, 2, D, device)
+    rng = np.random.default_rng(3)
+    L = rng.integers(0, S + 1, B)
+    parents = random_parents(rng, B, T)
+    sees, token = zip(*(ref.tree_sees(p) for p in parents))
+    lengths = torch.from_numpy(L).to(device)
+    out, lse = tree_attention(q, k, v, parents=parents, kv_lengths=lengths, return_lse=True)
+    check(out, lse, ref.tree_attention(*host, L, sees, token, D ** -0.5), torch.bfloat16, D, S)
+    zero, keep = np.zeros((B, 2, S)), np.arange(S)[None, None, :] < L[:, None, None]
+    out, w, lse = attention_with_key_weights(q[:, :1], k, v, mask=masks.KVLenMask(lengths), return_lse=True)
+    want = ref.key_weight_attention(host[0][:, :1], host[1], host[2], zero, keep, D ** -0.5)
+    check(out, lse, want, torch.bfloat16, D, S)
+    check_weights(w, want, zero, D, S, Hq // 2)
