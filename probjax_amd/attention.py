@@ -44,8 +44,8 @@ from typing import NamedTuple
 import torch
 
 from . import hip_attention as hip
-from .masks import (LoweredBias, LoweredMask, dense_distance, dense_keep, dense_relpos, dense_supported, lower_bias,
-                    lower_mask, split_low_rank_bias)
+from .masks import (KVLenMask, LoweredBias, LoweredMask, dense_distance, dense_keep, dense_relpos, dense_supported,
+                    lower_bias, lower_mask, split_low_rank_bias)
 
 HIP_ARCH = "gfx950"
 HALF_DTYPES = (torch.bfloat16, torch.float16)  # the 16-bit (MFMA bf16 / fp16) kernels
@@ -645,41 +645,47 @@ def attention_with_key_weights(q, k, v, key_weights=None, *, mask=None, sm_scale
 
     Steps of up to 64 rows ``(Hq/Hkv)*T`` without a causal mask run the
     split-KV decode, which keeps its scores; longer ones the flash forward and a
-    second pass over the scores.  No gradient: inputs that require one raise.
+    second pass over the scores.  Keys past a sequence's length reach nothing,
+    whatever they hold; what a causal mask hides enters products with weights of
+    0, as in ``mha``, so V has to be finite there.  No gradient: inputs that
+    require one raise.
     """
     who = "attention with key weights"
     if q.ndim != 4 or k.ndim != 4 or v.ndim != 4:
         raise ValueError(f"{who}: q must be [B, T, Hq, D], k and v [B, S, Hkv, D]")
-    _gqa_group(q.shape[-2], k.shape[-2])
     B, T, Hq, D = q.shape
-    if _needs_grad(q, k, v) or (key_weights is not None and _needs_grad(key_weights)):
-        raise ValueError(f"{who} has no gradient: call it under torch.no_grad() or on detached tensors")
-    lm = lower_mask(mask)
-    if lm is not None and lm.row_kv_lengths is not None and T == 1:  # one row: per-batch lengths
-        lm.kv_lengths, lm.row_kv_lengths = _row_kv_lengths(lm.row_kv_lengths, B, 1, q.device)[:, 0], None
-    if lm is None or lm.q_valid is not None or lm.kv_valid is not None or lm.extended and not _only_shifted(lm):
-        raise ValueError(f"{who} takes no mask, KVLenMask and causal masks, got {type(mask).__name__}")
+    group = _gqa_group(Hq, k.shape[2])
+    causal, lengths = False, None
+    if type(mask) is KVLenMask:  # (a decode step's: nothing to lower)
+        lengths = mask.kv_lengths
+    elif mask is not None:
+        lm = lower_mask(mask)
+        if lm is not None and lm.row_kv_lengths is not None and T == 1:  # one row: per-batch lengths
+            lm.kv_lengths, lm.row_kv_lengths = _row_kv_lengths(lm.row_kv_lengths, B, 1, q.device)[:, 0], None
+        if lm is None or lm.q_valid is not None or lm.kv_valid is not None or lm.extended and not _only_shifted(lm):
+            raise ValueError(f"{who} takes no mask, KVLenMask and causal masks, got {type(mask).__name__}")
+        causal, lengths = lm.causal, lm.kv_lengths
     if sm_scale is None:
         sm_scale = 1.0 / math.sqrt(D)
-    lse = None
-    if not lm.causal and (Hq // k.shape[2]) * T <= hip.WEIGHTED_DECODE_MAX_ROWS and T > 0:
-        out, weights, *lse = hip.weighted_decode(q, k, v, key_weights, sm_scale=sm_scale, kv_lengths=lm.kv_lengths,
-                                                 return_lse=return_lse)
-        lse = lse[0] if lse else None
-    else:
-        width = _kernel_width(D, q.dtype)
-        if width is None:
-            raise ValueError(f"{who}: head dims up to {FLASH_HEAD_DIMS[-1]}, got {D}")
-        rows = None
-        if width != D:
-            rows = hip.rows_width(D, max(Hq, k.shape[2])) if q.dtype in HALF_DTYPES else None
-            if rows is None:
-                q, k, v = _pad_features(q, width), _pad_features(k, width), _pad_features(v, width)
-        mods = hip.ScoreModsArgs(causal_shift=lm.causal_shift) if lm.causal_shift else None
-        out, lse = hip.flash_attention_fwd(q, k, v, sm_scale=float(sm_scale), causal=lm.causal,
-                                           kv_lengths=lm.kv_lengths, return_lse=True, mods=mods, width=rows)
-        weights = hip.key_weights(q, k, lse, key_weights, sm_scale=float(sm_scale), causal=lm.causal,
-                                  causal_shift=lm.causal_shift or 0, kv_lengths=lm.kv_lengths, width=rows)
+    if not causal and 0 < group * T <= hip.WEIGHTED_DECODE_MAX_ROWS:
+        res = hip.weighted_decode(q, k, v, key_weights, sm_scale=sm_scale, kv_lengths=lengths, return_lse=return_lse)
+        return res if res[0].shape[-1] == D else (res[0][..., :D], *res[1:])
+    if _needs_grad(q, k, v) or (key_weights is not None and _needs_grad(key_weights)):
+        raise ValueError(f"{who} has no gradient: call it under torch.no_grad() or on detached tensors")
+    width = _kernel_width(D, q.dtype)
+    if width is None:
+        raise ValueError(f"{who}: head dims up to {FLASH_HEAD_DIMS[-1]}, got {D}")
+    rows = None
+    if width != D:
+        rows = hip.rows_width(D, max(Hq, k.shape[2])) if q.dtype in HALF_DTYPES else None
+        if rows is None:
+            q, k, v = _pad_features(q, width), _pad_features(k, width), _pad_features(v, width)
+    shift = (lm.causal_shift if causal else None) or 0
+    mods = hip.ScoreModsArgs(causal_shift=shift) if shift else None
+    out, lse = hip.flash_attention_fwd(q, k, v, sm_scale=float(sm_scale), causal=causal, kv_lengths=lengths,
+                                       return_lse=True, mods=mods, width=rows)
+    weights = hip.key_weights(q, k, lse, key_weights, sm_scale=float(sm_scale), causal=causal, causal_shift=shift,
+                              kv_lengths=lengths, width=rows)
     if out.shape[-1] != D:
         out = out[..., :D]
     return (out, weights, lse) if return_lse else (out, weights)

@@ -768,6 +768,8 @@ def _key_weights(weights, like, B, H, S):
     if not isinstance(weights, torch.Tensor) or weights.get_device() != like.get_device() \
             or weights.dtype is not torch.float32:
         raise ValueError(f"key weights must be a float32 tensor on {like.device}")
+    if weights.requires_grad and torch.is_grad_enabled():
+        raise ValueError("key weights have no gradient: pass them detached or call under torch.no_grad()")
     if weights.shape != (B, H, S):
         raise ValueError(f"key weights must have shape {(B, H, S)}, got {tuple(weights.shape)}")
     return weights.contiguous()
@@ -859,7 +861,7 @@ def evict_keys(k, v, weights, keep: int, *, kv_lengths=None, sinks: int = 0, rec
                          f"{tuple(v.shape)} {v.dtype}")
     if k.dtype not in _DTYPES:
         raise ValueError(f"unsupported dtype {k.dtype}; expected bfloat16, float16 or float32")
-    if (k.requires_grad or v.requires_grad or weights.requires_grad) and torch.is_grad_enabled():
+    if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
         raise ValueError("eviction has no gradient: call it under torch.no_grad() or on detached tensors")
     B, S, H, D = k.shape
     keep, sinks, recent = int(keep), int(sinks), int(recent)

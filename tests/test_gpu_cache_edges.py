@@ -170,3 +170,31 @@ def test_more_sequences_than_the_schedule_sorts(device, Hq):
     want = ref.key_weight_attention(host[0][:, :1], host[1], host[2], zero, keep, D ** -0.5)
     check(out, lse, want, torch.bfloat16, D, S)
     check_weights(w, want, zero, D, S, Hq // 2)
+
+
+@pytest.mark.parametrize("name,D", [("bf16", 64), ("bf16", 128), ("f16", 80), ("bf16", 256), ("f32", 64)])
+def test_a_padded_prompt(device, name, D):
+    """NaN and infinities behind the sequences' lengths, under a causal mask, and
+    NaN in keys that the mask hides, reach no weight and no earlier row."""
+    import torch
+    from probjax_amd import masks
+    from probjax_amd.attention import attention_with_key_weights
+
+    B, T, dtype = 2, 200, _types()[name]
+    (q, k, v), host = _inputs(10, dtype, B, T, T, 4, 2, D, device)
+    L, scale = [150, 200], 1.0 / math.sqrt(D)
+    k[0, 150:], v[0, 150:] = float("nan"), float("inf")
+    mask = masks.ComposeMask("and", masks.CausalMask(), masks.KVLenMask(torch.tensor(L, dtype=torch.int32, device=device)))
+    out, w, lse = attention_with_key_weights(q, k, v, mask=mask, return_lse=True)
+    keep = np.tri(T, dtype=bool)[None] & (np.arange(T)[None, None, :] < np.array(L)[:, None, None])
+    zero = np.zeros((B, 2, T))
+    want = ref.key_weight_attention(*host, zero, keep, scale)
+    check(out, lse, want, dtype, D, T)
+    check_weights(w, want, zero, D, T, 2 * T)
+    v[0, 150:] = 0
+    out, w = attention_with_key_weights(q, k, v, mask=masks.CausalMask())
+    want = ref.key_weight_attention(*host, zero, np.broadcast_to(np.tri(T, dtype=bool), (B, T, T)), scale)
+    assert torch.isfinite(out[0, :150].float()).all() and torch.isfinite(out[1].float()).all()
+    assert not torch.isfinite(w[0, :, 150:]).any()
+    first = {n: want[n][:1, :, :150] if n == "reach" else want[n][:1, :150] for n in ("out", "spread", "reach")}
+    check(out[:1, :150], None, first, dtype, D, T)
