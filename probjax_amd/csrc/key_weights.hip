@@ -7,7 +7,7 @@
 // scores, 4 bytes a row and key beside the 2 (D + D) bytes of a 16-bit key, and
 // a second kernel sums their exponentials once the rows' statistics are known.
 // Forming the scores again instead would read K, half of the cache, again.  bf16, 8 KV
-// heads of 128, 4 rows each: 32 sequences of 512 .. 8192 keys (588 MB) 125 us, bound by
+// heads of 128, 4 rows each: 32 sequences of 512 .. 8192 keys (588 MB) 119 us, bound by
 // HBM (the decode without scores 107), and 12 us for the second kernel; one of 4096
 // keys 8 and 4.7 us, bound by latency.
 //
@@ -136,6 +136,13 @@ template <int D>
 static int run_scored_f32(DecodeArgs& a, int nrb, const float* wi, float* wo, void* ws, size_t n, hipStream_t s) {
   return nrb == 1 ? run_scored<scored_decode_f32_kernel<D, 1>>(a, wi, wo, ws, n, s)
                   : run_scored<scored_decode_f32_kernel<D, 2>>(a, wi, wo, ws, n, s);
+}
+
+// The automatic chunk: the decode's, up to 1024 keys.  MI355X, us, 1024 / 2048 keys,
+// 8 KV heads of 128, 4 rows each: 32 sequences of 512 .. 8192 keys 131 / 137, 8 of up to
+// 32768 133 / 141, 32 full ones of 8192 225 / 221.
+static int64_t scored_chunk(int64_t batch, int64_t groups, int64_t kv_len, int64_t chunk) {
+  return chunk ? chunk : std::min<int64_t>(auto_chunk(batch, groups, kv_len, kGqaItems), 1024);
 }
 
 // Workspace of a weighted decode: the decode's partials, then the scores.
@@ -452,7 +459,7 @@ using namespace pjx;
 
 extern "C" size_t pjx_weighted_decode_workspace_size(int64_t batch, int64_t kv_heads, int64_t rows, int64_t kv_len,
                                                      int64_t head_dim, int64_t chunk) {
-  return partial_bytes(batch, kv_heads, rows, kv_len, head_dim, chunk) +
+  return partial_bytes(batch, kv_heads, rows, kv_len, head_dim, scored_chunk(batch, kv_heads, kv_len, chunk)) +
          (size_t)(batch * kv_heads * rows * score_stride(kv_len)) * 4;
 }
 
@@ -465,7 +472,7 @@ extern "C" int pjx_weighted_decode(int dtype, const void* q, const void* k, cons
   const char* who = "pjx_weighted_decode";
   DecodeArgs a = {};
   const int rc = fill_cache_decode(a, who, dtype, q, k, v, kv_lengths, o, lse, batch, q_len, kv_len, q_heads, kv_heads,
-                                   head_dim, row_dim, strides, sm_scale, chunk);
+                                   head_dim, row_dim, strides, sm_scale, scored_chunk(batch, kv_heads, kv_len, chunk));
   if (rc != PJX_OK) return rc;
   const int64_t rows = q_heads / kv_heads * q_len;
   if (rows > kMaxScoredRows) return fail(PJX_ERR_INVALID, "pjx_weighted_decode: at most 64 rows per KV head");
