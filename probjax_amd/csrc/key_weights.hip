@@ -7,8 +7,8 @@
 // scores, 4 bytes a row and key beside the 2 (D + D) bytes of a 16-bit key, and
 // a second kernel sums their exponentials once the rows' statistics are known.
 // Forming the scores again instead would read K, half of the cache, again.  bf16, 8 KV
-// heads of 128, 4 rows each: 32 sequences of 512 .. 8192 keys (588 MB) 119 us, bound by
-// HBM (the decode without scores 107), and 12 us for the second kernel; one of 4096
+// heads of 128, 4 rows each: 32 sequences of 512 .. 8192 keys (588 MB) 118 us, bound by
+// HBM (the decode without scores 107), and 11 us for the second kernel; one of 4096
 // keys 8 and 4.7 us, bound by latency.
 //
 // Prompts (many rows): the scores are too many to keep.  They are formed again
@@ -38,6 +38,7 @@ __global__ __launch_bounds__(256, 1) void scored_decode_f32_kernel(DecodeArgs a)
 constexpr int kWeightThreads = 128;  // the merge's, which shares the launch
 constexpr int kWeightKeys = 4 * kWeightThreads;
 constexpr int kMaxScoredRows = 64;
+constexpr int kRowsAhead = 4;
 static_assert(kWeightThreads == kMergeThreads && kMaxScoredRows <= kWeightThreads, "one launch");
 
 // After the chunk kernel: the first merge_blocks workgroups merge the outputs,
@@ -54,6 +55,19 @@ __global__ __launch_bounds__(kWeightThreads) void scored_merge_kernel(DecodeArgs
   const int b = bg / a.G, tid = threadIdx.x;
   const int L = seq_len(a, b), n = (L + a.chunk - 1) / a.chunk;
   const int j0 = block % key_blocks * kWeightKeys + 4 * tid;
+  // The weights so far and, of few rows, the scores, on their way while the statistics
+  // are found (4 rows, 32 sequences of 512 .. 8192 keys: 131.8 -> 129.7 us for the step).
+  const float* s = a.scores + (size_t)bg * a.rows * a.score_ld + j0;
+  f32x4 first[kRowsAhead] = {};
+  const bool ahead = a.rows <= kRowsAhead;
+  if (ahead && j0 < L)
+#pragma unroll
+    for (int r = 0; r < kRowsAhead; ++r) first[r] = *(const f32x4*)(s + (size_t)min(r, a.rows - 1) * a.score_ld);
+  const size_t at = (size_t)bg * a.Lk + j0;
+  float w[4] = {};
+  if (w_in)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = w_in[(size_t)bg * a.Lk + min(j0 + e, a.Lk - 1)];
   // each row's chunks over the lanes it gets: a power of two of them, in one wave
   int per = 64;
   while (per * a.rows > kWeightThreads) per /= 2;
@@ -77,19 +91,21 @@ __global__ __launch_bounds__(kWeightThreads) void scored_merge_kernel(DecodeArgs
   __syncthreads();
   if (j0 >= a.Lk) return;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  if (j0 < L) {
-    const float* s = a.scores + (size_t)bg * a.rows * a.score_ld + j0;
-#pragma unroll 4
-    for (int r = 0; r < a.rows; ++r) {
-      const f32x4 x = *(const f32x4*)(s + (size_t)r * a.score_ld);
-      const float2 st = stat[r];
+  auto add = [&](const f32x4& x, const float2 st) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] = fmaf(fast_exp2(x[e] - st.x), st.y, acc[e]);
-    }
+    for (int e = 0; e < 4; ++e) acc[e] = fmaf(fast_exp2(x[e] - st.x), st.y, acc[e]);
+  };
+  if (ahead) {
+#pragma unroll
+    for (int r = 0; r < kRowsAhead; ++r)
+      if (r < a.rows) add(first[r], stat[r]);
+  } else if (j0 < L) {
+#pragma unroll 4
+    for (int r = 0; r < a.rows; ++r) add(*(const f32x4*)(s + (size_t)r * a.score_ld), stat[r]);
   }
-  const size_t at = (size_t)bg * a.Lk + j0;
-  for (int e = 0; e < 4 && j0 + e < a.Lk; ++e)
-    w_out[at + e] = (w_in ? w_in[at + e] : 0.f) + (j0 + e < L ? acc[e] : 0.f);
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (j0 + e < a.Lk) w_out[at + e] = w[e] + (j0 + e < L ? acc[e] : 0.f);
 }
 
 template <auto K>
@@ -139,8 +155,8 @@ static int run_scored_f32(DecodeArgs& a, int nrb, const float* wi, float* wo, vo
 }
 
 // The automatic chunk: the decode's, up to 1024 keys.  MI355X, us, 1024 / 2048 keys,
-// 8 KV heads of 128, 4 rows each: 32 sequences of 512 .. 8192 keys 131 / 137, 8 of up to
-// 32768 133 / 141, 32 full ones of 8192 225 / 221.
+// 8 KV heads of 128, 4 rows each: 32 sequences of 512 .. 8192 keys 130 / 137, 8 of up to
+// 32768 130 / 140, 32 full ones of 8192 221 / 218.
 static int64_t scored_chunk(int64_t batch, int64_t groups, int64_t kv_len, int64_t chunk) {
   return chunk ? chunk : std::min<int64_t>(auto_chunk(batch, groups, kv_len, kGqaItems), 1024);
 }
