@@ -1197,7 +1197,8 @@ int run_chunks(DecodeArgs& a, void* workspace, size_t ws_bytes, hipStream_t stre
 template <auto K>
 int run_decode(DecodeArgs& a, void* workspace, size_t ws_bytes, hipStream_t stream, const char* name) {
   const int rc = run_chunks<K>(a, workspace, ws_bytes, stream, name);
-  if (rc) return rc;
+  // (a draft has a key at least, so one chunk's kernel wrote every row)
+  if (rc || (a.extra && a.nch == 1)) return rc;
   return a.extra && a.nch <= kFewChunks ? launch_merge_few(a, stream, name) : launch_decode_merge(a, stream, name);
 }
 
