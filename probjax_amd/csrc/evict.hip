@@ -5,11 +5,12 @@
 // Two kernels.  The selection runs one workgroup per (sequence, head), its weights
 // in registers as order-preserving integers, and finds the threshold by counting
 // digits of 11 bits in LDS, two or three passes; one more pass ranks the kept keys.
-// It is bound by the latency of those steps (8 x 4096 weights 9 us, 128 x 8192 of
-// them 11; bits counted two a round by ballots kept the scalar unit, which 16 waves
-// share, busy for 9 us more).  The gather reads and writes every kept K and V row
-// once, 16 bytes a lane, bound by HBM (16 x 8192 keys of 8 heads of 128 cut to half
-// their capacity, 490 MB: 97 us, 5.0 TB/s).
+// It is bound by the latency of those steps and, of long caches, by the scalar unit
+// that its 16 waves share (8 x 4096 weights 8.4 us, 128 x 8192 of them 11, 8 x 32768
+// 31; read again in every pass, 2 x 40000: 46.  Bits counted two a round by ballots
+// kept the scalar unit busy for 9 us more).  The gather reads and writes every kept K
+// and V row once, 16 bytes a lane, bound by HBM (16 x 8192 keys of 8 heads of 128 cut
+// to half their capacity, 490 MB: 97 us, 5.0 TB/s).
 #include <stdio.h>
 
 #include "pjx_common.h"
@@ -108,18 +109,17 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
     T = 0u;
     int skip = hi - lo - need;
 #pragma unroll 1
-    for (int shift = 32 - kDigit, before = 32;;) {
+    for (int shift = 32 - kDigit, known = 32;;) {
       auto look = [&](uint32_t u) {
-        const bool in = (u != 0u) & (before == 32 || (u ^ T) >> (before & 31) == 0u);
-        const int d = (int)(u >> shift) & (kBins - 1);
-        const uint64_t m = __builtin_amdgcn_ballot_w64(in);
-        if (!m) return;
+        const bool in = (u != 0u) & (known == 32 || (u ^ T) >> (known & 31) == 0u);
+        if (!in) return;
         // One atomic for all lanes of the first one's digit: weights often share one,
         // and atomics on one word take their turns.
-        const int d0 = __builtin_amdgcn_readlane(d, __builtin_ctzll(m));
-        const uint64_t same = __builtin_amdgcn_ballot_w64(in & (d == d0));
-        if (lane == __builtin_ctzll(m)) atomicAdd(&bins[d0], __popcll(same));
-        else if (in & (d != d0)) atomicAdd(&bins[d], 1);
+        const int d = (int)(u >> shift) & (kBins - 1), d0 = __builtin_amdgcn_readfirstlane(d);
+        const uint64_t same = __builtin_amdgcn_ballot_w64(d == d0);
+        const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(same >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)same, 0));
+        const int add = d != d0 ? 1 : before == 0 ? __popcll(same) : 0;
+        if (add) atomicAdd(&bins[d], add);
       };
       if constexpr (R > 0) {
 #pragma unroll
@@ -158,7 +158,7 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
         ties = count - skip;
         break;
       }
-      before = shift;
+      known = shift;
       shift = max(shift - kDigit, 0);
     }
   }

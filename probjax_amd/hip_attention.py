@@ -879,8 +879,8 @@ def evict_keys(k, v, weights, keep: int, *, kv_lengths=None, sinks: int = 0, rec
         k_out, v_out, w_out = out
         _check_evict_out(out, (k, v, weights), keep)
         out_strides = _pair_strides(k_out, v_out)
-    lengths_index = torch.empty((B * (1 + H * keep),), dtype=torch.int32, device=k.device)
-    lengths, index_out = lengths_index[:B], lengths_index[B:].view(B, H, keep)
+    lengths = torch.empty((B,), dtype=torch.int32, device=k.device)
+    index_out = torch.empty((B, H, keep), dtype=torch.int32, device=k.device)
     k, v = _features_contiguous(k), _features_contiguous(v)
     _call(
         index, native.load().pjx_evict_keys, k.element_size(), k.data_ptr(), v.data_ptr(), weights.data_ptr(), _ptr(L),
