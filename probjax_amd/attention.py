@@ -387,7 +387,9 @@ class _AttentionFunction(torch.autograd.Function):
 
 
 def _needs_grad(*ts) -> bool:
-    return torch.is_grad_enabled() and any(t.requires_grad for t in ts)
+    """Whether a derivative is taken through one of ``ts``, in reverse or forward
+    mode (an autograd function without a forward-mode rule then raises)."""
+    return hip._tracked(*ts)
 
 
 def _kernel_width(d: int, dtype=torch.bfloat16):
@@ -738,10 +740,23 @@ class _RotaryFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, positions, options):
         ctx.save_for_backward(positions)
+        ctx.save_for_forward(positions)
         ctx.options = options
         ctx.set_materialize_grads(False)
         q, k = hip.rotary(q, k, positions, *options)
+        ctx.shapes = [x.shape for x in (q, k) if x is not None]
         return q if k is None else (q, k)
+
+    @staticmethod
+    def jvp(ctx, dq, dk, *_):
+        """The tangents turn as q and k do (in one launch, as those do)."""
+        (positions,) = ctx.saved_tensors
+        given = [x for x in (dq, dk) if x is not None]
+        turned = _rotate(given[0], given[1] if len(given) > 1 else None, positions, ctx.options)
+        turned = iter(turned if isinstance(turned, tuple) else (turned,))
+        # (a tangent that is not given is zero)
+        out = [given[0].new_zeros(n) if x is None else next(turned) for x, n in zip((dq, dk), ctx.shapes)]
+        return out[0] if len(out) == 1 else tuple(out)
 
     @staticmethod
     def backward(ctx, dq, dk=None):
@@ -751,12 +766,16 @@ class _RotaryFunction(torch.autograd.Function):
         *options, inverse = ctx.options
         options = (*options, not inverse)
         one, two = (dk, None) if dq is None else (dq, dk)
-        if _needs_grad(one) or (two is not None and _needs_grad(two)):
-            res = _RotaryFunction.apply(one, two, positions, options)
-            one, two = res if two is not None else (res, None)
-        else:
-            one, two = hip.rotary(one, two, positions, *options)
+        res = _rotate(one, two, positions, options)
+        one, two = res if two is not None else (res, None)
         return (None, one, None, None) if dq is None else (one, two, None, None)
+
+
+def _rotate(q, k, positions, options):
+    if _needs_grad(q) or (k is not None and _needs_grad(k)):
+        return _RotaryFunction.apply(q, k, positions, options)
+    y, z = hip.rotary(q, k, positions, *options)
+    return y if z is None else (y, z)
 
 
 def rotary(q, k, positions, *, sections=None, base: float = 10000.0, interleaved: bool = True,
@@ -779,7 +798,7 @@ def rotary(q, k, positions, *, sections=None, base: float = 10000.0, interleaved
     in float64, so far positions keep their fraction of a turn.
 
     bf16, fp16 or fp32, D up to 256, any strides (a slice of the features is read
-    in place).  Differentiable in q and k.
+    in place).  Differentiable in q and k, in reverse and forward mode.
     """
     if q.ndim != 4 or (k is not None and k.ndim != 4):
         raise ValueError("rotary: q and k must be [B, T, H, D]")
@@ -798,7 +817,7 @@ def rotary(q, k, positions, *, sections=None, base: float = 10000.0, interleaved
     if positions.shape not in ((T, A), (B, T, A)) or not 1 <= A <= 4:
         raise ValueError(f"rotary: positions must be [{T}], [{T}, A] or [{B}, {T}, A] with 1 to 4 axes, got "
                          f"{tuple(positions.shape)}")
-    if positions.requires_grad:
+    if positions.requires_grad or _needs_grad(positions):
         raise ValueError("rotary has no gradient in the positions")
     if positions.dtype not in hip._POSITION_TYPES:
         if positions.dtype == torch.bool or positions.dtype.is_complex:
@@ -816,10 +835,7 @@ def rotary(q, k, positions, *, sections=None, base: float = 10000.0, interleaved
         raise ValueError(f"rotary: base must be positive, got {base}")
     # sections, base, interleaved, shared_spectrum, inverse, as hip.rotary takes them
     options = (sections, float(base), bool(interleaved), bool(shared_spectrum), False)
-    if _needs_grad(q) or (k is not None and _needs_grad(k)):
-        return _RotaryFunction.apply(q, k, positions, options)
-    y, z = hip.rotary(q, k, positions, *options)
-    return y if z is None else (y, z)
+    return _rotate(q, k, positions, options)
 
 
 class _MaterializedMLAFunction(torch.autograd.Function):

@@ -14,6 +14,7 @@ import os
 from dataclasses import dataclass
 
 import torch
+from torch.autograd import forward_ad
 
 from . import native
 
@@ -628,6 +629,16 @@ def _gpu(*ts) -> int:
     return index
 
 
+def _tracked(*ts) -> bool:
+    """Whether a derivative is taken through one of the tensors: they require a
+    gradient, or carry a tangent (which forward mode gives tensors that require none)."""
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t.requires_grad:
+                return True
+    return forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in ts)
+
+
 def _call(index: int, entry, *args) -> None:
     """``entry(*args, stream)``, raising on an error, on the current stream of
     device ``index`` and with it as the current device (a launch takes the current
@@ -689,7 +700,7 @@ def _cache_call(who: str, q, k, v):
         raise ValueError(f"{who} takes bfloat16, float16 or float32 q, k and v of one dtype")
     if not 1 <= D <= 256:
         raise ValueError(f"{who}: head dims up to 256, got {D}")
-    if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
+    if _tracked(q, k, v):
         raise ValueError(f"{who} has no gradient: call it under torch.no_grad() or on detached tensors")
     width = 64 if D <= 64 else 128 if D <= 128 else 256
     row = D
@@ -768,7 +779,7 @@ def _key_weights(weights, like, B, H, S):
     if not isinstance(weights, torch.Tensor) or weights.get_device() != like.get_device() \
             or weights.dtype is not torch.float32:
         raise ValueError(f"key weights must be a float32 tensor on {like.device}")
-    if weights.requires_grad and torch.is_grad_enabled():
+    if _tracked(weights):
         raise ValueError("key weights have no gradient: pass them detached or call under torch.no_grad()")
     if weights.shape != (B, H, S):
         raise ValueError(f"key weights must have shape {(B, H, S)}, got {tuple(weights.shape)}")
@@ -861,7 +872,7 @@ def evict_keys(k, v, weights, keep: int, *, kv_lengths=None, sinks: int = 0, rec
                          f"{tuple(v.shape)} {v.dtype}")
     if k.dtype not in _DTYPES:
         raise ValueError(f"unsupported dtype {k.dtype}; expected bfloat16, float16 or float32")
-    if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
+    if _tracked(k, v):
         raise ValueError("eviction has no gradient: call it under torch.no_grad() or on detached tensors")
     B, S, H, D = k.shape
     keep, sinks, recent = int(keep), int(sinks), int(recent)
@@ -905,7 +916,7 @@ def _check_evict_out(out, ins, keep: int) -> None:
         raise ValueError("out needs contiguous features and contiguous weights")
     if any(n > 1 and s == 0 for t in (k_out, v_out) for n, s in zip(t.shape, t.stride())):
         raise ValueError("out must not be expanded")
-    if any(t.requires_grad for t in out):
+    if _tracked(*out) or any(t.requires_grad for t in out):
         raise ValueError("out must not require a gradient")
     read = {t.untyped_storage().data_ptr() for t in ins if t.numel()}
     write = [t.untyped_storage().data_ptr() for t in out if t.numel()]
