@@ -727,7 +727,15 @@ def evict_keys(k, v, key_weights, keep: int, *, kv_lengths=None, sinks: int = 0,
     ``out=(k, v, key_weights)``, buffers of at least ``keep`` slots that share no
     memory with the inputs, those are written and returned, and what they hold
     behind the kept keys stays (a layer's spare caches, say, with room for the
-    tokens to come).  No gradient: inputs that require one raise.
+    tokens to come).  That goes for the weights too: a buffer used before holds
+    those of its old keys there, and a key appended over one of them would go on
+    from its weight.  Zero them before keys are appended::
+
+        kept = evict_keys(..., out=spare)
+        slots = torch.arange(kept.key_weights.shape[-1], device=k.device)
+        kept.key_weights.masked_fill_(slots >= kept.kv_lengths[:, None, None], 0)
+
+    No gradient: inputs that require one raise.
     """
     return EvictedKeys(*hip.evict_keys(k, v, key_weights, keep, kv_lengths=kv_lengths, sinks=sinks, recent=recent,
                                        out=out))
