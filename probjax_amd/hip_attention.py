@@ -918,10 +918,57 @@ def _check_evict_out(out, ins, keep: int) -> None:
         raise ValueError("out must not be expanded")
     if _tracked(*out) or any(t.requires_grad for t in out):
         raise ValueError("out must not require a gradient")
-    read = {t.untyped_storage().data_ptr() for t in ins if t.numel()}
-    write = [t.untyped_storage().data_ptr() for t in out if t.numel()]
-    if read & set(write) or len(set(write)) != len(write):
-        raise ValueError("out must not share memory with the inputs, nor its buffers with each other")
+    every = (*out, *ins)
+    home = [t.untyped_storage().data_ptr() for t in every]
+    if len(set(home[:3])) == 3 and not set(home[:3]) & set(home[3:]):
+        return
+    reach = [_reach(t) for t in every]
+    for i in range(3):
+        for j in range(i + 1, len(every)):
+            # (views of one allocation may lie between each other without meeting)
+            if reach[i][0] < reach[j][1] and reach[j][0] < reach[i][1] and _share_bytes(every[i], every[j]):
+                raise ValueError("out must not share memory with the inputs, nor its buffers with each other")
+
+
+def _reach(t):
+    """First byte of a tensor, and the one behind its last."""
+    first = t.data_ptr()
+    if not t.numel():
+        return first, first
+    return first, first + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
+
+
+def _share_bytes(a, b, most: int = 10000) -> bool:
+    """Whether two tensors have a byte in common, exactly: a search for indices i and
+    j whose addresses are equal, largest stride first, which leaves few choices on
+    each axis of a layout without overlaps.  Yes, if it takes more than ``most`` steps."""
+    span = {}  # stride -> range of the sum of indices (b's negative) that goes with it
+    for t, sign in ((a, 1), (b, -1)):
+        size = t.element_size()
+        for n, s in [(size, 1), *((n, s * size) for n, s in zip(t.shape, t.stride()))]:
+            lo, hi = span.get(s, (0, 0))
+            span[s] = (lo, hi + n - 1) if sign > 0 else (lo - n + 1, hi)
+    span.pop(0, None)
+    axes = [(s, *span[s]) for s in sorted(span)]
+    least, greatest = [0], [0]  # of the sums over the axes up to one
+    for s, lo, hi in axes:
+        least.append(least[-1] + s * lo)
+        greatest.append(greatest[-1] + s * hi)
+    todo = [(b.data_ptr() - a.data_ptr(), len(axes))]
+    for _ in range(most):
+        if not todo:
+            return False
+        gap, left = todo.pop()
+        if left == 0:  # (reached with a gap of 0 alone)
+            return True
+        s, lo, hi = axes[left - 1]
+        # what is left must lie in reach of the smaller strides
+        lo = max(lo, -((greatest[left - 1] - gap) // s))
+        hi = min(hi, (gap - least[left - 1]) // s)
+        if hi - lo > most:
+            return True
+        todo.extend((gap - s * d, left - 1) for d in range(lo, hi + 1))
+    return True
 
 
 _POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2, torch.float64: 3}  # PJX_POSITION_*

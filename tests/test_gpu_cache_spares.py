@@ -61,3 +61,30 @@ def test_spares_by_turns(device, name):
             fresh = slice(int(start[b]), int(L[b]))
             # the sums of the steps alone, whatever lay there before
             assert (np.abs(to_np(w)[b, :, fresh] - sums[b, :, fresh]) <= tol[b, :, fresh]).all(), (turn, b)
+
+
+@pytest.mark.parametrize("axis", [0, 2, 3])
+def test_buffers_and_inputs_of_one_allocation(device, axis):
+    """K and V of one tensor, whose spare slots take what is kept of the others."""
+    import torch
+    from probjax_amd.attention import evict_keys
+
+    B, S, H, D, keep, room = 2, 300, 2, 64, 50, 70
+    shape = [B, S + room, H, D]
+    pool = torch.randn((*shape[:axis], 2, *shape[axis:]), generator=torch.Generator(device=device).manual_seed(2),
+                       device=device).to(torch.bfloat16)
+    k, v = pool.select(axis, 0), pool.select(axis, 1)
+    w = torch.rand((B, H, S), device=device)
+    L = torch.tensor([300, 45], dtype=torch.int32, device=device)
+    want = evict_keys(k[:, :S].clone(), v[:, :S].clone(), w, keep, kv_lengths=L, recent=3)
+    before = pool.clone()
+    out = (k[:, S:], v[:, S:], torch.zeros((B, H, room), device=device))
+    got = evict_keys(k[:, :S], v[:, :S], w, keep, kv_lengths=L, recent=3, out=out)
+    torch.cuda.synchronize()
+    assert torch.equal(got.index, want.index) and torch.equal(got.kv_lengths, want.kv_lengths)
+    for x, y, z in ((k, got.k, want.k), (v, got.v, want.v)):
+        assert y.data_ptr() == x[:, S:].data_ptr()
+        for b, n in enumerate((50, 45)):
+            assert torch.equal(y[b, :n], z[b, :n])
+            y[b, :n] = before.select(axis, 0 if x is k else 1)[b, S:S + n]
+    assert torch.equal(pool, before)  # nothing else was written
