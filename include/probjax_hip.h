@@ -621,7 +621,8 @@ int pjx_rotary(int dtype, const void* q, const void* k, void* q_out, void* k_out
  *   k_out, v_out rows, weights_out [B, Hkv, out_len] (out_len >= keep): what they held
  * Rows at and behind lengths_out[b] up to keep are zeroed with fill != 0, and all
  * of them left as they are without (weights too: the caller zeroes those of slots
- * that it appends keys to).  Out buffers must not overlap the inputs.
+ * that it appends keys to).  Out buffers must not overlap the inputs, nor their rows
+ * each other.
  * elem_size: bytes of an element of k and v (2 or 4); strides in elements, features
  * contiguous (NULL: contiguous, [B, kv_len, Hkv, D] and [B, out_len, Hkv, D]).
  */

@@ -725,7 +725,8 @@ def evict_keys(k, v, key_weights, keep: int, *, kv_lengths=None, sinks: int = 0,
 
     Returns new caches of ``keep`` slots, zeros behind the kept keys.  With
     ``out=(k, v, key_weights)``, buffers of at least ``keep`` slots that share no
-    memory with the inputs, those are written and returned, and what they hold
+    memory with the inputs or each other (views of one allocation may lie between
+    each other), those are written and returned, and what they hold
     behind the kept keys stays (a layer's spare caches, say, with room for the
     tokens to come).  That goes for the weights too: a buffer used before holds
     those of its old keys there, and a key appended over one of them would go on

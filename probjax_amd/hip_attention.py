@@ -914,8 +914,12 @@ def _check_evict_out(out, ins, keep: int) -> None:
                              f"{(B, H, f'>= {keep}')} of float32 on {k.device}")
     if (D > 1 and (k_out.stride(3) != 1 or v_out.stride(3) != 1)) or not w_out.is_contiguous():
         raise ValueError("out needs contiguous features and contiguous weights")
-    if any(n > 1 and s == 0 for t in (k_out, v_out) for n, s in zip(t.shape, t.stride())):
-        raise ValueError("out must not be expanded")
+    for t in (k_out, v_out):
+        end = 0  # of what the smaller strides reach
+        for s, n in sorted((s, n) for n, s in zip(t.shape, t.stride()) if n > 1):
+            if s <= end:
+                raise ValueError("out must not be expanded, nor its rows overlap each other")
+            end += (n - 1) * s
     if _tracked(*out) or any(t.requires_grad for t in out):
         raise ValueError("out must not require a gradient")
     every = (*out, *ins)

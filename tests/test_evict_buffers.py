@@ -65,6 +65,19 @@ def test_views_that_meet_are_refused():
             hip._check_evict_out(out, ins, KEEP)
 
 
+@pytest.mark.parametrize("stride", [(0, 16, 8, 1), (16, 16, 8, 1), (100, 16, 8, 1), (160, 12, 8, 1), (160, 16, 4, 1)])
+def test_buffers_whose_rows_overlap_each_other_are_refused(stride):
+    """Two rows would be written to one place, in an order that is not defined."""
+    k, v, w = _room()
+    wide = torch.as_strided(torch.zeros(1000, dtype=torch.bfloat16), (B, KEEP, H, D), stride)
+    for out in ((wide, v, w), (k, wide, w)):
+        with pytest.raises(ValueError, match="overlap"):
+            hip._check_evict_out(out, _inputs(), KEEP)
+    for t in (torch.zeros((KEEP, H, B, D), dtype=torch.bfloat16).permute(2, 0, 1, 3),
+              torch.zeros((B, 40, H, 24), dtype=torch.bfloat16)[:, 3:23:2, :, 8:16]):
+        hip._check_evict_out((t, v, w), _inputs(), KEEP)
+
+
 def test_shared_bytes_of_random_views():
     """Against the bytes themselves."""
     rng = random.Random(0)
