@@ -663,7 +663,10 @@ def attention_with_key_weights(q, k, v, key_weights=None, *, mask=None, sm_scale
     elif mask is not None:
         lm = lower_mask(mask)
         if lm is not None and lm.row_kv_lengths is not None and T == 1:  # one row: per-batch lengths
-            lm.kv_lengths, lm.row_kv_lengths = _row_kv_lengths(lm.row_kv_lengths, B, 1, q.device)[:, 0], None
+            rows = _row_kv_lengths(lm.row_kv_lengths, B, 1, q.device)
+            if rows is None:
+                raise ValueError(f"{who}: key lengths must be integers, one, [T] or [{B}, T]")
+            lm.kv_lengths, lm.row_kv_lengths = rows[:, 0], None
         if lm is None or lm.q_valid is not None or lm.kv_valid is not None or lm.extended and not _only_shifted(lm):
             raise ValueError(f"{who} takes no mask, KVLenMask and causal masks, got {type(mask).__name__}")
         causal, lengths = lm.causal, lm.kv_lengths
