@@ -666,6 +666,18 @@ def _int32(t, what: str, like, *shapes):
     return t
 
 
+def _key_lengths(kv_lengths, like, batch):
+    """``kv_lengths`` as int32 ``[batch]`` on the device of ``like`` (None: none);
+    like those of the other entry points they may come as ``[batch, 1]``."""
+    if kv_lengths is None:
+        return None
+    if not isinstance(kv_lengths, torch.Tensor):
+        kv_lengths = torch.as_tensor(kv_lengths)
+    if kv_lengths.ndim != 1:
+        kv_lengths = kv_lengths.reshape(-1)
+    return _int32(kv_lengths, "kv_lengths", like, (batch,))
+
+
 @functools.lru_cache(maxsize=256)
 def _workspace_size(entry: str, *sizes) -> int:
     """What the entry point's size query answers (a function of the sizes alone; a
@@ -756,7 +768,7 @@ def tree_decode(
         trees, m = (1 if tree.ndim == 2 else B), tree.data_ptr()
     if kv_lengths is None and S < T:
         raise ValueError(f"a cache of {S} slots does not hold {T} drafted tokens")
-    L = None if kv_lengths is None else _int32(kv_lengths, "kv_lengths", q, (B,))
+    L = _key_lengths(kv_lengths, q, B)
     lib = native.load()
     nbytes = _workspace_size("pjx_decode_workspace_size", B, Hkv, (Hq // Hkv) * T, S, width, chunk)
     ws = _scratch(nbytes, q, workspace)
@@ -801,7 +813,7 @@ def weighted_decode(
     if not 1 <= rows <= WEIGHTED_DECODE_MAX_ROWS:
         raise ValueError(f"a weighted decode step takes 1 to {WEIGHTED_DECODE_MAX_ROWS} rows per KV head, got {rows}")
     weights = _key_weights(weights, q, B, Hkv, S)
-    L = None if kv_lengths is None else _int32(kv_lengths, "kv_lengths", q, (B,))
+    L = _key_lengths(kv_lengths, q, B)
     lib = native.load()
     nbytes = _workspace_size("pjx_weighted_decode_workspace_size", B, Hkv, rows, S, width, chunk)
     ws = _scratch(nbytes, q, workspace)
@@ -834,7 +846,7 @@ def key_weights(
         raise ValueError("q and k must share a dtype and lse be float32")
     code = _dtype_code(q)
     weights = _key_weights(weights, q, B, Hkv, S)
-    L = None if kv_lengths is None else _int32(kv_lengths, "kv_lengths", q, (B,))
+    L = _key_lengths(kv_lengths, q, B)
     q, k, lse = _aligned(q.contiguous()), _aligned(k.contiguous()), lse.contiguous()
     lib = native.load()
     nbytes = _workspace_size("pjx_key_weights_workspace_size", B, T, S, Hq)
@@ -880,7 +892,7 @@ def evict_keys(k, v, weights, keep: int, *, kv_lengths=None, sinks: int = 0, rec
         raise ValueError(f"keep must be at least 1 and at least sinks + recent, got keep={keep}, sinks={sinks}, "
                          f"recent={recent}")
     weights = _key_weights(weights, k, B, H, S)
-    L = None if kv_lengths is None else _int32(kv_lengths, "kv_lengths", k, (B,))
+    L = _key_lengths(kv_lengths, k, B)
     out_strides = None
     if out is None:
         k_out = k.new_empty((B, keep, H, D))
