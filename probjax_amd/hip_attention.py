@@ -99,11 +99,17 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _stream(dev) -> int:
-    """The handle of torch's current stream on ``dev`` (as
-    ``torch.cuda.current_stream(dev).cuda_stream``, without building a Stream:
-    0.2 against 2.5 us on every call)."""
-    return torch._C._cuda_getCurrentRawStream(dev.index if dev.index is not None else torch.cuda.current_device())
+def _call(index: int, entry, *args) -> None:
+    """``entry(*args, stream)``, raising on an error, on the current stream of
+    device ``index`` and with it as the current device (a launch takes the current
+    device's kernels).  The raw handle: building a Stream takes 2.5 us against 0.2."""
+    if index == torch._C._cuda_getDevice():
+        rc = entry(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = entry(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        native.check(rc)
 
 
 def _lengths(kv_lengths, batch, dev):
@@ -212,13 +218,13 @@ def flash_attention_fwd(
     o = torch.empty_like(q)
     lse = torch.empty((B, Hq, Lq), dtype=torch.float32, device=dev) if return_lse else None
     lib = native.load()
-    rc = (lib.pjx_flash_fwd if width is None else lib.pjx_flash_fwd_rows)(
+    _call(
+        dev.index, lib.pjx_flash_fwd if width is None else lib.pjx_flash_fwd_rows,
         code, _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(lse), _ptr(L), _ptr(bias), bb, bh,
         B, Lq, Lk, Hq, Hkv, *((D,) if width is None else (width, D)), Lq if q_valid is None else int(q_valid),
         Lk if kv_valid is None else int(kv_valid), int(bool(causal)), float(sm_scale),
-        None if ms is None else ctypes.byref(ms[0]), _stream(dev),
+        None if ms is None else ctypes.byref(ms[0]),
     )
-    native.check(rc)
     return (o, lse) if return_lse else o
 
 
@@ -299,22 +305,22 @@ def flash_attention_bwd(
             split = lib.pjx_flash_bwd_split_workspace_size(code, B, Hq, Hkv, Lq, Lk, KD, int(bool(causal)))
             nbytes = max(nbytes, int(split))
     ws = _workspace(nbytes, dev, workspace)
-    rc = (lib.pjx_flash_bwd if width is None else lib.pjx_flash_bwd_rows)(
+    _call(
+        dev.index, lib.pjx_flash_bwd if width is None else lib.pjx_flash_bwd_rows,
         code, _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(do), _ptr(lse), _ptr(dq),
         _ptr(dk), _ptr(dv), _ptr(dbias), _ptr(ws), ws.numel(), _ptr(L), _ptr(bias), bb, bh, B, Lq, Lk, Hq, Hkv,
         *((D,) if width is None else (KD, D)),
         Lq if q_valid is None else int(q_valid), Lk if kv_valid is None else int(kv_valid),
-        int(bool(causal)), float(sm_scale), None if ms is None else ctypes.byref(ms[0]), _stream(dev),
+        int(bool(causal)), float(sm_scale), None if ms is None else ctypes.byref(ms[0]),
     )
-    native.check(rc)
     if fold:
         dbias = torch.empty_like(bias)
-        rc = lib.pjx_flash_dbias(
+        _call(
+            dev.index, lib.pjx_flash_dbias,
             code, _ptr(q), _ptr(k), _ptr(v), _ptr(do), _ptr(ws), _ptr(dbias), _ptr(L), _ptr(bias), bb, bh, B, Lq, Lk,
             Hq, Hkv, KD, D, Lq if q_valid is None else int(q_valid), Lk if kv_valid is None else int(kv_valid),
-            int(bool(causal)), float(sm_scale), None if ms is None else ctypes.byref(ms[0]), _stream(dev),
+            int(bool(causal)), float(sm_scale), None if ms is None else ctypes.byref(ms[0]),
         )
-        native.check(rc)
         return dq, dk, dv, dbias
     if dbias is None:
         return dq, dk, dv
@@ -337,9 +343,8 @@ def empty_rows(lse, src, dst, *, grad: bool) -> None:
     if out.dtype != val.dtype or not dst.is_contiguous():
         raise ValueError("output and V must share a dtype and the written one be contiguous")
     lse, src = lse.contiguous(), src.contiguous()
-    rc = native.load().pjx_empty_rows(_dtype_code(out), int(grad), _ptr(lse), _ptr(src), _ptr(dst), B, Lq, Lk, Hq,
-                                      Hkv, D, _stream(dev))
-    native.check(rc)
+    _call(dev.index, native.load().pjx_empty_rows, _dtype_code(out), int(grad), _ptr(lse), _ptr(src), _ptr(dst), B, Lq,
+          Lk, Hq, Hkv, D)
 
 
 def zero_empty_rows(lse, o, dout):
@@ -351,9 +356,8 @@ def zero_empty_rows(lse, o, dout):
         raise ValueError(f"incompatible shapes: output {tuple(o.shape)}, dO {tuple(dout.shape)}, lse {tuple(lse.shape)}")
     lse, o, dout = lse.contiguous(), _aligned(o.contiguous()), _aligned(dout.contiguous())
     o_rows, dout_rows = torch.empty_like(o), torch.empty_like(dout)
-    rc = native.load().pjx_zero_empty_rows(_dtype_code(o), _ptr(lse), _ptr(o), _ptr(dout), _ptr(o_rows),
-                                           _ptr(dout_rows), B, Lq, Hq, D, _stream(dev))
-    native.check(rc)
+    _call(dev.index, native.load().pjx_zero_empty_rows, _dtype_code(o), _ptr(lse), _ptr(o), _ptr(dout), _ptr(o_rows),
+          _ptr(dout_rows), B, Lq, Hq, D)
     return o_rows, dout_rows
 
 
@@ -427,11 +431,11 @@ def splitkv_decode(
     else:
         entry, dims = native.load().pjx_splitkv_decode_rows, (width, D)
         q, k, v = _aligned(q), _aligned(k), _aligned(v)
-    rc = entry(
+    _call(
+        dev.index, entry,
         _dtype_code(q), _ptr(q), _ptr(k), _ptr(v), _ptr(L), _ptr(o), _ptr(lse), _ptr(ws),
-        nbytes, B, Lq, S, Hq, Hkv, *dims, float(sm_scale), int(chunk), _stream(dev),
+        nbytes, B, Lq, S, Hq, Hkv, *dims, float(sm_scale), int(chunk),
     )
-    native.check(rc)
     return (o, lse) if return_lse else o
 
 
@@ -461,11 +465,11 @@ def mla_decode(
     ws = _workspace(nbytes, dev, workspace)
     o = torch.empty((B, Lq, H, dv), dtype=q.dtype, device=dev)
     lse = torch.empty((B, H, Lq), dtype=torch.float32, device=dev) if return_lse else None
-    rc = native.load().pjx_mla_decode(
+    _call(
+        dev.index, native.load().pjx_mla_decode,
         code, _ptr(q), _ptr(cache), _ptr(L), _ptr(o), _ptr(lse), _ptr(ws),
-        nbytes, B, Lq, H, S, R, dv, float(sm_scale), int(chunk), _stream(dev),
+        nbytes, B, Lq, H, S, R, dv, float(sm_scale), int(chunk),
     )
-    native.check(rc)
     return (o, lse) if return_lse else o
 
 
@@ -502,12 +506,12 @@ def mla_fwd(
     ms = _mods_struct(mods, B, Lq, S, H, dev)
     o = torch.empty((B, Lq, H, dv), dtype=q.dtype, device=dev)
     lse = torch.empty((B, H, Lq), dtype=torch.float32, device=dev) if return_lse else None
-    rc = native.load().pjx_mla_fwd(
+    _call(
+        dev.index, native.load().pjx_mla_fwd,
         code, _ptr(q), _ptr(cache), _ptr(o), _ptr(lse), _ptr(L), _ptr(bias), bb, bh,
         B, Lq, S, H, R, dv, Lq if q_valid is None else int(q_valid), S if kv_valid is None else int(kv_valid),
-        int(bool(causal)), float(sm_scale), None if ms is None else ctypes.byref(ms[0]), _stream(dev),
+        int(bool(causal)), float(sm_scale), None if ms is None else ctypes.byref(ms[0]),
     )
-    native.check(rc)
     return (o, lse) if return_lse else o
 
 
@@ -545,13 +549,13 @@ def mla_bwd(
     ws = _workspace(int(lib.pjx_mla_bwd_workspace_size(B, H, Lq, S, R)), dev, workspace)
     dq = torch.empty_like(q)
     dc = torch.empty_like(cache)
-    rc = lib.pjx_mla_bwd(
+    _call(
+        dev.index, lib.pjx_mla_bwd,
         code, _ptr(q), _ptr(cache), _ptr(o), _ptr(do), _ptr(lse), _ptr(dq), _ptr(dc),
         _ptr(ws), ws.numel(), _ptr(L), _ptr(bias), bb, bh, B, Lq, S, H, R, dv,
         Lq if q_valid is None else int(q_valid), S if kv_valid is None else int(kv_valid),
-        int(bool(causal)), float(sm_scale), None if ms is None else ctypes.byref(ms[0]), _stream(dev),
+        int(bool(causal)), float(sm_scale), None if ms is None else ctypes.byref(ms[0]),
     )
-    native.check(rc)
     return dq, dc
 
 
@@ -572,11 +576,11 @@ def mla_project(cache, wk, wv, *, width: int):
     cache, wk, wv = cache.contiguous(), wk.contiguous(), wv.contiguous()
     k = torch.empty((B, S, H, width), dtype=cache.dtype, device=dev)
     v = torch.empty((B, S, H, width), dtype=cache.dtype, device=dev)
-    rc = native.load().pjx_mla_project(
+    _call(
+        dev.index, native.load().pjx_mla_project,
         _DTYPES[cache.dtype], _ptr(cache), _ptr(wk), _ptr(wv), _ptr(k), _ptr(v),
-        B, S, H, R, dk, dv, int(width), _stream(dev),
+        B, S, H, R, dk, dv, int(width),
     )
-    native.check(rc)
     return k, v
 
 
@@ -594,11 +598,11 @@ def mla_project_bwd(cache, wk, wv, dk, dv):
     dcache, dwk, dwv = torch.empty_like(cache), torch.empty_like(wk), torch.empty_like(wv)
     lib = native.load()
     ws = _workspace(int(lib.pjx_mla_project_bwd_workspace_size(B, S, H, R, width)), dev, None)
-    rc = lib.pjx_mla_project_bwd(
+    _call(
+        dev.index, lib.pjx_mla_project_bwd,
         code, _ptr(cache), _ptr(wk), _ptr(wv), _ptr(dk), _ptr(dv), _ptr(dcache), _ptr(dwk), _ptr(dwv), _ptr(ws),
-        ws.numel(), B, S, H, R, dk_dim, dv_dim, width, _stream(dev),
+        ws.numel(), B, S, H, R, dk_dim, dv_dim, width,
     )
-    native.check(rc)
     return dcache, dwk, dwv
 
 
@@ -637,19 +641,6 @@ def _tracked(*ts) -> bool:
             if t.requires_grad:
                 return True
     return forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in ts)
-
-
-def _call(index: int, entry, *args) -> None:
-    """``entry(*args, stream)``, raising on an error, on the current stream of
-    device ``index`` and with it as the current device (a launch takes the current
-    device's kernels)."""
-    if index == torch._C._cuda_getDevice():
-        rc = entry(*args, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(index):
-            rc = entry(*args, torch._C._cuda_getCurrentRawStream(index))
-    if rc:
-        native.check(rc)
 
 
 def _int32(t, what: str, like, *shapes):
