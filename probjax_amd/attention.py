@@ -618,8 +618,12 @@ def tree_attention(q, k, v, *, parents=None, tree_mask=None, kv_lengths=None, sm
     What a token does not see does not reach its output, infinities and NaN
     included; a token that sees nothing gets 0 and LSE +inf.  bf16, fp16 or
     fp32, head dims up to 256, caches in any order of their first three axes.
-    ``sm_scale`` defaults to ``1/sqrt(D)``.  With ``return_lse`` also the
-    natural-log LSE ``[B, Hq, T]``.  No gradient: inputs that require one raise.
+    Lengths and parents are read as 32-bit integers (wider ones cost a conversion,
+    and their values have to fit).  In 16 bits the softmax weights are rounded to
+    the type before their product with V, as in ``mha``; scores, sums and partial
+    outputs are float32.  ``sm_scale`` defaults to ``1/sqrt(D)``.  With
+    ``return_lse`` also the natural-log LSE ``[B, Hq, T]``.  No gradient: inputs
+    that require one, or carry a tangent, raise.
     """
     if sm_scale is None:
         sm_scale = 1.0 / math.sqrt(q.shape[-1])
@@ -645,12 +649,16 @@ def attention_with_key_weights(q, k, v, key_weights=None, *, mask=None, sm_scale
     their intersections.  bf16, fp16 or fp32, head dims up to 256; ``sm_scale``
     defaults to ``1/sqrt(D)``.  With ``return_lse`` also the LSE ``[B, Hq, T]``.
 
+    Every row counts: those of padding in a batch of prompts too, and under
+    ``KVLenMask`` alone each token of a step sees the later ones of its own step.
     Steps of up to 64 rows ``(Hq/Hkv)*T`` without a causal mask run the
     split-KV decode, which keeps its scores; longer ones the flash forward and a
     second pass over the scores.  Keys past a sequence's length reach nothing,
     whatever they hold; what a causal mask hides enters products with weights of
-    0, as in ``mha``, so V has to be finite there.  No gradient: inputs that
-    require one raise.
+    0, as in ``mha``, so V has to be finite there.  In 16 bits the softmax weights
+    are rounded to the type before their product with V, as in ``mha``; scores and
+    the sums of key weights are float32.  No gradient: inputs that require one, or
+    carry a tangent, raise.
     """
     who = "attention with key weights"
     if q.ndim != 4 or k.ndim != 4 or v.ndim != 4:
@@ -739,7 +747,7 @@ def evict_keys(k, v, key_weights, keep: int, *, kv_lengths=None, sinks: int = 0,
         slots = torch.arange(kept.key_weights.shape[-1], device=k.device)
         kept.key_weights.masked_fill_(slots >= kept.kv_lengths[:, None, None], 0)
 
-    No gradient: inputs that require one raise.
+    No gradient: inputs that require one, or carry a tangent, raise.
     """
     return EvictedKeys(*hip.evict_keys(k, v, key_weights, keep, kv_lengths=kv_lengths, sinks=sinks, recent=recent,
                                        out=out))

@@ -785,6 +785,9 @@ __device__ __forceinline__ void gqa_decode(const DecodeArgs& a) {
           s[rb][kb][r] = p;
         }
       l_run[rb] = fmaf(l_run[rb], corr[rb], rs);
+      // The weights enter their product with V rounded to the 16-bit type, as the flash
+      // forward's do (the matrix instruction takes both operands in it; at most half a
+      // step of sum p |v|); their sum takes them unrounded.
       // P^T as the B operand: slot j < 4 <-> key 4*q4 + j, slot j >= 4 <-> key 16 + 4*q4 + j - 4.
       u32x4 pk;
       pk[0] = E::pack2(s[rb][0][0], s[rb][0][1]);

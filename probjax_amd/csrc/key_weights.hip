@@ -14,8 +14,11 @@
 // Prompts (many rows): the scores are too many to keep.  They are formed again
 // on the matrix units, keys as MFMA rows, so a lane's accumulators are sums of
 // its own 16 keys and nothing is exchanged until the end.  bf16, 4096 causal rows of
-// 16 heads over 4 KV heads of 128: 58 us, 590 TFLOP/s, bound by the exponentials (one
-// for every 256 operations) beside the products; the sum over the splits 4.8 us.
+// 16 heads over 4 KV heads of 128: 57 to 59 us, 590 to 600 TFLOP/s; the sum over the
+// splits 4.6 us.  No unit bounds it alone: while a CU is busy its matrix units work 41%
+// of the cycles and its VALUs 55% (a third of that exponentials, one for every 256
+// operations), two waves a SIMD, which leave gaps at each tile's barrier; and the CUs
+// are busy 77% of the time, the causal halves of the workgroups being uneven.
 //
 // Scores, their exponentials and every sum are float32, in a fixed order.
 #include <stdio.h>

@@ -13,7 +13,7 @@
 // Row groups of one work item are placed 8 workgroups apart, on one XCD, whose
 // L2 gives all but the first their K and V (HBM traffic of 244 rows, two groups:
 // that of one).  Bound by latency on one sequence (launch, lengths, first tile and
-// four tiles in turn, 1 us each: 15 us), by HBM on 16 (285 MB in 68 us, 4.2 TB/s), on
+// four tiles in turn, 1 us each: 15 us), by HBM on 16 (285 MB in 70 us, 4.1 TB/s), on
 // the widest by a tile's work on each SIMD and in LDS, about 1000 cycles each of
 // matrix instructions, exponentials and reads for the 2500 that a tile takes.
 // The weights p enter their product with V rounded to the 16-bit type, as the flash
