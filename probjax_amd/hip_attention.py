@@ -703,7 +703,8 @@ def _cache_call(who: str, q, k, v):
         raise ValueError(f"{who} takes bfloat16, float16 or float32 q, k and v of one dtype")
     if not 1 <= D <= 256:
         raise ValueError(f"{who}: head dims up to 256, got {D}")
-    if _tracked(q, k, v):
+    # (looked at here first, which spares the call: 0.3 us)
+    if (forward_ad._current_level >= 0 or q.requires_grad or k.requires_grad or v.requires_grad) and _tracked(q, k, v):
         raise ValueError(f"{who} has no gradient: call it under torch.no_grad() or on detached tensors")
     width = 64 if D <= 64 else 128 if D <= 128 else 256
     row = D
@@ -782,7 +783,7 @@ def _key_weights(weights, like, B, H, S):
     if not isinstance(weights, torch.Tensor) or weights.get_device() != like.get_device() \
             or weights.dtype is not torch.float32:
         raise ValueError(f"key weights must be a float32 tensor on {like.device}")
-    if _tracked(weights):
+    if (weights.requires_grad or forward_ad._current_level >= 0) and _tracked(weights):
         raise ValueError("key weights have no gradient: pass them detached or call under torch.no_grad()")
     if weights.shape != (B, H, S):
         raise ValueError(f"key weights must have shape {(B, H, S)}, got {tuple(weights.shape)}")
