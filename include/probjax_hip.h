@@ -632,6 +632,78 @@ int pjx_evict_keys(int64_t elem_size, const void* k, const void* v, const float*
                    int64_t recent, const pjx_cache_strides* strides, const pjx_cache_strides* out_strides, int fill,
                    void* stream);
 
+/*
+ * A paged KV cache: pools of pages that sequences share, and a row of page numbers
+ * per sequence.  No counterpart in the reference, whose caches are contiguous.
+ *
+ * Key j of sequence b lies in slot j % page_size of page table[b * table_stride +
+ * j / page_size]; a sequence holds up to table_len * page_size (at most 2^30) keys.
+ * An entry below 0, or of no page (>= pages), names none: what would be written
+ * there is dropped, zeros are read, and no row sees its keys.  Without a table
+ * (NULL) sequence b has the one page b (table_len 1): a contiguous cache
+ * [batch, page_size, kv_heads, head_dim].
+ *
+ * k, v: slot t of page p, head h at p * k_page + t * k_token + h * k_head (in
+ * elements, whole 16-byte chunks; features contiguous); rows are whole 16-byte
+ * chunks of at most 256 features, the pools start on 16 bytes.
+ *
+ * PJX_DTYPE_E4M3: rows in 8 bits.  A row (one key or value of one head) is held as
+ * e4m3 codes (4 bits of exponent, bias 7, 3 of fraction, no infinities) and one
+ * exponent, x = code * 2^(exponent - 127): the least, from 1 on, that brings the
+ * row's largest finite value to at most 448.  Values are rounded once, to the
+ * nearest code, ties to even; infinities and NaN become NaN; a value that would
+ * read back past the range of the type it came in is held at 240.  Exponents are
+ * contiguous bytes [pages, kv_heads, page_size] (NULL for other types).
+ */
+#define PJX_DTYPE_E4M3 3
+typedef struct pjx_pages {
+  void *k, *v;
+  uint8_t *k_exponents, *v_exponents;
+  const int32_t* table;
+  int64_t table_stride, table_len, pages, page_size;
+  int64_t k_page, k_token, k_head, v_page, v_token, v_head;
+} pjx_pages;
+
+/*
+ * Appends len new keys and values [batch, len, kv_heads, head_dim] (strides as for
+ * the caches above, NULL: contiguous) to their sequences: token t < new_lengths[b]
+ * (clamped to [0, len]; NULL: len) of sequence b becomes its key kv_lengths[b] + t
+ * (below 0: 0; NULL: 0), as far as the sequence has room.  lengths_out [batch]: the
+ * keys it has then, at most table_len * page_size.  Everything else in the pools
+ * stays.  Two tokens of one call must not name the same slot (sequences that share
+ * the page they write to).  dtype: of k and v; cache_dtype: dtype (copied) or
+ * PJX_DTYPE_E4M3.
+ */
+int pjx_write_pages(int dtype, int cache_dtype, const void* k, const void* v, const pjx_pages* cache,
+                    const int32_t* kv_lengths, const int32_t* new_lengths, int32_t* lengths_out, int64_t batch,
+                    int64_t len, int64_t kv_heads, int64_t head_dim, const pjx_cache_strides* strides, void* stream);
+
+/*
+ * Gathers the first out_len keys and values of every sequence into contiguous
+ * [batch, out_len, kv_heads, head_dim] tensors of dtype (the cache's, or of e4m3 any):
+ * code * 2^(exponent - 127) rounded once.  Zeros from kv_lengths[b] (NULL: all it has
+ * room for) on.
+ */
+int pjx_read_pages(int dtype, int cache_dtype, const pjx_pages* cache, const int32_t* kv_lengths, void* k_out,
+                   void* v_out, int64_t batch, int64_t out_len, int64_t kv_heads, int64_t head_dim, void* stream);
+
+/*
+ * Attention of every sequence's q_len newest tokens, whose keys the cache holds
+ * already: token t of q [batch, q_len, Hq, head_dim] sees the first
+ * kv_lengths[b] - (q_len - 1 - t) keys (kv_lengths clamped to what the sequence has
+ * room for; NULL: that), less those of missing pages.  What a row does not see does
+ * not reach it, infinities and NaN included; a row that sees nothing gives output 0
+ * and LSE +inf.  dtype of q and o; cache_dtype: dtype or PJX_DTYPE_E4M3.  lse:
+ * optional fp32 [batch, Hq, q_len], natural log.  q, o contiguous, on 16 bytes.
+ * workspace: on 16 bytes, at least pjx_paged_decode_workspace_size(batch, kv_heads,
+ * (Hq / kv_heads) * q_len, table_len * page_size, head_dim) bytes.
+ */
+size_t pjx_paged_decode_workspace_size(int64_t batch, int64_t kv_heads, int64_t rows, int64_t capacity,
+                                       int64_t head_dim);
+int pjx_paged_decode(int dtype, int cache_dtype, const void* q, const pjx_pages* cache, const int32_t* kv_lengths,
+                     void* o, float* lse, void* workspace, size_t workspace_bytes, int64_t batch, int64_t q_len,
+                     int64_t q_heads, int64_t kv_heads, int64_t head_dim, float sm_scale, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

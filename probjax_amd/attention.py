@@ -39,6 +39,7 @@ from __future__ import annotations
 import functools
 import math
 import os
+from dataclasses import dataclass
 from typing import NamedTuple
 
 import torch
@@ -751,6 +752,118 @@ def evict_keys(k, v, key_weights, keep: int, *, kv_lengths=None, sinks: int = 0,
     """
     return EvictedKeys(*hip.evict_keys(k, v, key_weights, keep, kv_lengths=kv_lengths, sinks=sinks, recent=recent,
                                        out=out))
+
+
+@dataclass(frozen=True, eq=False)
+class PagedCache:
+    """A KV cache in pages (no counterpart in the reference, whose caches are
+    contiguous): sequences of any length share a pool, and a page given back by one
+    serves another.
+
+    ``k`` / ``v`` ``[pages, page_size, Hkv, D]``, in any order of the first three axes
+    (say ``[pages, Hkv, page_size, D]`` transposed): bfloat16, float16, float32, or
+    float8_e4m3fn with ``k_exponents`` / ``v_exponents`` (uint8 ``[pages, Hkv,
+    page_size]``), which hold a row (one key or value of one head) as ``code *
+    2^(exponent - 127)``.  ``D`` up to 256, a row whole 16-byte chunks (multiples of 4
+    float32, 8 16-bit or 16 8-bit features).
+
+    ``page_table`` int32 ``[B, N]``: key j of sequence b lies in slot ``j % page_size``
+    of page ``page_table[b, j // page_size]``.  An entry below 0 (or of no page) names
+    none: writes to it are dropped, reads give zeros and no row sees its keys.  None:
+    page b is sequence b's only one, which makes ``k`` / ``v`` contiguous caches
+    ``[B, S, Hkv, D]``.
+
+    The tensors are used in place; their contents, the table's too, may change between
+    calls.  ``dataclasses.replace(cache, page_table=...)`` is the same pools for other
+    sequences.  Pools that are expanded, or share memory with each other, can be read
+    and attended over, not written to.  How many keys each sequence has is the caller's to keep: what
+    ``write_pages`` returns.
+    """
+
+    k: torch.Tensor
+    v: torch.Tensor
+    page_table: torch.Tensor | None = None
+    k_exponents: torch.Tensor | None = None
+    v_exponents: torch.Tensor | None = None
+
+    def __post_init__(self):
+        index, pages, unwritable = hip.pages_struct(self.k, self.v, self.page_table, self.k_exponents, self.v_exponents)
+        batch = self.k.shape[0] if self.page_table is None else self.page_table.shape[0]
+        for name, value in (("index", index), ("_pages", pages), ("unwritable", unwritable), ("batch", batch),
+                            ("code", hip.CACHE_DTYPES[self.k.dtype]), ("page_size", pages.page_size),
+                            ("capacity", pages.page_size * pages.table_len)):
+            object.__setattr__(self, name, value)
+
+    @classmethod
+    def allocate(cls, pages: int, page_size: int, kv_heads: int, head_dim: int, *, page_table=None,
+                 dtype=torch.bfloat16, device=None):
+        """A cache of new pools (their contents undefined) on the device of
+        ``page_table`` (or ``device``); ``dtype=torch.float8_e4m3fn``: in 8 bits."""
+        if device is None:
+            device = "cuda" if page_table is None else page_table.device
+        k, v = (torch.empty((pages, page_size, kv_heads, head_dim), dtype=dtype, device=device) for _ in range(2))
+        exponents = (None, None)
+        if dtype is torch.float8_e4m3fn:
+            exponents = [torch.empty((pages, kv_heads, page_size), dtype=torch.uint8, device=device) for _ in range(2)]
+        return cls(k, v, page_table, *exponents)
+
+    def pages(self):
+        """The tensors as the C entry points take them (``pjx_pages``)."""
+        return hip.set_pages(self._pages, self.k, self.v, self.page_table, self.k_exponents, self.v_exponents)
+
+
+def write_pages(cache: PagedCache, k, v, *, kv_lengths=None, new_lengths=None):
+    """Appends new keys and values to the sequences of a paged cache, in its type or
+    quantised to 8 bits (no counterpart in the reference).
+
+    ``k`` / ``v`` ``[B, T, Hkv, D]``, any strides (slices of a projection are read in
+    place).  Token t < ``new_lengths[b]`` (int ``[B]``, None: all T) becomes key
+    ``kv_lengths[b] + t`` of sequence b (``kv_lengths`` int ``[B]``, the keys it has;
+    None: none yet), as far as the sequence has room and a page for it; later tokens
+    are padding.  Returns the sequences' lengths then (int32 ``[B]``, at most the
+    capacity).  Nothing else in the pools changes.  Sequences that share pages must
+    not write to the same slot in one call.
+
+    In 8 bits (``cache.k.dtype`` float8_e4m3fn, k and v of any type) a row's exponent
+    is the least that brings its largest finite value to at most 448, so codes keep 4
+    significant bits (off by at most 2^-4 of a value) down to 2^-13 of the largest;
+    infinities and NaN become NaN, and a value that would read back past the range of
+    its own type is held at 240 * 2^exponent.  No gradient: inputs that require one, or
+    carry a tangent, raise.
+    """
+    return hip.write_pages(cache, k, v, kv_lengths=kv_lengths, new_lengths=new_lengths)
+
+
+def read_pages(cache: PagedCache, *, kv_lengths=None, length: int | None = None, dtype=None):
+    """The keys and values of a paged cache as contiguous ``(k, v)`` ``[B, length, Hkv,
+    D]`` (no counterpart in the reference): for a prompt's attention over what is
+    cached, say, with ``flex_attention``.
+
+    ``length``: None for all a sequence has room for.  Zeros from ``kv_lengths[b]``
+    (int ``[B]``, None: that room) on, and where a page is missing.  ``dtype``: the
+    cache's; of an 8-bit cache bfloat16 (default), float16 or float32, ``code *
+    2^exponent`` rounded once.  No gradient.
+    """
+    return hip.read_pages(cache, kv_lengths=kv_lengths, length=length, dtype=dtype)
+
+
+def paged_decode(q, cache: PagedCache, *, kv_lengths=None, sm_scale: float | None = None, return_lse: bool = False):
+    """Attention of every sequence's newest tokens over a paged cache that holds their
+    keys already (no counterpart in the reference, whose split-KV decode
+    (kernels/attention_splitkv.py:137-250) takes contiguous caches).
+
+    ``q [B, T, Hq, D]``, T tokens per sequence (1 as a rule); ``kv_lengths`` int
+    ``[B]`` counts all of its keys, the new tokens' too (None: all it has room for).
+    Token t sees the first ``kv_lengths[b] - (T - 1 - t)`` keys, less those of missing
+    pages.  What it does not see does not reach its output, infinities and NaN
+    included; a token that sees nothing gets 0 and LSE +inf.  bf16, fp16 or fp32 over a
+    cache of that type or of 8 bits; ``sm_scale`` defaults to ``1/sqrt(D)``.  With
+    ``return_lse`` also the natural-log LSE ``[B, Hq, T]``.  No gradient: inputs that
+    require one, or carry a tangent, raise.
+    """
+    if sm_scale is None:
+        sm_scale = 1.0 / math.sqrt(q.shape[-1])
+    return hip.paged_decode(q, cache, kv_lengths=kv_lengths, sm_scale=sm_scale, return_lse=return_lse)
 
 
 class _RotaryFunction(torch.autograd.Function):

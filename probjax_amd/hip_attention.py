@@ -657,7 +657,7 @@ def _int32(t, what: str, like, *shapes):
     return t
 
 
-def _key_lengths(kv_lengths, like, batch):
+def _key_lengths(kv_lengths, like, batch, what="kv_lengths"):
     """``kv_lengths`` as int32 ``[batch]`` on the device of ``like`` (None: none);
     like those of the other entry points they may come as ``[batch, 1]``."""
     if kv_lengths is None:
@@ -666,7 +666,7 @@ def _key_lengths(kv_lengths, like, batch):
         kv_lengths = torch.as_tensor(kv_lengths)
     if kv_lengths.ndim != 1:
         kv_lengths = kv_lengths.reshape(-1)
-    return _int32(kv_lengths, "kv_lengths", like, (batch,))
+    return _int32(kv_lengths, what, like, (batch,))
 
 
 @functools.lru_cache(maxsize=256)
@@ -1018,3 +1018,173 @@ def rotary(q, k, positions, sections, base: float, interleaved: bool, shared_spe
 def _int_array(values):
     """``values`` (a tuple) as a C array of int32."""
     return (ctypes.c_int32 * len(values))(*values)
+
+
+# ---------------------------------------------------------------------------
+# Paged caches
+# ---------------------------------------------------------------------------
+
+# dtypes of a paged cache's pools
+CACHE_DTYPES = {**_DTYPES, torch.float8_e4m3fn: native.PJX_DTYPE_E4M3}
+
+
+def pages_struct(k, v, page_table, k_exponents, v_exponents):
+    """``(index, pjx_pages, unwritable)`` of a paged cache's tensors (see
+    ``PagedCache``), checked; the struct's pointers are the caller's to set on every
+    call (``set_pages``).  ``unwritable``: why ``write_pages`` cannot take it, or None."""
+    if k.ndim != 4 or k.shape != v.shape or k.dtype is not v.dtype:
+        raise ValueError(f"a paged cache's k and v must be [pages, page_size, Hkv, D] of one shape and dtype, got "
+                         f"{tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}")
+    P, page, H, D = k.shape
+    if k.dtype not in CACHE_DTYPES:
+        raise ValueError(f"unsupported cache dtype {k.dtype}; expected bfloat16, float16, float32 or float8_e4m3fn")
+    if page < 1 or H < 1:
+        raise ValueError(f"a paged cache needs slots and heads, got {tuple(k.shape)}")
+    chunk = 16 // k.element_size()
+    if not 1 <= D <= 256 or D % chunk:
+        raise ValueError(f"a paged cache of {k.dtype} takes head dims up to 256 that are multiples of {chunk}, got {D}")
+    quantised = k.dtype is torch.float8_e4m3fn
+    if (k_exponents is None) == quantised or (v_exponents is None) == quantised:
+        raise ValueError("a cache of float8_e4m3fn needs k_exponents and v_exponents, other caches take none")
+    for what, x in (("k", k), ("v", v)):
+        if (D > 1 and x.stride(3) != 1) or x.data_ptr() % 16 or any(
+                n > 1 and s % chunk for n, s in zip(x.shape[:3], x.stride())):
+            raise ValueError(f"a paged cache's {what} needs contiguous features and rows that start on 16 bytes, got "
+                             f"strides {x.stride()} of {x.dtype}")
+    if quantised:
+        for what, x in (("k_exponents", k_exponents), ("v_exponents", v_exponents)):
+            if x.dtype is not torch.uint8 or x.shape != (P, H, page) or not x.is_contiguous():
+                raise ValueError(f"{what} must be contiguous uint8 {(P, H, page)}, got {x.dtype} {tuple(x.shape)}")
+    if page_table is None:
+        step, most = 0, 1
+    else:
+        if page_table.dtype is not torch.int32 or page_table.ndim != 2 or (
+                page_table.shape[1] > 1 and page_table.stride(1) != 1):
+            raise ValueError(f"page_table must be int32 [batch, pages of a sequence] with contiguous rows, got "
+                             f"{page_table.dtype} {tuple(page_table.shape)}")
+        step, most = page_table.stride(0), page_table.shape[1]
+    if page * most > 1 << 30:
+        raise ValueError(f"a sequence of a paged cache holds at most 2^30 keys, got room for {page * most}")
+    if any(t is not None and t.requires_grad for t in (k, v)) or _tracked(k, v):
+        raise ValueError("a paged cache has no gradient: its k and v must not require one")
+    index = _gpu(k, v, page_table, k_exponents, v_exponents)
+    # (an axis of one element has a stride of no meaning)
+    strides = [x.stride(i) if x.shape[i] > 1 else 0 for x in (k, v) for i in range(3)]
+    pages = native.Pages(None, None, None, None, None, step, most, P, page, *strides)
+    return index, pages, _unwritable([k, v] + [k_exponents, v_exponents] * quantised)
+
+
+def _unwritable(ts):
+    """Why tensors cannot be written by a launch whose order is open: an element that
+    lies in two places of one of them, or in two of them; None if none does."""
+    for t in ts:
+        end = 0  # of what the smaller strides reach
+        for s, n in sorted((s, n) for n, s in zip(t.shape, t.stride()) if n > 1):
+            if s <= end:
+                return "its pools are expanded, or their rows overlap each other"
+            end += (n - 1) * s
+    for i, a in enumerate(ts):
+        for b in ts[i + 1:]:
+            (x, x_end), (y, y_end) = _reach(a), _reach(b)
+            if x < y_end and y < x_end and _share_bytes(a, b):
+                return "its tensors share memory"
+    return None
+
+
+def set_pages(pages, k, v, page_table, k_exponents, v_exponents):
+    """``pages`` with the tensors' addresses."""
+    pages.k, pages.v, pages.table = k.data_ptr(), v.data_ptr(), _ptr(page_table)
+    if k_exponents is not None:
+        pages.k_exponents, pages.v_exponents = k_exponents.data_ptr(), v_exponents.data_ptr()
+    return pages
+
+
+def _rows_of_chunks(x):
+    """``x [B, T, H, D]``, copied unless its rows can be read 16 bytes at a time."""
+    n = 16 // x.element_size()
+    if x.is_contiguous() and x.data_ptr() % 16 == 0:
+        return x
+    if (x.stride(3) == 1 or x.shape[3] == 1) and x.data_ptr() % 16 == 0 and all(
+            x.shape[i] == 1 or x.stride(i) % n == 0 for i in range(3)):
+        return x
+    return _aligned(x.contiguous())
+
+
+def write_pages(cache, k, v, *, kv_lengths=None, new_lengths=None):
+    """``pjx_write_pages``: appends ``k``, ``v`` ``[B, T, Hkv, D]`` to the sequences of
+    a ``PagedCache`` -> their lengths then, int32 ``[B]``."""
+    if k.ndim != 4 or k.shape != v.shape or k.dtype is not v.dtype:
+        raise ValueError(f"k and v must be [B, T, Hkv, D] of one shape and dtype, got {tuple(k.shape)} {k.dtype} and "
+                         f"{tuple(v.shape)} {v.dtype}")
+    B, T, H, D = k.shape
+    _, _, Hc, Dc = cache.k.shape
+    if B != cache.batch or H != Hc or D != Dc:
+        raise ValueError(f"k {tuple(k.shape)} does not fit a cache of {cache.batch} sequences, {Hc} heads of {Dc}")
+    if cache.unwritable is not None:
+        raise ValueError(f"cannot write to this cache: {cache.unwritable}")
+    code = _dtype_code(k)
+    if cache.code != native.PJX_DTYPE_E4M3 and code != cache.code:
+        raise ValueError(f"a cache of {cache.k.dtype} takes keys and values of that dtype, got {k.dtype}")
+    if (forward_ad._current_level >= 0 or k.requires_grad or v.requires_grad) and _tracked(k, v):
+        raise ValueError("writing to a cache has no gradient: call it under torch.no_grad() or on detached tensors")
+    index = _gpu(k, v, cache.k)
+    k, v = _rows_of_chunks(k), _rows_of_chunks(v)
+    L, new = _key_lengths(kv_lengths, k, B), _key_lengths(new_lengths, k, B, "new_lengths")
+    lengths = torch.empty((B,), dtype=torch.int32, device=k.device)
+    _call(
+        index, native.load().pjx_write_pages, code, cache.code, k.data_ptr(), v.data_ptr(), cache.pages(), _ptr(L),
+        _ptr(new), lengths.data_ptr(), B, T, H, D, _pair_strides(k, v),
+    )
+    return lengths
+
+
+def read_pages(cache, *, kv_lengths=None, length: int | None = None, dtype=None):
+    """``pjx_read_pages``: the first ``length`` keys and values of every sequence of a
+    ``PagedCache`` -> ``(k, v)`` ``[B, length, Hkv, D]``, zeros behind ``kv_lengths``."""
+    k = cache.k
+    if dtype is None:
+        dtype = torch.bfloat16 if cache.code == native.PJX_DTYPE_E4M3 else k.dtype
+    if dtype not in _DTYPES or (cache.code != native.PJX_DTYPE_E4M3 and dtype is not k.dtype):
+        raise ValueError(f"a cache of {k.dtype} is read as " + (
+            "bfloat16, float16 or float32" if cache.code == native.PJX_DTYPE_E4M3 else "what it holds") + f", not {dtype}")
+    length = cache.capacity if length is None else int(length)
+    if not 0 <= length <= 1 << 30:
+        raise ValueError(f"length must be 0 to 2^30, got {length}")
+    B = cache.batch
+    _, _, H, D = k.shape
+    L = _key_lengths(kv_lengths, k, B)
+    out = k.new_empty((B, length, H, D), dtype=dtype), k.new_empty((B, length, H, D), dtype=dtype)
+    _call(
+        cache.index, native.load().pjx_read_pages, _DTYPES[dtype], cache.code, cache.pages(), _ptr(L),
+        out[0].data_ptr(), out[1].data_ptr(), B, length, H, D,
+    )
+    return out
+
+
+def paged_decode(q, cache, *, sm_scale: float, kv_lengths=None, return_lse: bool = False, workspace=None):
+    """``pjx_paged_decode``: attention of the newest tokens ``q [B, T, Hq, D]`` over a
+    ``PagedCache`` -> ``o`` (and the LSE ``[B, Hq, T]``)."""
+    if q.ndim != 4:
+        raise ValueError(f"paged attention: q must be [B, T, Hq, D], got {tuple(q.shape)}")
+    B, T, Hq, D = q.shape
+    _, _, H, Dc = cache.k.shape
+    if B != cache.batch or D != Dc or Hq < 1 or Hq % H or T < 1:
+        raise ValueError(f"paged attention: q {tuple(q.shape)} does not fit a cache of {cache.batch} sequences, {H} "
+                         f"heads of {Dc}")
+    code = _dtype_code(q)
+    if cache.code != native.PJX_DTYPE_E4M3 and code != cache.code:
+        raise ValueError(f"paged attention over a cache of {cache.k.dtype} takes q of that dtype, got {q.dtype}")
+    if (forward_ad._current_level >= 0 or q.requires_grad) and _tracked(q):
+        raise ValueError("paged attention has no gradient: call it under torch.no_grad() or on detached tensors")
+    index = _gpu(q, cache.k)
+    q = _aligned(q.contiguous())
+    L = _key_lengths(kv_lengths, q, B)
+    nbytes = _workspace_size("pjx_paged_decode_workspace_size", B, H, (Hq // H) * T, cache.capacity, D)
+    ws = _scratch(nbytes, q, workspace)
+    o = torch.empty_like(q)
+    lse = torch.empty((B, Hq, T), dtype=torch.float32, device=q.device) if return_lse else None
+    _call(
+        index, native.load().pjx_paged_decode, code, cache.code, q.data_ptr(), cache.pages(), _ptr(L), o.data_ptr(),
+        _ptr(lse), ws.data_ptr(), nbytes, B, T, Hq, H, D, sm_scale,
+    )
+    return (o, lse) if return_lse else o

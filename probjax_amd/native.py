@@ -16,6 +16,7 @@ LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libprobjax_hip.so"
 PJX_DTYPE_F32 = 0
 PJX_DTYPE_BF16 = 1
 PJX_DTYPE_F16 = 2
+PJX_DTYPE_E4M3 = 3  # of a paged cache
 PJX_OK = 0
 PJX_DECODE_STATIC_SCRATCH_BYTES = 32 << 20  # include/probjax_hip.h
 
@@ -49,11 +50,20 @@ class CacheStrides(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int64) for n in ("k_batch", "k_token", "k_head", "v_batch", "v_token", "v_head")]
 
 
+class Pages(ctypes.Structure):
+    """``pjx_pages``: the pools, exponents and page table of a paged cache."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "k_exponents", "v_exponents", "table")] + [
+        (n, ctypes.c_int64) for n in ("table_stride", "table_len", "pages", "page_size", "k_page", "k_token", "k_head",
+                                      "v_page", "v_token", "v_head")]
+
+
 # (name, restype, argtypes) of every exported entry point.
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _MODS = ctypes.POINTER(ScoreMods)
 _STRIDES = ctypes.POINTER(CacheStrides)
+_PAGES = ctypes.POINTER(Pages)
 _SIGNATURES = {
     "pjx_version": (ctypes.c_int, []),
     "pjx_last_error": (ctypes.c_char_p, []),
@@ -163,6 +173,20 @@ _SIGNATURES = {
         ctypes.c_int,
         [_I64, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _STRIDES, _STRIDES,
          ctypes.c_int, _P],
+    ),
+    "pjx_write_pages": (
+        ctypes.c_int,
+        [ctypes.c_int, ctypes.c_int, _P, _P, _PAGES, _P, _P, _P, _I64, _I64, _I64, _I64, _STRIDES, _P],
+    ),
+    "pjx_read_pages": (
+        ctypes.c_int,
+        [ctypes.c_int, ctypes.c_int, _PAGES, _P, _P, _P, _I64, _I64, _I64, _I64, _P],
+    ),
+    "pjx_paged_decode_workspace_size": (ctypes.c_size_t, [_I64, _I64, _I64, _I64, _I64]),
+    "pjx_paged_decode": (
+        ctypes.c_int,
+        [ctypes.c_int, ctypes.c_int, _P, _PAGES, _P, _P, _P, _P, ctypes.c_size_t, _I64, _I64, _I64, _I64, _I64,
+         ctypes.c_float, _P],
     ),
 }
 EXPORTED = tuple(_SIGNATURES)
