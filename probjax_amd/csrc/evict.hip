@@ -41,21 +41,6 @@ __device__ __forceinline__ uint32_t weight_key(uint32_t u) {
   return u >> 31 ? ~u : u | 0x80000000u;
 }
 
-// Inclusive prefix sums over the 16 lanes of a row, and over a wave.
-__device__ __forceinline__ int row_scan(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);  // row_shr:1
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
-  return x;
-}
-__device__ __forceinline__ int wave_scan(int x) {
-  x = row_scan(x);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1 and 3
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2 and 3
-  return x;
-}
-
 // R: weights of a thread's registers (the cache has at most R * kSelThreads); 0:
 // read again in every pass.
 constexpr int kTiles = 8;  // tiles of kSelThreads keys ranked, or loaded, together

@@ -3,13 +3,27 @@
 //   o_t = sum_j softmax_j(scale q_t.k_j) v_j,  j < L - (T-1-t),
 // L keys of the sequence, T new tokens (one as a rule).
 //
-// A workgroup per (sequence, token, query head); its waves take keys in turn, a wave
-// per key, and join at the end.
+// A workgroup takes a part of one sequence's keys for one KV head, with its (Hq/Hkv)*T
+// packed query rows as the columns of the matrix instructions (NRB blocks of 16); its
+// four waves take a quarter of the part each, 32 keys a step, and join at the end.  A
+// second kernel joins the parts.  How long a part is follows from the lengths, which
+// only the device knows: every wave works it out from all of them (plan), so a grid made
+// for the capacity, or captured once, is shared by whatever keys there are.
+//
+// A wave's K and V rows go from memory to LDS by loads of 16 bytes a lane that no
+// register waits for, whole rows each, one step ahead.  The lanes look up a page each, once per key, and hand the rows'
+// addresses around in LDS, so pages of any size and order cost the same.  K rows are read
+// back as the matrix operand; V is transposed by the LDS reads (ds_read_b64_tr).
+// 8-bit rows stay codes until they are operands, exact in bf16 and fp16; their powers of
+// two go to the scores (K) and to the softmax weights (V), after and before the products.
 #include <stdio.h>
 
 #include "pages.h"
 
 namespace pjx {
+
+constexpr int kPagedThreads = 256, kPagedWaves = 4;
+constexpr int kMinPart = 128;  // keys of a part at least (but for the last)
 
 struct PagedArgs {
   PageArgs p;
@@ -17,98 +31,723 @@ struct PagedArgs {
   char* o;
   float* lse;
   const int32_t* lengths;
-  int B, T, Hq, D;
-  float cx;
+  float* ws_o;   // [items][rows][W] unnormalised outputs of the parts
+  float* ws_ml;  // [items][rows][2] running max (log2 units), sum
+  int B, T, Hq, D, rows;
+  int items;     // most work items (parts of all sequences and KV heads) there may be
+  FastDiv by_g, by_t;
+  float cx;      // sm_scale * log2(e)
 };
 
-template <typename C, typename E>
-__global__ __launch_bounds__(256) void paged_decode_simple_kernel(PagedArgs a) {
-  constexpr int CS = fmt_size<C>(), ES = fmt_size<E>();
-  __shared__ float red[4][256 + 2];
-  const PageArgs& p = a.p;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int t = blockIdx.x / a.Hq, hq = blockIdx.x % a.Hq, b = blockIdx.y, h = hq / (a.Hq / p.H);
-  const int room = p.most * p.page;
-  const int L = (a.lengths ? min(max(a.lengths[b], 0), room) : room) - (a.T - 1 - t);
-  const bool in = 4 * lane < a.D;
-  auto load4 = [](const char* x, auto fmt, float* y) {
-    typedef decltype(fmt) F;
-    if constexpr (std::is_same<F, F32Fmt>::value) {
-      const f32x4 r = *(const f32x4*)x;
-      y[0] = r[0], y[1] = r[1], y[2] = r[2], y[3] = r[3];
-    } else if constexpr (std::is_same<F, E4m3Fmt>::value) {
-      const int r = *(const int*)x;
-      const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(r, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(r, true);
-      y[0] = lo[0], y[1] = lo[1], y[2] = hi[0], y[3] = hi[1];
-    } else {
-      const u32x2 r = *(const u32x2*)x;
-      y[0] = F::lo(r[0]), y[1] = F::hi(r[0]), y[2] = F::lo(r[1]), y[3] = F::hi(r[1]);
-    }
-  };
-  const int64_t row = ((int64_t)b * a.T + t) * a.Hq + hq;
-  float q[4] = {}, o[4] = {}, m = kMaxInit, l = 0.f;
-  if (in) load4(a.q + (row * a.D + 4 * lane) * ES, E{}, q);
-  for (int j = w; j < L; j += 4) {
-    const int i = p.by_page(j), slot = j - i * p.page;
-    const uint32_t page = page_entry(p, b, i);
-    if (page >= p.pages) continue;
-    float k[4] = {}, v[4] = {};
-    if (in) {
-      load4(p.k + page * p.kp + slot * p.kt + h * p.kh + 4 * lane * CS, C{}, k);
-      load4(p.v + page * p.vp + slot * p.vt + h * p.vh + 4 * lane * CS, C{}, v);
-    }
-    float s = (q[0] * k[0] + q[1] * k[1]) + (q[2] * k[2] + q[3] * k[3]);
-    for (int x = 32; x; x >>= 1) s += __shfl_xor(s, x);
-    float vs = 1.f;
-    if constexpr (CS == 1) {
-      const int64_t e = ((int64_t)page * p.H + h) * p.page + slot;
-      s *= exponent_scale(p.ke[e]);
-      vs = exponent_scale(p.ve[e]);
-    }
-    s *= a.cx;
-    const float mn = fmaxf(m, s), corr = fast_exp2(m - mn), pr = fast_exp2(s - mn);
-    m = mn;
-    l = fmaf(l, corr, pr);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = fmaf(o[e], corr, pr * vs * v[e]);
-  }
-#pragma unroll
-  for (int e = 0; e < 4; ++e) red[w][4 * lane + e] = o[e];
-  if (lane == 0) red[w][256] = m, red[w][257] = l;
-  __syncthreads();
-  if (w) return;
-  float M = kMaxInit, den = 0.f, sum[4] = {};
-  for (int x = 0; x < 4; ++x) M = fmaxf(M, red[x][256]);
-  for (int x = 0; x < 4; ++x) {
-    const float f = fast_exp2(red[x][256] - M);
-    den = fmaf(red[x][257], f, den);
-    for (int e = 0; e < 4; ++e) sum[e] = fmaf(red[x][4 * lane + e], f, sum[e]);
-  }
-  uint32_t bits = __float_as_uint(den);
-  asm volatile("" : "+v"(bits));  // (compiled without NaN in mind: a NaN sum is one of some key)
-  const bool some = bits != 0u;
-  float out[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) out[e] = some ? sum[e] / den : 0.f;
-  if (in) {
-    char* to = a.o + (row * a.D + 4 * lane) * ES;
-    if constexpr (ES == 4) *(f32x4*)to = f32x4{out[0], out[1], out[2], out[3]};
-    else *(u32x2*)to = u32x2{E::pack2(out[0], out[1]), E::pack2(out[2], out[3])};
-  }
-  if (a.lse && lane == 0) a.lse[((int64_t)b * a.Hq + hq) * a.T + t] = some ? (M + __log2f(den)) * kLn2 : INFINITY;
+__device__ __forceinline__ int paged_len(const PagedArgs& a, int b) {
+  const int room = a.p.most * a.p.page;
+  return a.lengths ? min(max(a.lengths[b], 0), room) : room;
 }
 
-template <typename C, typename E>
-static int run_simple(const PagedArgs& a, hipStream_t s, const char* who) {
-  launch_kernel<paged_decode_simple_kernel<C, E>>(dim3((unsigned)(a.Hq * a.T), (unsigned)a.B), dim3(256), 0, s, a);
+__device__ __forceinline__ int wave_sum(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
+
+// How the sequences are cut: into ceil(L / chunk) equal parts each (up to a rounding to
+// kMinPart), chunk the least power of two from kMinPart on that leaves at most a.items
+// work items.  The host's a.items allows a part per sequence and head, so there is one.
+struct Plan {
+  int chunk_log;
+  __device__ __forceinline__ int parts(int L) const { return (int)(((uint32_t)L + (1u << chunk_log) - 1u) >> chunk_log); }
+  __device__ __forceinline__ static int part_keys(int L, int n) { return n > 0 ? ((L - 1) / n + kMinPart) & ~(kMinPart - 1) : 0; }
+};
+// first: the length of sequence `lane` (0: none).
+__device__ __forceinline__ Plan make_plan(const PagedArgs& a, int first) {
+  const int lane = threadIdx.x & 63, most = a.items / a.p.H;  // parts of all sequences
+  Plan p = {7};
+  for (;; ++p.chunk_log) {
+    int n = min(p.parts(first), most + 1);
+    for (int b0 = 64; b0 < a.B; b0 += 64)
+      n = min(n + (b0 + lane < a.B ? p.parts(paged_len(a, b0 + lane)) : 0), most + 1);
+    if (wave_sum(n) <= most) return p;
+  }
+}
+// Part `item` of all sequences' parts in order: sequence b, its part c of n, the keys L.
+struct Part {
+  int b, c, n, L;
+};
+__device__ __forceinline__ bool find_part(const PagedArgs& a, const Plan& p, int first, int item, Part& w) {
+  const int lane = threadIdx.x & 63;
+  int run = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const int L = b0 == 0 ? first : b0 + lane < a.B ? paged_len(a, b0 + lane) : 0;
+    const int n = p.parts(L), upto = run + wave_scan(n);
+    const uint64_t past = __builtin_amdgcn_ballot_w64(upto > item);
+    if (past) {
+      const int src = __builtin_ctzll(past);
+      w.b = b0 + src;
+      w.n = __builtin_amdgcn_readlane(n, src);
+      w.L = __builtin_amdgcn_readlane(L, src);
+      w.c = item - (__builtin_amdgcn_readlane(upto, src) - w.n);
+      return true;
+    }
+    run = __builtin_amdgcn_readlane(upto, 63);
+  }
+  return false;
+}
+// Parts before those of sequence b, and b's.
+__device__ __forceinline__ int parts_before(const PagedArgs& a, const Plan& p, int first, int b, int& n_b) {
+  const int lane = threadIdx.x & 63;
+  int run = 0;
+  for (int b0 = 0;; b0 += 64) {
+    const int n = p.parts(b0 == 0 ? first : b0 + lane < a.B ? paged_len(a, b0 + lane) : 0);
+    const int upto = run + wave_scan(n);
+    if (b < b0 + 64) {
+      n_b = __builtin_amdgcn_readlane(n, b - b0);
+      return __builtin_amdgcn_readlane(upto, b - b0) - n_b;
+    }
+    run = __builtin_amdgcn_readlane(upto, 63);
+  }
+}
+
+// A step's K or V rows in LDS: rows of W elements of C, their 16-byte chunks at chunk ^
+// swz(row).  So that no read meets in a bank: a matrix operand of K (16 rows at one chunk
+// for 16 lanes, the next for the following 16), and the transposing reads of V (8 rows at
+// two chunks, 16 rows of codes at one).
+template <typename C, int W>
+struct PageTile {
+  static constexpr int CS = fmt_size<C>(), ROWB = W * CS, NC = ROWB / 16;
+  static constexpr int KS = ROWB > 512 ? 16 : 32;  // keys of a step
+  static constexpr int BYTES = KS * ROWB;
+  static constexpr int NL = BYTES / 1024;          // loads of a wave
+  static constexpr int RPI = 64 / NC;              // rows of a load
+  __device__ __forceinline__ static constexpr int swz(int r) {
+    return NC == 4 ? ((r >> 2) ^ ((r >> 4) << 1)) & 3 : NC == 8 ? (r & 6) | ((r >> 4) & 1) : ((r & 7) << 1) | ((r >> 4) & 1);
+  }
+  __device__ __forceinline__ static int at(int r, int chunk) { return r * ROWB + 16 * (chunk ^ swz(r)); }
+};
+
+// Loads from an address of each lane's own into LDS: lane l's 16 bytes land at lds + 16 * l
+// (dword or byte: at lds + 4 * l).  Written in assembly (they have no result a register
+// waits for): the compiler makes every transposing read of LDS wait for all loads it knows
+// of.  So it knows of none in the key loop, where arrived() counts them.  (M0 is not
+// in the clobbers, which may not name it; nothing else here uses it.)
+__device__ __forceinline__ uint32_t lds_offset(const void* p) {
+  return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p);
+}
+__device__ __forceinline__ void load_lds16(uint64_t from, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(lds) : "memory");
+}
+__device__ __forceinline__ void load_lds4(uint64_t from, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(lds) : "memory");
+}
+__device__ __forceinline__ void load_lds1(uint64_t from, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_ubyte %0, off" ::"v"(from), "s"(lds) : "memory");
+}
+
+// This wave's LDS accesses so far are done, and stay before this point.
+__device__ __forceinline__ void lds_done() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt(15 | (7 << 4) | (0 << 8) | (3 << 14));  // lgkmcnt(0)
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// All of this wave's loads but the last N have arrived.
+template <int N>
+__device__ __forceinline__ void arrived() {
+  __builtin_amdgcn_sched_barrier(0);
+  wait_vmcnt<N>();
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+__device__ __forceinline__ uint32_t bits_of(float x) {
+  uint32_t u = __float_as_uint(x);
+  asm volatile("" : "+v"(u));  // (the sources are compiled without NaN in mind)
+  return u;
+}
+
+// Whether any element of a dword of C is infinite or NaN.
+template <typename C>
+__device__ __forceinline__ bool odd_dword(uint32_t x) {
+  if constexpr (std::is_same<C, F32Fmt>::value) {
+    return (x & 0x7f800000u) == 0x7f800000u;
+  } else if constexpr (std::is_same<C, E4m3Fmt>::value) {
+    const uint32_t y = ~x & 0x7f7f7f7fu;  // a byte is 0 where the code is NaN
+    return ((y - 0x01010101u) & ~y & 0x80808080u) != 0u;
+  } else {
+    constexpr uint32_t ex = C::kF16 ? 0x7c00u : 0x7f80u;
+    return (x & ex) == ex || (x & (ex << 16)) == ex << 16;
+  }
+}
+
+// 8 codes as an operand of E (bf16 or fp16).
+template <typename E>
+__device__ __forceinline__ typename E::v8 codes8(uint32_t lo, uint32_t hi) {
+  u32x4 r;
+  if constexpr (E::kF16) {
+    r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, false));
+    r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, true));
+    r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, false));
+    r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, true));
+  } else {
+    r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, false));
+    r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, true));
+    r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, false));
+    r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, true));
+  }
+  return E::as8(r);
+}
+__device__ __forceinline__ f32x4 codes4(uint32_t w) {
+  const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+  return f32x4{lo[0], lo[1], hi[0], hi[1]};
+}
+
+// Workgroups of a compute unit, by their LDS.
+template <typename C, int W>
+constexpr int paged_occupancy() {
+  return W * fmt_size<C>() >= 512 ? 1 : 2;
+}
+
+// What the chunks behind a row's end are loaded from.
+__device__ const __attribute__((aligned(16))) uint32_t kZeros[4] = {};
+
+// C: format of the cache, E: of q and o; W: features of a row in LDS (64, 128, 256), ROWS:
+// a row has fewer, and zeros behind them; NRB: blocks of 16 query rows.
+template <typename C, typename E, int W, int NRB, bool ROWS>
+__global__ __launch_bounds__(kPagedThreads, (paged_occupancy<C, W>())) void paged_decode_kernel(PagedArgs a) {
+  using T = PageTile<C, W>;
+  constexpr bool F32 = std::is_same<E, F32Fmt>::value, QUANT = std::is_same<C, E4m3Fmt>::value;
+  // The weights' product with V: in 16 bits they are rounded to the type, in two parts
+  // (the rounding's rest is the second) where V is 8-bit codes: their scales have bf16's
+  // range, and fp16 outputs more bits than a bf16 weight has.
+  typedef typename std::conditional<QUANT && !F32, Bf16Fmt, E>::type EV;
+  constexpr bool SPLIT = QUANT && !F32 && std::is_same<E, F16Fmt>::value;
+  constexpr int KS = T::KS, KB = KS / 16, NL = T::NL, CS = T::CS, ES = fmt_size<E>();
+  constexpr int NDB = W / 16;
+  __shared__ __attribute__((aligned(1024))) unsigned char k_lds[kPagedWaves * T::BYTES];
+  __shared__ __attribute__((aligned(1024))) unsigned char v_lds[kPagedWaves * T::BYTES];
+  __shared__ __attribute__((aligned(16))) uint64_t rows_lds[kPagedWaves * 64];  // addresses of a step's K, V rows
+  __shared__ __attribute__((aligned(16))) uint32_t exp_lds[QUANT ? kPagedWaves * 64 : 4];
+  __shared__ __attribute__((aligned(16))) uint32_t page_lds[kPagedWaves * 64];  // pages of the next step's keys
+  __shared__ float2 ml_lds[kPagedWaves * 16];
+
+  const PageArgs& p = a.p;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c16 = lane & 15, q4 = lane >> 4;
+  const int q = a.by_g(blockIdx.x), g = blockIdx.x - q * p.H;
+  const int first = lane < a.B ? paged_len(a, lane) : 0;
+  const Plan plan = make_plan(a, first);
+  Part part;
+  if (!find_part(a, plan, first, q, part)) return;
+  const int b = part.b, keys = Plan::part_keys(part.L, part.n);
+  const int c0 = part.c * keys, c1 = min(c0 + keys, part.L);
+  const int per_wave = ((c1 - c0 + 127) >> 7) << 5;
+  const int w0 = c0 + w * per_wave, w1 = min(w0 + per_wave, c1);
+  const int row0 = blockIdx.y * 16 * NRB;
+
+  unsigned char* kl = k_lds + w * T::BYTES;
+  unsigned char* vl = v_lds + w * T::BYTES;
+  uint64_t* rl = rows_lds + w * 64;
+  uint32_t* el = exp_lds + (QUANT ? w * 64 : 0);
+  uint32_t* pl = page_lds + w * 64;
+  const uint32_t kl_at = lds_offset(kl), vl_at = lds_offset(vl), el_at = lds_offset(el), pl_at = lds_offset(pl);
+
+  // ---- the rows of a step, one lane per key and tensor (K: lanes 0..31, V: 32..63) ----
+  const int half = lane >> 5, lk = lane & 31;
+  const uint64_t pool = (uint64_t)(half ? p.v : p.k) + (uint64_t)g * (uint64_t)(half ? p.vh : p.kh);
+  const int64_t page_step = half ? p.vp : p.kp, token_step = half ? p.vt : p.kt;
+  const uint64_t exps = (uint64_t)(half ? p.ve : p.ke);
+  const uint64_t entries = p.table ? (uint64_t)(p.table + b * p.table_step) : (uint64_t)a.q;  // (read in any case)
+  auto look_up = [&](int k0) {  // the pages of a step's keys
+    load_lds4(entries + 4ull * (uint32_t)(p.table ? p.by_page(min(k0 + (lk & (KS - 1)), w1 - 1)) : 0), pl_at);
+  };
+  uint64_t exp_at = 0;
+  auto place = [&](int k0) -> uint32_t {  // their rows' addresses to LDS; which keys are there
+    const uint32_t page = p.table ? pl[lane] : (uint32_t)b;
+    const int key = k0 + (lk & (KS - 1)), kc = min(key, w1 - 1);
+    const bool some = page < p.pages;
+    const uint32_t pg = some ? page : 0u;
+    const int slot = kc - p.by_page(kc) * p.page;
+    rl[lane] = pool + (uint64_t)(pg * page_step + slot * token_step);
+    if constexpr (QUANT) exp_at = exps + (uint64_t)((int64_t)(pg * (uint64_t)p.H + g) * p.page + slot);
+    return (uint32_t)__builtin_amdgcn_ballot_w64(some && key < w1) & (uint32_t)((1ull << KS) - 1);
+  };
+  const int row_chunks = a.D * CS / 16;
+  auto fetch = [&](uint32_t to, int first) {
+    uint64_t at[NL];
+#pragma unroll
+    for (int i = 0; i < NL; ++i) at[i] = rl[first + i * T::RPI + lane / T::NC];
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int c = (lane % T::NC) ^ T::swz(i * T::RPI + lane / T::NC);
+      load_lds16(!ROWS || c < row_chunks ? at[i] + 16 * c : (uint64_t)kZeros, to + 1024 * i);
+    }
+  };
+  auto fetch_exps = [&]() {
+    if constexpr (QUANT) load_lds1(exp_at, el_at);
+  };
+
+  // ---- q as the B operand, features in the order the cache's rows are read in ----
+  int lim[NRB];  // keys that the lane's row sees
+  typename std::conditional<F32, f32x4, u32x4>::type qf[NRB][F32 ? W / 16 : W / 32];
+#pragma unroll
+  for (int rb = 0; rb < NRB; ++rb) {
+    const int row = row0 + 16 * rb + c16;
+    const bool in = row < a.rows;
+    const int gi = a.by_t(in ? row : 0), t = (in ? row : 0) - gi * a.T;
+    lim[rb] = part.L - (a.T - 1 - t);
+    const char* x = a.q + (((int64_t)b * a.T + t) * a.Hq + g * (a.Hq / p.H) + gi) * a.D * ES;
+    if constexpr (F32) {
+#pragma unroll
+      for (int j = 0; j < W / 16; ++j) {
+        const int d = QUANT ? 64 * (j / 4) + 16 * q4 + 4 * (j % 4) : 16 * j + 4 * q4;
+        qf[rb][j] = in && (!ROWS || d < a.D) ? *(const f32x4*)(x + 4 * d) : f32x4{};
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < W / 32; ++j) {
+        const int d = QUANT ? 64 * (j / 2) + 16 * q4 + 8 * (j % 2) : 32 * j + 8 * q4;
+        qf[rb][j] = in && (!ROWS || d < a.D) ? *(const u32x4*)(x + 2 * d) : u32x4{0u, 0u, 0u, 0u};
+      }
+    }
+  }
+
+  f32x4 acc[NRB][NDB];
+  float m_run[NRB], l_run[NRB];
+#pragma unroll
+  for (int rb = 0; rb < NRB; ++rb) {
+    m_run[rb] = kMaxInit;
+    l_run[rb] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NDB; ++i) acc[rb][i] = f32x4{};
+  }
+
+  uint32_t there = 0;
+  if (w0 < w1) {
+    look_up(w0);
+    arrived<0>();
+    there = place(w0);
+    lds_done();
+    look_up(w0 + KS);
+    fetch_exps();
+    fetch(kl_at, 0);
+    fetch(vl_at, 32);
+  }
+  for (int k0 = w0; k0 < w1; k0 += KS) {
+    arrived<NL>();  // K's rows and the next step's pages; behind them V's rows
+    u32x4 kf[KB][T::NC / 4];  // chunk 4j + q4 of key 16kb + c16
+    f32x4 ks[KB], vs[KB];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+      for (int j = 0; j < T::NC / 4; ++j) kf[kb][j] = *(const u32x4*)(kl + T::at(16 * kb + c16, 4 * j + q4));
+      if constexpr (QUANT) {
+        const u32x4 ke = *(const u32x4*)(el + 16 * kb + 4 * q4), ve = *(const u32x4*)(el + 32 + 16 * kb + 4 * q4);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          ks[kb][r] = exponent_scale(ke[r]) * a.cx;
+          vs[kb][r] = exponent_scale(ve[r]);
+        }
+      }
+    }
+    // The next step's rows: as soon as this one's are in registers.  (The last step's next
+    // one is its last key again, which no one reads.)
+    const uint32_t here = there;
+    there = place(k0 + KS);
+    lds_done();
+    look_up(k0 + 2 * KS);
+    fetch_exps();
+    fetch(kl_at, 0);
+
+    // ---- scores: keys 16kb + 4q4 + r, query row 16rb + c16 ----
+    f32x4 s[NRB][KB];
+#pragma unroll
+    for (int rb = 0; rb < NRB; ++rb)
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        s[rb][kb] = f32x4{};
+        if constexpr (F32) {
+#pragma unroll
+          for (int j = 0; j < W / 16; ++j) {
+            f32x4 k;
+            if constexpr (QUANT) k = codes4(kf[kb][j / 4][j % 4]);
+            else k = __builtin_bit_cast(f32x4, kf[kb][j]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              s[rb][kb] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[e], qf[rb][j][e], s[rb][kb], 0, 0, 0);
+          }
+        } else if constexpr (QUANT) {
+#pragma unroll
+          for (int j = 0; j < W / 32; ++j)
+            s[rb][kb] = E::mma16(codes8<E>(kf[kb][j / 2][2 * (j % 2)], kf[kb][j / 2][2 * (j % 2) + 1]), E::as8(qf[rb][j]),
+                                 s[rb][kb]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < W / 32; ++j) s[rb][kb] = E::mma16(E::as8(kf[kb][j]), E::as8(qf[rb][j]), s[rb][kb]);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[rb][kb][r] *= QUANT ? ks[kb][r] : a.cx;
+      }
+    // Keys that some row does not see: past its own, past the wave's, of missing pages.
+    const bool whole = here == (uint32_t)((1ull << KS) - 1) && k0 + KS <= part.L - (a.T - 1);
+    auto sees = [&](int rb, int j) { return (here >> j & 1u) != 0u && k0 + j < lim[rb]; };
+    if (!whole) {
+#pragma unroll
+      for (int rb = 0; rb < NRB; ++rb)
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (!sees(rb, 16 * kb + 4 * q4 + r)) s[rb][kb][r] = -INFINITY;
+    }
+
+    // ---- online softmax; the running maximum is raised when it is 2^8 behind ----
+#pragma unroll
+    for (int rb = 0; rb < NRB; ++rb) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[rb][kb][r]);
+      mx = xor32_max(xor16_max(mx));
+      if (wave_any(mx > m_run[rb] + kRescaleLog2)) {
+        const float m_new = fmaxf(m_run[rb], mx), corr = fast_exp2(m_run[rb] - m_new);
+        m_run[rb] = m_new;
+        l_run[rb] *= corr;
+#pragma unroll
+        for (int i = 0; i < NDB; ++i) acc[rb][i] *= corr;
+      }
+      float rs = 0.f;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float x = fast_exp2(s[rb][kb][r] - m_run[rb]);
+          rs += x;
+          s[rb][kb][r] = QUANT ? x * vs[kb][r] : x;
+        }
+      l_run[rb] += rs;
+    }
+
+    // ---- O += P V ----
+    arrived<NL + (QUANT ? 2 : 1)>();  // V's rows; behind them the next step's pages, exponents and K
+    // V: the operand blocks' rows are dims, their columns the keys 4q4 + j and 16 + 4q4 + j
+    // (float32: the rows of four blocks are 4 c16 + i of 64 dims, keys 4q4 + e)
+    u32x4 vf[F32 ? KB * NDB : NDB];
+    if constexpr (F32) {
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int i = 0; i < NDB / 4; ++i) {
+            const int r = 16 * kb + 4 * q4 + e;
+            if constexpr (QUANT) vf[kb * NDB + i * 4][e] = *(const uint32_t*)(vl + T::at(r, 4 * i + c16 / 4) + 4 * (c16 & 3));
+            else vf[kb * NDB + e * (NDB / 4) + i] = *(const u32x4*)(vl + T::at(r, 16 * i + c16));
+          }
+    } else if constexpr (QUANT) {
+      const int r = (c16 & 8 ? 16 : 0) + 4 * q4 + ((c16 >> 1) & 3);
+#pragma unroll
+      for (int i = 0; i < NDB; ++i) {
+        typedef int i32x2 __attribute__((ext_vector_type(2)));
+        const auto x = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+            (__attribute__((address_space(3))) i32x2*)(vl + T::at(r, i) + 8 * (c16 & 1)));
+        vf[i][0] = (uint32_t)x[0];
+        vf[i][1] = (uint32_t)x[1];
+      }
+    } else {
+      const int r = 4 * q4 + (c16 >> 2);
+#pragma unroll
+      for (int i = 0; i < NDB; ++i) {
+        const u32x2 lo = lds_read_tr16(vl + T::at(r, 2 * i + ((c16 >> 1) & 1)) + 8 * (c16 & 1));
+        const u32x2 hi = lds_read_tr16(vl + T::at(16 + r, 2 * i + ((c16 >> 1) & 1)) + 8 * (c16 & 1));
+        vf[i] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+      }
+    }
+
+    bool apart = false;
+    if (!whole) {  // (an infinity or NaN must not reach the rows that do not see its key)
+      bool odd = false;
+      if constexpr (F32 && QUANT) {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int i = 0; i < NDB / 4; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) odd |= odd_dword<C>(vf[kb * NDB + i * 4][e]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < (F32 ? KB * NDB : NDB); ++i)
+#pragma unroll
+          for (int e = 0; e < (QUANT ? 2 : 4); ++e) odd |= odd_dword<C>(vf[i][e]);
+      }
+      apart = wave_any(odd);
+    }
+    if (apart) {
+      // one key after the other, for the rows that see it
+#pragma unroll 1
+      for (int j = 0; j < KS; ++j) {
+#pragma unroll
+        for (int rb = 0; rb < NRB; ++rb) {
+          float x = 0.f;  // the weight of key j = 16kb + 4qq + r, which lane 16qq + c16 holds
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const float y = __shfl(s[rb][kb][r], 16 * ((j >> 2) & 3) + c16);
+              x = 16 * kb + r == (j & 19) ? y : x;
+            }
+          const bool see = sees(rb, j);
+#pragma unroll
+          for (int i = 0; i < NDB; ++i) {
+            f32x4 v;
+            if constexpr (F32) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int d = 64 * (i / 4) + 4 * (4 * q4 + e) + i % 4;
+                if constexpr (QUANT) v[e] = codes4(vl[T::at(j, d / 16) + d % 16])[0];
+                else v[e] = *(const float*)(vl + T::at(j, d / 4) + 4 * (d % 4));
+              }
+            } else if constexpr (QUANT) {
+              v = codes4(*(const uint32_t*)(vl + T::at(j, i) + 4 * q4));
+            } else {
+              const u32x2 u = *(const u32x2*)(vl + T::at(j, 2 * i + (q4 >> 1)) + 8 * (q4 & 1));
+              v = f32x4{C::lo(u[0]), C::hi(u[0]), C::lo(u[1]), C::hi(u[1])};
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (see) acc[rb][i][e] = fmaf(x, v[e], acc[rb][i][e]);
+          }
+        }
+      }
+    }
+    lds_done();
+    fetch(vl_at, 32);
+    if (!apart) {
+#pragma unroll
+      for (int rb = 0; rb < NRB; ++rb) {
+        if constexpr (F32) {
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+              for (int i = 0; i < NDB / 4; ++i) {
+                f32x4 v;
+                if constexpr (QUANT) v = codes4(vf[kb * NDB + i * 4][e]);
+                else v = __builtin_bit_cast(f32x4, vf[kb * NDB + e * (NDB / 4) + i]);
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+                  acc[rb][4 * i + t] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[t], s[rb][kb][e], acc[rb][4 * i + t], 0, 0, 0);
+              }
+        } else {
+          u32x4 pk, rest;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float x = s[rb][i / 2][2 * (i % 2)], y = s[rb][i / 2][2 * (i % 2) + 1];
+            pk[i] = EV::pack2(x, y);
+            if constexpr (SPLIT) rest[i] = EV::pack2(x - EV::lo(pk[i]), y - EV::hi(pk[i]));
+          }
+#pragma unroll
+          for (int i = 0; i < NDB; ++i) {
+            typename EV::v8 v;
+            if constexpr (QUANT) v = codes8<EV>(vf[i][0], vf[i][1]);
+            else v = EV::as8(vf[i]);
+            acc[rb][i] = EV::mma16(v, EV::as8(pk), acc[rb][i]);
+            if constexpr (SPLIT) acc[rb][i] = EV::mma16(v, EV::as8(rest), acc[rb][i]);
+          }
+        }
+      }
+    }
+  }
+
+  arrived<0>();
+
+  // ---- the four waves' (max, sum, O), one block of rows at a time; the first half of the
+  // dims through K's memory, the second through V's: quad c of row r at c ^ r ----
+  constexpr int NQ = W / 4, HQ = NQ / 2;  // quads of dims of a row, and of a half
+#pragma unroll
+  for (int rb = 0; rb < NRB; ++rb) {
+    const float l = xor32_sum(xor16_sum(l_run[rb]));
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NDB; ++i) {
+      f32x4 x = acc[rb][i];
+      int quad = 4 * i + q4;
+      if constexpr (F32) {  // quad 16j + 4q4 + r: element r of the four blocks 4j ..
+#pragma unroll
+        for (int t = 0; t < 4; ++t) x[t] = acc[rb][i / 4 * 4 + t][i % 4];
+        quad = i / 4 * 16 + 4 * q4 + i % 4;
+      }
+      unsigned char* to = quad < HQ ? k_lds : v_lds;
+      *(f32x4*)(to + ((w * 16 + c16) * HQ + ((quad % HQ) ^ (c16 & (HQ - 1)))) * 16) = x;
+    }
+    if (q4 == 0) ml_lds[w * 16 + c16] = make_float2(m_run[rb], l);
+    __syncthreads();
+    const int nr = min(16, a.rows - row0 - 16 * rb);
+    for (int e = tid; e < nr * NQ; e += kPagedThreads) {
+      const int r = e / NQ, c = e % NQ;
+      if (4 * c >= a.D) continue;
+      float2 ml[kPagedWaves];
+      float M = kMaxInit;
+#pragma unroll
+      for (int x = 0; x < kPagedWaves; ++x) {
+        ml[x] = ml_lds[x * 16 + r];
+        M = fmaxf(M, ml[x].x);
+      }
+      float den = 0.f;
+      f32x4 O = {};
+      const unsigned char* from = c < HQ ? k_lds : v_lds;
+#pragma unroll
+      for (int x = 0; x < kPagedWaves; ++x) {
+        const float f = fast_exp2(ml[x].x - M);
+        den = fmaf(f, ml[x].y, den);
+        const f32x4 o = *(const f32x4*)(from + ((x * 16 + r) * HQ + ((c % HQ) ^ (r & (HQ - 1)))) * 16);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) O[i] = fmaf(f, o[i], O[i]);
+      }
+      const int row = row0 + 16 * rb + r;
+      if (part.n == 1) {
+        const int gi = a.by_t(row), t = row - gi * a.T, hq = g * (a.Hq / p.H) + gi;
+        const bool some = bits_of(den) != 0u;
+        f32x4 out;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) out[i] = some ? O[i] / den : 0.f;
+        char* to = a.o + ((((int64_t)b * a.T + t) * a.Hq + hq) * a.D + 4 * c) * ES;
+        if constexpr (F32) *(f32x4*)to = out;
+        else *(u32x2*)to = u32x2{E::pack2(out[0], out[1]), E::pack2(out[2], out[3])};
+        if (a.lse && c == 0) a.lse[((int64_t)b * a.Hq + hq) * a.T + t] = some ? (M + __log2f(den)) * kLn2 : INFINITY;
+      } else {
+        const int64_t at = (int64_t)blockIdx.x * a.rows + row;
+        *(f32x4*)(a.ws_o + at * W + 4 * c) = O;
+        if (c == 0) *(float2*)(a.ws_ml + 2 * at) = make_float2(M, den);
+      }
+    }
+  }
+}
+
+// Joins the parts of a sequence: a workgroup per (sequence, KV head, query row), 256 / (W
+// / 4) parts at a time and up to 8 of a thread in flight.  Sequences of one part are
+// finished; those without keys give 0 and LSE +inf.
+template <typename E, int W>
+__global__ __launch_bounds__(kPagedThreads) void paged_join_kernel(PagedArgs a) {
+  constexpr int NQ = W / 4, SL = kPagedThreads / NQ, U = 8;
+  __shared__ float2 ml_lds[SL];
+  __shared__ f32x4 o_lds[SL * NQ];
+  const int tid = threadIdx.x, c = tid % NQ, sl = tid / NQ;
+  const int row = blockIdx.x;
+  const int len = (tid & 63) < a.B ? paged_len(a, tid & 63) : 0;
+  const Plan plan = make_plan(a, len);
+  for (int pair = blockIdx.y; pair < a.B * a.p.H; pair += gridDim.y) {
+    const int b = a.by_g(pair), g = pair - b * a.p.H;
+    int n;
+    const int before = parts_before(a, plan, len, b, n);
+    if (n == 1) continue;
+    const int64_t step = (int64_t)a.p.H * a.rows, first = ((int64_t)before * a.p.H + g) * a.rows + row;
+    float M = kMaxInit, den = 0.f;
+    f32x4 O = {};
+    for (int x0 = sl; x0 < n; x0 += U * SL) {
+      float2 ml[U];
+      f32x4 o[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t at = first + min(x0 + u * SL, n - 1) * step;
+        ml[u] = *(const float2*)(a.ws_ml + 2 * at);
+        o[u] = 4 * c < a.D ? *(const f32x4*)(a.ws_o + at * W + 4 * c) : f32x4{};
+      }
+      float m = M;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (x0 + u * SL < n) m = fmaxf(m, ml[u].x);
+      const float f = fast_exp2(M - m);
+      M = m;
+      den *= f;
+      O *= f;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (x0 + u * SL < n) {
+          const float y = fast_exp2(ml[u].x - M);
+          den = fmaf(y, ml[u].y, den);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) O[i] = fmaf(y, o[u][i], O[i]);
+        }
+    }
+    __syncthreads();  // (the pair before is done with the memory)
+    if (c == 0) ml_lds[sl] = make_float2(M, den);
+    o_lds[tid] = O;
+    __syncthreads();
+    if (sl) continue;
+#pragma unroll
+    for (int x = 0; x < SL; ++x) M = fmaxf(M, ml_lds[x].x);
+    den = 0.f;
+    O = f32x4{};
+#pragma unroll
+    for (int x = 0; x < SL; ++x) {
+      const float y = fast_exp2(ml_lds[x].x - M);
+      den = fmaf(y, ml_lds[x].y, den);
+      const f32x4 o = o_lds[x * NQ + c];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) O[i] = fmaf(y, o[i], O[i]);
+    }
+    const int gi = a.by_t(row), t = row - gi * a.T, hq = g * (a.Hq / a.p.H) + gi;
+    const bool some = bits_of(den) != 0u;
+    f32x4 out;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[i] = some ? O[i] / den : 0.f;
+    if (4 * c < a.D) {
+      char* to = a.o + ((((int64_t)b * a.T + t) * a.Hq + hq) * a.D + 4 * c) * fmt_size<E>();
+      if constexpr (std::is_same<E, F32Fmt>::value) *(f32x4*)to = out;
+      else *(u32x2*)to = u32x2{E::pack2(out[0], out[1]), E::pack2(out[2], out[3])};
+    }
+    if (a.lse && c == 0) a.lse[((int64_t)b * a.Hq + hq) * a.T + t] = some ? (M + __log2f(den)) * kLn2 : INFINITY;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host
+// ---------------------------------------------------------------------------
+constexpr int64_t kPagedItems = 1024;  // work items that fill the device
+
+// Most work items: kPagedItems, or two parts per sequence and head where those are more;
+// never more than there are parts of kMinPart keys.
+static int64_t paged_items(int64_t batch, int64_t kv_heads, int64_t capacity) {
+  const int64_t pairs = batch * kv_heads, most = std::max<int64_t>((capacity + kMinPart - 1) / kMinPart, 1);
+  const int64_t want = std::max(kPagedItems / kv_heads * kv_heads, 2 * pairs);
+  return pairs > 0 && most > want / pairs ? std::max(want, pairs) : pairs * most;
+}
+static int paged_width(int64_t head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
+static size_t paged_ws(int64_t batch, int64_t kv_heads, int64_t rows, int64_t capacity, int64_t head_dim) {
+  return (size_t)(paged_items(batch, kv_heads, capacity) * rows * (paged_width(head_dim) + 2)) * sizeof(float) + 16;
+}
+
+template <typename C, typename E, int W, bool ROWS>
+static int run_paged(PagedArgs& a, hipStream_t s, const char* who) {
+  constexpr bool WIDE = W == 256;  // (32 rows of 256 features spill registers)
+  const bool two = !WIDE && a.rows > 16;
+  const dim3 grid((unsigned)a.items, (unsigned)((a.rows + (two ? 31 : 15)) / (two ? 32 : 16)));
+  if (two) launch_kernel<paged_decode_kernel<C, E, W, WIDE ? 1 : 2, ROWS>>(grid, dim3(kPagedThreads), 0, s, a);
+  else launch_kernel<paged_decode_kernel<C, E, W, 1, ROWS>>(grid, dim3(kPagedThreads), 0, s, a);
+  int rc = check_launch(who);
+  if (rc) return rc;
+  // (sequences of more than one part, or of none)
+  launch_kernel<paged_join_kernel<E, W>>(dim3((unsigned)a.rows, (unsigned)std::min(a.B * a.p.H, 65535)), dim3(kPagedThreads), 0, s, a);
   return check_launch(who);
+}
+template <typename C, typename E, int W>
+static int run_paged(PagedArgs& a, hipStream_t s, const char* who) {
+  return a.D < W ? run_paged<C, E, W, true>(a, s, who) : run_paged<C, E, W, false>(a, s, who);
+}
+template <typename C, typename E>
+static int run_paged(PagedArgs& a, hipStream_t s, const char* who) {
+  const int w = paged_width(a.D);
+  return w == 64 ? run_paged<C, E, 64>(a, s, who) : w == 128 ? run_paged<C, E, 128>(a, s, who) : run_paged<C, E, 256>(a, s, who);
 }
 
 }  // namespace pjx
 
 using namespace pjx;
 
-extern "C" size_t pjx_paged_decode_workspace_size(int64_t, int64_t, int64_t, int64_t, int64_t) { return 16; }
+extern "C" size_t pjx_paged_decode_workspace_size(int64_t batch, int64_t kv_heads, int64_t rows, int64_t capacity,
+                                                  int64_t head_dim) {
+  if (batch < 0 || kv_heads <= 0 || rows < 0 || capacity < 0) return 16;
+  return paged_ws(batch, kv_heads, rows, capacity, head_dim);
+}
 
 extern "C" int pjx_paged_decode(int dtype, int cache_dtype, const void* q, const pjx_pages* cache,
                                 const int32_t* kv_lengths, void* o, float* lse, void* workspace,
@@ -121,23 +760,33 @@ extern "C" int pjx_paged_decode(int dtype, int cache_dtype, const void* q, const
   if (rc != PJX_OK) return rc;
   if (dtype != PJX_DTYPE_BF16 && dtype != PJX_DTYPE_F16 && dtype != PJX_DTYPE_F32)
     return fail(PJX_ERR_INVALID, "pjx_paged_decode: dtype must be PJX_DTYPE_BF16, PJX_DTYPE_F16 or PJX_DTYPE_F32");
-  const bool quant = cache_dtype == PJX_DTYPE_E4M3;
+  const bool quant = cache_dtype == PJX_DTYPE_E4M3, f32 = dtype == PJX_DTYPE_F32;
   if (!quant && cache_dtype != dtype) return fail(PJX_ERR_INVALID, "pjx_paged_decode: the cache has another dtype");
   if (q_len <= 0 || q_heads <= 0 || q_heads % kv_heads) return fail(PJX_ERR_INVALID, "pjx_paged_decode: bad sizes");
-  if (q_len > (1 << 20) || q_heads > (1 << 20) || batch * q_heads > (1 << 30) || batch * q_heads * q_len > (1 << 30))
+  const int64_t rows = q_heads / kv_heads * q_len, capacity = cache->page_size * cache->table_len;
+  if (q_len > (1 << 20) || q_heads > (1 << 20) || rows > (1 << 19) || batch * kv_heads > (1 << 22) ||
+      batch * kv_heads * rows > (1 << 30))
     return fail(PJX_ERR_INVALID, "pjx_paged_decode: sizes out of range");
   if (!(sm_scale > 0.f)) return fail(PJX_ERR_INVALID, "pjx_paged_decode: sm_scale must be > 0");
   if (batch == 0) return PJX_OK;
   if (!q || !o) return fail(PJX_ERR_INVALID, "pjx_paged_decode: null pointer");
   if (((uintptr_t)q | (uintptr_t)o) % 16) return fail(PJX_ERR_INVALID, "pjx_paged_decode: q and o must start on 16 bytes");
-  if (!workspace || workspace_bytes < 16) return fail(PJX_ERR_WORKSPACE, "pjx_paged_decode: workspace missing or too small");
-  a.q = (const char*)q; a.o = (char*)o; a.lse = lse; a.lengths = kv_lengths;
-  a.B = (int)batch; a.T = (int)q_len; a.Hq = (int)q_heads; a.D = (int)head_dim;
-  a.cx = sm_scale * kLog2e;
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == PJX_DTYPE_F32)
-    return quant ? run_simple<E4m3Fmt, F32Fmt>(a, s, who) : run_simple<F32Fmt, F32Fmt>(a, s, who);
-  if (dtype == PJX_DTYPE_BF16)
-    return quant ? run_simple<E4m3Fmt, Bf16Fmt>(a, s, who) : run_simple<Bf16Fmt, Bf16Fmt>(a, s, who);
-  return quant ? run_simple<E4m3Fmt, F16Fmt>(a, s, who) : run_simple<F16Fmt, F16Fmt>(a, s, who);
+  if (capacity == 0 || cache->pages == 0)
+    return write_keyless(o, lse, (size_t)(batch * q_len * q_heads * head_dim), f32, (size_t)(batch * q_heads * q_len), s,
+                         who);
+  if (!workspace || workspace_bytes < paged_ws(batch, kv_heads, rows, capacity, head_dim))
+    return fail(PJX_ERR_WORKSPACE, "pjx_paged_decode: workspace missing or too small");
+  if ((uintptr_t)workspace % 16) return fail(PJX_ERR_INVALID, "pjx_paged_decode: the workspace must start on 16 bytes");
+  a.q = (const char*)q; a.o = (char*)o; a.lse = lse; a.lengths = kv_lengths;
+  a.B = (int)batch; a.T = (int)q_len; a.Hq = (int)q_heads; a.D = (int)head_dim; a.rows = (int)rows;
+  a.items = (int)paged_items(batch, kv_heads, capacity);
+  a.by_g = fast_div(kv_heads);
+  a.by_t = fast_div(q_len);
+  a.cx = sm_scale * kLog2e;
+  a.ws_o = (float*)workspace;
+  a.ws_ml = a.ws_o + (int64_t)a.items * rows * paged_width(head_dim);
+  if (f32) return quant ? run_paged<E4m3Fmt, F32Fmt>(a, s, who) : run_paged<F32Fmt, F32Fmt>(a, s, who);
+  if (dtype == PJX_DTYPE_BF16) return quant ? run_paged<E4m3Fmt, Bf16Fmt>(a, s, who) : run_paged<Bf16Fmt, Bf16Fmt>(a, s, who);
+  return quant ? run_paged<E4m3Fmt, F16Fmt>(a, s, who) : run_paged<F16Fmt, F16Fmt>(a, s, who);
 }
