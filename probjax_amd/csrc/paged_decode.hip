@@ -22,8 +22,8 @@
 
 namespace pjx {
 
-constexpr int kPagedThreads = 256, kPagedWaves = 4;
-constexpr int kMinPart = 128;  // keys of a part at least (but for the last)
+constexpr int kPagedWaves = 4;
+constexpr int kMinPart = 64;  // keys of a part at least (but for the last)
 
 struct PagedArgs {
   PageArgs p;
@@ -35,6 +35,8 @@ struct PagedArgs {
   float* ws_ml;  // [items][rows][2] running max (log2 units), sum
   int B, T, Hq, D, rows;
   int items;     // most work items (parts of all sequences and KV heads) there may be
+  int cut;       // 0: enough for parts of kMinPart keys whatever the lengths
+  int unit;      // kMinPart, or as many times that as keeps the sum of all lengths in 30 bits
   FastDiv by_g, by_t;
   float cx;      // sm_scale * log2(e)
 };
@@ -46,24 +48,29 @@ __device__ __forceinline__ int paged_len(const PagedArgs& a, int b) {
 
 __device__ __forceinline__ int wave_sum(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
 
-// How the sequences are cut: into ceil(L / chunk) equal parts each (up to a rounding to
-// kMinPart), chunk the least power of two from kMinPart on that leaves at most a.items
-// work items.  The host's a.items allows a part per sequence and head, so there is one.
+// How the sequences are cut: into ceil(L / chunk) parts each, equal but for a rounding to
+// kMinPart, with a chunk for all of them that leaves at most a.items work items.  With u =
+// chunk / a.unit and m_b = ceil(L_b / a.unit), B' sequences of any keys have at most
+//   sum ceil(m_b / u) <= (sum m_b) / u + B'
+// parts, so u = ceil(sum m_b / (parts wanted - B')) will do; chunk = kMinPart where there
+// may be as many items as that makes.
 struct Plan {
-  int chunk_log;
-  __device__ __forceinline__ int parts(int L) const { return (int)(((uint32_t)L + (1u << chunk_log) - 1u) >> chunk_log); }
+  int chunk;
+  __device__ __forceinline__ int parts(int L) const { return (int)(((uint32_t)L + (uint32_t)chunk - 1u) / (uint32_t)chunk); }
   __device__ __forceinline__ static int part_keys(int L, int n) { return n > 0 ? ((L - 1) / n + kMinPart) & ~(kMinPart - 1) : 0; }
 };
 // first: the length of sequence `lane` (0: none).
 __device__ __forceinline__ Plan make_plan(const PagedArgs& a, int first) {
-  const int lane = threadIdx.x & 63, most = a.items / a.p.H;  // parts of all sequences
-  Plan p = {7};
-  for (;; ++p.chunk_log) {
-    int n = min(p.parts(first), most + 1);
-    for (int b0 = 64; b0 < a.B; b0 += 64)
-      n = min(n + (b0 + lane < a.B ? p.parts(paged_len(a, b0 + lane)) : 0), most + 1);
-    if (wave_sum(n) <= most) return p;
+  if (!a.cut) return {kMinPart};
+  const int lane = threadIdx.x & 63;
+  int all = (first + a.unit - 1) / a.unit, some = first > 0;
+  for (int b0 = 64; b0 < a.B; b0 += 64) {
+    const int L = b0 + lane < a.B ? paged_len(a, b0 + lane) : 0;
+    all += (L + a.unit - 1) / a.unit;
+    some += L > 0;
   }
+  const int want = a.items / a.p.H - wave_sum(some);
+  return {max((wave_sum(all) + want - 1) / want, 1) * a.unit};
 }
 // Part `item` of all sequences' parts in order: sequence b, its part c of n, the keys L.
 struct Part {
@@ -129,7 +136,7 @@ __device__ __forceinline__ uint32_t lds_offset(const void* p) {
   return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p);
 }
 __device__ __forceinline__ void load_lds16(uint64_t from, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(lds) : "memory");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt" ::"v"(from), "s"(lds) : "memory");
 }
 __device__ __forceinline__ void load_lds4(uint64_t from, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(lds) : "memory");
@@ -209,7 +216,7 @@ __device__ const __attribute__((aligned(16))) uint32_t kZeros[4] = {};
 // C: format of the cache, E: of q and o; W: features of a row in LDS (64, 128, 256), ROWS:
 // a row has fewer, and zeros behind them; NRB: blocks of 16 query rows.
 template <typename C, typename E, int W, int NRB, bool ROWS>
-__global__ __launch_bounds__(kPagedThreads, (paged_occupancy<C, W>())) void paged_decode_kernel(PagedArgs a) {
+__global__ __launch_bounds__(64 * kPagedWaves, (paged_occupancy<C, W>())) void paged_decode_kernel(PagedArgs a) {
   using T = PageTile<C, W>;
   constexpr bool F32 = std::is_same<E, F32Fmt>::value, QUANT = std::is_same<C, E4m3Fmt>::value;
   // The weights' product with V: in 16 bits they are rounded to the type, in two parts
@@ -224,28 +231,21 @@ __global__ __launch_bounds__(kPagedThreads, (paged_occupancy<C, W>())) void page
   __shared__ __attribute__((aligned(16))) uint64_t rows_lds[kPagedWaves * 64];  // addresses of a step's K, V rows
   __shared__ __attribute__((aligned(16))) uint32_t exp_lds[QUANT ? kPagedWaves * 64 : 4];
   __shared__ __attribute__((aligned(16))) uint32_t page_lds[kPagedWaves * 64];  // pages of the next step's keys
-  __shared__ float2 ml_lds[kPagedWaves * 16];
-
   const PageArgs& p = a.p;
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int c16 = lane & 15, q4 = lane >> 4;
-  const int q = a.by_g(blockIdx.x), g = blockIdx.x - q * p.H;
+  const int lane = threadIdx.x & 63, c16 = lane & 15, q4 = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int item = blockIdx.x * kPagedWaves + w, q = a.by_g(item), g = item - q * p.H;
   const int first = lane < a.B ? paged_len(a, lane) : 0;
   const Plan plan = make_plan(a, first);
   Part part;
   if (!find_part(a, plan, first, q, part)) return;
   const int b = part.b, keys = Plan::part_keys(part.L, part.n);
-  const int c0 = part.c * keys, c1 = min(c0 + keys, part.L);
-  const int per_wave = ((c1 - c0 + 127) >> 7) << 5;
-  const int w0 = c0 + w * per_wave, w1 = min(w0 + per_wave, c1);
+  const int w0 = part.c * keys, w1 = min(w0 + keys, part.L);
   const int row0 = blockIdx.y * 16 * NRB;
 
-  unsigned char* kl = k_lds + w * T::BYTES;
-  unsigned char* vl = v_lds + w * T::BYTES;
+  unsigned char *kl = k_lds + w * T::BYTES, *vl = v_lds + w * T::BYTES;
   uint64_t* rl = rows_lds + w * 64;
-  uint32_t* el = exp_lds + (QUANT ? w * 64 : 0);
-  uint32_t* pl = page_lds + w * 64;
+  uint32_t *el = exp_lds + (QUANT ? w * 64 : 0), *pl = page_lds + w * 64;
   const uint32_t kl_at = lds_offset(kl), vl_at = lds_offset(vl), el_at = lds_offset(el), pl_at = lds_offset(pl);
 
   // ---- the rows of a step, one lane per key and tensor (K: lanes 0..31, V: 32..63) ----
@@ -318,17 +318,14 @@ __global__ __launch_bounds__(kPagedThreads, (paged_occupancy<C, W>())) void page
     for (int i = 0; i < NDB; ++i) acc[rb][i] = f32x4{};
   }
 
-  uint32_t there = 0;
-  if (w0 < w1) {
-    look_up(w0);
-    arrived<0>();
-    there = place(w0);
-    lds_done();
-    look_up(w0 + KS);
-    fetch_exps();
-    fetch(kl_at, 0);
-    fetch(vl_at, 32);
-  }
+  look_up(w0);
+  arrived<0>();
+  uint32_t there = place(w0);
+  lds_done();
+  look_up(w0 + KS);
+  fetch_exps();
+  fetch(kl_at, 0);
+  fetch(vl_at, 32);
   for (int k0 = w0; k0 < w1; k0 += KS) {
     arrived<NL>();  // K's rows and the next step's pages; behind them V's rows
     u32x4 kf[KB][T::NC / 4];  // chunk 4j + q4 of key 16kb + c16
@@ -358,32 +355,36 @@ __global__ __launch_bounds__(kPagedThreads, (paged_occupancy<C, W>())) void page
     // ---- scores: keys 16kb + 4q4 + r, query row 16rb + c16 ----
     f32x4 s[NRB][KB];
 #pragma unroll
-    for (int rb = 0; rb < NRB; ++rb)
+    for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
-        s[rb][kb] = f32x4{};
-        if constexpr (F32) {
+      for (int rb = 0; rb < NRB; ++rb) s[rb][kb] = f32x4{};
+      if constexpr (F32) {
 #pragma unroll
-          for (int j = 0; j < W / 16; ++j) {
-            f32x4 k;
-            if constexpr (QUANT) k = codes4(kf[kb][j / 4][j % 4]);
-            else k = __builtin_bit_cast(f32x4, kf[kb][j]);
+        for (int j = 0; j < W / 16; ++j) {
+          f32x4 k;
+          if constexpr (QUANT) k = codes4(kf[kb][j / 4][j % 4]);
+          else k = __builtin_bit_cast(f32x4, kf[kb][j]);
+#pragma unroll
+          for (int rb = 0; rb < NRB; ++rb)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               s[rb][kb] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[e], qf[rb][j][e], s[rb][kb], 0, 0, 0);
-          }
-        } else if constexpr (QUANT) {
-#pragma unroll
-          for (int j = 0; j < W / 32; ++j)
-            s[rb][kb] = E::mma16(codes8<E>(kf[kb][j / 2][2 * (j % 2)], kf[kb][j / 2][2 * (j % 2) + 1]), E::as8(qf[rb][j]),
-                                 s[rb][kb]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < W / 32; ++j) s[rb][kb] = E::mma16(E::as8(kf[kb][j]), E::as8(qf[rb][j]), s[rb][kb]);
         }
+      } else {
+#pragma unroll
+        for (int j = 0; j < W / 32; ++j) {
+          typename E::v8 k;
+          if constexpr (QUANT) k = codes8<E>(kf[kb][j / 2][2 * (j % 2)], kf[kb][j / 2][2 * (j % 2) + 1]);
+          else k = E::as8(kf[kb][j]);
+#pragma unroll
+          for (int rb = 0; rb < NRB; ++rb) s[rb][kb] = E::mma16(k, E::as8(qf[rb][j]), s[rb][kb]);
+        }
+      }
+#pragma unroll
+      for (int rb = 0; rb < NRB; ++rb)
 #pragma unroll
         for (int r = 0; r < 4; ++r) s[rb][kb][r] *= QUANT ? ks[kb][r] : a.cx;
-      }
+    }
     // Keys that some row does not see: past its own, past the wave's, of missing pages.
     const bool whole = here == (uint32_t)((1ull << KS) - 1) && k0 + KS <= part.L - (a.T - 1);
     auto sees = [&](int rb, int j) { return (here >> j & 1u) != 0u && k0 + j < lim[rb]; };
@@ -520,114 +521,89 @@ __global__ __launch_bounds__(kPagedThreads, (paged_occupancy<C, W>())) void page
     lds_done();
     fetch(vl_at, 32);
     if (!apart) {
+      if constexpr (F32) {
 #pragma unroll
-      for (int rb = 0; rb < NRB; ++rb) {
-        if constexpr (F32) {
+        for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-          for (int kb = 0; kb < KB; ++kb)
+          for (int e = 0; e < 4; ++e)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
+            for (int i = 0; i < NDB / 4; ++i) {
+              f32x4 v;
+              if constexpr (QUANT) v = codes4(vf[kb * NDB + i * 4][e]);
+              else v = __builtin_bit_cast(f32x4, vf[kb * NDB + e * (NDB / 4) + i]);
 #pragma unroll
-              for (int i = 0; i < NDB / 4; ++i) {
-                f32x4 v;
-                if constexpr (QUANT) v = codes4(vf[kb * NDB + i * 4][e]);
-                else v = __builtin_bit_cast(f32x4, vf[kb * NDB + e * (NDB / 4) + i]);
+              for (int rb = 0; rb < NRB; ++rb)
 #pragma unroll
                 for (int t = 0; t < 4; ++t)
                   acc[rb][4 * i + t] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[t], s[rb][kb][e], acc[rb][4 * i + t], 0, 0, 0);
-              }
-        } else {
-          u32x4 pk, rest;
+            }
+      } else {
+        u32x4 pk[NRB], rest[NRB];
+#pragma unroll
+        for (int rb = 0; rb < NRB; ++rb)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float x = s[rb][i / 2][2 * (i % 2)], y = s[rb][i / 2][2 * (i % 2) + 1];
-            pk[i] = EV::pack2(x, y);
-            if constexpr (SPLIT) rest[i] = EV::pack2(x - EV::lo(pk[i]), y - EV::hi(pk[i]));
+            pk[rb][i] = EV::pack2(x, y);
+            if constexpr (SPLIT) rest[rb][i] = EV::pack2(x - EV::lo(pk[rb][i]), y - EV::hi(pk[rb][i]));
           }
 #pragma unroll
-          for (int i = 0; i < NDB; ++i) {
-            typename EV::v8 v;
-            if constexpr (QUANT) v = codes8<EV>(vf[i][0], vf[i][1]);
-            else v = EV::as8(vf[i]);
-            acc[rb][i] = EV::mma16(v, EV::as8(pk), acc[rb][i]);
-            if constexpr (SPLIT) acc[rb][i] = EV::mma16(v, EV::as8(rest), acc[rb][i]);
+        for (int i = 0; i < NDB; ++i) {
+          typename EV::v8 v;
+          if constexpr (QUANT) v = codes8<EV>(vf[i][0], vf[i][1]);
+          else v = EV::as8(vf[i]);
+#pragma unroll
+          for (int rb = 0; rb < NRB; ++rb) {
+            acc[rb][i] = EV::mma16(v, EV::as8(pk[rb]), acc[rb][i]);
+            if constexpr (SPLIT) acc[rb][i] = EV::mma16(v, EV::as8(rest[rb]), acc[rb][i]);
           }
         }
       }
     }
   }
+  arrived<0>();  // (nothing may come to LDS that is another's by then)
 
-  arrived<0>();
-
-  // ---- the four waves' (max, sum, O), one block of rows at a time; the first half of the
-  // dims through K's memory, the second through V's: quad c of row r at c ^ r ----
-  constexpr int NQ = W / 4, HQ = NQ / 2;  // quads of dims of a row, and of a half
 #pragma unroll
   for (int rb = 0; rb < NRB; ++rb) {
-    const float l = xor32_sum(xor16_sum(l_run[rb]));
-    __syncthreads();
+    const int row = row0 + 16 * rb + c16;
+    const float den = xor32_sum(xor16_sum(l_run[rb]));
+    if (row >= a.rows) continue;
+    const bool some = bits_of(den) != 0u;
+    const int gi = a.by_t(row), t = row - gi * a.T, hq = g * (a.Hq / p.H) + gi;
+    const int64_t at = part.n == 1 ? ((int64_t)b * a.T + t) * a.Hq + hq : (int64_t)item * a.rows + row;
 #pragma unroll
     for (int i = 0; i < NDB; ++i) {
       f32x4 x = acc[rb][i];
-      int quad = 4 * i + q4;
-      if constexpr (F32) {  // quad 16j + 4q4 + r: element r of the four blocks 4j ..
+      int d = 16 * i + 4 * q4;
+      if constexpr (F32) {  // dims 64j + 16q4 + 4r ..: element r of the four blocks 4j ..
 #pragma unroll
-        for (int t = 0; t < 4; ++t) x[t] = acc[rb][i / 4 * 4 + t][i % 4];
-        quad = i / 4 * 16 + 4 * q4 + i % 4;
+        for (int u = 0; u < 4; ++u) x[u] = acc[rb][i / 4 * 4 + u][i % 4];
+        d = 64 * (i / 4) + 16 * q4 + 4 * (i % 4);
       }
-      unsigned char* to = quad < HQ ? k_lds : v_lds;
-      *(f32x4*)(to + ((w * 16 + c16) * HQ + ((quad % HQ) ^ (c16 & (HQ - 1)))) * 16) = x;
-    }
-    if (q4 == 0) ml_lds[w * 16 + c16] = make_float2(m_run[rb], l);
-    __syncthreads();
-    const int nr = min(16, a.rows - row0 - 16 * rb);
-    for (int e = tid; e < nr * NQ; e += kPagedThreads) {
-      const int r = e / NQ, c = e % NQ;
-      if (4 * c >= a.D) continue;
-      float2 ml[kPagedWaves];
-      float M = kMaxInit;
-#pragma unroll
-      for (int x = 0; x < kPagedWaves; ++x) {
-        ml[x] = ml_lds[x * 16 + r];
-        M = fmaxf(M, ml[x].x);
-      }
-      float den = 0.f;
-      f32x4 O = {};
-      const unsigned char* from = c < HQ ? k_lds : v_lds;
-#pragma unroll
-      for (int x = 0; x < kPagedWaves; ++x) {
-        const float f = fast_exp2(ml[x].x - M);
-        den = fmaf(f, ml[x].y, den);
-        const f32x4 o = *(const f32x4*)(from + ((x * 16 + r) * HQ + ((c % HQ) ^ (r & (HQ - 1)))) * 16);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) O[i] = fmaf(f, o[i], O[i]);
-      }
-      const int row = row0 + 16 * rb + r;
+      if (ROWS && d >= a.D) continue;
       if (part.n == 1) {
-        const int gi = a.by_t(row), t = row - gi * a.T, hq = g * (a.Hq / p.H) + gi;
-        const bool some = bits_of(den) != 0u;
-        f32x4 out;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) out[i] = some ? O[i] / den : 0.f;
-        char* to = a.o + ((((int64_t)b * a.T + t) * a.Hq + hq) * a.D + 4 * c) * ES;
-        if constexpr (F32) *(f32x4*)to = out;
-        else *(u32x2*)to = u32x2{E::pack2(out[0], out[1]), E::pack2(out[2], out[3])};
-        if (a.lse && c == 0) a.lse[((int64_t)b * a.Hq + hq) * a.T + t] = some ? (M + __log2f(den)) * kLn2 : INFINITY;
+        for (int u = 0; u < 4; ++u) x[u] = some ? x[u] / den : 0.f;
+        char* to = a.o + (at * a.D + d) * ES;
+        if constexpr (F32) *(f32x4*)to = x;
+        else *(u32x2*)to = u32x2{E::pack2(x[0], x[1]), E::pack2(x[2], x[3])};
       } else {
-        const int64_t at = (int64_t)blockIdx.x * a.rows + row;
-        *(f32x4*)(a.ws_o + at * W + 4 * c) = O;
-        if (c == 0) *(float2*)(a.ws_ml + 2 * at) = make_float2(M, den);
+        *(f32x4*)(a.ws_o + at * W + d) = x;
       }
+    }
+    if (q4 == 0) {
+      if (part.n > 1) *(float2*)(a.ws_ml + 2 * at) = make_float2(m_run[rb], den);
+      else if (a.lse) a.lse[((int64_t)b * a.Hq + hq) * a.T + t] = some ? (m_run[rb] + __log2f(den)) * kLn2 : INFINITY;
     }
   }
 }
 
-// Joins the parts of a sequence: a workgroup per (sequence, KV head, query row), 256 / (W
-// / 4) parts at a time and up to 8 of a thread in flight.  Sequences of one part are
-// finished; those without keys give 0 and LSE +inf.
-template <typename E, int W>
-__global__ __launch_bounds__(kPagedThreads) void paged_join_kernel(PagedArgs a) {
-  constexpr int NQ = W / 4, SL = kPagedThreads / NQ, U = 8;
+// Joins the parts of a sequence: a workgroup of N threads per (sequence, KV head, query
+// row), N / (W / 4) parts at a time and up to 8 of a thread in flight.  Sequences of one
+// part are finished; those without keys give 0 and LSE +inf.
+template <typename E, int W, int N>
+__global__ __launch_bounds__(N) void paged_join_kernel(PagedArgs a) {
+  constexpr int NQ = W / 4, SL = N / NQ, U = 8;
   __shared__ float2 ml_lds[SL];
   __shared__ f32x4 o_lds[SL * NQ];
   const int tid = threadIdx.x, c = tid % NQ, sl = tid / NQ;
@@ -702,31 +678,35 @@ __global__ __launch_bounds__(kPagedThreads) void paged_join_kernel(PagedArgs a) 
 // ---------------------------------------------------------------------------
 // Host
 // ---------------------------------------------------------------------------
-constexpr int64_t kPagedItems = 1024;  // work items that fill the device
-
-// Most work items: kPagedItems, or two parts per sequence and head where those are more;
-// never more than there are parts of kMinPart keys.
-static int64_t paged_items(int64_t batch, int64_t kv_heads, int64_t capacity) {
+// Most work items, with `waves` of them to a compute unit at a time: as many as fill the
+// device once, or two parts per sequence and head where those are more; no more than parts
+// of kMinPart keys come to.
+static int64_t paged_items(int64_t batch, int64_t kv_heads, int64_t capacity, int waves) {
   const int64_t pairs = batch * kv_heads, most = std::max<int64_t>((capacity + kMinPart - 1) / kMinPart, 1);
-  const int64_t want = std::max(kPagedItems / kv_heads * kv_heads, 2 * pairs);
-  return pairs > 0 && most > want / pairs ? std::max(want, pairs) : pairs * most;
+  const int64_t want = std::max((int64_t)256 * waves / kv_heads * kv_heads, 2 * pairs);
+  return most <= want / std::max<int64_t>(pairs, 1) ? pairs * most : want;
 }
 static int paged_width(int64_t head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
 static size_t paged_ws(int64_t batch, int64_t kv_heads, int64_t rows, int64_t capacity, int64_t head_dim) {
-  return (size_t)(paged_items(batch, kv_heads, capacity) * rows * (paged_width(head_dim) + 2)) * sizeof(float) + 16;
+  return (size_t)(paged_items(batch, kv_heads, capacity, 2 * kPagedWaves) * rows * (paged_width(head_dim) + 2)) * sizeof(float) + 16;
 }
 
 template <typename C, typename E, int W, bool ROWS>
 static int run_paged(PagedArgs& a, hipStream_t s, const char* who) {
   constexpr bool WIDE = W == 256;  // (32 rows of 256 features spill registers)
   const bool two = !WIDE && a.rows > 16;
-  const dim3 grid((unsigned)a.items, (unsigned)((a.rows + (two ? 31 : 15)) / (two ? 32 : 16)));
-  if (two) launch_kernel<paged_decode_kernel<C, E, W, WIDE ? 1 : 2, ROWS>>(grid, dim3(kPagedThreads), 0, s, a);
-  else launch_kernel<paged_decode_kernel<C, E, W, 1, ROWS>>(grid, dim3(kPagedThreads), 0, s, a);
+  a.items = (int)paged_items(a.B, a.p.H, (int64_t)a.p.most * a.p.page, paged_occupancy<C, W>() * kPagedWaves);
+  a.cut = a.items < (int64_t)a.B * a.p.H * (((int64_t)a.p.most * a.p.page + kMinPart - 1) / kMinPart);
+  const int gx = (a.items + kPagedWaves - 1) / kPagedWaves;
+  const dim3 grid((unsigned)gx, (unsigned)((a.rows + (two ? 31 : 15)) / (two ? 32 : 16)));
+  if (two) launch_kernel<paged_decode_kernel<C, E, W, WIDE ? 1 : 2, ROWS>>(grid, dim3(64 * kPagedWaves), 0, s, a);
+  else launch_kernel<paged_decode_kernel<C, E, W, 1, ROWS>>(grid, dim3(64 * kPagedWaves), 0, s, a);
   int rc = check_launch(who);
   if (rc) return rc;
-  // (sequences of more than one part, or of none)
-  launch_kernel<paged_join_kernel<E, W>>(dim3((unsigned)a.rows, (unsigned)std::min(a.B * a.p.H, 65535)), dim3(kPagedThreads), 0, s, a);
+  // Sequences of more than one part, or of none.
+  const dim3 rows((unsigned)a.rows, (unsigned)std::min(a.B * a.p.H, 65535));
+  if (a.items / (a.B * a.p.H) > 8 * 256 / (W / 4)) launch_kernel<paged_join_kernel<E, W, 1024>>(rows, dim3(1024), 0, s, a);
+  else launch_kernel<paged_join_kernel<E, W, 256>>(rows, dim3(256), 0, s, a);
   return check_launch(who);
 }
 template <typename C, typename E, int W>
@@ -780,12 +760,14 @@ extern "C" int pjx_paged_decode(int dtype, int cache_dtype, const void* q, const
   if ((uintptr_t)workspace % 16) return fail(PJX_ERR_INVALID, "pjx_paged_decode: the workspace must start on 16 bytes");
   a.q = (const char*)q; a.o = (char*)o; a.lse = lse; a.lengths = kv_lengths;
   a.B = (int)batch; a.T = (int)q_len; a.Hq = (int)q_heads; a.D = (int)head_dim; a.rows = (int)rows;
-  a.items = (int)paged_items(batch, kv_heads, capacity);
+  int64_t unit = kMinPart;
+  while (batch * ((capacity + unit - 1) / unit) > (1 << 30)) unit *= 2;
+  a.unit = (int)unit;
   a.by_g = fast_div(kv_heads);
   a.by_t = fast_div(q_len);
   a.cx = sm_scale * kLog2e;
   a.ws_o = (float*)workspace;
-  a.ws_ml = a.ws_o + (int64_t)a.items * rows * paged_width(head_dim);
+  a.ws_ml = a.ws_o + paged_items(batch, kv_heads, capacity, 2 * kPagedWaves) * rows * paged_width(head_dim);
   if (f32) return quant ? run_paged<E4m3Fmt, F32Fmt>(a, s, who) : run_paged<F32Fmt, F32Fmt>(a, s, who);
   if (dtype == PJX_DTYPE_BF16) return quant ? run_paged<E4m3Fmt, Bf16Fmt>(a, s, who) : run_paged<Bf16Fmt, Bf16Fmt>(a, s, who);
   return quant ? run_paged<E4m3Fmt, F16Fmt>(a, s, who) : run_paged<F16Fmt, F16Fmt>(a, s, who);
