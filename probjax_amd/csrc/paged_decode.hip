@@ -36,6 +36,7 @@ struct PagedArgs {
   int B, T, Hq, D, rows;
   int items;     // most work items (parts of all sequences and KV heads) there may be
   int cut;       // 0: enough for parts of kMinPart keys whatever the lengths
+  int slices;    // paged_join_kernel
   int unit;      // kMinPart, or as many times that as keeps the sum of all lengths in 30 bits
   FastDiv by_g, by_t;
   float cx;      // sm_scale * log2(e)
@@ -598,16 +599,18 @@ __global__ __launch_bounds__(64 * kPagedWaves, (paged_occupancy<C, W>())) void p
   }
 }
 
-// Joins the parts of a sequence: a workgroup of N threads per (sequence, KV head, query
-// row), N / (W / 4) parts at a time and up to 8 of a thread in flight.  Sequences of one
-// part are finished; those without keys give 0 and LSE +inf.
-template <typename E, int W, int N>
-__global__ __launch_bounds__(N) void paged_join_kernel(PagedArgs a) {
-  constexpr int NQ = W / 4, SL = N / NQ, U = 8;
-  __shared__ float2 ml_lds[SL];
-  __shared__ f32x4 o_lds[SL * NQ];
-  const int tid = threadIdx.x, c = tid % NQ, sl = tid / NQ;
-  const int row = blockIdx.x;
+// Joins the parts of a sequence: 256 >> a.slices quads of dims of a (sequence, KV head) to
+// a workgroup, 1 << a.slices threads to a quad, which take every so manieth part, 8 of a
+// thread in flight.  Sequences of one part are finished; those without keys give 0 and LSE
+// +inf.
+template <typename E, int W>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
+  constexpr int NQ = W / 4, U = 8;
+  __shared__ f32x4 o_lds[256];
+  __shared__ float2 ml_lds[256];
+  const int tid = threadIdx.x, per = 256 >> a.slices, sl = tid >> (8 - a.slices), step = 1 << a.slices;
+  const int quad = blockIdx.x * per + (tid & (per - 1)), row = quad / NQ, c = quad % NQ;
+  const bool in = row < a.rows && 4 * c < a.D;
   const int len = (tid & 63) < a.B ? paged_len(a, tid & 63) : 0;
   const Plan plan = make_plan(a, len);
   for (int pair = blockIdx.y; pair < a.B * a.p.H; pair += gridDim.y) {
@@ -615,62 +618,61 @@ __global__ __launch_bounds__(N) void paged_join_kernel(PagedArgs a) {
     int n;
     const int before = parts_before(a, plan, len, b, n);
     if (n == 1) continue;
-    const int64_t step = (int64_t)a.p.H * a.rows, first = ((int64_t)before * a.p.H + g) * a.rows + row;
     float M = kMaxInit, den = 0.f;
     f32x4 O = {};
-    for (int x0 = sl; x0 < n; x0 += U * SL) {
+    const int64_t first = ((int64_t)before * a.p.H + g) * a.rows + (in ? row : 0), apart = (int64_t)a.p.H * a.rows;
+    for (int x0 = sl; x0 < n; x0 += U * step) {
       float2 ml[U];
       f32x4 o[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int64_t at = first + min(x0 + u * SL, n - 1) * step;
-        ml[u] = *(const float2*)(a.ws_ml + 2 * at);
-        o[u] = 4 * c < a.D ? *(const f32x4*)(a.ws_o + at * W + 4 * c) : f32x4{};
+        const bool ok = in && x0 + u * step < n;
+        const int64_t at = first + (ok ? x0 + u * step : x0) * apart;
+        ml[u] = ok ? *(const float2*)(a.ws_ml + 2 * at) : make_float2(kMaxInit, 0.f);
+        o[u] = ok ? *(const f32x4*)(a.ws_o + at * W + 4 * c) : f32x4{};
       }
       float m = M;
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (x0 + u * SL < n) m = fmaxf(m, ml[u].x);
+      for (int u = 0; u < U; ++u) m = fmaxf(m, ml[u].x);
       const float f = fast_exp2(M - m);
       M = m;
       den *= f;
       O *= f;
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (x0 + u * SL < n) {
-          const float y = fast_exp2(ml[u].x - M);
-          den = fmaf(y, ml[u].y, den);
+      for (int u = 0; u < U; ++u) {
+        const float y = fast_exp2(ml[u].x - M);
+        den = fmaf(y, ml[u].y, den);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) O[i] = fmaf(y, o[u][i], O[i]);
-        }
+        for (int i = 0; i < 4; ++i) O[i] = fmaf(y, o[u][i], O[i]);
+      }
     }
-    __syncthreads();  // (the pair before is done with the memory)
-    if (c == 0) ml_lds[sl] = make_float2(M, den);
-    o_lds[tid] = O;
-    __syncthreads();
-    if (sl) continue;
+    if (a.slices) {
+      __syncthreads();  // (the pair before is done with the memory)
+      ml_lds[tid] = make_float2(M, den);
+      o_lds[tid] = O;
+      __syncthreads();
+      if (sl) continue;
+      for (int x = 1; x < step; ++x) M = fmaxf(M, ml_lds[tid + x * per].x);
+      den = 0.f;
+      O = f32x4{};
+      for (int x = 0; x < step; ++x) {
+        const float2 ml = ml_lds[tid + x * per];
+        const f32x4 o = o_lds[tid + x * per];
+        const float y = fast_exp2(ml.x - M);
+        den = fmaf(y, ml.y, den);
 #pragma unroll
-    for (int x = 0; x < SL; ++x) M = fmaxf(M, ml_lds[x].x);
-    den = 0.f;
-    O = f32x4{};
-#pragma unroll
-    for (int x = 0; x < SL; ++x) {
-      const float y = fast_exp2(ml_lds[x].x - M);
-      den = fmaf(y, ml_lds[x].y, den);
-      const f32x4 o = o_lds[x * NQ + c];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) O[i] = fmaf(y, o[i], O[i]);
+        for (int i = 0; i < 4; ++i) O[i] = fmaf(y, o[i], O[i]);
+      }
     }
+    if (!in) continue;
     const int gi = a.by_t(row), t = row - gi * a.T, hq = g * (a.Hq / a.p.H) + gi;
     const bool some = bits_of(den) != 0u;
     f32x4 out;
 #pragma unroll
     for (int i = 0; i < 4; ++i) out[i] = some ? O[i] / den : 0.f;
-    if (4 * c < a.D) {
-      char* to = a.o + ((((int64_t)b * a.T + t) * a.Hq + hq) * a.D + 4 * c) * fmt_size<E>();
-      if constexpr (std::is_same<E, F32Fmt>::value) *(f32x4*)to = out;
-      else *(u32x2*)to = u32x2{E::pack2(out[0], out[1]), E::pack2(out[2], out[3])};
-    }
+    char* to = a.o + ((((int64_t)b * a.T + t) * a.Hq + hq) * a.D + 4 * c) * fmt_size<E>();
+    if constexpr (std::is_same<E, F32Fmt>::value) *(f32x4*)to = out;
+    else *(u32x2*)to = u32x2{E::pack2(out[0], out[1]), E::pack2(out[2], out[3])};
     if (a.lse && c == 0) a.lse[((int64_t)b * a.Hq + hq) * a.T + t] = some ? (M + __log2f(den)) * kLn2 : INFINITY;
   }
 }
@@ -703,10 +705,14 @@ static int run_paged(PagedArgs& a, hipStream_t s, const char* who) {
   else launch_kernel<paged_decode_kernel<C, E, W, 1, ROWS>>(grid, dim3(64 * kPagedWaves), 0, s, a);
   int rc = check_launch(who);
   if (rc) return rc;
-  // Sequences of more than one part, or of none.
-  const dim3 rows((unsigned)a.rows, (unsigned)std::min(a.B * a.p.H, 65535));
-  if (a.items / (a.B * a.p.H) > 8 * 256 / (W / 4)) launch_kernel<paged_join_kernel<E, W, 1024>>(rows, dim3(1024), 0, s, a);
-  else launch_kernel<paged_join_kernel<E, W, 256>>(rows, dim3(256), 0, s, a);
+  // Sequences of more than one part, or of none.  Threads enough that each takes up to 8
+  // parts of an even cut (131072 keys of one sequence, 255 parts: 5.1 us against 9.5 with a
+  // workgroup to a row), and that the rows fill a workgroup.
+  const int64_t quads = (int64_t)a.rows * (W / 4), parts = a.items / ((int64_t)a.B * a.p.H);
+  while (a.slices < 5 && (parts > 8 << a.slices || quads << a.slices < 256)) ++a.slices;
+  const int per = 256 >> a.slices;
+  launch_kernel<paged_join_kernel<E, W>>(dim3((unsigned)((quads + per - 1) / per), (unsigned)std::min(a.B * a.p.H, 65535)),
+                                         dim3(256), 0, s, a);
   return check_launch(who);
 }
 template <typename C, typename E, int W>
