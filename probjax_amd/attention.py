@@ -791,6 +791,7 @@ class PagedCache:
         batch = self.k.shape[0] if self.page_table is None else self.page_table.shape[0]
         for name, value in (("index", index), ("_pages", pages), ("unwritable", unwritable), ("batch", batch),
                             ("code", hip.CACHE_DTYPES[self.k.dtype]), ("page_size", pages.page_size),
+                            ("kv_heads", self.k.shape[2]), ("head_dim", self.k.shape[3]),
                             ("capacity", pages.page_size * pages.table_len)):
             object.__setattr__(self, name, value)
 

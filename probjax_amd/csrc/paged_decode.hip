@@ -3,12 +3,18 @@
 //   o_t = sum_j softmax_j(scale q_t.k_j) v_j,  j < L - (T-1-t),
 // L keys of the sequence, T new tokens (one as a rule).
 //
-// A workgroup takes a part of one sequence's keys for one KV head, with its (Hq/Hkv)*T
-// packed query rows as the columns of the matrix instructions (NRB blocks of 16); its
-// four waves take a quarter of the part each, 32 keys a step, and join at the end.  A
-// second kernel joins the parts.  How long a part is follows from the lengths, which
-// only the device knows: every wave works it out from all of them (plan), so a grid made
-// for the capacity, or captured once, is shared by whatever keys there are.
+// A wave takes a share of the keys of all sequences, laid end to end in steps of 32, for
+// one KV head, with its (Hq/Hkv)*T packed query rows as the columns of the matrix
+// instructions (NRB blocks of 16).  Shares are equal whatever the lengths, and as many as
+// the device holds waves: each compute unit streams the same bytes at the same time (parts
+// of whole sequences left the last units 82 us for a share that the first had in 58).  A
+// share that runs into the next sequence leaves a partial result and goes on; a second
+// kernel joins the parts of a sequence.  What a share is follows from the lengths, which
+// only the device knows: every wave works it out from all of them, so a grid made for the
+// capacity, or captured once, is shared by whatever keys there are.  A workgroup's four
+// waves are neighbouring heads on the same keys, so rows that lie side by side are read
+// side by side (8-bit rows of 64 features, [page, H, D]: 43 us against 58 as workgroups of
+// their own).
 //
 // A wave's K and V rows go from memory to LDS by loads of 16 bytes a lane that no
 // register waits for, whole rows each, one step ahead.  The lanes look up a page each, once per key, and hand the rows'
@@ -23,7 +29,7 @@
 namespace pjx {
 
 constexpr int kPagedWaves = 4;
-constexpr int kMinPart = 64;  // keys of a part at least (but for the last)
+constexpr int kLeastShare = 64;  // keys of a share at least
 
 struct PagedArgs {
   PageArgs p;
@@ -31,14 +37,14 @@ struct PagedArgs {
   char* o;
   float* lse;
   const int32_t* lengths;
-  float* ws_o;   // [items][rows][W] unnormalised outputs of the parts
-  float* ws_ml;  // [items][rows][2] running max (log2 units), sum
+  float* ws_o;   // [shares + B][H][rows][W] unnormalised outputs of the parts
+  float* ws_ml;  // [shares + B][H][rows][2] running max (log2 units), sum
   int B, T, Hq, D, rows;
-  int items;     // most work items (parts of all sequences and KV heads) there may be
-  int cut;       // 0: enough for parts of kMinPart keys whatever the lengths
+  int shares;    // of a KV head, at most
+  int least;     // steps of a share at least
+  int step_log;  // keys of a step, as a power of two
   int slices;    // paged_join_kernel
-  int unit;      // kMinPart, or as many times that as keeps the sum of all lengths in 30 bits
-  FastDiv by_g, by_t;
+  FastDiv by_g, by_t, by_shares;
   float cx;      // sm_scale * log2(e)
 };
 
@@ -47,68 +53,74 @@ __device__ __forceinline__ int paged_len(const PagedArgs& a, int b) {
   return a.lengths ? min(max(a.lengths[b], 0), room) : room;
 }
 
-__device__ __forceinline__ int wave_sum(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
+// The steps of all sequences, end to end, and a share of them.  Lane l knows sequence l's
+// length (0 behind the last) and the steps up to its end.
+__device__ __forceinline__ int steps_of(const PagedArgs& a, int L) { return (L + (1 << a.step_log) - 1) >> a.step_log; }
+struct Lane {
+  int len, upto;
+};
+__device__ __forceinline__ Lane lane_steps(const PagedArgs& a) {
+  const int lane = threadIdx.x & 63, L = lane < a.B ? paged_len(a, lane) : 0;
+  return {L, wave_scan(steps_of(a, L))};
+}
+__device__ __forceinline__ int all_steps(const PagedArgs& a, const Lane& s) {
+  const int lane = threadIdx.x & 63;
+  int all = __builtin_amdgcn_readlane(s.upto, 63), n = 0;
+  if (a.B <= 64) return all;
+  for (int b0 = 64; b0 < a.B; b0 += 64) n += b0 + lane < a.B ? steps_of(a, paged_len(a, b0 + lane)) : 0;
+  return all + __builtin_amdgcn_readlane(wave_scan(n), 63);
+}
+__device__ __forceinline__ int share_of(const PagedArgs& a, int all) { return max(a.by_shares(all + a.shares - 1), a.least); }
 
-// How the sequences are cut: into ceil(L / chunk) parts each, equal but for a rounding to
-// kMinPart, with a chunk for all of them that leaves at most a.items work items.  With u =
-// chunk / a.unit and m_b = ceil(L_b / a.unit), B' sequences of any keys have at most
-//   sum ceil(m_b / u) <= (sum m_b) / u + B'
-// parts, so u = ceil(sum m_b / (parts wanted - B')) will do; chunk = kMinPart where there
-// may be as many items as that makes.
-struct Plan {
-  int chunk;
-  __device__ __forceinline__ int parts(int L) const { return (int)(((uint32_t)L + (uint32_t)chunk - 1u) / (uint32_t)chunk); }
-  __device__ __forceinline__ static int part_keys(int L, int n) { return n > 0 ? ((L - 1) / n + kMinPart) & ~(kMinPart - 1) : 0; }
+// A step of a wave: keys k0 .. of sequence b, which has `len`; `left` steps of the share
+// from this one on.
+struct Cursor {
+  int b, k0, len, left;
 };
-// first: the length of sequence `lane` (0: none).
-__device__ __forceinline__ Plan make_plan(const PagedArgs& a, int first) {
-  if (!a.cut) return {kMinPart};
+// Step `at` of all steps.
+__device__ __forceinline__ Cursor find_step(const PagedArgs& a, const Lane& s, int at) {
   const int lane = threadIdx.x & 63;
-  int all = (first + a.unit - 1) / a.unit, some = first > 0;
-  for (int b0 = 64; b0 < a.B; b0 += 64) {
-    const int L = b0 + lane < a.B ? paged_len(a, b0 + lane) : 0;
-    all += (L + a.unit - 1) / a.unit;
-    some += L > 0;
-  }
-  const int want = a.items / a.p.H - wave_sum(some);
-  return {max((wave_sum(all) + want - 1) / want, 1) * a.unit};
-}
-// Part `item` of all sequences' parts in order: sequence b, its part c of n, the keys L.
-struct Part {
-  int b, c, n, L;
-};
-__device__ __forceinline__ bool find_part(const PagedArgs& a, const Plan& p, int first, int item, Part& w) {
-  const int lane = threadIdx.x & 63;
-  int run = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const int L = b0 == 0 ? first : b0 + lane < a.B ? paged_len(a, b0 + lane) : 0;
-    const int n = p.parts(L), upto = run + wave_scan(n);
-    const uint64_t past = __builtin_amdgcn_ballot_w64(upto > item);
+  int L = s.len, upto = s.upto;
+  for (int b0 = 0;;) {
+    const uint64_t past = __builtin_amdgcn_ballot_w64(upto > at);
     if (past) {
-      const int src = __builtin_ctzll(past);
-      w.b = b0 + src;
-      w.n = __builtin_amdgcn_readlane(n, src);
-      w.L = __builtin_amdgcn_readlane(L, src);
-      w.c = item - (__builtin_amdgcn_readlane(upto, src) - w.n);
-      return true;
+      const int src = __builtin_ctzll(past), len = __builtin_amdgcn_readlane(L, src);
+      const int before = __builtin_amdgcn_readlane(upto, src) - steps_of(a, len);
+      return {b0 + src, (at - before) << a.step_log, len, 0};
     }
-    run = __builtin_amdgcn_readlane(upto, 63);
+    const int run = __builtin_amdgcn_readlane(upto, 63);
+    b0 += 64;
+    if (b0 >= a.B) return {0, 0, 0, 0};
+    L = b0 + lane < a.B ? paged_len(a, b0 + lane) : 0;
+    upto = run + wave_scan(steps_of(a, L));
   }
-  return false;
 }
-// Parts before those of sequence b, and b's.
-__device__ __forceinline__ int parts_before(const PagedArgs& a, const Plan& p, int first, int b, int& n_b) {
-  const int lane = threadIdx.x & 63;
-  int run = 0;
-  for (int b0 = 0;; b0 += 64) {
-    const int n = p.parts(b0 == 0 ? first : b0 + lane < a.B ? paged_len(a, b0 + lane) : 0);
-    const int upto = run + wave_scan(n);
-    if (b < b0 + 64) {
-      n_b = __builtin_amdgcn_readlane(n, b - b0);
-      return __builtin_amdgcn_readlane(upto, b - b0) - n_b;
-    }
-    run = __builtin_amdgcn_readlane(upto, 63);
+// The next step of the share; its last one stays (with left = 0).  lens: lane l's length.
+__device__ __forceinline__ Cursor next_step(const PagedArgs& a, int lens, Cursor c) {
+  if (c.left <= 1) return {c.b, c.k0, c.len, 0};
+  c.left -= 1;
+  c.k0 += 1 << a.step_log;
+  if (c.k0 >= c.len) {
+    c.k0 = 0;
+    do {  // (a step is left, so a sequence follows that has keys)
+      c.b += 1;
+      c.len = c.b < 64 ? __builtin_amdgcn_readlane(lens, c.b) : __builtin_amdgcn_readfirstlane(paged_len(a, c.b));
+    } while (c.len == 0);
   }
+  return c;
+}
+// Steps before those of sequence b, and b's.
+__device__ __forceinline__ int steps_before(const PagedArgs& a, const Lane& s, int b, int& n_b) {
+  const int lane = threadIdx.x & 63;
+  int L = s.len, upto = s.upto, b0 = 0;
+  for (; b >= b0 + 64;) {
+    const int run = __builtin_amdgcn_readlane(upto, 63);
+    b0 += 64;
+    L = b0 + lane < a.B ? paged_len(a, b0 + lane) : 0;
+    upto = run + wave_scan(steps_of(a, L));
+  }
+  n_b = steps_of(a, __builtin_amdgcn_readlane(L, b - b0));
+  return __builtin_amdgcn_readlane(upto, b - b0) - n_b;
 }
 
 // A step's K or V rows in LDS: rows of W elements of C, their 16-byte chunks at chunk ^
@@ -137,12 +149,15 @@ __device__ __forceinline__ uint32_t lds_offset(const void* p) {
   return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p);
 }
 __device__ __forceinline__ void load_lds16(uint64_t from, uint32_t lds) {
+  lds = __builtin_amdgcn_readfirstlane(lds);
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt" ::"v"(from), "s"(lds) : "memory");
 }
 __device__ __forceinline__ void load_lds4(uint64_t from, uint32_t lds) {
+  lds = __builtin_amdgcn_readfirstlane(lds);
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(lds) : "memory");
 }
 __device__ __forceinline__ void load_lds1(uint64_t from, uint32_t lds) {
+  lds = __builtin_amdgcn_readfirstlane(lds);
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_ubyte %0, off" ::"v"(from), "s"(lds) : "memory");
 }
 
@@ -161,6 +176,13 @@ __device__ __forceinline__ void arrived() {
   __builtin_amdgcn_sched_barrier(0);
   wait_vmcnt<N>();
   __builtin_amdgcn_sched_barrier(0);
+}
+
+// x, as the compiler cannot know it: what is made of it is made where it is used, and not
+// kept in registers through a loop that seldom comes there.
+__device__ __forceinline__ int once(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
 }
 
 __device__ __forceinline__ uint32_t bits_of(float x) {
@@ -205,19 +227,37 @@ __device__ __forceinline__ f32x4 codes4(uint32_t w) {
   return f32x4{lo[0], lo[1], hi[0], hi[1]};
 }
 
-// Workgroups of a compute unit, by their LDS.
+// Waves of a compute unit at a time: four, one to a SIMD and with 64 rows each on their
+// way, keep the memory busy from rows of 128 bytes on (32 x 512-8192 keys of 8 heads of 128
+// in 8 bits: 51 us with four, 54 with eight, 57 and more where units hold different numbers
+// of them); eight on shorter ones (64 features in 8 bits: 30 us against 40).
 template <typename C, int W>
+constexpr int paged_waves() {
+  return W * fmt_size<C>() >= 128 ? 4 : 8;
+}
+// Waves of a SIMD that the registers are to leave room for (256 features, and float32 sums
+// of more than 64, need more than half of them).
+template <typename C, typename E, int W>
 constexpr int paged_occupancy() {
-  return W * fmt_size<C>() >= 512 ? 1 : 2;
+  return W == 256 || (std::is_same<E, F32Fmt>::value && W > 64) ? 1 : 2;
+}
+
+// Waves of a workgroup that has a whole sequence (WHOLE): as many as its LDS and registers
+// allow.
+template <typename C, typename E, int W, int NRB>
+constexpr int paged_whole_waves() {
+  return W * fmt_size<C>() > 256 || W == 256 || (W > 64 && (std::is_same<E, F32Fmt>::value || NRB > 1)) ? 4 : 8;
 }
 
 // What the chunks behind a row's end are loaded from.
 __device__ const __attribute__((aligned(16))) uint32_t kZeros[4] = {};
 
 // C: format of the cache, E: of q and o; W: features of a row in LDS (64, 128, 256), ROWS:
-// a row has fewer, and zeros behind them; NRB: blocks of 16 query rows.
-template <typename C, typename E, int W, int NRB, bool ROWS>
-__global__ __launch_bounds__(64 * kPagedWaves, (paged_occupancy<C, W>())) void paged_decode_kernel(PagedArgs a) {
+// a row has fewer, and zeros behind them; NRB: blocks of 16 query rows.  WHOLE: a workgroup
+// takes one sequence's keys for a KV head, an equal number of steps to each of its waves,
+// and joins them itself.
+template <typename C, typename E, int W, int NRB, bool ROWS, bool WHOLE>
+__global__ __launch_bounds__(64 * (WHOLE ? paged_whole_waves<C, E, W, NRB>() : kPagedWaves), (paged_occupancy<C, E, W>())) void paged_decode_kernel(PagedArgs a) {
   using T = PageTile<C, W>;
   constexpr bool F32 = std::is_same<E, F32Fmt>::value, QUANT = std::is_same<C, E4m3Fmt>::value;
   // The weights' product with V: in 16 bits they are rounded to the type, in two parts
@@ -227,21 +267,37 @@ __global__ __launch_bounds__(64 * kPagedWaves, (paged_occupancy<C, W>())) void p
   constexpr bool SPLIT = QUANT && !F32 && std::is_same<E, F16Fmt>::value;
   constexpr int KS = T::KS, KB = KS / 16, NL = T::NL, CS = T::CS, ES = fmt_size<E>();
   constexpr int NDB = W / 16;
-  __shared__ __attribute__((aligned(1024))) unsigned char k_lds[kPagedWaves * T::BYTES];
-  __shared__ __attribute__((aligned(1024))) unsigned char v_lds[kPagedWaves * T::BYTES];
-  __shared__ __attribute__((aligned(16))) uint64_t rows_lds[kPagedWaves * 64];  // addresses of a step's K, V rows
-  __shared__ __attribute__((aligned(16))) uint32_t exp_lds[QUANT ? kPagedWaves * 64 : 4];
-  __shared__ __attribute__((aligned(16))) uint32_t page_lds[kPagedWaves * 64];  // pages of the next step's keys
+  constexpr int NW = WHOLE ? paged_whole_waves<C, E, W, NRB>() : kPagedWaves;
+  __shared__ __attribute__((aligned(1024))) unsigned char k_lds[NW * T::BYTES];
+  __shared__ __attribute__((aligned(1024))) unsigned char v_lds[NW * T::BYTES];
+  __shared__ __attribute__((aligned(16))) uint64_t rows_lds[NW * 64];  // addresses of a step's K, V rows
+  __shared__ __attribute__((aligned(16))) uint32_t exp_lds[QUANT ? NW * 64 : 4];
+  __shared__ __attribute__((aligned(16))) uint32_t page_lds[NW * 64];  // pages of the next step's keys
+  __shared__ float2 ml_lds[WHOLE ? NW * 16 : 1];
   const PageArgs& p = a.p;
   const int lane = threadIdx.x & 63, c16 = lane & 15, q4 = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int item = blockIdx.x * kPagedWaves + w, q = a.by_g(item), g = item - q * p.H;
-  const int first = lane < a.B ? paged_len(a, lane) : 0;
-  const Plan plan = make_plan(a, first);
-  Part part;
-  if (!find_part(a, plan, first, q, part)) return;
-  const int b = part.b, keys = Plan::part_keys(part.L, part.n);
-  const int w0 = part.c * keys, w1 = min(w0 + keys, part.L);
+  int share = 0, g, lens = 0;
+  Cursor cur;
+  if constexpr (WHOLE) {
+    cur.b = a.by_g(blockIdx.x);
+    g = blockIdx.x - cur.b * p.H;
+    cur.len = __builtin_amdgcn_readfirstlane(paged_len(a, cur.b));
+    const int steps = steps_of(a, cur.len), per = (steps + NW - 1) / NW;
+    cur.k0 = (w * per) * KS;
+    cur.left = min(per, steps - w * per);
+  } else {
+    const int item = blockIdx.x * NW + w;
+    share = a.by_g(item);
+    g = item - share * p.H;
+    const Lane steps = lane_steps(a);
+    lens = steps.len;
+    const int all = all_steps(a, steps), size = share_of(a, all);
+    if ((int64_t)share * size >= all) return;
+    cur = find_step(a, steps, share * size);
+    cur.left = min(size, all - share * size);
+  }
+  Cursor nxt = next_step(a, lens, cur), then = next_step(a, lens, nxt);
   const int row0 = blockIdx.y * 16 * NRB;
 
   unsigned char *kl = k_lds + w * T::BYTES, *vl = v_lds + w * T::BYTES;
@@ -254,20 +310,20 @@ __global__ __launch_bounds__(64 * kPagedWaves, (paged_occupancy<C, W>())) void p
   const uint64_t pool = (uint64_t)(half ? p.v : p.k) + (uint64_t)g * (uint64_t)(half ? p.vh : p.kh);
   const int64_t page_step = half ? p.vp : p.kp, token_step = half ? p.vt : p.kt;
   const uint64_t exps = (uint64_t)(half ? p.ve : p.ke);
-  const uint64_t entries = p.table ? (uint64_t)(p.table + b * p.table_step) : (uint64_t)a.q;  // (read in any case)
-  auto look_up = [&](int k0) {  // the pages of a step's keys
-    load_lds4(entries + 4ull * (uint32_t)(p.table ? p.by_page(min(k0 + (lk & (KS - 1)), w1 - 1)) : 0), pl_at);
+  auto look_up = [&](const Cursor& c) {  // the pages of a step's keys (without a table something else, unused)
+    const uint64_t entry = p.table ? (uint64_t)(p.table + c.b * p.table_step) : (uint64_t)a.q;
+    load_lds4(entry + 4ull * (uint32_t)(p.table ? p.by_page(min(c.k0 + (lk & (KS - 1)), c.len - 1)) : 0), pl_at);
   };
   uint64_t exp_at = 0;
-  auto place = [&](int k0) -> uint32_t {  // their rows' addresses to LDS; which keys are there
-    const uint32_t page = p.table ? pl[lane] : (uint32_t)b;
-    const int key = k0 + (lk & (KS - 1)), kc = min(key, w1 - 1);
+  auto place = [&](const Cursor& c) -> uint32_t {  // their rows' addresses to LDS; which keys are there
+    const uint32_t page = p.table ? pl[lane] : (uint32_t)c.b;
+    const int key = c.k0 + (lk & (KS - 1)), kc = min(key, c.len - 1);
     const bool some = page < p.pages;
     const uint32_t pg = some ? page : 0u;
     const int slot = kc - p.by_page(kc) * p.page;
     rl[lane] = pool + (uint64_t)(pg * page_step + slot * token_step);
     if constexpr (QUANT) exp_at = exps + (uint64_t)((int64_t)(pg * (uint64_t)p.H + g) * p.page + slot);
-    return (uint32_t)__builtin_amdgcn_ballot_w64(some && key < w1) & (uint32_t)((1ull << KS) - 1);
+    return (uint32_t)__builtin_amdgcn_ballot_w64(some && key < c.len) & (uint32_t)((1ull << KS) - 1);
   };
   const int row_chunks = a.D * CS / 16;
   auto fetch = [&](uint32_t to, int first) {
@@ -284,50 +340,69 @@ __global__ __launch_bounds__(64 * kPagedWaves, (paged_occupancy<C, W>())) void p
     if constexpr (QUANT) load_lds1(exp_at, el_at);
   };
 
-  // ---- q as the B operand, features in the order the cache's rows are read in ----
+  // ---- a sequence: q as the B operand, features in the order the cache's rows are read in ----
   int lim[NRB];  // keys that the lane's row sees
   typename std::conditional<F32, f32x4, u32x4>::type qf[NRB][F32 ? W / 16 : W / 32];
-#pragma unroll
-  for (int rb = 0; rb < NRB; ++rb) {
-    const int row = row0 + 16 * rb + c16;
-    const bool in = row < a.rows;
-    const int gi = a.by_t(in ? row : 0), t = (in ? row : 0) - gi * a.T;
-    lim[rb] = part.L - (a.T - 1 - t);
-    const char* x = a.q + (((int64_t)b * a.T + t) * a.Hq + g * (a.Hq / p.H) + gi) * a.D * ES;
-    if constexpr (F32) {
-#pragma unroll
-      for (int j = 0; j < W / 16; ++j) {
-        const int d = QUANT ? 64 * (j / 4) + 16 * q4 + 4 * (j % 4) : 16 * j + 4 * q4;
-        qf[rb][j] = in && (!ROWS || d < a.D) ? *(const f32x4*)(x + 4 * d) : f32x4{};
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < W / 32; ++j) {
-        const int d = QUANT ? 64 * (j / 2) + 16 * q4 + 8 * (j % 2) : 32 * j + 8 * q4;
-        qf[rb][j] = in && (!ROWS || d < a.D) ? *(const u32x4*)(x + 2 * d) : u32x4{0u, 0u, 0u, 0u};
-      }
-    }
-  }
-
   f32x4 acc[NRB][NDB];
   float m_run[NRB], l_run[NRB];
+  bool from_start = false;
+  auto begin = [&](const Cursor& c) {
+    from_start = c.k0 == 0;
+    const int r16 = once(c16), d4 = once(q4);
 #pragma unroll
-  for (int rb = 0; rb < NRB; ++rb) {
-    m_run[rb] = kMaxInit;
-    l_run[rb] = 0.f;
+    for (int rb = 0; rb < NRB; ++rb) {
+      const int row = row0 + 16 * rb + r16;
+      const bool in = row < a.rows;
+      const int gi = a.by_t(in ? row : 0), t = (in ? row : 0) - gi * a.T;
+      lim[rb] = c.len - (a.T - 1 - t);
+      const char* x = a.q + (((int64_t)c.b * a.T + t) * a.Hq + g * (a.Hq / p.H) + gi) * a.D * ES;
+      if constexpr (F32) {
 #pragma unroll
-    for (int i = 0; i < NDB; ++i) acc[rb][i] = f32x4{};
-  }
+        for (int j = 0; j < W / 16; ++j) {
+          const int d = QUANT ? 64 * (j / 4) + 16 * d4 + 4 * (j % 4) : 16 * j + 4 * d4;
+          qf[rb][j] = in && (!ROWS || d < a.D) ? *(const f32x4*)(x + 4 * d) : f32x4{};
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < W / 32; ++j) {
+          const int d = QUANT ? 64 * (j / 2) + 16 * d4 + 8 * (j % 2) : 32 * j + 8 * d4;
+          qf[rb][j] = in && (!ROWS || d < a.D) ? *(const u32x4*)(x + 2 * d) : u32x4{0u, 0u, 0u, 0u};
+        }
+      }
+      m_run[rb] = kMaxInit;
+      l_run[rb] = 0.f;
+#pragma unroll
+      for (int i = 0; i < NDB; ++i) acc[rb][i] = f32x4{};
+    }
+    arrived<0>();  // (here, or the compiler waits for all loads at q's first use in every step)
+  };
 
-  look_up(w0);
-  arrived<0>();
-  uint32_t there = place(w0);
-  lds_done();
-  look_up(w0 + KS);
-  fetch_exps();
-  fetch(kl_at, 0);
-  fetch(vl_at, 32);
-  for (int k0 = w0; k0 < w1; k0 += KS) {
+  auto begin_empty = [&]() {
+#pragma unroll
+    for (int rb = 0; rb < NRB; ++rb) {
+      m_run[rb] = kMaxInit;
+      l_run[rb] = 0.f;
+#pragma unroll
+      for (int i = 0; i < NDB; ++i) acc[rb][i] = f32x4{};
+    }
+  };
+
+  uint32_t there = 0;
+  const bool any = !WHOLE || cur.left > 0;
+  if (any) {
+    look_up(cur);
+    begin(cur);
+    there = place(cur);
+    lds_done();
+    look_up(nxt);
+    fetch_exps();
+    fetch(kl_at, 0);
+    fetch(vl_at, 32);
+  } else {
+    begin_empty();
+  }
+  while (any) {
+    const int k0 = cur.k0;
     arrived<NL>();  // K's rows and the next step's pages; behind them V's rows
     u32x4 kf[KB][T::NC / 4];  // chunk 4j + q4 of key 16kb + c16
     f32x4 ks[KB], vs[KB];
@@ -344,12 +419,12 @@ __global__ __launch_bounds__(64 * kPagedWaves, (paged_occupancy<C, W>())) void p
         }
       }
     }
-    // The next step's rows: as soon as this one's are in registers.  (The last step's next
-    // one is its last key again, which no one reads.)
+    // The next step's rows: as soon as this one's are in registers.  (The share's last step
+    // is fetched once more, for no one.)
     const uint32_t here = there;
-    there = place(k0 + KS);
+    there = place(nxt);
     lds_done();
-    look_up(k0 + 2 * KS);
+    look_up(then);
     fetch_exps();
     fetch(kl_at, 0);
 
@@ -387,7 +462,7 @@ __global__ __launch_bounds__(64 * kPagedWaves, (paged_occupancy<C, W>())) void p
         for (int r = 0; r < 4; ++r) s[rb][kb][r] *= QUANT ? ks[kb][r] : a.cx;
     }
     // Keys that some row does not see: past its own, past the wave's, of missing pages.
-    const bool whole = here == (uint32_t)((1ull << KS) - 1) && k0 + KS <= part.L - (a.T - 1);
+    const bool whole = here == (uint32_t)((1ull << KS) - 1) && k0 + KS <= cur.len - (a.T - 1);
     auto sees = [&](int rb, int j) { return (here >> j & 1u) != 0u && k0 + j < lim[rb]; };
     if (!whole) {
 #pragma unroll
@@ -561,40 +636,107 @@ __global__ __launch_bounds__(64 * kPagedWaves, (paged_occupancy<C, W>())) void p
         }
       }
     }
+
+    if constexpr (WHOLE) {
+      if (cur.left <= 1) break;
+    }
+    // ---- the end of a sequence, or of the share ----
+    if (!WHOLE && (cur.left <= 1 || nxt.b != cur.b)) {
+      const bool alone = from_start && k0 + KS >= cur.len;  // the whole sequence
+      const int r16 = once(c16), d4 = once(q4);
+#pragma unroll
+      for (int rb = 0; rb < NRB; ++rb) {
+        const int row = row0 + 16 * rb + r16;
+        const float den = xor32_sum(xor16_sum(l_run[rb]));
+        if (row >= a.rows) continue;
+        const bool some = bits_of(den) != 0u;
+        const float inv = some ? 1.f / den : 0.f;
+        const int gi = a.by_t(row), t = row - gi * a.T, hq = g * (a.Hq / p.H) + gi;
+        const int64_t at = alone ? ((int64_t)cur.b * a.T + t) * a.Hq + hq : ((int64_t)(share + cur.b) * p.H + g) * a.rows + row;
+#pragma unroll
+        for (int i = 0; i < NDB; ++i) {
+          f32x4 x = acc[rb][i];
+          int d = 16 * i + 4 * d4;
+          if constexpr (F32) {  // dims 64j + 16q4 + 4r ..: element r of the four blocks 4j ..
+#pragma unroll
+            for (int u = 0; u < 4; ++u) x[u] = acc[rb][i / 4 * 4 + u][i % 4];
+            d = 64 * (i / 4) + 16 * d4 + 4 * (i % 4);
+          }
+          if (ROWS && d >= a.D) continue;
+          if (alone) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) x[u] *= inv;
+            char* to = a.o + (at * a.D + d) * ES;
+            if constexpr (F32) *(f32x4*)to = x;
+            else *(u32x2*)to = u32x2{E::pack2(x[0], x[1]), E::pack2(x[2], x[3])};
+          } else {
+            *(f32x4*)(a.ws_o + at * W + d) = x;
+          }
+        }
+        if (d4 == 0) {
+          if (!alone) *(float2*)(a.ws_ml + 2 * at) = make_float2(m_run[rb], den);
+          else if (a.lse) a.lse[((int64_t)cur.b * a.Hq + hq) * a.T + t] = some ? (m_run[rb] + __log2f(den)) * kLn2 : INFINITY;
+        }
+      }
+      if (cur.left <= 1) break;
+      begin(nxt);
+    }
+    cur = nxt;
+    nxt = then;
+    then = next_step(a, lens, then);
   }
   arrived<0>();  // (nothing may come to LDS that is another's by then)
 
+  if constexpr (WHOLE) {
+    // ---- the waves' (max, sum, O), one block of rows at a time; the first half of the dims
+    // through K's memory, the second through V's: quad c of row r at c ^ r ----
+    constexpr int NQ = W / 4, HQ = NQ / 2;  // quads of dims of a row, and of a half
 #pragma unroll
-  for (int rb = 0; rb < NRB; ++rb) {
-    const int row = row0 + 16 * rb + c16;
-    const float den = xor32_sum(xor16_sum(l_run[rb]));
-    if (row >= a.rows) continue;
-    const bool some = bits_of(den) != 0u;
-    const int gi = a.by_t(row), t = row - gi * a.T, hq = g * (a.Hq / p.H) + gi;
-    const int64_t at = part.n == 1 ? ((int64_t)b * a.T + t) * a.Hq + hq : (int64_t)item * a.rows + row;
+    for (int rb = 0; rb < NRB; ++rb) {
+      const float l = xor32_sum(xor16_sum(l_run[rb]));
+      __syncthreads();
 #pragma unroll
-    for (int i = 0; i < NDB; ++i) {
-      f32x4 x = acc[rb][i];
-      int d = 16 * i + 4 * q4;
-      if constexpr (F32) {  // dims 64j + 16q4 + 4r ..: element r of the four blocks 4j ..
+      for (int i = 0; i < NDB; ++i) {
+        f32x4 x = acc[rb][i];
+        int quad = 4 * i + q4;
+        if constexpr (F32) {  // quad 16j + 4q4 + r: element r of the four blocks 4j ..
 #pragma unroll
-        for (int u = 0; u < 4; ++u) x[u] = acc[rb][i / 4 * 4 + u][i % 4];
-        d = 64 * (i / 4) + 16 * q4 + 4 * (i % 4);
+          for (int u = 0; u < 4; ++u) x[u] = acc[rb][i / 4 * 4 + u][i % 4];
+          quad = i / 4 * 16 + 4 * q4 + i % 4;
+        }
+        unsigned char* to = quad < HQ ? k_lds : v_lds;
+        *(f32x4*)(to + ((w * 16 + c16) * HQ + ((quad % HQ) ^ (c16 & (HQ - 1)))) * 16) = x;
       }
-      if (ROWS && d >= a.D) continue;
-      if (part.n == 1) {
+      if (q4 == 0) ml_lds[w * 16 + c16] = make_float2(m_run[rb], l);
+      __syncthreads();
+      const int nr = min(16, a.rows - row0 - 16 * rb);
+      for (int e = threadIdx.x; e < nr * NQ; e += 64 * NW) {
+        const int r = e / NQ, c = e % NQ;
+        if (ROWS && 4 * c >= a.D) continue;
+        float M = kMaxInit, den = 0.f;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) x[u] = some ? x[u] / den : 0.f;
-        char* to = a.o + (at * a.D + d) * ES;
-        if constexpr (F32) *(f32x4*)to = x;
-        else *(u32x2*)to = u32x2{E::pack2(x[0], x[1]), E::pack2(x[2], x[3])};
-      } else {
-        *(f32x4*)(a.ws_o + at * W + d) = x;
+        for (int x = 0; x < NW; ++x) M = fmaxf(M, ml_lds[x * 16 + r].x);
+        f32x4 O = {};
+        const unsigned char* from = c < HQ ? k_lds : v_lds;
+#pragma unroll
+        for (int x = 0; x < NW; ++x) {
+          const float2 ml = ml_lds[x * 16 + r];
+          const float f = fast_exp2(ml.x - M);
+          den = fmaf(f, ml.y, den);
+          const f32x4 o = *(const f32x4*)(from + ((x * 16 + r) * HQ + ((c % HQ) ^ (r & (HQ - 1)))) * 16);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) O[i] = fmaf(f, o[i], O[i]);
+        }
+        const int row = row0 + 16 * rb + r, gi = a.by_t(row), t = row - gi * a.T, hq = g * (a.Hq / p.H) + gi;
+        const bool some = bits_of(den) != 0u;
+        const float inv = some ? 1.f / den : 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) O[i] *= inv;
+        char* to = a.o + ((((int64_t)cur.b * a.T + t) * a.Hq + hq) * a.D + 4 * c) * ES;
+        if constexpr (F32) *(f32x4*)to = O;
+        else *(u32x2*)to = u32x2{E::pack2(O[0], O[1]), E::pack2(O[2], O[3])};
+        if (a.lse && c == 0) a.lse[((int64_t)cur.b * a.Hq + hq) * a.T + t] = some ? (M + __log2f(den)) * kLn2 : INFINITY;
       }
-    }
-    if (q4 == 0) {
-      if (part.n > 1) *(float2*)(a.ws_ml + 2 * at) = make_float2(m_run[rb], den);
-      else if (a.lse) a.lse[((int64_t)b * a.Hq + hq) * a.T + t] = some ? (m_run[rb] + __log2f(den)) * kLn2 : INFINITY;
     }
   }
 }
@@ -611,16 +753,17 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
   const int tid = threadIdx.x, per = 256 >> a.slices, sl = tid >> (8 - a.slices), step = 1 << a.slices;
   const int quad = blockIdx.x * per + (tid & (per - 1)), row = quad / NQ, c = quad % NQ;
   const bool in = row < a.rows && 4 * c < a.D;
-  const int len = (tid & 63) < a.B ? paged_len(a, tid & 63) : 0;
-  const Plan plan = make_plan(a, len);
+  const Lane all = lane_steps(a);
+  const int size = share_of(a, all_steps(a, all));
   for (int pair = blockIdx.y; pair < a.B * a.p.H; pair += gridDim.y) {
     const int b = a.by_g(pair), g = pair - b * a.p.H;
-    int n;
-    const int before = parts_before(a, plan, len, b, n);
+    int steps;
+    const int from = steps_before(a, all, b, steps), share = from / size;
+    const int n = steps ? (from + steps - 1) / size - share + 1 : 0;
     if (n == 1) continue;
     float M = kMaxInit, den = 0.f;
     f32x4 O = {};
-    const int64_t first = ((int64_t)before * a.p.H + g) * a.rows + (in ? row : 0), apart = (int64_t)a.p.H * a.rows;
+    const int64_t first = ((int64_t)(share + b) * a.p.H + g) * a.rows + (in ? row : 0), apart = (int64_t)a.p.H * a.rows;
     for (int x0 = sl; x0 < n; x0 += U * step) {
       float2 ml[U];
       f32x4 o[U];
@@ -680,35 +823,53 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
 // ---------------------------------------------------------------------------
 // Host
 // ---------------------------------------------------------------------------
-// Most work items, with `waves` of them to a compute unit at a time: as many as fill the
-// device once, or two parts per sequence and head where those are more; no more than parts
-// of kMinPart keys come to.
-static int64_t paged_items(int64_t batch, int64_t kv_heads, int64_t capacity, int waves) {
-  const int64_t pairs = batch * kv_heads, most = std::max<int64_t>((capacity + kMinPart - 1) / kMinPart, 1);
-  const int64_t want = std::max((int64_t)256 * waves / kv_heads * kv_heads, 2 * pairs);
-  return most <= want / std::max<int64_t>(pairs, 1) ? pairs * most : want;
-}
+// Shares of a KV head, with `waves` waves to a compute unit at a time: as many as fill the
+// device once.
+static int64_t paged_shares(int64_t kv_heads, int waves) { return std::max<int64_t>((int64_t)256 * waves / kv_heads, 1); }
 static int paged_width(int64_t head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
-static size_t paged_ws(int64_t batch, int64_t kv_heads, int64_t rows, int64_t capacity, int64_t head_dim) {
-  return (size_t)(paged_items(batch, kv_heads, capacity, 2 * kPagedWaves) * rows * (paged_width(head_dim) + 2)) * sizeof(float) + 16;
+// Parts of a KV head at most: one of every share, and one more where a sequence begins.
+static int64_t paged_parts(int64_t batch, int64_t kv_heads) { return paged_shares(kv_heads, 2 * kPagedWaves) + batch; }
+static size_t paged_ws(int64_t batch, int64_t kv_heads, int64_t rows, int64_t head_dim) {
+  return (size_t)(paged_parts(batch, kv_heads) * kv_heads * rows * (paged_width(head_dim) + 2)) * sizeof(float) + 16;
 }
+
+// Whether a workgroup takes a sequence whole, and nothing is joined after it: where one
+// compute unit has little enough to read (by itself it reads some 40 GB/s).  us, shares and
+// join / whole: 256 bf16 keys of 8 heads of 128, one sequence 9.1 / 6.6, 32 of them 12.4 /
+// 11.0; 512 keys 9.5 / 8.3 and 14.7 / 15.1; 512 keys in 8 bits 9.4 / 7.4 and 12.7 / 10.6;
+// 1024 float32 keys of 4 heads of 64 10.9 / 18.2.
+constexpr int64_t kWholeBytes = 128 << 10;
+static bool paged_whole(int64_t capacity, int64_t row_bytes) { return capacity * 2 * row_bytes <= kWholeBytes; }
 
 template <typename C, typename E, int W, bool ROWS>
 static int run_paged(PagedArgs& a, hipStream_t s, const char* who) {
   constexpr bool WIDE = W == 256;  // (32 rows of 256 features spill registers)
   const bool two = !WIDE && a.rows > 16;
-  a.items = (int)paged_items(a.B, a.p.H, (int64_t)a.p.most * a.p.page, paged_occupancy<C, W>() * kPagedWaves);
-  a.cut = a.items < (int64_t)a.B * a.p.H * (((int64_t)a.p.most * a.p.page + kMinPart - 1) / kMinPart);
-  const int gx = (a.items + kPagedWaves - 1) / kPagedWaves;
-  const dim3 grid((unsigned)gx, (unsigned)((a.rows + (two ? 31 : 15)) / (two ? 32 : 16)));
-  if (two) launch_kernel<paged_decode_kernel<C, E, W, WIDE ? 1 : 2, ROWS>>(grid, dim3(64 * kPagedWaves), 0, s, a);
-  else launch_kernel<paged_decode_kernel<C, E, W, 1, ROWS>>(grid, dim3(64 * kPagedWaves), 0, s, a);
+  a.step_log = PageTile<C, W>::KS == 16 ? 4 : 5;
+  const int64_t capacity = (int64_t)a.p.most * a.p.page;
+  const unsigned groups = (unsigned)((a.rows + (two ? 31 : 15)) / (two ? 32 : 16));
+  if (paged_whole(capacity, PageTile<C, W>::ROWB)) {
+    constexpr int NRB = WIDE ? 1 : 2;
+    const dim3 grid((unsigned)(a.B * a.p.H), groups);
+    if (two) launch_kernel<paged_decode_kernel<C, E, W, NRB, ROWS, true>>(grid, dim3(64 * paged_whole_waves<C, E, W, NRB>()), 0, s, a);
+    else launch_kernel<paged_decode_kernel<C, E, W, 1, ROWS, true>>(grid, dim3(64 * paged_whole_waves<C, E, W, 1>()), 0, s, a);
+    return check_launch(who);
+  }
+  a.shares = (int)paged_shares(a.p.H, paged_waves<C, W>());
+  a.by_shares = fast_div(a.shares);
+  a.least = kLeastShare >> a.step_log;
+  const int64_t steps = a.B * ((capacity + PageTile<C, W>::KS - 1) >> a.step_log);
+  if (a.shares > (steps + a.least - 1) / a.least) a.shares = (int)((steps + a.least - 1) / a.least), a.by_shares = fast_div(a.shares);
+  const int gx = (a.shares * a.p.H + kPagedWaves - 1) / kPagedWaves;
+  const dim3 grid((unsigned)gx, groups);
+  if (two) launch_kernel<paged_decode_kernel<C, E, W, WIDE ? 1 : 2, ROWS, false>>(grid, dim3(64 * kPagedWaves), 0, s, a);
+  else launch_kernel<paged_decode_kernel<C, E, W, 1, ROWS, false>>(grid, dim3(64 * kPagedWaves), 0, s, a);
   int rc = check_launch(who);
   if (rc) return rc;
   // Sequences of more than one part, or of none.  Threads enough that each takes up to 8
   // parts of an even cut (131072 keys of one sequence, 255 parts: 5.1 us against 9.5 with a
   // workgroup to a row), and that the rows fill a workgroup.
-  const int64_t quads = (int64_t)a.rows * (W / 4), parts = a.items / ((int64_t)a.B * a.p.H);
+  const int64_t quads = (int64_t)a.rows * (W / 4), parts = a.shares / a.B + 1;
   while (a.slices < 5 && (parts > 8 << a.slices || quads << a.slices < 256)) ++a.slices;
   const int per = 256 >> a.slices;
   launch_kernel<paged_join_kernel<E, W>>(dim3((unsigned)((quads + per - 1) / per), (unsigned)std::min(a.B * a.p.H, 65535)),
@@ -732,7 +893,7 @@ using namespace pjx;
 extern "C" size_t pjx_paged_decode_workspace_size(int64_t batch, int64_t kv_heads, int64_t rows, int64_t capacity,
                                                   int64_t head_dim) {
   if (batch < 0 || kv_heads <= 0 || rows < 0 || capacity < 0) return 16;
-  return paged_ws(batch, kv_heads, rows, capacity, head_dim);
+  return paged_ws(batch, kv_heads, rows, head_dim);
 }
 
 extern "C" int pjx_paged_decode(int dtype, int cache_dtype, const void* q, const pjx_pages* cache,
@@ -753,6 +914,8 @@ extern "C" int pjx_paged_decode(int dtype, int cache_dtype, const void* q, const
   if (q_len > (1 << 20) || q_heads > (1 << 20) || rows > (1 << 19) || batch * kv_heads > (1 << 22) ||
       batch * kv_heads * rows > (1 << 30))
     return fail(PJX_ERR_INVALID, "pjx_paged_decode: sizes out of range");
+  if (batch * ((capacity + 15) / 16) > (1 << 30))
+    return fail(PJX_ERR_INVALID, "pjx_paged_decode: the sequences have room for more than 2^34 keys");
   if (!(sm_scale > 0.f)) return fail(PJX_ERR_INVALID, "pjx_paged_decode: sm_scale must be > 0");
   if (batch == 0) return PJX_OK;
   if (!q || !o) return fail(PJX_ERR_INVALID, "pjx_paged_decode: null pointer");
@@ -761,19 +924,16 @@ extern "C" int pjx_paged_decode(int dtype, int cache_dtype, const void* q, const
   if (capacity == 0 || cache->pages == 0)
     return write_keyless(o, lse, (size_t)(batch * q_len * q_heads * head_dim), f32, (size_t)(batch * q_heads * q_len), s,
                          who);
-  if (!workspace || workspace_bytes < paged_ws(batch, kv_heads, rows, capacity, head_dim))
+  if (!workspace || workspace_bytes < paged_ws(batch, kv_heads, rows, head_dim))
     return fail(PJX_ERR_WORKSPACE, "pjx_paged_decode: workspace missing or too small");
   if ((uintptr_t)workspace % 16) return fail(PJX_ERR_INVALID, "pjx_paged_decode: the workspace must start on 16 bytes");
   a.q = (const char*)q; a.o = (char*)o; a.lse = lse; a.lengths = kv_lengths;
   a.B = (int)batch; a.T = (int)q_len; a.Hq = (int)q_heads; a.D = (int)head_dim; a.rows = (int)rows;
-  int64_t unit = kMinPart;
-  while (batch * ((capacity + unit - 1) / unit) > (1 << 30)) unit *= 2;
-  a.unit = (int)unit;
   a.by_g = fast_div(kv_heads);
   a.by_t = fast_div(q_len);
   a.cx = sm_scale * kLog2e;
   a.ws_o = (float*)workspace;
-  a.ws_ml = a.ws_o + paged_items(batch, kv_heads, capacity, 2 * kPagedWaves) * rows * paged_width(head_dim);
+  a.ws_ml = a.ws_o + paged_parts(batch, kv_heads) * kv_heads * rows * paged_width(head_dim);
   if (f32) return quant ? run_paged<E4m3Fmt, F32Fmt>(a, s, who) : run_paged<F32Fmt, F32Fmt>(a, s, who);
   if (dtype == PJX_DTYPE_BF16) return quant ? run_paged<E4m3Fmt, Bf16Fmt>(a, s, who) : run_paged<Bf16Fmt, Bf16Fmt>(a, s, who);
   return quant ? run_paged<E4m3Fmt, F16Fmt>(a, s, who) : run_paged<F16Fmt, F16Fmt>(a, s, who);

@@ -1083,10 +1083,10 @@ def _unwritable(ts):
             if s <= end:
                 return "its pools are expanded, or their rows overlap each other"
             end += (n - 1) * s
-    for i, a in enumerate(ts):
-        for b in ts[i + 1:]:
-            (x, x_end), (y, y_end) = _reach(a), _reach(b)
-            if x < y_end and y < x_end and _share_bytes(a, b):
+    reach = [_reach(t) for t in ts]
+    for i, (x, x_end) in enumerate(reach):
+        for j, (y, y_end) in enumerate(reach[:i]):
+            if x < y_end and y < x_end and _share_bytes(ts[i], ts[j]):
                 return "its tensors share memory"
     return None
 
@@ -1099,15 +1099,17 @@ def set_pages(pages, k, v, page_table, k_exponents, v_exponents):
     return pages
 
 
-def _rows_of_chunks(x):
-    """``x [B, T, H, D]``, copied unless its rows can be read 16 bytes at a time."""
-    n = 16 // x.element_size()
-    if x.is_contiguous() and x.data_ptr() % 16 == 0:
-        return x
-    if (x.stride(3) == 1 or x.shape[3] == 1) and x.data_ptr() % 16 == 0 and all(
-            x.shape[i] == 1 or x.stride(i) % n == 0 for i in range(3)):
-        return x
-    return _aligned(x.contiguous())
+def _new_rows(k, v):
+    """``(k, v, strides)`` of new keys and values ``[B, T, H, D]``, copied unless their
+    rows can be read 16 bytes at a time."""
+    if k.is_contiguous() and v.is_contiguous():
+        return (k, v, None) if (k.data_ptr() | v.data_ptr()) % 16 == 0 else (_aligned(k), _aligned(v), None)
+    n = 16 // k.element_size()
+    given = k.stride(), v.stride()
+    if not any(s % n for strides in given for s in strides[:3]) and given[0][3] == given[1][3] == 1 \
+            and (k.data_ptr() | v.data_ptr()) % 16 == 0:
+        return k, v, native.CacheStrides(*given[0][:3], *given[1][:3])
+    return _aligned(k.contiguous()), _aligned(v.contiguous()), None
 
 
 def write_pages(cache, k, v, *, kv_lengths=None, new_lengths=None):
@@ -1117,23 +1119,23 @@ def write_pages(cache, k, v, *, kv_lengths=None, new_lengths=None):
         raise ValueError(f"k and v must be [B, T, Hkv, D] of one shape and dtype, got {tuple(k.shape)} {k.dtype} and "
                          f"{tuple(v.shape)} {v.dtype}")
     B, T, H, D = k.shape
-    _, _, Hc, Dc = cache.k.shape
-    if B != cache.batch or H != Hc or D != Dc:
-        raise ValueError(f"k {tuple(k.shape)} does not fit a cache of {cache.batch} sequences, {Hc} heads of {Dc}")
+    if B != cache.batch or H != cache.kv_heads or D != cache.head_dim:
+        raise ValueError(f"k {tuple(k.shape)} does not fit a cache of {cache.batch} sequences, {cache.kv_heads} heads of "
+                         f"{cache.head_dim}")
     if cache.unwritable is not None:
         raise ValueError(f"cannot write to this cache: {cache.unwritable}")
     code = _dtype_code(k)
-    if cache.code != native.PJX_DTYPE_E4M3 and code != cache.code:
+    if code != cache.code and cache.code != native.PJX_DTYPE_E4M3:
         raise ValueError(f"a cache of {cache.k.dtype} takes keys and values of that dtype, got {k.dtype}")
     if (forward_ad._current_level >= 0 or k.requires_grad or v.requires_grad) and _tracked(k, v):
         raise ValueError("writing to a cache has no gradient: call it under torch.no_grad() or on detached tensors")
     index = _gpu(k, v, cache.k)
-    k, v = _rows_of_chunks(k), _rows_of_chunks(v)
+    k, v, strides = _new_rows(k, v)
     L, new = _key_lengths(kv_lengths, k, B), _key_lengths(new_lengths, k, B, "new_lengths")
-    lengths = torch.empty((B,), dtype=torch.int32, device=k.device)
+    lengths = torch.empty((B,), dtype=torch.int32, device=k.device) if L is None else torch.empty_like(L)
     _call(
         index, native.load().pjx_write_pages, code, cache.code, k.data_ptr(), v.data_ptr(), cache.pages(), _ptr(L),
-        _ptr(new), lengths.data_ptr(), B, T, H, D, _pair_strides(k, v),
+        _ptr(new), lengths.data_ptr(), B, T, H, D, strides,
     )
     return lengths
 
@@ -1150,15 +1152,15 @@ def read_pages(cache, *, kv_lengths=None, length: int | None = None, dtype=None)
     length = cache.capacity if length is None else int(length)
     if not 0 <= length <= 1 << 30:
         raise ValueError(f"length must be 0 to 2^30, got {length}")
-    B = cache.batch
-    _, _, H, D = k.shape
+    B, H, D = cache.batch, cache.kv_heads, cache.head_dim
     L = _key_lengths(kv_lengths, k, B)
-    out = k.new_empty((B, length, H, D), dtype=dtype), k.new_empty((B, length, H, D), dtype=dtype)
+    k_out = k.new_empty((B, length, H, D), dtype=dtype)
+    v_out = torch.empty_like(k_out)
     _call(
         cache.index, native.load().pjx_read_pages, _DTYPES[dtype], cache.code, cache.pages(), _ptr(L),
-        out[0].data_ptr(), out[1].data_ptr(), B, length, H, D,
+        k_out.data_ptr(), v_out.data_ptr(), B, length, H, D,
     )
-    return out
+    return k_out, v_out
 
 
 def paged_decode(q, cache, *, sm_scale: float, kv_lengths=None, return_lse: bool = False, workspace=None):
@@ -1167,24 +1169,25 @@ def paged_decode(q, cache, *, sm_scale: float, kv_lengths=None, return_lse: bool
     if q.ndim != 4:
         raise ValueError(f"paged attention: q must be [B, T, Hq, D], got {tuple(q.shape)}")
     B, T, Hq, D = q.shape
-    _, _, H, Dc = cache.k.shape
-    if B != cache.batch or D != Dc or Hq < 1 or Hq % H or T < 1:
+    H = cache.kv_heads
+    if B != cache.batch or D != cache.head_dim or Hq < 1 or Hq % H or T < 1:
         raise ValueError(f"paged attention: q {tuple(q.shape)} does not fit a cache of {cache.batch} sequences, {H} "
-                         f"heads of {Dc}")
+                         f"heads of {cache.head_dim}")
     code = _dtype_code(q)
-    if cache.code != native.PJX_DTYPE_E4M3 and code != cache.code:
+    if code != cache.code and cache.code != native.PJX_DTYPE_E4M3:
         raise ValueError(f"paged attention over a cache of {cache.k.dtype} takes q of that dtype, got {q.dtype}")
     if (forward_ad._current_level >= 0 or q.requires_grad) and _tracked(q):
         raise ValueError("paged attention has no gradient: call it under torch.no_grad() or on detached tensors")
     index = _gpu(q, cache.k)
     q = _aligned(q.contiguous())
     L = _key_lengths(kv_lengths, q, B)
+    lib = native.load()
     nbytes = _workspace_size("pjx_paged_decode_workspace_size", B, H, (Hq // H) * T, cache.capacity, D)
     ws = _scratch(nbytes, q, workspace)
     o = torch.empty_like(q)
     lse = torch.empty((B, Hq, T), dtype=torch.float32, device=q.device) if return_lse else None
     _call(
-        index, native.load().pjx_paged_decode, code, cache.code, q.data_ptr(), cache.pages(), _ptr(L), o.data_ptr(),
+        index, lib.pjx_paged_decode, code, cache.code, q.data_ptr(), cache.pages(), _ptr(L), o.data_ptr(),
         _ptr(lse), ws.data_ptr(), nbytes, B, T, Hq, H, D, sm_scale,
     )
     return (o, lse) if return_lse else o

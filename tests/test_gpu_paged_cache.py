@@ -206,7 +206,7 @@ def test_strided_rows_are_read_in_place_and_others_copied(device):
     turned = torch.randn((B, H, T, D), generator=gen, device=device).to(torch.bfloat16).transpose(1, 2)
     apart = torch.randn((B, T, H, D + 1), generator=gen, device=device).to(torch.bfloat16)[..., :D]
     one = torch.randn((1, 1, H, D), generator=gen, device=device).to(torch.bfloat16).expand(B, T, H, D)
-    assert hip._rows_of_chunks(fused[:, :, H:2 * H]).data_ptr() == fused[:, :, H:].data_ptr()
+    assert hip._new_rows(fused[:, :, H:2 * H], fused[:, :, 3 * H:])[0].data_ptr() == fused[:, :, H:].data_ptr()
     for x, y in ((fused[:, :, H:2 * H], fused[:, :, 3 * H:]), (odd, turned), (apart, one), (turned, odd)):
         caches = [PagedCache.allocate(B, T, H, D, dtype=torch.float8_e4m3fn, device=device) for _ in range(2)]
         write_pages(caches[0], x, y)
