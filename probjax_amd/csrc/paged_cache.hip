@@ -26,7 +26,7 @@ struct WriteArgs {
   int32_t* lengths_out;
   int B, T, D;
   int tokens;  // of a workgroup
-  FastDiv by_2h;
+  FastDiv by_h;
 };
 
 // Keys of sequence b before the call, and its new tokens.
@@ -53,108 +53,131 @@ __device__ __forceinline__ uint32_t group_max(uint32_t x) {
   return x;
 }
 
-// 8 elements of a row: their values, and which of them are infinite or NaN (tested on
-// the loaded bits: the sources are compiled without NaN in mind).
+// What 8 elements of a row in format E are made of.
 template <typename E>
-__device__ __forceinline__ uint32_t unpack8(const u32x4* raw, float* x) {
-  uint32_t odd = 0;
-  if constexpr (std::is_same<E, F32Fmt>::value) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t u = raw[i / 4][i % 4];
-      odd |= (u & 0x7f800000u) == 0x7f800000u ? 1u << i : 0u;
-      x[i] = __uint_as_float(u);
-    }
-  } else {
-    constexpr uint32_t ex = E::kF16 ? 0x7c00u : 0x7f80u;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t u = raw[0][i];
-      odd |= ((u & ex) == ex ? 1u << 2 * i : 0u) | ((u & (ex << 16)) == ex << 16 ? 2u << 2 * i : 0u);
-      x[2 * i] = E::lo(u);
-      x[2 * i + 1] = E::hi(u);
-    }
+struct Row8 {
+  static constexpr bool k32 = std::is_same<E, F32Fmt>::value, kF16 = std::is_same<E, F16Fmt>::value;
+  // The largest magnitude that reads back inside the type's range is 240 * 2^e, of those
+  // below 256 * 2^e: past it a row takes the long way.  (As the type's own bits; infinities
+  // and NaN are past it too.  Bits, since the sources are compiled without NaN in mind.)
+  static constexpr uint32_t kMost = k32 ? 0x7f700000u : kF16 ? 0x7b80u : 0x7f70u;
+  static constexpr uint32_t kInf = k32 ? 0x7f800000u : kF16 ? 0x7c00u : 0x7f80u;
+
+  __device__ __forceinline__ static uint32_t magnitude(const u32x4* raw, int i) {
+    if constexpr (k32) return raw[i / 4][i % 4] & 0x7fffffffu;
+    else return (raw[0][i / 2] >> 16 * (i % 2)) & 0x7fffu;
   }
-  return odd;
+  __device__ __forceinline__ static float value(const u32x4* raw, int i) {
+    if constexpr (k32) return __uint_as_float(raw[i / 4][i % 4]);
+    else return i % 2 ? E::hi(raw[0][i / 2]) : E::lo(raw[0][i / 2]);
+  }
+  __device__ __forceinline__ static uint32_t float_bits(uint32_t m) {  // of a magnitude
+    if constexpr (k32) return m;
+    else return __float_as_uint(E::lo(m));
+  }
+  __device__ __forceinline__ static uint32_t largest(const u32x4* raw) {
+    uint32_t m = 0;
+    if constexpr (k32) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m = max(m, magnitude(raw, i));
+    } else {  // two at a time
+      typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+      u16x2 x = __builtin_bit_cast(u16x2, raw[0][0] & 0x7fff7fffu);
+#pragma unroll
+      for (int i = 1; i < 4; ++i) x = __builtin_elementwise_max(x, __builtin_bit_cast(u16x2, raw[0][i] & 0x7fff7fffu));
+      m = max((uint32_t)x[0], (uint32_t)x[1]);
+    }
+    return m;
+  }
+};
+
+// The exponent byte of a row whose largest finite value has these float bits: 448 is 1.75 *
+// 2^8, its fraction's bits 0x600000; a scale below 2^-126 would be subnormal.
+__device__ __forceinline__ int row_exponent(uint32_t bits) {
+  return max((int)(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0), 1);
 }
 
 // E: format of the new rows.  QUANT: into 8 bits, 8 elements a lane; else copied, 16
 // bytes a lane.  LPR lanes per row.
 template <typename E, bool QUANT, int LPR>
 __global__ __launch_bounds__(kPageThreads) void write_pages_kernel(WriteArgs a) {
+  typedef Row8<E> R;
   constexpr int SZ = fmt_size<E>();
   constexpr int EPL = QUANT ? 8 : 16 / SZ;  // elements of a lane
   constexpr int LDS16 = EPL * SZ / 16;      // its 16-byte loads
   constexpr int RPB = kPageThreads / LPR;   // rows of a pass
   constexpr int U = 4;                      // passes in flight
   const PageArgs& p = a.p;
-  const int tid = threadIdx.x, sub = tid % LPR;
+  const int tid = threadIdx.x, sub = tid % LPR, kv = blockIdx.z;
   const bool in_row = sub * EPL < a.D;
+  char* pool = kv ? p.v : p.k;
+  uint8_t* exps = kv ? p.ve : p.ke;
+  const int64_t sp = kv ? p.vp : p.kp, st = kv ? p.vt : p.kt, sh = kv ? p.vh : p.kh;
+  const int64_t xt = a.xt[kv], xh = a.xh[kv];
   for (int b = blockIdx.y; b < a.B; b += gridDim.y) {
     int64_t before;
     int n;
     new_tokens(a, b, before, n);
     const int64_t room = (int64_t)p.most * p.page;
-    if (blockIdx.x == 0 && tid == 0) a.lengths_out[b] = (int32_t)min(before + n, room);
+    if (blockIdx.x == 0 && kv == 0 && tid == 0) a.lengths_out[b] = (int32_t)min(before + n, room);
     const int64_t first = (int64_t)blockIdx.x * a.tokens;
     if (first >= n || before + first >= room) continue;
     const int nt = (int)min((int64_t)a.tokens, min((int64_t)n - first, room - before - first));
-    const int rows = nt * 2 * p.H;
-    for (int r0 = tid / LPR; r0 < rows; r0 += U * RPB) {
+    const int rows = nt * p.H;
+    const char* x = a.x[kv] + b * a.xb[kv] + first * xt + sub * EPL * SZ;
+    for (int r0 = 0; r0 < rows; r0 += U * RPB) {
       u32x4 raw[U][LDS16];
       uint32_t page[U];
-      int slot[U], kv[U], h[U];
-      bool ok[U];
+      int slot[U], h[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int r = r0 + u * RPB;
-        ok[u] = r < rows;
-        const int t = a.by_2h(ok[u] ? r : 0), rest = (ok[u] ? r : 0) - t * 2 * p.H;
-        kv[u] = rest >= p.H;
-        h[u] = rest - kv[u] * p.H;
+        if (r0 + u * RPB >= rows) break;
+        const int mine = r0 + u * RPB + tid / LPR, r = min(mine, rows - 1), t = a.by_h(r);
+        h[u] = r - t * p.H;
         const int pos = (int)(before + first) + t, i = p.by_page(pos);
         slot[u] = pos - i * p.page;
-        page[u] = ok[u] ? page_entry(p, b, i) : ~0u;
-        const char* x = (kv[u] ? a.x[1] + b * a.xb[1] + (first + t) * a.xt[1] + h[u] * a.xh[1]
-                               : a.x[0] + b * a.xb[0] + (first + t) * a.xt[0] + h[u] * a.xh[0]) + sub * EPL * SZ;
+        page[u] = mine < rows ? page_entry(p, b, i) : ~0u;
 #pragma unroll
-        for (int i2 = 0; i2 < LDS16; ++i2)
-          raw[u][i2] = ok[u] && in_row ? *(const u32x4*)(x + 16 * i2) : u32x4{0u, 0u, 0u, 0u};
+        for (int j = 0; j < LDS16; ++j)
+          raw[u][j] = in_row ? *(const u32x4*)(x + t * xt + h[u] * xh + 16 * j) : u32x4{0u, 0u, 0u, 0u};
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
+        if (r0 + u * RPB >= rows) break;
         const bool there = page[u] < p.pages;
-        char* to = (kv[u] ? p.v + page[u] * p.vp + slot[u] * p.vt + h[u] * p.vh
-                          : p.k + page[u] * p.kp + slot[u] * p.kt + h[u] * p.kh);
+        char* to = pool + page[u] * sp + slot[u] * st + h[u] * sh;
         if constexpr (QUANT) {
-          float x[8];
-          const uint32_t odd = unpack8<E>(raw[u], x);
-          uint32_t m = 0;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) m = max(m, odd >> i & 1 ? 0u : __float_as_uint(x[i]) & 0x7fffffffu);
-          m = group_max<LPR>(m);
-          // 448 is 1.75 * 2^8, its fraction's bits 0x600000; a scale below 2^-126 would be subnormal
-          const int e = max((int)(m >> 23) - 8 + ((m & 0x7fffffu) > 0x600000u ? 1 : 0), 1);
-          const float back = exponent_scale(254 - e);
-          // (what would read back past the range of the rows' type: 240 is the largest below 256)
-          constexpr float most = std::is_same<E, F16Fmt>::value ? 61440.f : 0x1.ep127f;
-          float y[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) y[i] = fminf(fmaxf(x[i], -most), most) * back;
+          uint32_t m = group_max<LPR>(R::largest(raw[u]));
+          int e = row_exponent(R::float_bits(m));
+          float back = exponent_scale(254 - e);
           u32x2 c;
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i], y[4 * i + 1], 0, false);
-            c[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i + 2], y[4 * i + 3], w, true);
+            int w = __builtin_amdgcn_cvt_pk_fp8_f32(R::value(raw[u], 4 * i) * back, R::value(raw[u], 4 * i + 1) * back, 0, false);
+            c[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(R::value(raw[u], 4 * i + 2) * back,
+                                                             R::value(raw[u], 4 * i + 3) * back, w, true);
           }
-          if (odd) {
+          if (m > R::kMost) {
+            m = 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (odd >> i & 1) c[i / 4] = (c[i / 4] & ~(0xffu << 8 * (i % 4))) | 0x7fu << 8 * (i % 4);
+            for (int i = 0; i < 8; ++i) {
+              const uint32_t y = R::magnitude(raw[u], i);
+              m = max(m, y < R::kInf ? y : 0u);
+            }
+            m = group_max<LPR>(m);
+            e = row_exponent(R::float_bits(m));
+            back = exponent_scale(254 - e);
+            const float most = __uint_as_float(R::float_bits(R::kMost));
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float y = fminf(fmaxf(R::value(raw[u], i), -most), most) * back;
+              const uint32_t code = R::magnitude(raw[u], i) < R::kInf ? (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y, y, 0, false) & 0xffu : 0x7fu;
+              c[i / 4] = (c[i / 4] & ~(0xffu << 8 * (i % 4))) | code << 8 * (i % 4);
+            }
           }
           if (there) {
             if (in_row) *(u32x2*)(to + sub * EPL) = c;
-            if (sub == 0) (kv[u] ? p.ve : p.ke)[((int64_t)page[u] * p.H + h[u]) * p.page + slot[u]] = (uint8_t)e;
+            if (sub == 0) exps[((int64_t)page[u] * p.H + h[u]) * p.page + slot[u]] = (uint8_t)e;
           }
         } else if (there && in_row) {
           *(u32x4*)(to + sub * 16) = raw[u][0];
@@ -175,13 +198,16 @@ struct ReadArgs {
   FastDiv by_token, by_row;  // units of a token (H rows), of a row
 };
 
-// C: format of the cache, E: of the output (C, unless C is e4m3).
-template <typename C, typename E>
+// C: format of the cache, E: of the output (C, unless C is e4m3).  STREAM: more than the
+// 256 MB cache holds, past its reuse hint and twice the rows in flight (16 x 1000-8192 keys
+// of 8 heads of 128 from 8 bits, 545 MB written: 134 us against 162; 134 MB: 45 and 46, 67
+// MB: 27 and 19).
+template <typename C, typename E, bool STREAM>
 __global__ __launch_bounds__(kPageThreads) void read_pages_kernel(ReadArgs a) {
   constexpr bool QUANT = std::is_same<C, E4m3Fmt>::value;
   constexpr int EPU = 16 / fmt_size<E>();         // elements of a unit
   constexpr int IN = EPU * fmt_size<C>();         // its bytes in the cache
-  constexpr int U = 4;
+  constexpr int U = STREAM ? 8 : 4;
   typedef typename std::conditional<IN == 16, u32x4, typename std::conditional<IN == 8, u32x2, uint32_t>::type>::type Raw;
   const PageArgs& p = a.p;
   const int tid = threadIdx.x, kv = blockIdx.z;
@@ -213,7 +239,9 @@ __global__ __launch_bounds__(kPageThreads) void read_pages_kernel(ReadArgs a) {
           const uint32_t page = page_entry(p, b, i);
           there[u] = page < p.pages;
           if (there[u]) {
-            raw[u] = *(const Raw*)(pool + page * sp + slot * st + h * sh + c * IN);
+            const Raw* x = (const Raw*)(pool + page * sp + slot * st + h * sh + c * IN);
+            if constexpr (STREAM) raw[u] = __builtin_nontemporal_load(x);
+            else raw[u] = *x;
             if constexpr (QUANT) e[u] = exps[((int64_t)page * p.H + h) * p.page + slot];
           }
         }
@@ -245,7 +273,9 @@ __global__ __launch_bounds__(kPageThreads) void read_pages_kernel(ReadArgs a) {
           }
           if (!there[u]) out = u32x4{0u, 0u, 0u, 0u};
         }
-        *(u32x4*)(y + (int64_t)unit * 16) = out;
+        u32x4* to = (u32x4*)(y + (int64_t)unit * 16);
+        if constexpr (STREAM) __builtin_nontemporal_store(out, to);
+        else *to = out;
       }
     }
   }
@@ -296,6 +326,8 @@ int fill_pages(PageArgs& a, const char* who, int cache_dtype, const pjx_pages* c
   return PJX_OK;
 }
 
+constexpr int64_t kStreamRead = (int64_t)256 << 20;  // bytes read_pages writes past which they are streamed
+
 // Tokens of a workgroup whose tokens are `per_token` units of work, `passes` x 256 of
 // them wanted.
 static int tokens_of(int64_t per_token, int passes) {
@@ -304,9 +336,9 @@ static int tokens_of(int64_t per_token, int passes) {
 
 template <typename E, bool QUANT, int LPR>
 static int run_write(WriteArgs& a, hipStream_t s, const char* who) {
-  a.tokens = tokens_of((int64_t)2 * a.p.H * LPR, 8);
+  a.tokens = tokens_of((int64_t)a.p.H * LPR, 4);
   const unsigned x = (unsigned)std::max((a.T + a.tokens - 1) / a.tokens, 1);
-  launch_kernel<write_pages_kernel<E, QUANT, LPR>>(dim3(x, (unsigned)std::min(a.B, 65535)), dim3(kPageThreads), 0, s, a);
+  launch_kernel<write_pages_kernel<E, QUANT, LPR>>(dim3(x, (unsigned)std::min(a.B, 65535), 2), dim3(kPageThreads), 0, s, a);
   return check_launch(who);
 }
 
@@ -328,11 +360,13 @@ template <typename C, typename E>
 static int run_read(ReadArgs& a, hipStream_t s, const char* who) {
   a.upr = a.D * fmt_size<E>() / 16;
   const int64_t per_token = (int64_t)a.p.H * a.upr;
-  a.tokens = tokens_of(per_token, 4);
+  const bool stream = 2 * a.B * a.L * per_token * 16 >= kStreamRead;
+  a.tokens = tokens_of(per_token, stream ? 8 : 4);
   a.by_token = fast_div(per_token);
   a.by_row = fast_div(a.upr);
-  const int64_t x = (a.L + a.tokens - 1) / a.tokens;
-  launch_kernel<read_pages_kernel<C, E>>(dim3((unsigned)x, (unsigned)std::min(a.B, 65535), 2), dim3(kPageThreads), 0, s, a);
+  const dim3 grid((unsigned)((a.L + a.tokens - 1) / a.tokens), (unsigned)std::min(a.B, 65535), 2);
+  if (stream) launch_kernel<read_pages_kernel<C, E, true>>(grid, dim3(kPageThreads), 0, s, a);
+  else launch_kernel<read_pages_kernel<C, E, false>>(grid, dim3(kPageThreads), 0, s, a);
   return check_launch(who);
 }
 
@@ -374,7 +408,7 @@ extern "C" int pjx_write_pages(int dtype, int cache_dtype, const void* k, const 
   }
   a.lengths = kv_lengths; a.fresh = new_lengths; a.lengths_out = lengths_out;
   a.B = (int)batch; a.T = (int)len; a.D = (int)head_dim;
-  a.by_2h = fast_div(2 * kv_heads);
+  a.by_h = fast_div(kv_heads);
   hipStream_t s = (hipStream_t)stream;
   return dtype == PJX_DTYPE_F32    ? run_write<F32Fmt>(a, quant, s, who)
          : dtype == PJX_DTYPE_BF16 ? run_write<Bf16Fmt>(a, quant, s, who)
