@@ -96,11 +96,14 @@ CASES = [
 ]
 
 
+@pytest.mark.parametrize("times", [1, 12])  # sequences short enough for a workgroup each, and cut into shares
 @pytest.mark.parametrize("case", CASES, ids=lambda c: "-".join(map(str, c)))
-def test_matches_definition(device, case):
+def test_matches_definition(device, case, times):
     import torch
+    from probjax_amd import native
 
     name, held, B, T, Hq, Hkv, D, page, N, layout = case
+    N *= times
     rng = np.random.default_rng(D + page + T)
     S, dtype = N * page, types()[name]
     pages = B * N + 1
@@ -109,6 +112,9 @@ def test_matches_definition(device, case):
     cache = make_cache(device, rng, held, pages, page, Hkv, D, table, layout, spread=3)
     q = torch.from_numpy(rng.standard_normal((B, T, Hq, D), dtype=np.float32)).to(device, dtype)
     run(device, cache, table, lengths, q, dtype, "full and random lengths")
+    width = 64 if D <= 64 else 128 if D <= 128 else 256
+    whole = S * 2 * width * cache.k.element_size() <= 128 << 10
+    assert len(native.last_launches()) == (1 if whole else 2), native.last_launches()
     run(device, cache, table, [max(S - 1, 0)] + [min(T, S)] * (B - 1), q, dtype, "as many keys as tokens")
     run(device, cache, table, [1] + [0] * (B - 1), q, dtype, "one key, none")
     run(device, cache, table, [S + 100] + [-5] * (B - 1), q, dtype, "past the capacity, negative")
@@ -116,19 +122,25 @@ def test_matches_definition(device, case):
 
 
 @pytest.mark.parametrize("name,held", [("bf16", "bf16"), ("f16", "e4m3"), ("f32", "f32"), ("bf16", "e4m3"), ("f32", "e4m3")])
-@pytest.mark.parametrize("B,S", [(1, 5000), (5, 1100), (300, 40), (70, 300)])
+@pytest.mark.parametrize("B,S", [(1, 5000), (5, 1100), (300, 40), (70, 300), (64, 2100), (65, 2100), (130, 2500), (300, 2100)])
 def test_lengths_of_every_kind(device, name, held, B, S):
-    """One long sequence, ragged batches, more sequences than threads of a workgroup."""
+    """One long sequence, ragged batches, more sequences than a wave has lanes (shares
+    that run through several short ones among them)."""
     import torch
 
     Hq, Hkv, D, page = 4, 2, 64, 16
     rng = np.random.default_rng(B)
     N, dtype = -(-S // page), types()[name]
     lengths = [S] + [int(x) for x in rng.integers(0, S + 1, B - 1)]
+    if B >= 64:  # long runs of short ones
+        lengths = [n if b % 9 == 0 else n % 40 for b, n in enumerate(lengths)]
+        lengths[3:7] = [0] * 4
+        lengths[-2:] = [0, 0]
     table = make_table(rng, B, N, B * N, lengths, page)
     cache = make_cache(device, rng, held, B * N, page, Hkv, D, table)
     q = torch.from_numpy(rng.standard_normal((B, 1, Hq, D), dtype=np.float32)).to(device, dtype)
     run(device, cache, table, lengths, q, dtype)
+    run(device, cache, table, [0] * B, q, dtype, "no keys")
 
 
 def _spoil(pool, at, value):
@@ -142,19 +154,19 @@ def _spoil(pool, at, value):
 
 
 @pytest.mark.parametrize("name,held", [("bf16", "bf16"), ("f16", "f16"), ("f32", "f32"), ("bf16", "e4m3"), ("f32", "e4m3")])
-@pytest.mark.parametrize("T,page", [(1, 16), (4, 16), (4, 5), (1, 64)])
-def test_what_is_not_seen_does_not_reach_the_output(device, name, held, T, page):
+@pytest.mark.parametrize("T,page,keys", [(1, 16, 300), (4, 16, 300), (4, 5, 300), (1, 64, 300), (1, 16, 2500), (5, 16, 2500), (20, 7, 2500)])
+def test_what_is_not_seen_does_not_reach_the_output(device, name, held, T, page, keys):
     """NaN and infinities behind the lengths, in pages of no sequence, in keys that the
     earlier tokens do not see; missing pages among the others."""
     import torch
     from probjax_amd.attention import paged_decode
 
     B, Hq, Hkv, D, dtype = 3, 4, 2, 64, types()[name]
-    N = -(-300 // page)
+    N = -(-keys // page)
     rng = np.random.default_rng(7)
     pages = B * N + 2
     table = rng.permutation(pages)[:B * N].reshape(B, N).astype(np.int32)
-    lengths = [N * page - 7, 131, T + 1]
+    lengths = [N * page - 7, keys // 2 - 19, T + 1]
     table[0, 3], table[0, N // 2], table[1, 0], table[2, 0] = -1, pages + 3, -2 ** 31, -1
     cache = make_cache(device, rng, held, pages, page, Hkv, D, table)
     clean_k, clean_v, there = gathered(cache, table, lengths)
@@ -262,3 +274,33 @@ def test_scales_far_apart(device):
         cache.k_exponents.copy_(torch.from_numpy(rng.integers(60, 119, cache.k_exponents.shape).astype(np.uint8)))
         q = torch.from_numpy(rng.standard_normal((B, 1, Hq, D), dtype=np.float32)).to(device, types()[dtype])
         run(device, cache, table, [N * page, 20], q, types()[dtype])
+
+
+def test_many_heads(device):
+    """More KV heads than the device holds waves, and numbers that no workgroup divides."""
+    import torch
+
+    rng = np.random.default_rng(4)
+    for H, D, N, held in ((2053, 16, 33, "e4m3"), (37, 64, 40, "bf16"), (6, 128, 70, "bf16")):
+        B, page, G = 2, 64, 2
+        lengths = [N * page - 3, 70]
+        table = make_table(rng, B, N, B * N, lengths, page)
+        cache = make_cache(device, rng, held, B * N, page, H, D, table)
+        q = torch.from_numpy(rng.standard_normal((B, 1, H * G, D), dtype=np.float32)).to(device, torch.bfloat16)
+        run(device, cache, table, lengths, q, torch.bfloat16)
+
+
+def test_a_share_of_keys_in_missing_pages(device):
+    """Nothing but missing pages in whole parts of a sequence, and in all of it."""
+    import torch
+
+    rng = np.random.default_rng(5)
+    B, Hq, Hkv, D, page, N = 3, 4, 2, 64, 16, 300
+    lengths = [N * page, 4000, 700]
+    for dtype, held in (("bf16", "bf16"), ("f16", "e4m3"), ("f32", "f32")):
+        table = make_table(rng, B, N, B * N, lengths, page)
+        table[0, 20:250], table[1, :200], table[2] = -1, -1, -1
+        cache = make_cache(device, rng, held, B * N, page, Hkv, D, table)
+        q = torch.from_numpy(rng.standard_normal((B, 2, Hq, D), dtype=np.float32)).to(device, types()[dtype])
+        got, lse = run(device, cache, table, lengths, q, types()[dtype])
+        assert not got[2].any() and torch.isposinf(lse[2]).all()
