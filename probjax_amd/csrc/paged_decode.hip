@@ -266,11 +266,11 @@ template <typename C, typename E, int W, int NRB, bool ROWS, bool WHOLE>
 __global__ __launch_bounds__(64 * (WHOLE ? paged_whole_waves<C, E, W, NRB>() : kPagedWaves), (paged_occupancy<C, E, W>())) void paged_decode_kernel(PagedArgs a) {
   using T = PageTile<C, W>;
   constexpr bool F32 = std::is_same<E, F32Fmt>::value, QUANT = std::is_same<C, E4m3Fmt>::value;
-  // The weights' product with V: in 16 bits they are rounded to the type, in two parts
-  // (the rounding's rest is the second) where V is 8-bit codes: their scales have bf16's
-  // range, and fp16 outputs more bits than a bf16 weight has.
+  // The weights enter their product with V in 16 bits, in two parts: rounded to the type,
+  // and the rounding's rest.  That leaves the output's own rounding (without the second
+  // part errors are 1.3 times it) and costs nothing where the memory is waited for.  Codes
+  // take them as bf16 whatever E is: their rows' powers of two have its range, not fp16's.
   typedef typename std::conditional<QUANT && !F32, Bf16Fmt, E>::type EV;
-  constexpr bool SPLIT = QUANT && !F32 && std::is_same<E, F16Fmt>::value;
   constexpr int KS = T::KS, KB = KS / 16, NL = T::NL, CS = T::CS, ES = fmt_size<E>();
   constexpr int NDB = W / 16;
   constexpr int NW = WHOLE ? paged_whole_waves<C, E, W, NRB>() : kPagedWaves;
@@ -627,7 +627,7 @@ __global__ __launch_bounds__(64 * (WHOLE ? paged_whole_waves<C, E, W, NRB>() : k
           for (int i = 0; i < 4; ++i) {
             const float x = s[rb][i / 2][2 * (i % 2)], y = s[rb][i / 2][2 * (i % 2) + 1];
             pk[rb][i] = EV::pack2(x, y);
-            if constexpr (SPLIT) rest[rb][i] = EV::pack2(x - EV::lo(pk[rb][i]), y - EV::hi(pk[rb][i]));
+            rest[rb][i] = EV::pack2(x - EV::lo(pk[rb][i]), y - EV::hi(pk[rb][i]));
           }
 #pragma unroll
         for (int i = 0; i < NDB; ++i) {
@@ -637,7 +637,7 @@ __global__ __launch_bounds__(64 * (WHOLE ? paged_whole_waves<C, E, W, NRB>() : k
 #pragma unroll
           for (int rb = 0; rb < NRB; ++rb) {
             acc[rb][i] = EV::mma16(v, EV::as8(pk[rb]), acc[rb][i]);
-            if constexpr (SPLIT) acc[rb][i] = EV::mma16(v, EV::as8(rest[rb]), acc[rb][i]);
+            acc[rb][i] = EV::mma16(v, EV::as8(rest[rb]), acc[rb][i]);
           }
         }
       }
