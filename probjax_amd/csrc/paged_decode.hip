@@ -506,6 +506,15 @@ __global__ __launch_bounds__(64 * (WHOLE ? paged_whole_waves<C, E, W, NRB>() : k
           s[rb][kb][r] = QUANT ? x * vs[kb][r] : x;
         }
       l_run[rb] += rs;
+      if constexpr (QUANT) {
+        if (!whole) {  // (what no key was written to may hold 255, an infinite power)
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (!sees(rb, 16 * kb + 4 * q4 + r)) s[rb][kb][r] = 0.f;
+        }
+      }
     }
 
     // ---- O += P V ----

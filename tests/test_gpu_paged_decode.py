@@ -202,6 +202,47 @@ def test_what_is_not_seen_does_not_reach_the_output(device, name, held, T, page,
         assert torch.isnan(got[:2, T - 2:]).any(-1).all()
 
 
+@pytest.mark.parametrize("name", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("T,D,page,keys", [(1, 64, 16, 300), (4, 64, 5, 300), (5, 128, 16, 2500), (1, 256, 16, 200)])
+def test_exponents_of_unwritten_slots(device, name, T, D, page, keys):
+    """Any byte may stand where nothing was written, 255 (a power of two that is
+    infinite) too: behind the lengths, in page 0 (where missing pages are read from)
+    and, for the keys that the last token alone sees, for the earlier ones."""
+    import torch
+    from probjax_amd.attention import paged_decode
+
+    B, Hq, Hkv, dtype = 2, 4, 2, types()[name]
+    N = -(-keys // page)
+    rng = np.random.default_rng(8)
+    pages = B * N + 1
+    table = (1 + rng.permutation(B * N)).reshape(B, N).astype(np.int32)  # page 0: no one's
+    lengths = [N * page - 3, keys // 2 - 19]
+    table[0, 2], table[1, 1] = -1, pages
+    cache = make_cache(device, rng, "e4m3", pages, page, Hkv, D, table)
+    k, v, there = gathered(cache, table, lengths)
+    used = np.zeros((pages, page), bool)
+    for b in range(B):
+        p, s = ref.slots(table, page, pages, b, np.arange(lengths[b]))
+        used[p[p >= 0], s[p >= 0]] = True
+    spoil = torch.from_numpy(~used).to(device)[:, None].expand(pages, Hkv, page)
+    cache.k_exponents[spoil] = 255
+    cache.v_exponents[spoil] = 255
+    q = torch.from_numpy(rng.standard_normal((B, T, Hq, D), dtype=np.float32)).to(device, dtype)
+    L = torch.tensor(lengths, dtype=torch.int32, device=device)
+    want = ref.paged_decode(to_np(q), k, v, there, lengths, 1.0 / math.sqrt(D))
+    got, lse = paged_decode(q, cache, kv_lengths=L, return_lse=True)
+    torch.cuda.synchronize()
+    check(got, lse, want, dtype, D, N * page)
+    if T > 1:
+        for b in range(B):
+            p, s = ref.slots(table, page, pages, b, [lengths[b] - 1])
+            cache.v_exponents[p[0], :, s[0]] = 255
+        got, lse = paged_decode(q, cache, kv_lengths=L, return_lse=True)
+        torch.cuda.synchronize()
+        early = {n: x[:, :T - 1] if n in ("out", "spread") else x[..., :T - 1] for n, x in want.items()}
+        check(got[:, :T - 1], lse[..., :T - 1], early, dtype, D, N * page)
+
+
 @pytest.mark.parametrize("name,held", [("bf16", "bf16"), ("f16", "e4m3"), ("f32", "f32")])
 def test_nan_and_infinities_that_are_seen(device, name, held):
     """As the definition has them: NaN in a seen value spoils its feature, in a seen key
