@@ -145,7 +145,7 @@ __global__ __launch_bounds__(kPageThreads) void write_pages_kernel(WriteArgs a) 
       for (int u = 0; u < U; ++u) {
         if (r0 + u * RPB >= rows) break;
         const bool there = page[u] < p.pages;
-        char* to = pool + page[u] * sp + slot[u] * st + h[u] * sh;
+        char* to = pool + page[u] * (uint64_t)sp + slot[u] * st + h[u] * sh;
         if constexpr (QUANT) {
           uint32_t m = group_max<LPR>(R::largest(raw[u]));
           int e = row_exponent(R::float_bits(m));
@@ -176,7 +176,7 @@ __global__ __launch_bounds__(kPageThreads) void write_pages_kernel(WriteArgs a) 
             }
           }
           if (there) {
-            if (in_row) *(u32x2*)(to + sub * EPL) = c;
+            if (in_row) __builtin_nontemporal_store(c, (u32x2*)(to + sub * EPL));
             if (sub == 0) exps[((int64_t)page[u] * p.H + h[u]) * p.page + slot[u]] = (uint8_t)e;
           }
         } else if (there && in_row) {
