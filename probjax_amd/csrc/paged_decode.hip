@@ -69,12 +69,19 @@ __device__ __forceinline__ Lane lane_steps(const PagedArgs& a) {
   const int lane = threadIdx.x & 63, L = lane < a.B ? paged_len(a, lane) : 0;
   return {L, wave_scan(steps_of(a, L))};
 }
+// The sum over the lanes' sequences behind the first 64 and before `end`, in all lanes.
+__device__ __forceinline__ int later_steps(const PagedArgs& a, int end) {
+  int n = 0;
+#pragma unroll 8
+  for (int b0 = 64; b0 < end; b0 += 64) {
+    const int b = b0 + (threadIdx.x & 63), L = paged_len(a, min(b, a.B - 1));
+    n += b < end ? steps_of(a, L) : 0;
+  }
+  return __builtin_amdgcn_readlane(wave_scan(n), 63);
+}
 __device__ __forceinline__ int all_steps(const PagedArgs& a, const Lane& s) {
-  const int lane = threadIdx.x & 63;
-  int all = __builtin_amdgcn_readlane(s.upto, 63), n = 0;
-  if (a.B <= 64) return all;
-  for (int b0 = 64; b0 < a.B; b0 += 64) n += b0 + lane < a.B ? steps_of(a, paged_len(a, b0 + lane)) : 0;
-  return all + __builtin_amdgcn_readlane(wave_scan(n), 63);
+  const int all = __builtin_amdgcn_readlane(s.upto, 63);
+  return a.B <= 64 ? all : all + later_steps(a, a.B);
 }
 __device__ __forceinline__ int share_of(const PagedArgs& a, int all) { return max(a.by_shares(all + a.shares - 1), a.least); }
 
@@ -117,16 +124,12 @@ __device__ __forceinline__ Cursor next_step(const PagedArgs& a, int lens, Cursor
 }
 // Steps before those of sequence b, and b's.
 __device__ __forceinline__ int steps_before(const PagedArgs& a, const Lane& s, int b, int& n_b) {
-  const int lane = threadIdx.x & 63;
-  int L = s.len, upto = s.upto, b0 = 0;
-  for (; b >= b0 + 64;) {
-    const int run = __builtin_amdgcn_readlane(upto, 63);
-    b0 += 64;
-    L = b0 + lane < a.B ? paged_len(a, b0 + lane) : 0;
-    upto = run + wave_scan(steps_of(a, L));
+  if (b < 64) {
+    n_b = steps_of(a, __builtin_amdgcn_readlane(s.len, b));
+    return __builtin_amdgcn_readlane(s.upto, b) - n_b;
   }
-  n_b = steps_of(a, __builtin_amdgcn_readlane(L, b - b0));
-  return __builtin_amdgcn_readlane(upto, b - b0) - n_b;
+  n_b = steps_of(a, __builtin_amdgcn_readfirstlane(paged_len(a, b)));
+  return __builtin_amdgcn_readlane(s.upto, 63) + later_steps(a, b);
 }
 
 // A step's K or V rows in LDS: rows of W elements of C, their 16-byte chunks at chunk ^
