@@ -841,15 +841,27 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
 // ---------------------------------------------------------------------------
 // Host
 // ---------------------------------------------------------------------------
-// Shares of a KV head, with `waves` waves to a compute unit at a time: as many as fill the
-// device once.
-static int64_t paged_shares(int64_t kv_heads, int waves) { return std::max<int64_t>((int64_t)256 * waves / kv_heads, 1); }
 static int paged_width(int64_t head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
-// Parts of a KV head at most: one of every share, and one more where a sequence begins.
-static int64_t paged_parts(int64_t batch, int64_t kv_heads) { return paged_shares(kv_heads, 2 * kPagedWaves) + batch; }
-static size_t paged_ws(int64_t batch, int64_t kv_heads, int64_t rows, int64_t head_dim) {
-  return (size_t)(paged_parts(batch, kv_heads) * kv_heads * rows * (paged_width(head_dim) + 2)) * sizeof(float) + 16;
+// Blocks of 16 query rows of a wave: 32 rows of 256 features spill registers.
+static int paged_blocks(int64_t rows, int64_t head_dim) { return rows > 16 && paged_width(head_dim) < 256 ? 2 : 1; }
+static int64_t paged_groups(int64_t rows, int64_t head_dim) {
+  const int64_t n = 16 * paged_blocks(rows, head_dim);
+  return std::max<int64_t>((rows + n - 1) / n, 1);
 }
+// Shares of a KV head, with `waves` waves to a compute unit at a time: as many as fill the
+// device once, each of the groups of rows taking all of them.
+static int64_t paged_shares(int64_t kv_heads, int64_t rows, int64_t head_dim, int waves) {
+  return std::max<int64_t>((int64_t)256 * waves / (kv_heads * paged_groups(rows, head_dim)), 1);
+}
+// Parts of a KV head at most: one of every share, and one more where a sequence begins.
+static int64_t paged_parts(int64_t batch, int64_t kv_heads, int64_t rows, int64_t head_dim) {
+  return paged_shares(kv_heads, rows, head_dim, 2 * kPagedWaves) + batch;
+}
+static size_t paged_ws(int64_t batch, int64_t kv_heads, int64_t rows, int64_t head_dim) {
+  return (size_t)(paged_parts(batch, kv_heads, rows, head_dim) * kv_heads * rows * (paged_width(head_dim) + 2)) * sizeof(float) + 16;
+}
+static_assert(paged_waves<Bf16Fmt, 64>() <= 2 * kPagedWaves && paged_waves<E4m3Fmt, 64>() <= 2 * kPagedWaves,
+              "paged_parts counts the shares of so many waves");
 
 // Whether a workgroup takes a sequence whole, and nothing is joined after it: where one
 // compute unit has little enough to read (by itself it reads some 40 GB/s).  us, shares and
@@ -861,26 +873,25 @@ static bool paged_whole(int64_t capacity, int64_t row_bytes) { return capacity *
 
 template <typename C, typename E, int W, bool ROWS>
 static int run_paged(PagedArgs& a, hipStream_t s, const char* who) {
-  constexpr bool WIDE = W == 256;  // (32 rows of 256 features spill registers)
-  const bool two = !WIDE && a.rows > 16;
+  constexpr int NRB = W == 256 ? 1 : 2;
+  const bool two = paged_blocks(a.rows, W) == 2;
   a.step_log = PageTile<C, W>::KS == 16 ? 4 : 5;
   const int64_t capacity = (int64_t)a.p.most * a.p.page;
-  const unsigned groups = (unsigned)((a.rows + (two ? 31 : 15)) / (two ? 32 : 16));
+  const unsigned groups = (unsigned)paged_groups(a.rows, W);
   if (paged_whole(capacity, PageTile<C, W>::ROWB)) {
-    constexpr int NRB = WIDE ? 1 : 2;
     const dim3 grid((unsigned)(a.B * a.p.H), groups);
     if (two) launch_kernel<paged_decode_kernel<C, E, W, NRB, ROWS, true>>(grid, dim3(64 * paged_whole_waves<C, E, W, NRB>()), 0, s, a);
     else launch_kernel<paged_decode_kernel<C, E, W, 1, ROWS, true>>(grid, dim3(64 * paged_whole_waves<C, E, W, 1>()), 0, s, a);
     return check_launch(who);
   }
-  a.shares = (int)paged_shares(a.p.H, paged_waves<C, W>());
+  a.shares = (int)paged_shares(a.p.H, a.rows, W, paged_waves<C, W>());
   a.by_shares = fast_div(a.shares);
   a.least = least_share<E>() >> a.step_log;
   const int64_t steps = a.B * ((capacity + PageTile<C, W>::KS - 1) >> a.step_log);
   if (a.shares > (steps + a.least - 1) / a.least) a.shares = (int)((steps + a.least - 1) / a.least), a.by_shares = fast_div(a.shares);
   const int gx = (a.shares * a.p.H + kPagedWaves - 1) / kPagedWaves;
   const dim3 grid((unsigned)gx, groups);
-  if (two) launch_kernel<paged_decode_kernel<C, E, W, WIDE ? 1 : 2, ROWS, false>>(grid, dim3(64 * kPagedWaves), 0, s, a);
+  if (two) launch_kernel<paged_decode_kernel<C, E, W, NRB, ROWS, false>>(grid, dim3(64 * kPagedWaves), 0, s, a);
   else launch_kernel<paged_decode_kernel<C, E, W, 1, ROWS, false>>(grid, dim3(64 * kPagedWaves), 0, s, a);
   int rc = check_launch(who);
   if (rc) return rc;
@@ -951,7 +962,7 @@ extern "C" int pjx_paged_decode(int dtype, int cache_dtype, const void* q, const
   a.by_t = fast_div(q_len);
   a.cx = sm_scale * kLog2e;
   a.ws_o = (float*)workspace;
-  a.ws_ml = a.ws_o + paged_parts(batch, kv_heads) * kv_heads * rows * paged_width(head_dim);
+  a.ws_ml = a.ws_o + paged_parts(batch, kv_heads, rows, head_dim) * kv_heads * rows * paged_width(head_dim);
   if (f32) return quant ? run_paged<E4m3Fmt, F32Fmt>(a, s, who) : run_paged<F32Fmt, F32Fmt>(a, s, who);
   if (dtype == PJX_DTYPE_BF16) return quant ? run_paged<E4m3Fmt, Bf16Fmt>(a, s, who) : run_paged<Bf16Fmt, Bf16Fmt>(a, s, who);
   return quant ? run_paged<E4m3Fmt, F16Fmt>(a, s, who) : run_paged<F16Fmt, F16Fmt>(a, s, who);
