@@ -671,8 +671,8 @@ typedef struct pjx_pages {
  * (below 0: 0; NULL: 0), as far as the sequence has room.  lengths_out [batch]: the
  * keys it has then, at most table_len * page_size.  Everything else in the pools
  * stays.  Two tokens of one call must not name the same slot (sequences that share
- * the page they write to).  dtype: of k and v; cache_dtype: dtype (copied) or
- * PJX_DTYPE_E4M3.
+ * the page they write to), k and v not overlap the pools, lengths_out not be one of
+ * the other lengths.  dtype: of k and v; cache_dtype: dtype (copied) or PJX_DTYPE_E4M3.
  */
 int pjx_write_pages(int dtype, int cache_dtype, const void* k, const void* v, const pjx_pages* cache,
                     const int32_t* kv_lengths, const int32_t* new_lengths, int32_t* lengths_out, int64_t batch,
@@ -682,7 +682,7 @@ int pjx_write_pages(int dtype, int cache_dtype, const void* k, const void* v, co
  * Gathers the first out_len keys and values of every sequence into contiguous
  * [batch, out_len, kv_heads, head_dim] tensors of dtype (the cache's, or of e4m3 any):
  * code * 2^(exponent - 127) rounded once.  Zeros from kv_lengths[b] (NULL: all it has
- * room for) on.
+ * room for) on, and of missing pages.
  */
 int pjx_read_pages(int dtype, int cache_dtype, const pjx_pages* cache, const int32_t* kv_lengths, void* k_out,
                    void* v_out, int64_t batch, int64_t out_len, int64_t kv_heads, int64_t head_dim, void* stream);
@@ -696,7 +696,9 @@ int pjx_read_pages(int dtype, int cache_dtype, const pjx_pages* cache, const int
  * and LSE +inf.  dtype of q and o; cache_dtype: dtype or PJX_DTYPE_E4M3.  lse:
  * optional fp32 [batch, Hq, q_len], natural log.  q, o contiguous, on 16 bytes.
  * workspace: on 16 bytes, at least pjx_paged_decode_workspace_size(batch, kv_heads,
- * (Hq / kv_heads) * q_len, table_len * page_size, head_dim) bytes.
+ * (Hq / kv_heads) * q_len, table_len * page_size, head_dim) bytes, undefined before and
+ * after; calls at the same time need one each.  At most 2^34 keys of room over the
+ * batch, 2^19 rows ((Hq / kv_heads) * q_len), 2^22 batch * kv_heads.
  */
 size_t pjx_paged_decode_workspace_size(int64_t batch, int64_t kv_heads, int64_t rows, int64_t capacity,
                                        int64_t head_dim);

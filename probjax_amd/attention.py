@@ -787,10 +787,11 @@ class PagedCache:
     v_exponents: torch.Tensor | None = None
 
     def __post_init__(self):
-        index, pages, unwritable = hip.pages_struct(self.k, self.v, self.page_table, self.k_exponents, self.v_exponents)
+        index, pages, unwritable, storages = hip.pages_struct(self.k, self.v, self.page_table, self.k_exponents,
+                                                              self.v_exponents)
         batch = self.k.shape[0] if self.page_table is None else self.page_table.shape[0]
-        for name, value in (("index", index), ("_pages", pages), ("unwritable", unwritable), ("batch", batch),
-                            ("code", hip.CACHE_DTYPES[self.k.dtype]), ("page_size", pages.page_size),
+        for name, value in (("index", index), ("_pages", pages), ("unwritable", unwritable), ("storages", storages),
+                            ("batch", batch), ("code", hip.CACHE_DTYPES[self.k.dtype]), ("page_size", pages.page_size),
                             ("kv_heads", self.k.shape[2]), ("head_dim", self.k.shape[3]),
                             ("capacity", pages.page_size * pages.table_len)):
             object.__setattr__(self, name, value)
@@ -818,7 +819,7 @@ def write_pages(cache: PagedCache, k, v, *, kv_lengths=None, new_lengths=None):
     quantised to 8 bits (no counterpart in the reference).
 
     ``k`` / ``v`` ``[B, T, Hkv, D]``, any strides (slices of a projection are read in
-    place).  Token t < ``new_lengths[b]`` (int ``[B]``, None: all T) becomes key
+    place; not slices of the pools).  Token t < ``new_lengths[b]`` (int ``[B]``, None: all T) becomes key
     ``kv_lengths[b] + t`` of sequence b (``kv_lengths`` int ``[B]``, the keys it has;
     None: none yet), as far as the sequence has room and a page for it; later tokens
     are padding.  Returns the sequences' lengths then (int32 ``[B]``, at most the
@@ -859,8 +860,8 @@ def paged_decode(q, cache: PagedCache, *, kv_lengths=None, sm_scale: float | Non
     pages.  What it does not see does not reach its output, infinities and NaN
     included; a token that sees nothing gets 0 and LSE +inf.  bf16, fp16 or fp32 over a
     cache of that type or of 8 bits; ``sm_scale`` defaults to ``1/sqrt(D)``.  With
-    ``return_lse`` also the natural-log LSE ``[B, Hq, T]``.  No gradient: inputs that
-    require one, or carry a tangent, raise.
+    ``return_lse`` also the natural-log LSE ``[B, Hq, T]``.  The batch may have room for
+    2^34 keys in all.  No gradient: inputs that require one, or carry a tangent, raise.
     """
     if sm_scale is None:
         sm_scale = 1.0 / math.sqrt(q.shape[-1])

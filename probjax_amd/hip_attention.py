@@ -1029,9 +1029,10 @@ CACHE_DTYPES = {**_DTYPES, torch.float8_e4m3fn: native.PJX_DTYPE_E4M3}
 
 
 def pages_struct(k, v, page_table, k_exponents, v_exponents):
-    """``(index, pjx_pages, unwritable)`` of a paged cache's tensors (see
+    """``(index, pjx_pages, unwritable, storages)`` of a paged cache's tensors (see
     ``PagedCache``), checked; the struct's pointers are the caller's to set on every
-    call (``set_pages``).  ``unwritable``: why ``write_pages`` cannot take it, or None."""
+    call (``set_pages``).  ``unwritable``: why ``write_pages`` cannot take it, or None;
+    ``storages``: addresses of the memory that k and v are views of."""
     if k.ndim != 4 or k.shape != v.shape or k.dtype is not v.dtype:
         raise ValueError(f"a paged cache's k and v must be [pages, page_size, Hkv, D] of one shape and dtype, got "
                          f"{tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}")
@@ -1071,7 +1072,8 @@ def pages_struct(k, v, page_table, k_exponents, v_exponents):
     # (an axis of one element has a stride of no meaning)
     strides = [x.stride(i) if x.shape[i] > 1 else 0 for x in (k, v) for i in range(3)]
     pages = native.Pages(None, None, None, None, None, step, most, P, page, *strides)
-    return index, pages, _unwritable([k, v] + [k_exponents, v_exponents] * quantised)
+    return (index, pages, _unwritable([k, v] + [k_exponents, v_exponents] * quantised),
+            (k.untyped_storage().data_ptr(), v.untyped_storage().data_ptr()))
 
 
 def _unwritable(ts):
@@ -1131,6 +1133,9 @@ def write_pages(cache, k, v, *, kv_lengths=None, new_lengths=None):
         raise ValueError("writing to a cache has no gradient: call it under torch.no_grad() or on detached tensors")
     index = _gpu(k, v, cache.k)
     k, v, strides = _new_rows(k, v)
+    for x in (k, v):
+        if x.untyped_storage().data_ptr() in cache.storages and (_share_bytes(x, cache.k) or _share_bytes(x, cache.v)):
+            raise ValueError("k and v must not share memory with the cache's pools")
     L, new = _key_lengths(kv_lengths, k, B), _key_lengths(new_lengths, k, B, "new_lengths")
     lengths = torch.empty((B,), dtype=torch.int32, device=k.device) if L is None else torch.empty_like(L)
     _call(

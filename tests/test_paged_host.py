@@ -137,6 +137,22 @@ def test_calls_that_are_refused(call, msg):
         call(cache())
 
 
+def test_new_rows_in_the_pools_are_refused(monkeypatch):
+    """What a launch would read and write in an open order; pools beside them are not."""
+    both = torch.zeros((PAGES, 3, PAGE, H, D), dtype=torch.bfloat16)
+    c = A.PagedCache(both[:, 0], both[:, 1], table())
+    flat = both.view(-1, H, D)
+    launched = []
+    monkeypatch.setattr(hip, "_call", lambda *args: launched.append(args))
+    for x in (both[:B, 0, :3], both[:B, 1, 1:4], flat[:10].view(B, 5, H, D)):
+        for k, v in ((x, torch.zeros_like(x)), (torch.zeros_like(x), x)):
+            with pytest.raises(ValueError, match="share memory"):
+                A.write_pages(c, k, v)
+    assert not launched
+    A.write_pages(c, both[:B, 2, :3], both[2:2 + B, 2, :3])
+    assert len(launched) == 1
+
+
 def test_reads_of_8_bits_name_a_float_type():
     with pytest.raises(ValueError, match="bfloat16, float16 or float32"):
         A.read_pages(cache(torch.float8_e4m3fn), dtype=torch.float8_e4m3fn)
