@@ -270,6 +270,28 @@ def test_nan_and_infinities_that_are_seen(device, name, held):
         assert torch.isnan(got[1]).all() and torch.isnan(lse[1]).all() and not torch.isnan(lse[0]).any()
 
 
+@pytest.mark.parametrize("name,held", [("bf16", "bf16"), ("f16", "e4m3"), ("f32", "f32")])
+def test_caches_without_a_page(device, name, held):
+    """No pool, no page of a sequence, no sequence: zeros, LSE +inf, lengths of 0."""
+    import torch
+    from probjax_amd.attention import PagedCache, paged_decode, read_pages, write_pages
+
+    dtype, pool = types()[name], types().get(held, torch.float8_e4m3fn)
+    for pages, shape in ((0, (2, 3)), (4, (2, 0)), (0, (2, 0)), (4, (0, 3)), (0, (0, 0))):
+        print(pages, shape, flush=True)
+        table = torch.zeros(shape, dtype=torch.int32, device=device)
+        cache = PagedCache.allocate(pages, 16, 2, 64, page_table=table, dtype=pool)
+        B = shape[0]
+        q = torch.full((B, 3, 4, 64), float("nan"), dtype=dtype, device=device)
+        out, lse = paged_decode(q, cache, return_lse=True)
+        k, v = read_pages(cache, length=20, dtype=dtype)
+        lengths = write_pages(cache, q[:, :, :2], q[:, :, 2:])
+        torch.cuda.synchronize()
+        assert out.shape == q.shape and not out.any() and torch.isposinf(lse).all() and lse.shape == (B, 4, 3)
+        assert k.shape == v.shape == (B, 20, 2, 64) and not k.any() and not v.any()
+        assert lengths.tolist() == [min(3, cache.capacity)] * B
+
+
 def test_contiguous_caches_and_views(device):
     """Without a table: page b is sequence b's; one sequence shared by the batch; the
     table a slice of a wider one; equal to the split-KV decode's result within both's
