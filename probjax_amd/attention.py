@@ -796,6 +796,9 @@ class PagedCache:
                             ("capacity", pages.page_size * pages.table_len)):
             object.__setattr__(self, name, value)
 
+    def __reduce__(self):
+        return type(self), (self.k, self.v, self.page_table, self.k_exponents, self.v_exponents)
+
     @classmethod
     def allocate(cls, pages: int, page_size: int, kv_heads: int, head_dim: int, *, page_table=None,
                  dtype=torch.bfloat16, device=None):

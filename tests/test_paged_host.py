@@ -1,6 +1,7 @@
 """What the paged cache and its operators take and refuse, and where they launch (host
 logic: devices, streams and launches are stubs, no GPU needed)."""
 
+import copy
 import dataclasses
 
 import pytest
@@ -54,6 +55,21 @@ def test_allocate():
     c = A.PagedCache.allocate(PAGES, PAGE, H, D, page_table=table(), dtype=torch.float8_e4m3fn)
     assert c.k.dtype is torch.float8_e4m3fn and c.k_exponents.shape == (PAGES, H, PAGE) and c.unwritable is None
     assert A.PagedCache.allocate(B, 100, H, D, device="cpu").capacity == 100
+
+
+def test_copies(tmp_path):
+    """A cache is copied, and saved, as its tensors are."""
+    c = cache(torch.float8_e4m3fn)
+    same, other = copy.copy(c), copy.deepcopy(c)
+    assert same.k is c.k and other.k is not c.k
+    st = other.pages()
+    assert (st.k, st.v_exponents, st.table) == (other.k.data_ptr(), other.v_exponents.data_ptr(), other.page_table.data_ptr())
+    pair = torch.zeros((2, PAGES, PAGE, H, D), dtype=torch.bfloat16)
+    both = copy.deepcopy(A.PagedCache(*pair, table()))
+    assert both.unwritable is None and both.v.data_ptr() - both.k.data_ptr() == 2 * both.k.numel()
+    torch.save(c, tmp_path / "cache")
+    back = torch.load(tmp_path / "cache", weights_only=False)
+    assert back.capacity == c.capacity and back.k.dtype is c.k.dtype and torch.equal(back.page_table, c.page_table)
 
 
 def _offset(t):
