@@ -11,7 +11,7 @@
 // share that runs into the next sequence leaves a partial result and goes on; a second
 // kernel joins the parts of a sequence.  What a share is follows from the lengths, which
 // only the device knows: every wave works it out from all of them, so a grid made for the
-// capacity, or captured once, is shared by whatever keys there are.  A workgroup's four
+// capacity, or captured once, is shared by whatever keys there are.  A workgroup's
 // waves are neighbouring heads on the same keys, so rows that lie side by side are read
 // side by side (8-bit rows of 64 features, [page, H, D]: 43 us against 58 as workgroups of
 // their own).
@@ -37,7 +37,6 @@
 
 namespace pjx {
 
-constexpr int kPagedWaves = 4;
 // Keys of a share at least: two steps, but of float32 one, whose products take as long as
 // its loads (512 keys of 4 heads of 64: 9.1 us against 10.6; bf16 heads of 128 11.3 against
 // 10.9).
@@ -253,6 +252,14 @@ template <typename C, int W>
 constexpr int paged_waves() {
   return W * fmt_size<C>() >= 128 ? 4 : 8;
 }
+constexpr int kPagedWaves = 8;  // of a compute unit at most
+// Waves of a workgroup: those of rows that together make up 512 bytes and more of a token,
+// if its heads lie side by side (64 features in 8 bits, 32 x 512-8192 keys: 36 us with eight, 38 with four,
+// 45 with two).
+template <typename C, int W>
+constexpr int paged_group() {
+  return W * fmt_size<C>() >= 128 ? 4 : 8;
+}
 // Waves of a SIMD that the registers are to leave room for (256 features, and float32 sums
 // of more than 64, need more than half of them).
 template <typename C, typename E, int W>
@@ -275,7 +282,7 @@ __device__ const __attribute__((aligned(16))) uint32_t kZeros[4] = {};
 // takes one sequence's keys for a KV head, an equal number of steps to each of its waves,
 // and joins them itself.
 template <typename C, typename E, int W, int NRB, bool ROWS, bool WHOLE>
-__global__ __launch_bounds__(64 * (WHOLE ? paged_whole_waves<C, E, W, NRB>() : kPagedWaves), (paged_occupancy<C, E, W>())) void paged_decode_kernel(PagedArgs a) {
+__global__ __launch_bounds__(64 * (WHOLE ? paged_whole_waves<C, E, W, NRB>() : paged_group<C, W>()), (paged_occupancy<C, E, W>())) void paged_decode_kernel(PagedArgs a) {
   using T = PageTile<C, W>;
   constexpr bool F32 = std::is_same<E, F32Fmt>::value, QUANT = std::is_same<C, E4m3Fmt>::value;
   // The weights enter their product with V in 16 bits, in two parts: rounded to the type,
@@ -285,7 +292,7 @@ __global__ __launch_bounds__(64 * (WHOLE ? paged_whole_waves<C, E, W, NRB>() : k
   typedef typename std::conditional<QUANT && !F32, Bf16Fmt, E>::type EV;
   constexpr int KS = T::KS, KB = KS / 16, NL = T::NL, CS = T::CS, ES = fmt_size<E>();
   constexpr int NDB = W / 16;
-  constexpr int NW = WHOLE ? paged_whole_waves<C, E, W, NRB>() : kPagedWaves;
+  constexpr int NW = WHOLE ? paged_whole_waves<C, E, W, NRB>() : paged_group<C, W>();
   __shared__ __attribute__((aligned(1024))) unsigned char k_lds[NW * T::BYTES];
   __shared__ __attribute__((aligned(1024))) unsigned char v_lds[NW * T::BYTES];
   __shared__ __attribute__((aligned(16))) uint64_t rows_lds[NW * 64];  // addresses of a step's K, V rows
@@ -864,12 +871,12 @@ static int64_t paged_shares(int64_t kv_heads, int64_t rows, int64_t head_dim, in
 }
 // Parts of a KV head at most: one of every share, and one more where a sequence begins.
 static int64_t paged_parts(int64_t batch, int64_t kv_heads, int64_t rows, int64_t head_dim) {
-  return paged_shares(kv_heads, rows, head_dim, 2 * kPagedWaves) + batch;
+  return paged_shares(kv_heads, rows, head_dim, kPagedWaves) + batch;
 }
 static size_t paged_ws(int64_t batch, int64_t kv_heads, int64_t rows, int64_t head_dim) {
   return (size_t)(paged_parts(batch, kv_heads, rows, head_dim) * kv_heads * rows * (paged_width(head_dim) + 2)) * sizeof(float) + 16;
 }
-static_assert(paged_waves<Bf16Fmt, 64>() <= 2 * kPagedWaves && paged_waves<E4m3Fmt, 64>() <= 2 * kPagedWaves,
+static_assert(paged_waves<Bf16Fmt, 64>() <= kPagedWaves && paged_waves<E4m3Fmt, 64>() <= kPagedWaves,
               "paged_parts counts the shares of so many waves");
 
 // Whether a workgroup takes a sequence whole, and nothing is joined after it: where one
@@ -898,10 +905,10 @@ static int run_paged(PagedArgs& a, hipStream_t s, const char* who) {
   a.least = least_share<E>() >> a.step_log;
   const int64_t steps = a.B * ((capacity + PageTile<C, W>::KS - 1) >> a.step_log);
   if (a.shares > (steps + a.least - 1) / a.least) a.shares = (int)((steps + a.least - 1) / a.least), a.by_shares = fast_div(a.shares);
-  const int gx = (a.shares * a.p.H + kPagedWaves - 1) / kPagedWaves;
+  const int group = paged_group<C, W>(), gx = (a.shares * a.p.H + group - 1) / group;
   const dim3 grid((unsigned)gx, groups);
-  if (two) launch_kernel<paged_decode_kernel<C, E, W, NRB, ROWS, false>>(grid, dim3(64 * kPagedWaves), 0, s, a);
-  else launch_kernel<paged_decode_kernel<C, E, W, 1, ROWS, false>>(grid, dim3(64 * kPagedWaves), 0, s, a);
+  if (two) launch_kernel<paged_decode_kernel<C, E, W, NRB, ROWS, false>>(grid, dim3(64 * group), 0, s, a);
+  else launch_kernel<paged_decode_kernel<C, E, W, 1, ROWS, false>>(grid, dim3(64 * group), 0, s, a);
   int rc = check_launch(who);
   if (rc) return rc;
   // Sequences of more than one part, or of none.  Threads enough that each takes up to 8
