@@ -254,8 +254,8 @@ constexpr int paged_waves() {
 }
 constexpr int kPagedWaves = 8;  // of a compute unit at most
 // Waves of a workgroup: those of rows that together make up 512 bytes and more of a token,
-// if its heads lie side by side (64 features in 8 bits, 32 x 512-8192 keys: 36 us with eight, 38 with four,
-// 45 with two).
+// if its heads lie side by side (64 features in 8 bits, 32 x 512-8192 keys: 36 us with
+// eight, 38 with four, 45 with two).
 template <typename C, int W>
 constexpr int paged_group() {
   return W * fmt_size<C>() >= 128 ? 4 : 8;
