@@ -143,6 +143,23 @@ def test_lengths_of_every_kind(device, name, held, B, S):
     run(device, cache, table, [0] * B, q, dtype, "no keys")
 
 
+@pytest.mark.parametrize("name,held,H,T,D,S", [("bf16", "e4m3", 16, 1040, 256, 300), ("f32", "f32", 32, 1100, 64, 600),
+                                               ("f16", "f16", 6, 333, 128, 900)])
+def test_prompts_of_many_rows(device, name, held, H, T, D, S):
+    """So many groups of rows that a wave has all sequences' keys to itself (the first
+    two), or a few have; tokens with no key, more tokens than keys."""
+    import torch
+
+    B, page, dtype = 3, 20, types()[name]
+    rng = np.random.default_rng(T)
+    N = -(-S // page)
+    lengths = [S, 0, S // 2]
+    table = make_table(rng, B, N, B * N, lengths, page)
+    cache = make_cache(device, rng, held, B * N, page, H, D, table)
+    q = torch.from_numpy(rng.standard_normal((B, T, H, D), dtype=np.float32)).to(device, dtype)
+    run(device, cache, table, lengths, q, dtype)
+
+
 def _spoil(pool, at, value):
     """Sets one feature of every head in slot ``at = (page, slot)``."""
     import torch
