@@ -338,11 +338,15 @@ static int tokens_of(int64_t per_token, int passes) {
   return (int)std::max<int64_t>((int64_t)passes * kPageThreads / per_token, 1);
 }
 
+// Whether a launch's 32 bits count the threads of so many workgroups.
+static bool countable(int64_t workgroups) { return workgroups * kPageThreads <= 0xffffffffLL; }
+
 template <typename E, bool QUANT, int LPR>
 static int run_write(WriteArgs& a, hipStream_t s, const char* who) {
   a.tokens = tokens_of((int64_t)a.p.H * LPR, 4);
-  const unsigned x = (unsigned)std::max((a.T + a.tokens - 1) / a.tokens, 1);
-  launch_kernel<write_pages_kernel<E, QUANT, LPR>>(dim3(x, (unsigned)std::min(a.B, 65535), 2), dim3(kPageThreads), 0, s, a);
+  const int64_t x = std::max<int64_t>(((int64_t)a.T + a.tokens - 1) / a.tokens, 1);
+  if (!countable(x)) return fail(PJX_ERR_INVALID, "pjx_write_pages: too many new tokens");
+  launch_kernel<write_pages_kernel<E, QUANT, LPR>>(dim3((unsigned)x, (unsigned)std::min(a.B, 65535), 2), dim3(kPageThreads), 0, s, a);
   return check_launch(who);
 }
 
@@ -368,7 +372,9 @@ static int run_read(ReadArgs& a, hipStream_t s, const char* who) {
   a.tokens = tokens_of(per_token, stream ? 8 : 4);
   a.by_token = fast_div(per_token);
   a.by_row = fast_div(a.upr);
-  const dim3 grid((unsigned)((a.L + a.tokens - 1) / a.tokens), (unsigned)std::min(a.B, 65535), 2);
+  const int64_t x = (a.L + a.tokens - 1) / a.tokens;
+  if (!countable(x)) return fail(PJX_ERR_INVALID, "pjx_read_pages: out_len is too long");
+  const dim3 grid((unsigned)x, (unsigned)std::min(a.B, 65535), 2);
   if (stream) launch_kernel<read_pages_kernel<C, E, true>>(grid, dim3(kPageThreads), 0, s, a);
   else launch_kernel<read_pages_kernel<C, E, false>>(grid, dim3(kPageThreads), 0, s, a);
   return check_launch(who);

@@ -93,6 +93,13 @@ def test_write_pages(lib, over, msg):
     refused(lib, "pjx_write_pages", _write(**over), msg)
 
 
+def test_more_than_a_launch_counts(lib):
+    wide = dict(H=256, T=1 << 30, strides=native.CacheStrides(0, 0, 64, 0, 0, 64))
+    refused(lib, "pjx_write_pages", _write(**wide), "too many new tokens")
+    refused(lib, "pjx_write_pages", _write(held=BF16, cache=pages(k_exponents=None), **wide), "too many new tokens")
+    refused(lib, "pjx_read_pages", _read(H=256, L=1 << 30), "too long")
+
+
 @pytest.mark.parametrize("over,msg", [(dict(L=-1), "out of range"), (dict(k=None), "null"), (dict(v=P(4)), "16 bytes")])
 def test_read_pages(lib, over, msg):
     refused(lib, "pjx_read_pages", _read(**over), msg)
