@@ -699,6 +699,8 @@ int pjx_read_pages(int dtype, int cache_dtype, const pjx_pages* cache, const int
  * (Hq / kv_heads) * q_len, table_len * page_size, head_dim) bytes, undefined before and
  * after; calls at the same time need one each.  At most 2^34 keys of room over the
  * batch, 2^19 rows ((Hq / kv_heads) * q_len), 2^22 batch * kv_heads.
+ * The same call gives the same bits; where a sequence's sums are cut follows from the
+ * lengths of all.
  */
 size_t pjx_paged_decode_workspace_size(int64_t batch, int64_t kv_heads, int64_t rows, int64_t capacity,
                                        int64_t head_dim);

@@ -864,7 +864,9 @@ def paged_decode(q, cache: PagedCache, *, kv_lengths=None, sm_scale: float | Non
     included; a token that sees nothing gets 0 and LSE +inf.  bf16, fp16 or fp32 over a
     cache of that type or of 8 bits; ``sm_scale`` defaults to ``1/sqrt(D)``.  With
     ``return_lse`` also the natural-log LSE ``[B, Hq, T]``.  The batch may have room for
-    2^34 keys in all.  No gradient: inputs that require one, or carry a tangent, raise.
+    2^34 keys in all.  The same call gives the same bits; where a sequence's sums are cut
+    follows from all lengths, so its last bits may differ next to other sequences.  No
+    gradient: inputs that require one, or carry a tangent, raise.
     """
     if sm_scale is None:
         sm_scale = 1.0 / math.sqrt(q.shape[-1])

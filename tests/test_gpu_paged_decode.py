@@ -160,6 +160,26 @@ def test_prompts_of_many_rows(device, name, held, H, T, D, S):
     run(device, cache, table, lengths, q, dtype)
 
 
+@pytest.mark.parametrize("held,S", [("bf16", 200), ("bf16", 3000), ("e4m3", 3000)])
+def test_the_same_call_gives_the_same_bits(device, held, S):
+    import torch
+    from probjax_amd.attention import paged_decode
+
+    B, H, D, page = 9, 4, 128, 16
+    rng = np.random.default_rng(S)
+    N = -(-S // page)
+    lengths = [S] + [int(x) for x in rng.integers(0, S + 1, B - 1)]
+    table = make_table(rng, B, N, B * N, lengths, page)
+    cache = make_cache(device, rng, held, B * N, page, H, D, table)
+    q = torch.from_numpy(rng.standard_normal((B, 2, 4 * H, D), dtype=np.float32)).to(device, torch.bfloat16)
+    L = torch.tensor(lengths, dtype=torch.int32, device=device)
+    first = paged_decode(q, cache, kv_lengths=L, return_lse=True)
+    for _ in range(20):
+        again = paged_decode(q, cache, kv_lengths=L, return_lse=True)
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(first, again))
+
+
 def _spoil(pool, at, value):
     """Sets one feature of every head in slot ``at = (page, slot)``."""
     import torch
