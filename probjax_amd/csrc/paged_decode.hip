@@ -208,18 +208,30 @@ __device__ __forceinline__ uint32_t bits_of(float x) {
   return u;
 }
 
-// Whether any element of a dword of C is infinite or NaN.
-template <typename C>
-__device__ __forceinline__ bool odd_dword(uint32_t x) {
+// Whether any element of N x 4 dwords of floats C is infinite or NaN.
+template <typename C, int N>
+__device__ __forceinline__ bool any_odd(const u32x4 (&x)[N]) {
   if constexpr (std::is_same<C, F32Fmt>::value) {
-    return (x & 0x7f800000u) == 0x7f800000u;
-  } else if constexpr (std::is_same<C, E4m3Fmt>::value) {
-    const uint32_t y = ~x & 0x7f7f7f7fu;  // a byte is 0 where the code is NaN
-    return ((y - 0x01010101u) & ~y & 0x80808080u) != 0u;
-  } else {
-    constexpr uint32_t ex = C::kF16 ? 0x7c00u : 0x7f80u;
-    return (x & ex) == ex || (x & (ex << 16)) == ex << 16;
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) odd |= (x[i][e] & 0x7f800000u) == 0x7f800000u;
+    return odd;
+  } else {  // by the largest magnitude, two elements at a time
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    u16x2 m = {0, 0};
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, x[i][e] & 0x7fff7fffu));
+    return max((uint32_t)m[0], (uint32_t)m[1]) >= (C::kF16 ? 0x7c00u : 0x7f80u);
   }
+}
+// Whether any of a dword's 4 codes is NaN.
+__device__ __forceinline__ bool odd_codes(uint32_t x) {
+  const uint32_t y = ~x & 0x7f7f7f7fu;  // a byte is 0 where the code is NaN
+  return ((y - 0x01010101u) & ~y & 0x80808080u) != 0u;
 }
 
 // 8 codes as an operand of E (bf16 or fp16).
@@ -572,23 +584,23 @@ __global__ __launch_bounds__(64 * (WHOLE ? paged_whole_waves<C, E, W, NRB>() : p
       }
     }
 
+    // An infinity or NaN must not reach the rows that do not see its key.  In the rows that
+    // do, the two parts of a 16-bit weight would make a NaN of an infinity (0 or less times
+    // it, from the second part), so 16 bits are looked at in every step.
     bool apart = false;
-    if (!whole) {  // (an infinity or NaN must not reach the rows that do not see its key)
-      bool odd = false;
-      if constexpr (F32 && QUANT) {
+    if constexpr (QUANT) {
+      if (!whole) {
+        bool odd = false;
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
+        for (int i = 0; i < (F32 ? KB * NDB : NDB); ++i) {
+          if (F32 && i % 4) continue;  // (four blocks' codes are in the first's dwords)
 #pragma unroll
-          for (int i = 0; i < NDB / 4; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) odd |= odd_dword<C>(vf[kb * NDB + i * 4][e]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < (F32 ? KB * NDB : NDB); ++i)
-#pragma unroll
-          for (int e = 0; e < (QUANT ? 2 : 4); ++e) odd |= odd_dword<C>(vf[i][e]);
+          for (int e = 0; e < (F32 ? 4 : 2); ++e) odd |= odd_codes(vf[i][e]);
+        }
+        apart = wave_any(odd);
       }
-      apart = wave_any(odd);
+    } else if (!F32 || !whole) {
+      apart = wave_any(any_odd<C>(vf));
     }
     if (apart) {
       // one key after the other, for the rows that see it
