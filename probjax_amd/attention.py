@@ -774,7 +774,8 @@ class PagedCache:
     ``[B, S, Hkv, D]``.
 
     The tensors are used in place; their contents, the table's too, may change between
-    calls.  ``dataclasses.replace(cache, page_table=...)`` is the same pools for other
+    calls.  One that was given other memory or another layout (``Tensor.set_``) is checked
+    and taken as it is then.  ``dataclasses.replace(cache, page_table=...)`` is the same pools for other
     sequences.  Pools that are expanded, or share memory with each other, can be read
     and attended over, not written to.  How many keys each sequence has is the caller's to keep: what
     ``write_pages`` returns.
@@ -787,11 +788,12 @@ class PagedCache:
     v_exponents: torch.Tensor | None = None
 
     def __post_init__(self):
-        index, pages, unwritable, storages = hip.pages_struct(self.k, self.v, self.page_table, self.k_exponents,
-                                                              self.v_exponents)
+        tensors = self.k, self.v, self.page_table, self.k_exponents, self.v_exponents
+        index, pages, unwritable, storages = hip.pages_struct(*tensors)
         batch = self.k.shape[0] if self.page_table is None else self.page_table.shape[0]
         for name, value in (("index", index), ("_pages", pages), ("unwritable", unwritable), ("storages", storages),
-                            ("batch", batch), ("code", hip.CACHE_DTYPES[self.k.dtype]), ("page_size", pages.page_size),
+                            ("_state", hip.pages_state(*tensors)), ("batch", batch),
+                            ("code", hip.CACHE_DTYPES[self.k.dtype]), ("page_size", pages.page_size),
                             ("kv_heads", self.k.shape[2]), ("head_dim", self.k.shape[3]),
                             ("capacity", pages.page_size * pages.table_len)):
             object.__setattr__(self, name, value)
@@ -813,8 +815,12 @@ class PagedCache:
         return cls(k, v, page_table, *exponents)
 
     def pages(self):
-        """The tensors as the C entry points take them (``pjx_pages``)."""
-        return hip.set_pages(self._pages, self.k, self.v, self.page_table, self.k_exponents, self.v_exponents)
+        """The tensors as the C entry points take them (``pjx_pages``); checked again, and
+        what the cache knows of them taken anew, if they were given other memory, sizes or
+        strides (``Tensor.set_``, ``Tensor.data``) since the last call."""
+        if hip.pages_state(self.k, self.v, self.page_table, self.k_exponents, self.v_exponents) != self._state:
+            self.__post_init__()
+        return self._pages
 
 
 def write_pages(cache: PagedCache, k, v, *, kv_lengths=None, new_lengths=None):

@@ -1030,8 +1030,7 @@ CACHE_DTYPES = {**_DTYPES, torch.float8_e4m3fn: native.PJX_DTYPE_E4M3}
 
 def pages_struct(k, v, page_table, k_exponents, v_exponents):
     """``(index, pjx_pages, unwritable, storages)`` of a paged cache's tensors (see
-    ``PagedCache``), checked; the struct's pointers are the caller's to set on every
-    call (``set_pages``).  ``unwritable``: why ``write_pages`` cannot take it, or None;
+    ``PagedCache``), checked.  ``unwritable``: why ``write_pages`` cannot take it, or None;
     ``storages``: addresses of the memory that k and v are views of."""
     if k.ndim != 4 or k.shape != v.shape or k.dtype is not v.dtype:
         raise ValueError(f"a paged cache's k and v must be [pages, page_size, Hkv, D] of one shape and dtype, got "
@@ -1071,7 +1070,8 @@ def pages_struct(k, v, page_table, k_exponents, v_exponents):
     index = _gpu(k, v, page_table, k_exponents, v_exponents)
     # (an axis of one element has a stride of no meaning)
     strides = [x.stride(i) if x.shape[i] > 1 else 0 for x in (k, v) for i in range(3)]
-    pages = native.Pages(None, None, None, None, None, step, most, P, page, *strides)
+    pages = native.Pages(k.data_ptr(), v.data_ptr(), _ptr(k_exponents), _ptr(v_exponents), _ptr(page_table), step, most,
+                         P, page, *strides)
     return (index, pages, _unwritable([k, v] + [k_exponents, v_exponents] * quantised),
             (k.untyped_storage().data_ptr(), v.untyped_storage().data_ptr()))
 
@@ -1093,12 +1093,15 @@ def _unwritable(ts):
     return None
 
 
-def set_pages(pages, k, v, page_table, k_exponents, v_exponents):
-    """``pages`` with the tensors' addresses."""
-    pages.k, pages.v, pages.table = k.data_ptr(), v.data_ptr(), _ptr(page_table)
+def pages_state(k, v, page_table, k_exponents, v_exponents):
+    """What of a paged cache's tensors ``pages_struct`` goes by, to compare with later.
+    (The exponents' one shape follows from the pools'.)"""
+    state = (k.data_ptr(), v.data_ptr(), k.shape, v.shape, k.stride(), v.stride(), k.dtype, v.dtype)
+    if page_table is not None:
+        state += page_table.data_ptr(), page_table.shape, page_table.stride()
     if k_exponents is not None:
-        pages.k_exponents, pages.v_exponents = k_exponents.data_ptr(), v_exponents.data_ptr()
-    return pages
+        state += k_exponents.data_ptr(), v_exponents.data_ptr()
+    return state
 
 
 def _new_rows(k, v):
@@ -1121,6 +1124,7 @@ def write_pages(cache, k, v, *, kv_lengths=None, new_lengths=None):
         raise ValueError(f"k and v must be [B, T, Hkv, D] of one shape and dtype, got {tuple(k.shape)} {k.dtype} and "
                          f"{tuple(v.shape)} {v.dtype}")
     B, T, H, D = k.shape
+    pages = cache.pages()
     if B != cache.batch or H != cache.kv_heads or D != cache.head_dim:
         raise ValueError(f"k {tuple(k.shape)} does not fit a cache of {cache.batch} sequences, {cache.kv_heads} heads of "
                          f"{cache.head_dim}")
@@ -1139,7 +1143,7 @@ def write_pages(cache, k, v, *, kv_lengths=None, new_lengths=None):
     L, new = _key_lengths(kv_lengths, k, B), _key_lengths(new_lengths, k, B, "new_lengths")
     lengths = torch.empty((B,), dtype=torch.int32, device=k.device) if L is None else torch.empty_like(L)
     _call(
-        index, native.load().pjx_write_pages, code, cache.code, k.data_ptr(), v.data_ptr(), cache.pages(), _ptr(L),
+        index, native.load().pjx_write_pages, code, cache.code, k.data_ptr(), v.data_ptr(), pages, _ptr(L),
         _ptr(new), lengths.data_ptr(), B, T, H, D, strides,
     )
     return lengths
@@ -1148,7 +1152,7 @@ def write_pages(cache, k, v, *, kv_lengths=None, new_lengths=None):
 def read_pages(cache, *, kv_lengths=None, length: int | None = None, dtype=None):
     """``pjx_read_pages``: the first ``length`` keys and values of every sequence of a
     ``PagedCache`` -> ``(k, v)`` ``[B, length, Hkv, D]``, zeros behind ``kv_lengths``."""
-    k = cache.k
+    pages, k = cache.pages(), cache.k
     if dtype is None:
         dtype = torch.bfloat16 if cache.code == native.PJX_DTYPE_E4M3 else k.dtype
     if dtype not in _DTYPES or (cache.code != native.PJX_DTYPE_E4M3 and dtype is not k.dtype):
@@ -1162,7 +1166,7 @@ def read_pages(cache, *, kv_lengths=None, length: int | None = None, dtype=None)
     k_out = k.new_empty((B, length, H, D), dtype=dtype)
     v_out = torch.empty_like(k_out)
     _call(
-        cache.index, native.load().pjx_read_pages, _DTYPES[dtype], cache.code, cache.pages(), _ptr(L),
+        cache.index, native.load().pjx_read_pages, _DTYPES[dtype], cache.code, pages, _ptr(L),
         k_out.data_ptr(), v_out.data_ptr(), B, length, H, D,
     )
     return k_out, v_out
@@ -1174,7 +1178,7 @@ def paged_decode(q, cache, *, sm_scale: float, kv_lengths=None, return_lse: bool
     if q.ndim != 4:
         raise ValueError(f"paged attention: q must be [B, T, Hq, D], got {tuple(q.shape)}")
     B, T, Hq, D = q.shape
-    H = cache.kv_heads
+    pages, H = cache.pages(), cache.kv_heads
     if B != cache.batch or D != cache.head_dim or Hq < 1 or Hq % H or T < 1:
         raise ValueError(f"paged attention: q {tuple(q.shape)} does not fit a cache of {cache.batch} sequences, {H} "
                          f"heads of {cache.head_dim}")
@@ -1192,7 +1196,7 @@ def paged_decode(q, cache, *, sm_scale: float, kv_lengths=None, return_lse: bool
     o = torch.empty_like(q)
     lse = torch.empty((B, Hq, T), dtype=torch.float32, device=q.device) if return_lse else None
     _call(
-        index, lib.pjx_paged_decode, code, cache.code, q.data_ptr(), cache.pages(), _ptr(L), o.data_ptr(),
+        index, lib.pjx_paged_decode, code, cache.code, q.data_ptr(), pages, _ptr(L), o.data_ptr(),
         _ptr(lse), ws.data_ptr(), nbytes, B, T, Hq, H, D, sm_scale,
     )
     return (o, lse) if return_lse else o
