@@ -31,15 +31,22 @@
 // The hint on the loads that rows are not read again (nt) matters most: 98 us against 165
 // without it behind other work that filled the caches (8 bits 63 against 106), though a
 // cache of 67-84 MB read over and over by itself would take 24-31 us for 30-33 without.
+// With several groups of rows, each of which reads all keys, it is mixed: 128 rows (four
+// groups of 32) of 4 KV heads of 128, 32 x 512-8192 bf16 keys, 124 us with it and 132
+// without, 128 rows of 256 features (eight groups of 16, 587 MB) 438 and 309.
 #include <stdio.h>
 
 #include "pages.h"
 
 namespace pjx {
 
-// Keys of a share at least: two steps, but of float32 one, whose products take as long as
-// its loads (512 keys of 4 heads of 64: 9.1 us against 10.6; bf16 heads of 128 11.3 against
-// 10.9).
+// Keys of a share at least: 64, but of float32 tokens 32 (a step; of a float32 cache's rows
+// of 256 features two), since their products take as long as the loads.  It counts where
+// there are few keys.  512 keys, 16 query on 4 KV heads of 64 / 128 / 256, us in a captured
+// graph with 32 and with 64: float32 8.6, 10.0 / 11.0, 13.5 / 14.7, 20.1; float32 over 8
+// bits 10.1, 12.7 / 10.5, 13.2 / 14.5, 19.7; bf16 7.5, 8.2 / 8.3, 9.4 / 10.2, 11.5; bf16
+// over 8 bits 8.0, 9.0 / 8.2, 9.1 / 9.5, 10.7.  So one step would be faster in 16 bits too,
+// by 1 us of a call that the host takes 11 for.
 template <typename E>
 constexpr int least_share() {
   return std::is_same<E, F32Fmt>::value ? 32 : 64;
@@ -258,8 +265,9 @@ __device__ __forceinline__ f32x4 codes4(uint32_t w) {
 
 // Waves of a compute unit at a time: four, one to a SIMD and with 64 rows each on their
 // way, keep the memory busy from rows of 128 bytes on (32 x 512-8192 keys of 8 heads of 128
-// in 8 bits: 51 us with four, 54 with eight, 57 and more where units hold different numbers
-// of them); eight on shorter ones (64 features in 8 bits: 30 us against 40).
+// in 8 bits: 51 us with four, 53 with eight, 57 and more where units hold different numbers
+// of them); eight on shorter ones (the same of 64 features: 34 us against 51, head-major
+// pages 31 against 49).
 template <typename C, int W>
 constexpr int paged_waves() {
   return W * fmt_size<C>() >= 128 ? 4 : 8;
@@ -916,10 +924,24 @@ static_assert(paged_waves<Bf16Fmt, 64>() <= kPagedWaves && paged_waves<E4m3Fmt, 
               "paged_parts counts the shares of so many waves");
 
 // Whether a workgroup takes a sequence whole, and nothing is joined after it: where one
-// compute unit has little enough to read (by itself it reads some 40 GB/s).  us, shares and
-// join / whole: 256 bf16 keys of 8 heads of 128, one sequence 9.1 / 6.6, 32 of them 12.4 /
-// 11.0; 512 keys 9.5 / 8.3 and 14.7 / 15.1; 512 keys in 8 bits 9.4 / 7.4 and 12.7 / 10.6;
-// 1024 float32 keys of 4 heads of 64 10.9 / 18.2.
+// compute unit has little enough to read (by itself it reads some 40 GB/s).  us in a
+// captured graph, whole / shares and join, 1, 8 and 32 sequences, 8 KV heads:
+//                        128 KB and less               256 KB
+//   bf16, 128 features   256 keys  6.3 / 8.9           512 keys  7.7 / 9.1
+//                                  6.9 / 10.3                    11.4 / 10.7
+//                                  9.1 / 12.1                    15.2 / 15.6
+//   8 bits, the same     512 keys  7.2 / 9.2           1024 keys 10.1 / 9.6
+//                                  7.6 / 10.5                    10.5 / 11.4
+//                                  9.2 / 14.6                    16.2 / 19.6
+//   bf16, 64 features    512 keys  5.7 / 8.1           1024 keys 7.8 / 8.3
+//                                  6.3 / 9.3                     11.9 / 9.9
+//                                  8.5 / 11.7                    14.5 / 15.8
+//   float32, 64          256 keys  7.8 / 8.4           512 keys  11.2 / 8.7
+//                                  8.5 / 9.2                     12.2 / 9.9
+//                                  10.7 / 12.6                   16.1 / 16.5
+// Up to 128 KB whole is faster at any number of sequences.  At 256 KB either side can be;
+// which one depends on the number of workgroups too, and the shares taken there cost up to
+// 1.4 us with one sequence and 3.4 with 32.
 constexpr int64_t kWholeBytes = 128 << 10;
 static bool paged_whole(int64_t capacity, int64_t row_bytes) { return capacity * 2 * row_bytes <= kWholeBytes; }
 
